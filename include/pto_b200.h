@@ -232,6 +232,53 @@ int pto_b200_gemm_mx_static(void* stream, uint8_t* out, const uint8_t* src0, con
                             int b_dtype, int out_dtype);
 
 /*
+ * NVFP4, two-level 4-bit floating point. No counterpart in the reference (its 4-bit tiles are MXFP4): e2m1 elements,
+ * one e4m3 scale per 16 elements of a row, one fp32 scale g per tensor; an element stands for code * scale * g.
+ * Codes are packed two per byte (element 2i in the low nibble of byte i). Scales are held in 512-byte tiles of 128 rows
+ * x 4 scales (64 elements), tile (row / 128, k / 64) in row-major order, scale j of row r of a tile at byte
+ * (r % 32) * 16 + r / 32 * 4 + j; bytes that only pad a tile are zero (pto_b200_nvfp4_quantize writes them).
+ */
+size_t pto_b200_nvfp4_scale_bytes(int rows, int k);
+
+/* The largest finite magnitude of a rows x k matrix (F32, BF16 or F16, leading dimension ld_src elements) -> *amax. */
+int pto_b200_amax(void* stream, float* amax, const uint8_t* src, int rows, int k, long long ld_src, int src_dtype);
+
+/*
+ * Quantise src (rows x k; F32, BF16 or F16; leading dimension ld_src elements) to NVFP4:
+ *   *tensor_scale = g = the smallest power of two >= *amax / 2688 (1 for 0; *amax is finite and not negative)
+ *   scale         = the e4m3 value nearest to max|x| / (6 g) of its 16 elements, at most 448
+ *   code          = the e2m1 value nearest to x / (scale g), ties to the even code, at most 6; 0 where the scale is 0
+ * Decisions are those of exact arithmetic. A block with an infinity or a NaN gets the scale NaN (0x7F) and zero codes;
+ * the last block of a row is filled up with zeros.
+ *   data   : rows runs of ceil(k / 16) * 8 bytes, leading dimension ld_data bytes (a multiple of 8), 8-byte aligned
+ *            (16 for pto_b200_gemm_nvfp4)
+ *   scales : pto_b200_nvfp4_scale_bytes(rows, k) bytes, 4-byte aligned (16 for pto_b200_gemm_nvfp4)
+ * transpose != 0: the same of src's transpose: data has k runs over ceil(rows / 16) * 16 elements, scales
+ * pto_b200_nvfp4_scale_bytes(k, rows) bytes.
+ */
+int pto_b200_nvfp4_quantize(void* stream, uint8_t* data, uint8_t* scales, float* tensor_scale, const uint8_t* src,
+                            const float* amax, int rows, int k, long long ld_src, long long ld_data, int src_dtype,
+                            int transpose);
+
+/*
+ * Back to numbers: out[r][i] = code * scale * g for the first k elements of each row (tensor_scale null: g = 1), F32, BF16
+ * or F16. data: leading dimension ld_data bytes (a multiple of 4, at least ceil(k / 8) * 4), 4-byte aligned.
+ */
+int pto_b200_nvfp4_dequantize(void* stream, uint8_t* out, const uint8_t* data, const uint8_t* scales,
+                              const float* tensor_scale, int rows, int k, long long ld_data, long long ld_out, int out_dtype);
+
+/*
+ * C = scale_a scale_b (A * B) (+ bias) of NVFP4 matrices, fp32 accumulation.
+ *   src0 / src1 : A (m x k) and B column-major (n x k) codes, 16-byte aligned; lda, ldb in 4-bit elements, multiples of 32
+ *   src2 / src3 : their scale tiles, 16-byte aligned; scale_a, scale_b: their tensor scales on the device, or null for 1
+ *   bias        : n floats or null, added before the store cast; out_dtype F32, BF16 or F16; k % 16 == 0.
+ * The result does not depend on timing; nothing is allocated and no workspace is needed.
+ */
+int pto_b200_gemm_nvfp4(void* stream, uint8_t* out, const uint8_t* src0, const uint8_t* src1, const uint8_t* src2,
+                        const uint8_t* src3, const float* scale_a, const float* scale_b, const float* bias, int m, int n, int k,
+                        long long lda, long long ldb, long long ldc, int out_dtype);
+
+/*
  * fp32 -> bf16 cast (round to nearest even) of `count` contiguous elements: the TSTORE cast applied to the
  * reduced K-split partials (gemm_ar: reduced_output -> fp16/bf16 result, kernels/manual/a2a3/gemm_ar/README.md:33-46).
  */

@@ -66,6 +66,14 @@ SYMBOLS = {
     "pto_b200_mx_quantize_e4m3": (_i, [ctypes.c_void_p, _u8p, _u8p, _u8p, _i, _i, _ll, _ll, _ll]),
     "pto_b200_mx_quantize_e4m3_ex": (_i, [ctypes.c_void_p, _u8p, _u8p, _u8p, _i, _i, _ll, _ll, _ll, _i]),
     "pto_b200_mx_quantize_e2m1": (_i, [ctypes.c_void_p, _u8p, _u8p, _u8p, _i, _i, _ll, _ll, _ll, _i]),
+    "pto_b200_nvfp4_scale_bytes": (ctypes.c_size_t, [_i, _i]),
+    "pto_b200_amax": (_i, [ctypes.c_void_p, _u8p, _u8p, _i, _i, _ll, _i]),
+    "pto_b200_nvfp4_quantize": (_i, [ctypes.c_void_p, _u8p, _u8p, _u8p, _u8p, _u8p, _i, _i, _ll, _ll, _i, _i]),
+    "pto_b200_nvfp4_dequantize": (_i, [ctypes.c_void_p, _u8p, _u8p, _u8p, _u8p, _i, _i, _ll, _ll, _i]),
+    "pto_b200_gemm_nvfp4": (
+        _i,
+        [ctypes.c_void_p, _u8p, _u8p, _u8p, _u8p, _u8p, _u8p, _u8p, _u8p, _i, _i, _i, _ll, _ll, _ll, _i],
+    ),
     "pto_b200_gemm_mx_static": (
         _i,
         [ctypes.c_void_p, _u8p, _u8p, _u8p, _u8p, _u8p, _i, _i, _i, _ll, _ll, _ll, _ll, _ll, _i, _i, _i],

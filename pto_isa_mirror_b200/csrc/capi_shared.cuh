@@ -1,0 +1,32 @@
+// What the sources behind the C ABI share on the host side: per-device set-up, tensor maps, error notes, launch counts.
+#pragma once
+#include "../../include/pto_b200.h"
+
+#include <cuda.h>
+#include <cuda_runtime.h>
+
+namespace pto_b200 {
+
+constexpr int kMaxDevices = 64;
+
+struct HostContext {
+    int device;           // ordinal of the current device, below kMaxDevices
+    int sm_count;
+    int* status;          // device address of the status word the kernels record a given-up wait in
+    long long wait_limit; // cycles one bounded wait may take
+};
+
+// The current device's context; a PTO_B200 code other than 0 when it is no sm_100 GPU or a CUDA call fails.
+int host_context(HostContext* out);
+
+// Records the text of a failed CUDA call for pto_b200_last_cuda_error; PTO_B200_OK or PTO_B200_ECUDA.
+int note_cuda_error(cudaError_t e, const char* what);
+
+// Counts kernel launches for pto_b200_launch_count.
+void count_launches(int n);
+
+// 2-D map of [rows, cols] elements of `type` with a row pitch in bytes and 128-byte swizzled (or plain) boxes.
+int encode_map_2d(CUtensorMap* map, CUtensorMapDataType type, const void* base, long long rows, long long cols,
+                  long long pitch_bytes, int box_cols, int box_rows, bool swizzle128);
+
+} // namespace pto_b200

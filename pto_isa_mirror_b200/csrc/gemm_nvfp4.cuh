@@ -1,0 +1,659 @@
+// Product of two NVFP4 matrices on sm_100a:
+//   C[i][j] = ga gb sum_k (a[i][k] sa[i][k/16]) (b[j][k] sb[j][k/16])  (+ bias[j])
+// with e2m1 elements, e4m3 scales and fp32 accumulation: tcgen05.mma kind::mxf4nvf4, which multiplies 64 elements of K
+// per instruction and applies a scale per 16 of them from tensor memory. A 128-byte swizzle row holds 256 packed
+// elements, so a ring stage is 256 elements of K: four instructions.
+//
+// Scales come in the 512-byte tiles nvfp4_quantize.cuh describes, which tcgen05.cp moves to tensor memory as they are.
+// The last stage of K may hold fewer than four 64-element groups: only those that exist are multiplied, so what stands
+// in the scale buffers past them never matters.
+//
+// gemm_nvfp4_2cta: a cluster of two CTAs owns a 256 x 256 tile (many rows). gemm_nvfp4_few_rows: few rows of A, the
+// bound is reading B; see there.
+#pragma once
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+
+#include <cstdint>
+
+#include "gemm_tile_loop.cuh"
+#include "sm100_ptx.cuh"
+
+namespace pto_b200 {
+
+enum NvOut : int { NV_OUT_F32 = 0, NV_OUT_BF16 = 1, NV_OUT_F16 = 2 };
+
+struct NvGemmParams {
+    void* c;
+    long long ldc;      // elements
+    int m, n;
+    int m_tiles, n_tiles, group_m;
+    int k_stages;       // 256-element stages of K
+    int k_atoms;        // 64-element groups of K
+    uint32_t idesc;
+    const float* ga;    // tensor scales, or null for 1
+    const float* gb;
+    const float* bias;  // n values, or null
+    const uint8_t* sfa; // tiled scales
+    const uint8_t* sfb;
+    int* status;
+    long long wait_limit;
+    int tma_store;      // pair kernel: C leaves through TMA stores
+};
+
+// status codes of bounded waits that gave up
+constexpr int ST_NV_PRODUCER = 21;
+constexpr int ST_NV_SCALES = 22;
+constexpr int ST_NV_MMA = 23;
+constexpr int ST_NV_EPILOGUE = 24;
+
+constexpr int kNvStageK = 256;       // elements of K per stage
+constexpr int kNvAtomBytes = 512;    // scales of 128 rows x 64 elements
+
+__device__ __forceinline__ float nv_alpha(const NvGemmParams& p)
+{
+    const float a = p.ga != nullptr ? __ldg(p.ga) : 1.0f;
+    const float b = p.gb != nullptr ? __ldg(p.gb) : 1.0f;
+    return a * b;
+}
+
+template <int OUT>
+__device__ __forceinline__ uint32_t nv_pack2(float lo, float hi)
+{
+    if constexpr (OUT == NV_OUT_F16) {
+        const __half2 h = __floats2half2_rn(lo, hi);
+        return *reinterpret_cast<const uint32_t*>(&h);
+    } else {
+        const __nv_bfloat162 h = __floats2bfloat162_rn(lo, hi);
+        return *reinterpret_cast<const uint32_t*>(&h);
+    }
+}
+
+// ---------------------------------------------------------------- many rows: CTA pairs, 256 x 256 tiles
+//
+// Roles per CTA: warp 0 loads (TMA), warp 1 multiplies (leader CTA) or copies scales to tensor memory (second CTA, whose
+// MMA warp has nothing else to do), warps 2..9 store. A 256-column accumulator and the scale columns of five stages
+// fill tensor memory, so there is one accumulator: the store warps - eight of them, so that a thread owns 128 columns
+// of its row - move it to registers in one go and hand it back before they convert and store, and the next tile's
+// products start some hundred cycles after the last one's end instead of after its stores.
+constexpr int kNvPairStages = 5;
+constexpr int kNvPairThreads = 320;
+constexpr int kNvStoreWarps = 8; // per CTA
+
+struct NvPairSmem {
+    static constexpr int kABytes = 128 * 128;
+    static constexpr int kBBytes = 128 * 128;
+    static constexpr int kSfaBytes = 4 * kNvAtomBytes;
+    static constexpr int kSfbBytes = 8 * kNvAtomBytes; // scales of all 256 columns, in both CTAs
+    static constexpr int kEpiBufBytes = 32 * 128;
+    static constexpr int kAOff = 0;
+    static constexpr int kBOff = kNvPairStages * kABytes;
+    static constexpr int kEpiOff = kBOff + kNvPairStages * kBBytes;
+    static constexpr int kSfaOff = kEpiOff + kNvStoreWarps * kEpiBufBytes;
+    static constexpr int kSfbOff = kSfaOff + kNvPairStages * kSfaBytes;
+    static constexpr int kBarOff = kSfbOff + kNvPairStages * kSfbBytes;
+    static constexpr int kNumBars = 4 * kNvPairStages + 2;
+    static constexpr int kMiscOff = kBarOff + kNumBars * 8;
+    static constexpr int kTotal = kMiscOff + 16 + 1024;
+};
+static_assert(NvPairSmem::kTotal <= 227 * 1024, "shared memory of the pair kernel");
+
+__device__ __forceinline__ void nv_tile_coords(int t, const NvGemmParams& p, int& mi, int& ni)
+{
+    const int group_size = p.group_m * p.n_tiles;
+    const int g = t / group_size;
+    const int first_m = g * p.group_m;
+    const int gm = min(p.m_tiles - first_m, p.group_m);
+    const int r = t - g * group_size;
+    mi = first_m + r % gm;
+    ni = r / gm;
+}
+
+template <int OUT>
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kNvPairThreads, 1)
+    gemm_nvfp4_2cta(const __grid_constant__ CUtensorMap tmap_a, const __grid_constant__ CUtensorMap tmap_b,
+                    const __grid_constant__ CUtensorMap tmap_sfa, const __grid_constant__ CUtensorMap tmap_sfb,
+                    const __grid_constant__ CUtensorMap tmap_c, const NvGemmParams p)
+{
+    using L = NvPairSmem;
+    constexpr int STAGES = kNvPairStages;
+    constexpr uint32_t kSfCol0 = 256;       // scale columns of stage s: [256 + 48 s, +16) for A, the next 32 for B
+    constexpr uint32_t kSfColsPerStage = 48;
+    static_assert(256 + STAGES * 48 <= kTmemCols, "accumulator and scale columns");
+
+    extern __shared__ uint8_t smem_raw[];
+    uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+    uint64_t* full_bar = reinterpret_cast<uint64_t*>(smem + L::kBarOff); // leader: both CTAs' operands landed
+    uint64_t* empty_bar = full_bar + STAGES;                            // each CTA
+    uint64_t* sf_landed_bar = empty_bar + STAGES;                       // second CTA: both CTAs' scales landed
+    uint64_t* sf_full_bar = sf_landed_bar + STAGES;                     // leader: scales are in tensor memory
+    uint64_t* acc_full_bar = sf_full_bar + STAGES;                      // each CTA
+    uint64_t* acc_empty_bar = acc_full_bar + 1;                         // leader: sixteen store warps
+    uint32_t* tmem_base_slot = reinterpret_cast<uint32_t*>(smem + L::kMiscOff);
+    volatile uint32_t* abort_flag = reinterpret_cast<volatile uint32_t*>(smem + L::kMiscOff + 4);
+
+    const int warp = threadIdx.x >> 5;
+    const int lane = threadIdx.x & 31;
+    const uint32_t cta_rank = ptx::cluster_ctarank();
+    const bool leader = (cta_rank == 0);
+    const int pair = blockIdx.x >> 1;
+    const int num_pairs = gridDim.x >> 1;
+    const int tiles = p.m_tiles * p.n_tiles;
+
+    if (threadIdx.x == 0) {
+        for (int s = 0; s < STAGES; ++s) {
+            ptx::mbar_init(&full_bar[s], 1);
+            ptx::mbar_init(&empty_bar[s], 1);
+            ptx::mbar_init(&sf_landed_bar[s], 1);
+            ptx::mbar_init(&sf_full_bar[s], 1);
+        }
+        ptx::mbar_init(acc_full_bar, 1);
+        ptx::mbar_init(acc_empty_bar, 2 * kNvStoreWarps);
+        *abort_flag = 0;
+        ptx::fence_mbar_init();
+        ptx::prefetch_tensormap(&tmap_a);
+        ptx::prefetch_tensormap(&tmap_b);
+        ptx::prefetch_tensormap(&tmap_sfa);
+        ptx::prefetch_tensormap(&tmap_sfb);
+        if (p.tma_store != 0) {
+            ptx::prefetch_tensormap(&tmap_c);
+        }
+    }
+    if (warp == 1) {
+        ptx::tmem_alloc_pair(tmem_base_slot, kTmemCols);
+        ptx::tmem_relinquish_alloc_permit_pair();
+    }
+    ptx::tc_fence_before_sync();
+    __syncthreads();
+    ptx::cluster_arrive(); // the peer's barriers must exist before anything is signalled across the pair
+    ptx::cluster_wait();
+    ptx::tc_fence_after_sync();
+    const uint32_t tmem_base = *tmem_base_slot;
+
+    if (warp == 0) {
+        // ---------------------------------------------------------------- loads (both CTAs)
+        if (lane == 0) {
+            int stage = 0;
+            uint32_t phase = 0;
+            bool ok = true;
+            for (int t = pair; ok && t < tiles; t += num_pairs) {
+                int mi, ni;
+                nv_tile_coords(t, p, mi, ni);
+                const int row_a = mi * 256 + static_cast<int>(cta_rank) * 128;
+                const int row_b = ni * 256 + static_cast<int>(cta_rank) * 128;
+                // scale tiles as rows of 256 bytes, two per 512-byte tile; tiles past the last row read as zero
+                const int sfa_row = (2 * mi + static_cast<int>(cta_rank)) * p.k_atoms * 2;
+                const int sfb_row = 2 * ni * p.k_atoms * 2;
+                for (int ks = 0; ks < p.k_stages; ++ks) {
+                    ok = bounded_wait(&empty_bar[stage], phase ^ 1u, abort_flag, p.status, ST_NV_PRODUCER, p.wait_limit);
+                    if (!ok) {
+                        break;
+                    }
+                    if (leader) {
+                        ptx::mbar_arrive_expect_tx(&full_bar[stage], 2u * (L::kABytes + L::kBBytes));
+                    } else {
+                        ptx::mbar_arrive_expect_tx(&sf_landed_bar[stage], 2u * (L::kSfaBytes + L::kSfbBytes));
+                    }
+                    const uint32_t full_addr = ptx::map_to_cta(ptx::smem_u32(&full_bar[stage]), 0);
+                    const uint32_t landed_addr = ptx::map_to_cta(ptx::smem_u32(&sf_landed_bar[stage]), 1);
+                    uint8_t* sfa = smem + L::kSfaOff + stage * L::kSfaBytes;
+                    uint8_t* sfb = smem + L::kSfbOff + stage * L::kSfbBytes;
+                    ptx::tma_load_2d_pair(sfa, &tmap_sfa, landed_addr, 0, sfa_row + ks * 8);
+                    ptx::tma_load_2d_pair(sfb, &tmap_sfb, landed_addr, 0, sfb_row + ks * 8);
+                    ptx::tma_load_2d_pair(sfb + 4 * kNvAtomBytes, &tmap_sfb, landed_addr, 0, sfb_row + p.k_atoms * 2 + ks * 8);
+                    ptx::tma_load_2d_pair(smem + L::kAOff + stage * L::kABytes, &tmap_a, full_addr, ks * 128, row_a);
+                    ptx::tma_load_2d_pair(smem + L::kBOff + stage * L::kBBytes, &tmap_b, full_addr, ks * 128, row_b);
+                    if (++stage == STAGES) {
+                        stage = 0;
+                        phase ^= 1u;
+                    }
+                }
+            }
+        }
+    } else if (warp == 1 && !leader) {
+        // ---------------------------------------------------------------- scales to tensor memory (second CTA)
+        // cta_group::2 copies the same shared-memory offsets of both CTAs into both CTAs' tensor memory
+        if (lane == 0) {
+            int stage = 0;
+            uint32_t phase = 0;
+            bool ok = true;
+            for (int t = pair; ok && t < tiles; t += num_pairs) {
+                for (int ks = 0; ks < p.k_stages; ++ks) {
+                    ok = bounded_wait(&sf_landed_bar[stage], phase, abort_flag, p.status, ST_NV_SCALES, p.wait_limit);
+                    if (!ok) {
+                        break;
+                    }
+                    ptx::tc_fence_after_sync();
+                    const uint32_t sfa = ptx::smem_u32(smem + L::kSfaOff + stage * L::kSfaBytes);
+                    const uint32_t sfb = ptx::smem_u32(smem + L::kSfbOff + stage * L::kSfbBytes);
+                    const uint32_t sf = tmem_base + kSfCol0 + kSfColsPerStage * static_cast<uint32_t>(stage);
+#pragma unroll
+                    for (uint32_t g = 0; g < 4; ++g) {
+                        ptx::tmem_cp_32x128b_warpx4_pair(sf + 4u * g, ptx::make_smem_desc(sfa + 512u * g, 0, 128, ptx::kSwizzleNone));
+                        ptx::tmem_cp_32x128b_warpx4_pair(sf + 16u + 8u * g,
+                                                         ptx::make_smem_desc(sfb + 512u * g, 0, 128, ptx::kSwizzleNone));
+                        ptx::tmem_cp_32x128b_warpx4_pair(sf + 20u + 8u * g,
+                                                         ptx::make_smem_desc(sfb + 2048u + 512u * g, 0, 128, ptx::kSwizzleNone));
+                    }
+                    ptx::umma_commit_pair(&sf_full_bar[stage], 0x1);
+                    if (++stage == STAGES) {
+                        stage = 0;
+                        phase ^= 1u;
+                    }
+                }
+            }
+        }
+    } else if (warp == 1) {
+        // ---------------------------------------------------------------- products (leader)
+        if (lane == 0) {
+            int stage = 0;
+            uint32_t phase = 0;
+            uint32_t acc_phase = 0;
+            bool ok = true;
+            for (int t = pair; ok && t < tiles; t += num_pairs) {
+                ok = bounded_wait(acc_empty_bar, acc_phase ^ 1u, abort_flag, p.status, ST_NV_MMA, p.wait_limit);
+                if (!ok) {
+                    break;
+                }
+                ptx::tc_fence_after_sync();
+                for (int ks = 0; ks < p.k_stages; ++ks) {
+                    ok = bounded_wait(&full_bar[stage], phase, abort_flag, p.status, ST_NV_MMA, p.wait_limit) &&
+                         bounded_wait(&sf_full_bar[stage], phase, abort_flag, p.status, ST_NV_MMA, p.wait_limit);
+                    if (!ok) {
+                        break;
+                    }
+                    ptx::tc_fence_after_sync();
+                    const uint32_t a_base = ptx::smem_u32(smem + L::kAOff + stage * L::kABytes);
+                    const uint32_t b_base = ptx::smem_u32(smem + L::kBOff + stage * L::kBBytes);
+                    const uint32_t sf = tmem_base + kSfCol0 + kSfColsPerStage * static_cast<uint32_t>(stage);
+                    const int groups = min(4, p.k_atoms - 4 * ks);
+#pragma unroll
+                    for (int g = 0; g < 4; ++g) {
+                        if (g < groups) {
+                            ptx::umma_nvf4_pair(tmem_base, ptx::make_smem_desc(a_base + g * 32, 16, 1024, ptx::kSwizzle128B),
+                                                ptx::make_smem_desc(b_base + g * 32, 16, 1024, ptx::kSwizzle128B), p.idesc,
+                                                sf + 4u * g, sf + 16u + 8u * g, (ks > 0 || g > 0) ? 1u : 0u);
+                        }
+                    }
+                    ptx::umma_commit_pair(&empty_bar[stage], 0x3);
+                    if (++stage == STAGES) {
+                        stage = 0;
+                        phase ^= 1u;
+                    }
+                }
+                if (!ok) {
+                    break;
+                }
+                ptx::umma_commit_pair(acc_full_bar, 0x3);
+                acc_phase ^= 1u;
+            }
+        }
+    } else {
+        // ---------------------------------------------------------------- stores (both CTAs)
+        constexpr bool kOut32 = (OUT == NV_OUT_F32);
+        constexpr int kBoxCols = kOut32 ? 32 : 64; // a box is 32 rows x 128 bytes
+        constexpr int kBoxes = 128 / kBoxCols;
+        const int quarter = warp & 3;
+        const int half = (warp - 2) >> 2; // which 128 columns
+        uint8_t* box = smem + L::kEpiOff + (warp - 2) * L::kEpiBufBytes;
+        const float alpha = nv_alpha(p);
+        uint32_t acc_phase = 0;
+        bool ok = true;
+        for (int t = pair; ok && t < tiles; t += num_pairs) {
+            int mi, ni;
+            nv_tile_coords(t, p, mi, ni);
+            ok = bounded_wait(acc_full_bar, acc_phase, abort_flag, p.status, ST_NV_EPILOGUE, p.wait_limit);
+            ok = __all_sync(0xFFFFFFFFu, ok);
+            if (!ok) {
+                break;
+            }
+            acc_phase ^= 1u;
+            ptx::tc_fence_after_sync();
+            uint32_t v[4][32];
+            const uint32_t t_row = tmem_base + static_cast<uint32_t>(half * 128) + (static_cast<uint32_t>(quarter * 32) << 16);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                ptx::tmem_ld_32x32b_x32(t_row + 32u * i, v[i]);
+            }
+            ptx::tmem_ld_wait();
+            ptx::tc_fence_before_sync();
+            __syncwarp();
+            if (lane == 0) {
+                if (leader) {
+                    ptx::mbar_arrive(acc_empty_bar);
+                } else {
+                    ptx::mbar_arrive_cluster(ptx::map_to_cta(ptx::smem_u32(acc_empty_bar), 0));
+                }
+            }
+            const int row0 = mi * 256 + static_cast<int>(cta_rank) * 128 + quarter * 32;
+            const int col0 = ni * 256 + half * 128;
+#pragma unroll
+            for (int b = 0; b < kBoxes; ++b) {
+                const int bc = col0 + b * kBoxCols;
+                if (bc >= p.n || row0 >= p.m) {
+                    break;
+                }
+                if (p.tma_store != 0 && lane == 0) {
+                    ptx::bulk_wait_group_read<0>(); // the box's last store has left shared memory
+                }
+                __syncwarp();
+                uint8_t* line = box + lane * 128;
+#pragma unroll
+                for (int q = 0; q < 8; ++q) { // 16-byte pieces of this thread's row, 128-byte swizzle
+                    uint32_t o[4];
+                    if constexpr (kOut32) {
+#pragma unroll
+                        for (int j = 0; j < 4; ++j) {
+                            const int col = q * 4 + j;
+                            float f = __uint_as_float(v[b][col]) * alpha;
+                            if (p.bias != nullptr && bc + col < p.n) {
+                                f += __ldg(p.bias + bc + col);
+                            }
+                            o[j] = __float_as_uint(f);
+                        }
+                    } else {
+#pragma unroll
+                        for (int j = 0; j < 4; ++j) {
+                            const int col = q * 8 + 2 * j;
+                            float lo = __uint_as_float(v[2 * b + col / 32][col % 32]) * alpha;
+                            float hi = __uint_as_float(v[2 * b + col / 32][col % 32 + 1]) * alpha;
+                            if (p.bias != nullptr) {
+                                lo += bc + col < p.n ? __ldg(p.bias + bc + col) : 0.0f;
+                                hi += bc + col + 1 < p.n ? __ldg(p.bias + bc + col + 1) : 0.0f;
+                            }
+                            o[j] = nv_pack2<OUT>(lo, hi);
+                        }
+                    }
+                    *reinterpret_cast<uint4*>(line + ((q ^ (lane & 7)) * 16)) = make_uint4(o[0], o[1], o[2], o[3]);
+                }
+                if (p.tma_store != 0) {
+                    ptx::fence_proxy_async_smem();
+                    __syncwarp();
+                    if (lane == 0) {
+                        ptx::tma_store_2d(&tmap_c, box, bc, row0);
+                        ptx::bulk_commit_group();
+                    }
+                } else {
+                    // C or its rows off the TMA's 16-byte grid: element by element, a warp along one row at a time
+                    __syncwarp();
+                    const int rows_here = min(32, p.m - row0);
+                    for (int r = 0; r < rows_here; ++r) {
+                        const uint8_t* src = box + r * 128;
+                        const long long base = (static_cast<long long>(row0) + r) * p.ldc + bc;
+                        if constexpr (kOut32) {
+                            if (bc + lane < p.n) {
+                                static_cast<uint32_t*>(p.c)[base + lane] =
+                                    *reinterpret_cast<const uint32_t*>(src + ((lane >> 2) ^ (r & 7)) * 16 + (lane & 3) * 4);
+                            }
+                        } else {
+#pragma unroll
+                            for (int h = 0; h < 2; ++h) {
+                                const int e = h * 32 + lane;
+                                if (bc + e < p.n) {
+                                    static_cast<uint16_t*>(p.c)[base + e] =
+                                        *reinterpret_cast<const uint16_t*>(src + ((e >> 3) ^ (r & 7)) * 16 + (e & 7) * 2);
+                                }
+                            }
+                        }
+                    }
+                    __syncwarp();
+                }
+            }
+        }
+        if (lane == 0) {
+            ptx::bulk_wait_group_read<0>(); // shared memory outlives the reads of the last boxes
+        }
+    }
+
+    ptx::tc_fence_before_sync();
+    __syncthreads();
+    if (*abort_flag != 0) {
+        for (int i = 0; i < 2000; ++i) { // copies and products in flight end before shared and tensor memory go away
+            __nanosleep(1000);
+        }
+    }
+    ptx::cluster_arrive_relaxed();
+    ptx::cluster_wait();
+    if (warp == 1) {
+        ptx::tc_fence_after_sync();
+        ptx::tmem_dealloc_pair(tmem_base, kTmemCols);
+    }
+}
+
+// ---------------------------------------------------------------- few rows of A
+//
+// With few rows the product reads B once and does little else, so B takes the instruction's 128-row side (128 columns
+// of C per CTA) and the rows of A its N side (BLOCK_T = 16 .. 128 of them): no MMA rows are wasted on rows that are not
+// there, and lane = column of C makes the stores of a row contiguous. When the tiles are fewer than the CTAs that fit
+// the GPU, a cluster of CTAs shares a tile along K: each keeps fp32 partial sums, which are added over distributed
+// shared memory in rank order, so the result does not depend on timing and no workspace is needed.
+// Shared memory is kept below half an SM's, so that two CTAs run per SM and one's loads cover the other's start and end.
+constexpr int kNvFewThreads = 192;
+
+template <int BLOCK_T>
+struct NvFewSmem {
+    static constexpr int kWBytes = 128 * 128;      // B: 128 columns of C
+    static constexpr int kXBytes = BLOCK_T * 128;  // A: BLOCK_T rows
+    static constexpr int kSfBytes = 4 * kNvAtomBytes;
+    static constexpr int kStageBytes = kWBytes + kXBytes + 2 * kSfBytes;
+    static constexpr int kStages = (111 * 1024) / kStageBytes;
+    static constexpr int kXOff = kStages * kWBytes;
+    static constexpr int kSfwOff = kXOff + kStages * kXBytes;
+    static constexpr int kSfxOff = kSfwOff + kStages * kSfBytes;
+    static constexpr int kBarOff = kSfxOff + kStages * kSfBytes;
+    static constexpr int kMiscOff = kBarOff + (2 * kStages + 1) * 8;
+    static constexpr int kTotal = kMiscOff + 16 + 1024;
+    static_assert(BLOCK_T * 128 * 4 <= kBarOff, "partial sums reuse the ring");
+    static_assert(kTotal <= 113 * 1024, "two CTAs per SM");
+    static constexpr int kSfCol = BLOCK_T < 32 ? 32 : BLOCK_T; // scale columns, 32 per stage, behind the accumulator
+    static constexpr int kTmem = 256;                          // half an SM's
+    static_assert(kSfCol + 32 * kStages <= kTmem, "accumulator and scale columns");
+};
+
+template <int OUT>
+__device__ __forceinline__ void nv_store_one(const NvGemmParams& p, long long row, int col, float f)
+{
+    const long long at = row * p.ldc + col;
+    if constexpr (OUT == NV_OUT_F32) {
+        static_cast<float*>(p.c)[at] = f;
+    } else if constexpr (OUT == NV_OUT_BF16) {
+        static_cast<__nv_bfloat16*>(p.c)[at] = __float2bfloat16_rn(f);
+    } else {
+        static_cast<__half*>(p.c)[at] = __float2half_rn(f);
+    }
+}
+
+// grid: splits (the cluster) x 128-column tiles x BLOCK_T-row tiles
+template <int BLOCK_T, int OUT>
+__global__ void __launch_bounds__(kNvFewThreads, 2)
+    gemm_nvfp4_few_rows(const __grid_constant__ CUtensorMap tmap_w, const __grid_constant__ CUtensorMap tmap_x,
+                        const NvGemmParams p)
+{
+    using L = NvFewSmem<BLOCK_T>;
+    constexpr int STAGES = L::kStages;
+    extern __shared__ uint8_t smem_raw[];
+    uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+    uint64_t* full_bar = reinterpret_cast<uint64_t*>(smem + L::kBarOff);
+    uint64_t* empty_bar = full_bar + STAGES;
+    uint64_t* acc_bar = empty_bar + STAGES;
+    uint32_t* tmem_base_slot = reinterpret_cast<uint32_t*>(smem + L::kMiscOff);
+    volatile uint32_t* abort_flag = reinterpret_cast<volatile uint32_t*>(smem + L::kMiscOff + 4);
+
+    const int warp = threadIdx.x >> 5;
+    const int lane = threadIdx.x & 31;
+    const int splits = static_cast<int>(gridDim.x);
+    const int rank = static_cast<int>(blockIdx.x);
+    const int ni = static_cast<int>(blockIdx.y);
+    const int ti = static_cast<int>(blockIdx.z);
+    const int ks0 = static_cast<int>(static_cast<long long>(p.k_stages) * rank / splits);
+    const int ks1 = static_cast<int>(static_cast<long long>(p.k_stages) * (rank + 1) / splits);
+
+    if (threadIdx.x == 0) {
+        for (int s = 0; s < STAGES; ++s) {
+            ptx::mbar_init(&full_bar[s], 1);
+            ptx::mbar_init(&empty_bar[s], 1);
+        }
+        ptx::mbar_init(acc_bar, 1);
+        *abort_flag = 0;
+        ptx::fence_mbar_init();
+        ptx::prefetch_tensormap(&tmap_w);
+        ptx::prefetch_tensormap(&tmap_x);
+    }
+    if (warp == 1) {
+        ptx::tmem_alloc(tmem_base_slot, L::kTmem);
+        ptx::tmem_relinquish_alloc_permit();
+    }
+    ptx::tc_fence_before_sync();
+    __syncthreads();
+    ptx::tc_fence_after_sync();
+    const uint32_t tmem_base = *tmem_base_slot;
+
+    if (warp == 0) {
+        if (lane == 0) {
+            int stage = 0;
+            uint32_t phase = 0;
+            const uint8_t* sfw = p.sfb + static_cast<size_t>(ni) * p.k_atoms * kNvAtomBytes;
+            const uint8_t* sfx = p.sfa + static_cast<size_t>(ti) * p.k_atoms * kNvAtomBytes;
+            for (int ks = ks0; ks < ks1; ++ks) {
+                if (!bounded_wait(&empty_bar[stage], phase ^ 1u, abort_flag, p.status, ST_NV_PRODUCER, p.wait_limit)) {
+                    break;
+                }
+                const uint32_t sf_bytes = static_cast<uint32_t>(min(4, p.k_atoms - 4 * ks)) * kNvAtomBytes;
+                ptx::mbar_arrive_expect_tx(&full_bar[stage], L::kWBytes + L::kXBytes + 2u * sf_bytes);
+                ptx::tma_load_2d(smem + stage * L::kWBytes, &tmap_w, &full_bar[stage], ks * 128, ni * 128);
+                ptx::tma_load_2d(smem + L::kXOff + stage * L::kXBytes, &tmap_x, &full_bar[stage], ks * 128, ti * BLOCK_T);
+                const size_t at = static_cast<size_t>(ks) * 4 * kNvAtomBytes;
+                ptx::bulk_load_1d(smem + L::kSfwOff + stage * L::kSfBytes, sfw + at, sf_bytes, &full_bar[stage]);
+                ptx::bulk_load_1d(smem + L::kSfxOff + stage * L::kSfBytes, sfx + at, sf_bytes, &full_bar[stage]);
+                if (++stage == STAGES) {
+                    stage = 0;
+                    phase ^= 1u;
+                }
+            }
+        }
+    } else if (warp == 1) {
+        if (lane == 0) {
+            int stage = 0;
+            uint32_t phase = 0;
+            bool ok = true;
+            for (int ks = ks0; ks < ks1; ++ks) {
+                ok = bounded_wait(&full_bar[stage], phase, abort_flag, p.status, ST_NV_MMA, p.wait_limit);
+                if (!ok) {
+                    break;
+                }
+                ptx::tc_fence_after_sync();
+                const uint32_t w_base = ptx::smem_u32(smem + stage * L::kWBytes);
+                const uint32_t x_base = ptx::smem_u32(smem + L::kXOff + stage * L::kXBytes);
+                const uint32_t sfw = ptx::smem_u32(smem + L::kSfwOff + stage * L::kSfBytes);
+                const uint32_t sfx = ptx::smem_u32(smem + L::kSfxOff + stage * L::kSfBytes);
+                // every stage has its own scale columns: a copy never meets a product that still reads them
+                const uint32_t sf = tmem_base + L::kSfCol + 32u * static_cast<uint32_t>(stage);
+                const int groups = min(4, p.k_atoms - 4 * ks);
+#pragma unroll
+                for (int g = 0; g < 4; ++g) {
+                    if (g < groups) {
+                        ptx::tmem_cp_32x128b_warpx4(sf + 4u * g, ptx::make_smem_desc(sfw + 512u * g, 0, 128, ptx::kSwizzleNone));
+                        ptx::tmem_cp_32x128b_warpx4(sf + 16u + 4u * g,
+                                                    ptx::make_smem_desc(sfx + 512u * g, 0, 128, ptx::kSwizzleNone));
+                    }
+                }
+#pragma unroll
+                for (int g = 0; g < 4; ++g) {
+                    if (g < groups) {
+                        ptx::umma_nvf4(tmem_base, ptx::make_smem_desc(w_base + g * 32, 16, 1024, ptx::kSwizzle128B),
+                                       ptx::make_smem_desc(x_base + g * 32, 16, 1024, ptx::kSwizzle128B), p.idesc, sf + 4u * g,
+                                       sf + 16u + 4u * g, (ks > ks0 || g > 0) ? 1u : 0u);
+                    }
+                }
+                ptx::umma_commit(&empty_bar[stage]);
+                if (++stage == STAGES) {
+                    stage = 0;
+                    phase ^= 1u;
+                }
+            }
+            if (ok) {
+                ptx::umma_commit(acc_bar);
+            }
+        }
+    } else {
+        bool ok = bounded_wait(acc_bar, 0, abort_flag, p.status, ST_NV_EPILOGUE, p.wait_limit);
+        ok = __all_sync(0xFFFFFFFFu, ok);
+        if (ok) {
+            ptx::tc_fence_after_sync();
+            const int quarter = warp & 3;
+            const int in_tile = quarter * 32 + lane;
+            const int col = ni * 128 + in_tile;
+            const float alpha = nv_alpha(p);
+            const float bias = (p.bias != nullptr && col < p.n) ? __ldg(p.bias + col) : 0.0f;
+            float* part = reinterpret_cast<float*>(smem); // [BLOCK_T][128]; every load and product of the ring is done
+            uint32_t v[32];
+#pragma unroll
+            for (int c = 0; c < (BLOCK_T + 31) / 32; ++c) {
+                const int t0 = ti * BLOCK_T + c * 32;
+                if (t0 >= p.m) {
+                    break;
+                }
+                ptx::tmem_ld_32x32b_x32(tmem_base + 32u * c + (static_cast<uint32_t>(quarter * 32) << 16), v);
+                ptx::tmem_ld_wait();
+                const int valid = min(min(32, BLOCK_T), p.m - t0);
+                if (splits == 1) {
+                    if (col < p.n) {
+#pragma unroll
+                        for (int i = 0; i < 32; ++i) {
+                            if (i < valid) {
+                                nv_store_one<OUT>(p, t0 + i, col, __uint_as_float(v[i]) * alpha + bias);
+                            }
+                        }
+                    }
+                } else {
+#pragma unroll
+                    for (int i = 0; i < 32; ++i) {
+                        if (i < valid) {
+                            part[(c * 32 + i) * 128 + in_tile] = __uint_as_float(v[i]);
+                        }
+                    }
+                }
+            }
+        }
+    }
+
+    ptx::tc_fence_before_sync();
+    __syncthreads();
+    if (*abort_flag != 0) {
+        for (int i = 0; i < 2000; ++i) {
+            __nanosleep(1000);
+        }
+    }
+    if (warp == 1) {
+        ptx::tc_fence_after_sync();
+        ptx::tmem_dealloc(tmem_base, L::kTmem);
+    }
+    if (splits > 1) {
+        ptx::cluster_arrive(); // every CTA's partial sums are in its shared memory
+        ptx::cluster_wait();
+        const int rows = min(BLOCK_T, p.m - ti * BLOCK_T);
+        const int items = rows * 128;
+        const int first = static_cast<int>(static_cast<long long>(items) * rank / splits);
+        const int last = static_cast<int>(static_cast<long long>(items) * (rank + 1) / splits);
+        const float alpha = nv_alpha(p);
+        const uint32_t base = ptx::smem_u32(smem);
+        for (int i = first + static_cast<int>(threadIdx.x); i < last; i += kNvFewThreads) {
+            const int col = ni * 128 + (i & 127);
+            if (col < p.n) {
+                float sum = 0.0f;
+                for (int r = 0; r < splits; ++r) {
+                    sum += ptx::ld_shared_cluster_f32(ptx::map_to_cta(base + 4u * static_cast<uint32_t>(i), static_cast<uint32_t>(r)));
+                }
+                sum *= alpha;
+                if (p.bias != nullptr) {
+                    sum += __ldg(p.bias + col);
+                }
+                nv_store_one<OUT>(p, static_cast<long long>(ti) * BLOCK_T + (i >> 7), col, sum);
+            }
+        }
+        ptx::cluster_arrive_relaxed(); // no CTA leaves while another still reads its shared memory
+        ptx::cluster_wait();
+    }
+}
+
+} // namespace pto_b200

@@ -660,7 +660,7 @@ __global__ void __launch_bounds__(kNumThreads, 1)
 // tcgen05.cp 32x128b.warpx4 copy expects: atom (k_block, row_block) holds 128 rows x 4 scales with
 // byte offset (r % 32) * 16 + (r / 32) * 4 + j. Rows / K-blocks past the end get 127 (= 2^0).
 // One launch re-tiles both operands' scales: items [0, a_blocks * k_blocks * 128) belong to A, the rest to B.
-__global__ void retile_scales_kernel(const uint8_t* __restrict__ src_a, uint8_t* __restrict__ dst_a, int rows_a,
+static __global__ void retile_scales_kernel(const uint8_t* __restrict__ src_a, uint8_t* __restrict__ dst_a, int rows_a,
                                      long long ld_a, int a_blocks, const uint8_t* __restrict__ src_b,
                                      uint8_t* __restrict__ dst_b, int rows_b, long long ld_b, int b_blocks, int k_groups,
                                      int k_blocks)
@@ -697,7 +697,7 @@ __global__ void retile_scales_kernel(const uint8_t* __restrict__ src_a, uint8_t*
 }
 
 // fp32 -> bf16 (round to nearest even) over a contiguous buffer; used after the K-split reduction.
-__global__ void cast_f32_bf16_kernel(const float* __restrict__ src, __nv_bfloat16* __restrict__ dst, long long count)
+static __global__ void cast_f32_bf16_kernel(const float* __restrict__ src, __nv_bfloat16* __restrict__ dst, long long count)
 {
     const long long n4 = count / 4;
     const long long tid = blockIdx.x * static_cast<long long>(blockDim.x) + threadIdx.x;

@@ -1,0 +1,369 @@
+// C ABI of the NVFP4 operators: argument checks, tensor maps, choice of kernel, launch.
+#include "capi_shared.cuh"
+
+#include <atomic>
+
+#include "gemm_nvfp4.cuh"
+#include "nvfp4_quantize.cuh"
+
+namespace pto_b200 {
+namespace {
+
+int source_of(int dtype)
+{
+    return dtype == PTO_B200_F32 ? NV_F32 : dtype == PTO_B200_BF16 ? NV_BF16 : dtype == PTO_B200_F16 ? NV_F16 : -1;
+}
+
+int size_of(int src) { return src == NV_F32 ? 4 : 2; }
+
+bool misaligned(const void* p, unsigned bytes) { return (reinterpret_cast<uintptr_t>(p) & (bytes - 1u)) != 0; }
+
+// Blocks for `items` single-thread items: one resident wave that walks them with a grid stride.
+template <typename Kernel>
+int one_wave(Kernel kernel, long long items, int sm_count, int* grid)
+{
+    int per_sm = 0;
+    if (int rc = note_cuda_error(cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per_sm, kernel, kNvQuantThreads, 0),
+                                 "nvfp4 occupancy")) {
+        return rc;
+    }
+    const long long want = (items + kNvQuantThreads - 1) / kNvQuantThreads;
+    const long long cap = static_cast<long long>(sm_count) * (per_sm > 0 ? per_sm : 1);
+    *grid = static_cast<int>(want < cap ? want : cap);
+    return PTO_B200_OK;
+}
+
+template <int SRC, bool VEC>
+int launch_quantize(cudaStream_t s, int sm_count, const void* src, const float* amax, uint8_t* data, uint8_t* scales,
+                    float* tensor_scale, int rows, int k, long long ld_src, long long ld_data, bool transpose)
+{
+    if (transpose) {
+        constexpr int kSmem = kNvTransRows / 16 * kNvTransGroupBytes<SRC>;
+        auto kernel = nvfp4_quantize_transposed_kernel<SRC, VEC>;
+        if (int rc = note_cuda_error(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem),
+                                     "cudaFuncSetAttribute(nvfp4 transpose)")) {
+            return rc;
+        }
+        // whole 128-row tiles of scales: columns past k are quantised as zeros, which fills the tiles' padding
+        const dim3 grid(static_cast<unsigned>((rows + kNvTransRows - 1) / kNvTransRows),
+                        static_cast<unsigned>((k + 127) / 128 * (128 / kNvTransCols)));
+        kernel<<<grid, kNvQuantThreads, kSmem, s>>>(src, amax, data, scales, tensor_scale, rows, k, ld_src, ld_data);
+    } else {
+        const long long items = (static_cast<long long>(rows) + 127) / 128 * 128 * ((k + 63) / 64 * 4);
+        int grid = 0;
+        if (int rc = one_wave(nvfp4_quantize_kernel<SRC, VEC>, items, sm_count, &grid)) {
+            return rc;
+        }
+        nvfp4_quantize_kernel<SRC, VEC>
+            <<<grid, kNvQuantThreads, 0, s>>>(src, amax, data, scales, tensor_scale, rows, k, ld_src, ld_data);
+    }
+    count_launches(1);
+    return note_cuda_error(cudaGetLastError(), "nvfp4_quantize launch");
+}
+
+template <int SRC, bool VEC>
+int launch_amax(cudaStream_t s, int sm_count, const void* src, float* amax, int rows, int k, long long ld_src)
+{
+    int grid = 0;
+    if (int rc = one_wave(amax_kernel<SRC, VEC>, static_cast<long long>(rows) * ((k + 15) / 16), sm_count, &grid)) {
+        return rc;
+    }
+    if (int rc = note_cuda_error(cudaMemsetAsync(amax, 0, sizeof(float), s), "amax memset")) {
+        return rc;
+    }
+    amax_kernel<SRC, VEC><<<grid, kNvQuantThreads, 0, s>>>(src, reinterpret_cast<uint32_t*>(amax), rows, k, ld_src);
+    count_launches(1);
+    return note_cuda_error(cudaGetLastError(), "amax launch");
+}
+
+template <int DST, bool VEC>
+int launch_dequantize(cudaStream_t s, int sm_count, const uint8_t* data, const uint8_t* scales, const float* tensor_scale,
+                      void* out, int rows, int k, long long ld_data, long long ld_out)
+{
+    int grid = 0;
+    if (int rc = one_wave(nvfp4_dequantize_kernel<DST, VEC>, static_cast<long long>(rows) * ((k + 7) / 8), sm_count, &grid)) {
+        return rc;
+    }
+    nvfp4_dequantize_kernel<DST, VEC>
+        <<<grid, kNvQuantThreads, 0, s>>>(data, scales, tensor_scale, out, rows, k, ld_data, ld_out);
+    count_launches(1);
+    return note_cuda_error(cudaGetLastError(), "nvfp4_dequantize launch");
+}
+
+// f(SRC, VEC) as template arguments
+#define PTO_NV_DISPATCH(src, vec, f, ...)                                                            \
+    ((src) == NV_F32 ? ((vec) ? f<NV_F32, true>(__VA_ARGS__) : f<NV_F32, false>(__VA_ARGS__))        \
+     : (src) == NV_BF16 ? ((vec) ? f<NV_BF16, true>(__VA_ARGS__) : f<NV_BF16, false>(__VA_ARGS__))   \
+                        : ((vec) ? f<NV_F16, true>(__VA_ARGS__) : f<NV_F16, false>(__VA_ARGS__)))
+
+// Instruction descriptor of kind::mxf4nvf4: e2m1 is 1 in both format fields ([7,10) and [10,12)), N >> 3 at [17,23),
+// scale format e4m3 (0) at 23, M >> 7 at [27,29), K = 64 (0) at 31; scale ids 0, since an instruction uses all four
+// bytes of a scale column.
+uint32_t nv_idesc(int m_inst, int n_inst)
+{
+    return (1u << 7) | (1u << 10) | (static_cast<uint32_t>(n_inst >> 3) << 17) | (static_cast<uint32_t>(m_inst >> 7) << 27);
+}
+
+struct NvProblem {
+    const uint8_t* a;
+    const uint8_t* b;
+    int m, n, k;
+    long long lda, ldb; // 4-bit elements
+};
+
+template <int OUT>
+int launch_nv_pair(cudaStream_t stream, const HostContext& host, const NvProblem& q, NvGemmParams p)
+{
+    auto kernel = gemm_nvfp4_2cta<OUT>;
+    static std::atomic<int> max_clusters[kMaxDevices];
+    cudaLaunchConfig_t cfg = {};
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = 2;
+    attr[0].val.clusterDim.y = 1;
+    attr[0].val.clusterDim.z = 1;
+    cfg.blockDim = dim3(kNvPairThreads, 1, 1);
+    cfg.dynamicSmemBytes = NvPairSmem::kTotal;
+    cfg.stream = stream;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    int clusters = max_clusters[host.device].load(std::memory_order_acquire);
+    if (clusters == 0) {
+        if (int rc = note_cuda_error(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, NvPairSmem::kTotal),
+                                     "cudaFuncSetAttribute(nvfp4 pair)")) {
+            return rc;
+        }
+        cfg.gridDim = dim3(2, 1, 1);
+        if (int rc = note_cuda_error(cudaOccupancyMaxActiveClusters(&clusters, kernel, &cfg), "cudaOccupancyMaxActiveClusters")) {
+            return rc;
+        }
+        clusters = clusters > 0 ? clusters : 1;
+        max_clusters[host.device].store(clusters, std::memory_order_release);
+    }
+    p.m_tiles = (q.m + 255) / 256;
+    p.n_tiles = (q.n + 255) / 256;
+    p.group_m = 8;
+    p.idesc = nv_idesc(256, 256);
+    CUtensorMap ta, tb, tsa, tsb, tc;
+    const long long sf_rows_a = (static_cast<long long>(q.m) + 127) / 128 * p.k_atoms * 2;
+    const long long sf_rows_b = (static_cast<long long>(q.n) + 127) / 128 * p.k_atoms * 2;
+    const CUtensorMapDataType u8 = CU_TENSOR_MAP_DATA_TYPE_UINT8;
+    int rc = encode_map_2d(&ta, u8, q.a, q.m, q.k / 2, q.lda / 2, 128, 128, true);
+    rc = rc ? rc : encode_map_2d(&tb, u8, q.b, q.n, q.k / 2, q.ldb / 2, 128, 128, true);
+    rc = rc ? rc : encode_map_2d(&tsa, u8, p.sfa, sf_rows_a, 256, 256, 256, 8, false);
+    rc = rc ? rc : encode_map_2d(&tsb, u8, p.sfb, sf_rows_b, 256, 256, 256, 8, false);
+    // C leaves through TMA stores when its base, its row pitch and the end of its rows lie on 16-byte boundaries (at a
+    // ragged end the store unit is a whole 16-byte piece)
+    constexpr int esize = OUT == NV_OUT_F32 ? 4 : 2;
+    p.tma_store = !misaligned(p.c, 16) && (p.ldc * esize) % 16 == 0 && (static_cast<long long>(q.n) * esize) % 16 == 0;
+    tc = ta;
+    if (p.tma_store) {
+        const CUtensorMapDataType type = OUT == NV_OUT_F32 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32 : CU_TENSOR_MAP_DATA_TYPE_UINT16;
+        rc = rc ? rc : encode_map_2d(&tc, type, p.c, q.m, q.n, p.ldc * esize, 128 / esize, 32, true);
+    }
+    if (rc) {
+        return rc;
+    }
+    const long long tiles = static_cast<long long>(p.m_tiles) * p.n_tiles;
+    cfg.gridDim = dim3(static_cast<unsigned>(2 * (tiles < clusters ? tiles : clusters)), 1, 1);
+    count_launches(1);
+    return note_cuda_error(cudaLaunchKernelEx(&cfg, kernel, ta, tb, tsa, tsb, tc, p), "gemm_nvfp4_2cta launch");
+}
+
+template <int BLOCK_T, int OUT>
+int launch_nv_few(cudaStream_t stream, const HostContext& host, const NvProblem& q, NvGemmParams p)
+{
+    using L = NvFewSmem<BLOCK_T>;
+    auto kernel = gemm_nvfp4_few_rows<BLOCK_T, OUT>;
+    static std::atomic<int> attr_done[kMaxDevices];
+    if (attr_done[host.device].load(std::memory_order_acquire) == 0) {
+        if (int rc = note_cuda_error(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, L::kTotal),
+                                     "cudaFuncSetAttribute(nvfp4 few rows)")) {
+            return rc;
+        }
+        attr_done[host.device].store(1, std::memory_order_release);
+    }
+    p.idesc = nv_idesc(128, BLOCK_T);
+    CUtensorMap tw, tx;
+    const CUtensorMapDataType u8 = CU_TENSOR_MAP_DATA_TYPE_UINT8;
+    int rc = encode_map_2d(&tw, u8, q.b, q.n, q.k / 2, q.ldb / 2, 128, 128, true);
+    rc = rc ? rc : encode_map_2d(&tx, u8, q.a, q.m, q.k / 2, q.lda / 2, 128, BLOCK_T, true);
+    if (rc) {
+        return rc;
+    }
+    const long long n_tiles = (static_cast<long long>(q.n) + 127) / 128;
+    const long long t_tiles = (static_cast<long long>(q.m) + BLOCK_T - 1) / BLOCK_T;
+    if (n_tiles > 65535 || t_tiles > 65535) {
+        return PTO_B200_EINVAL;
+    }
+    // K parts: as many as keep all of them resident at two CTAs per SM, each with two stages of K at least
+    int splits = 1;
+    while (splits < 8 && n_tiles * t_tiles * splits * 2 <= 2ll * host.sm_count && p.k_stages >= splits * 4) {
+        splits *= 2;
+    }
+    cudaLaunchConfig_t cfg = {};
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = static_cast<unsigned>(splits);
+    attr[0].val.clusterDim.y = 1;
+    attr[0].val.clusterDim.z = 1;
+    cfg.gridDim = dim3(static_cast<unsigned>(splits), static_cast<unsigned>(n_tiles), static_cast<unsigned>(t_tiles));
+    cfg.blockDim = dim3(kNvFewThreads, 1, 1);
+    cfg.dynamicSmemBytes = L::kTotal;
+    cfg.stream = stream;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    count_launches(1);
+    return note_cuda_error(cudaLaunchKernelEx(&cfg, kernel, tw, tx, p), "gemm_nvfp4_few_rows launch");
+}
+
+template <int OUT>
+int launch_nv(cudaStream_t stream, const HostContext& host, const NvProblem& q, const NvGemmParams& p)
+{
+    const long long tiles256 = ((static_cast<long long>(q.m) + 255) / 256) * ((static_cast<long long>(q.n) + 255) / 256);
+    if (q.m > 128 && tiles256 >= host.sm_count / 2) {
+        return launch_nv_pair<OUT>(stream, host, q, p);
+    }
+    if (q.m <= 16) {
+        return launch_nv_few<16, OUT>(stream, host, q, p);
+    }
+    if (q.m <= 32) {
+        return launch_nv_few<32, OUT>(stream, host, q, p);
+    }
+    if (q.m <= 64) {
+        return launch_nv_few<64, OUT>(stream, host, q, p);
+    }
+    return launch_nv_few<128, OUT>(stream, host, q, p);
+}
+
+} // namespace
+} // namespace pto_b200
+
+using namespace pto_b200;
+
+extern "C" size_t pto_b200_nvfp4_scale_bytes(int rows, int k)
+{
+    if (rows <= 0 || k <= 0) {
+        return 0;
+    }
+    return ((static_cast<size_t>(rows) + 127) / 128) * ((static_cast<size_t>(k) + 63) / 64) * kNvAtomBytes;
+}
+
+extern "C" int pto_b200_amax(void* stream, float* amax, const uint8_t* src, int rows, int k, long long ld_src, int src_dtype)
+{
+    if (amax == nullptr || src == nullptr || rows <= 0 || k <= 0 || ld_src < k) {
+        return PTO_B200_EINVAL;
+    }
+    const int type = source_of(src_dtype);
+    if (type < 0) {
+        return PTO_B200_EDTYPE;
+    }
+    const int es = size_of(type);
+    if (misaligned(src, es) || misaligned(amax, 4)) {
+        return PTO_B200_EALIGN;
+    }
+    HostContext host;
+    if (int rc = host_context(&host)) {
+        return rc;
+    }
+    const bool vec = !misaligned(src, 16) && (ld_src * es) % 16 == 0;
+    return PTO_NV_DISPATCH(type, vec, launch_amax, static_cast<cudaStream_t>(stream), host.sm_count, src, amax, rows, k, ld_src);
+}
+
+extern "C" int pto_b200_nvfp4_quantize(void* stream, uint8_t* data, uint8_t* scales, float* tensor_scale, const uint8_t* src,
+                                       const float* amax, int rows, int k, long long ld_src, long long ld_data,
+                                       int src_dtype, int transpose)
+{
+    const long long length = transpose ? rows : k; // of the result's rows
+    if (data == nullptr || scales == nullptr || tensor_scale == nullptr || src == nullptr || amax == nullptr || rows <= 0 ||
+        k <= 0 || ld_src < k || ld_data < (length + 15) / 16 * 8 || (transpose && (k + 127) / 128 * 2 > 65535)) {
+        return PTO_B200_EINVAL;
+    }
+    const int type = source_of(src_dtype);
+    if (type < 0) {
+        return PTO_B200_EDTYPE;
+    }
+    const int es = size_of(type);
+    if (misaligned(src, es) || misaligned(data, 8) || ld_data % 8 != 0 || misaligned(scales, 4) || misaligned(tensor_scale, 4) ||
+        misaligned(amax, 4)) {
+        return PTO_B200_EALIGN;
+    }
+    HostContext host;
+    if (int rc = host_context(&host)) {
+        return rc;
+    }
+    const bool vec = !misaligned(src, 16) && (ld_src * es) % 16 == 0;
+    return PTO_NV_DISPATCH(type, vec, launch_quantize, static_cast<cudaStream_t>(stream), host.sm_count, src, amax, data,
+                           scales, tensor_scale, rows, k, ld_src, ld_data, transpose != 0);
+}
+
+extern "C" int pto_b200_nvfp4_dequantize(void* stream, uint8_t* out, const uint8_t* data, const uint8_t* scales,
+                                         const float* tensor_scale, int rows, int k, long long ld_data, long long ld_out,
+                                         int out_dtype)
+{
+    if (out == nullptr || data == nullptr || scales == nullptr || rows <= 0 || k <= 0 ||
+        ld_data < (static_cast<long long>(k) + 7) / 8 * 4 || ld_out < k) {
+        return PTO_B200_EINVAL;
+    }
+    const int type = source_of(out_dtype);
+    if (type < 0) {
+        return PTO_B200_EDTYPE;
+    }
+    const int es = size_of(type);
+    if (misaligned(out, es) || misaligned(data, 4) || ld_data % 4 != 0 || misaligned(tensor_scale, 4)) {
+        return PTO_B200_EALIGN;
+    }
+    HostContext host;
+    if (int rc = host_context(&host)) {
+        return rc;
+    }
+    const bool vec = !misaligned(out, 16) && (ld_out * es) % 16 == 0;
+    return PTO_NV_DISPATCH(type, vec, launch_dequantize, static_cast<cudaStream_t>(stream), host.sm_count, data, scales,
+                           tensor_scale, out, rows, k, ld_data, ld_out);
+}
+
+extern "C" int pto_b200_gemm_nvfp4(void* stream, uint8_t* out, const uint8_t* src0, const uint8_t* src1, const uint8_t* src2,
+                                   const uint8_t* src3, const float* scale_a, const float* scale_b, const float* bias, int m,
+                                   int n, int k, long long lda, long long ldb, long long ldc, int out_dtype)
+{
+    if (out_dtype != PTO_B200_F32 && out_dtype != PTO_B200_BF16 && out_dtype != PTO_B200_F16) {
+        return PTO_B200_EDTYPE;
+    }
+    if (out == nullptr || src0 == nullptr || src1 == nullptr || src2 == nullptr || src3 == nullptr || m <= 0 || n <= 0 ||
+        k <= 0 || k % 16 != 0 || lda < k || ldb < k || ldc < n) {
+        return PTO_B200_EINVAL;
+    }
+    if (misaligned(src0, 16) || misaligned(src1, 16) || lda % 32 != 0 || ldb % 32 != 0 || misaligned(src2, 16) ||
+        misaligned(src3, 16) || misaligned(out, out_dtype == PTO_B200_F32 ? 4 : 2) || misaligned(scale_a, 4) ||
+        misaligned(scale_b, 4) || misaligned(bias, 4)) {
+        return PTO_B200_EALIGN;
+    }
+    HostContext host;
+    if (int rc = host_context(&host)) {
+        return rc;
+    }
+    NvGemmParams p = {};
+    p.c = out;
+    p.ldc = ldc;
+    p.m = m;
+    p.n = n;
+    p.k_atoms = (k + 63) / 64;
+    p.k_stages = (p.k_atoms + 3) / 4;
+    p.ga = scale_a;
+    p.gb = scale_b;
+    p.bias = bias;
+    p.sfa = src2;
+    p.sfb = src3;
+    p.status = host.status;
+    p.wait_limit = host.wait_limit;
+    const NvProblem q{src0, src1, m, n, k, lda, ldb};
+    cudaStream_t s = static_cast<cudaStream_t>(stream);
+    switch (out_dtype) {
+        case PTO_B200_F32:
+            return launch_nv<NV_OUT_F32>(s, host, q, p);
+        case PTO_B200_BF16:
+            return launch_nv<NV_OUT_BF16>(s, host, q, p);
+        default:
+            return launch_nv<NV_OUT_F16>(s, host, q, p);
+    }
+}

@@ -11,6 +11,7 @@
 #include <cuda.h>
 #include <cuda_runtime.h>
 
+#include "capi_shared.cuh"
 #include "gemm_tile_loop.cuh"
 #include "gemm_tile_loop_2cta.cuh"
 #include "gemv.cuh"
@@ -49,7 +50,6 @@ struct DeviceInfo {
     bool no_tma_store = false; // PTO_B200_NO_TMA_STORE=1: the two-CTA kernels store C from registers (A/B measurements)
 };
 
-constexpr int kMaxDevices = 64;
 std::mutex g_mutex;
 DeviceInfo g_devices[kMaxDevices];
 EncodeTiledFn g_encode = nullptr;
@@ -1493,6 +1493,45 @@ extern "C" const char* pto_b200_error_string(int code)
             return "unknown error code";
     }
 }
+
+namespace pto_b200 {
+
+int host_context(HostContext* out)
+{
+    DeviceInfo* dev = nullptr;
+    if (int rc = device_info(&dev)) {
+        return rc;
+    }
+    out->device = static_cast<int>(dev - g_devices);
+    out->sm_count = dev->sm_count;
+    out->status = dev->status_ptr;
+    out->wait_limit = g_wait_limit.load(std::memory_order_relaxed);
+    return PTO_B200_OK;
+}
+
+int note_cuda_error(cudaError_t e, const char* what) { return note_cuda(e, what); }
+
+void count_launches(int n) { g_launches.fetch_add(static_cast<unsigned long long>(n), std::memory_order_relaxed); }
+
+int encode_map_2d(CUtensorMap* map, CUtensorMapDataType type, const void* base, long long rows, long long cols,
+                  long long pitch_bytes, int box_cols, int box_rows, bool swizzle128)
+{
+    cuuint64_t dims[2] = {static_cast<cuuint64_t>(cols), static_cast<cuuint64_t>(rows)};
+    cuuint64_t strides[1] = {static_cast<cuuint64_t>(pitch_bytes)};
+    cuuint32_t box[2] = {static_cast<cuuint32_t>(box_cols), static_cast<cuuint32_t>(box_rows)};
+    cuuint32_t estr[2] = {1, 1};
+    CUresult r = g_encode(map, type, 2, const_cast<void*>(base), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                          swizzle128 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_NONE,
+                          CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    if (r != CUDA_SUCCESS) {
+        std::snprintf(t_cuda_error, sizeof(t_cuda_error), "cuTensorMapEncodeTiled failed with CUresult %d",
+                      static_cast<int>(r));
+        return PTO_B200_ECUDA;
+    }
+    return PTO_B200_OK;
+}
+
+} // namespace pto_b200
 
 extern "C" const char* pto_b200_last_cuda_error(void) { return t_cuda_error; }
 
