@@ -279,6 +279,31 @@ int pto_b200_gemm_nvfp4(void* stream, uint8_t* out, const uint8_t* src0, const u
                         long long lda, long long ldb, long long ldc, int out_dtype);
 
 /*
+ * pto_b200_mx_quantize_e4m3_ex with the source's type as an argument. F32: that call. BF16 / F16: the same bytes and scales
+ * as that call gives for the same numbers in fp32, read in 16 bits - an activation kept for the backward pass; a block
+ * with an infinity or a NaN is allowed and gets the scale 255 (NaN) and zero bytes.
+ *   src, 16-bit : 16-byte aligned, ld_src a multiple of 8;  data : 8-byte aligned, ld_data a multiple of 8
+ */
+int pto_b200_mx_quantize_e4m3_src(void* stream, uint8_t* data, uint8_t* scales, const uint8_t* src, int rows, int k,
+                                  long long ld_src, long long ld_data, long long ld_scales, int src_dtype, int scale_alg);
+
+/*
+ * Weight gradient of a linear layer from its 8-bit activations (no counterpart in the reference):
+ *   out[n][k] = sum_t dy[t][n] * data[t][k] * 2^(scales[t][k / 32] - 127)  (+ addend[n][k])
+ *   dy     : t x n, BF16 or F16, leading dimension ld_dy elements (a multiple of 8), 16-byte aligned
+ *   data   : t x k e4m3 bytes, leading dimension ld_data (a multiple of 16), 16-byte aligned; k % 32 == 0
+ *   scales : t x k/32 e8m0 bytes, leading dimension ld_scales (what pto_b200_mx_quantize_e4m3* writes)
+ *   addend : n x k of out's type or null; may be out itself (gradient accumulation)
+ *   out    : n x k, F32, BF16 or F16
+ * The activations are multiplied as the numbers they stand for, in dy's type: exact for BF16 down to 2^-126; for F16 what
+ * lies above 65504 becomes infinite and what lies below 2^-14 is rounded. Sums are fp32, rounded at least every 2048
+ * tokens where the tensor core's own sum cuts off. The result does not depend on timing; no workspace is needed.
+ */
+int pto_b200_gemm_wgrad_mx(void* stream, uint8_t* out, const uint8_t* dy, const uint8_t* data, const uint8_t* scales,
+                           const uint8_t* addend, int t, int n, int k, long long ld_dy, long long ld_data,
+                           long long ld_scales, long long ld_out, long long ld_addend, int dy_dtype, int out_dtype);
+
+/*
  * fp32 -> bf16 cast (round to nearest even) of `count` contiguous elements: the TSTORE cast applied to the
  * reduced K-split partials (gemm_ar: reduced_output -> fp16/bf16 result, kernels/manual/a2a3/gemm_ar/README.md:33-46).
  */

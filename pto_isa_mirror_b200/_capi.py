@@ -74,6 +74,11 @@ SYMBOLS = {
         _i,
         [ctypes.c_void_p, _u8p, _u8p, _u8p, _u8p, _u8p, _u8p, _u8p, _u8p, _i, _i, _i, _ll, _ll, _ll, _i],
     ),
+    "pto_b200_mx_quantize_e4m3_src": (_i, [ctypes.c_void_p, _u8p, _u8p, _u8p, _i, _i, _ll, _ll, _ll, _i, _i]),
+    "pto_b200_gemm_wgrad_mx": (
+        _i,
+        [ctypes.c_void_p, _u8p, _u8p, _u8p, _u8p, _u8p, _i, _i, _i, _ll, _ll, _ll, _ll, _ll, _i, _i],
+    ),
     "pto_b200_gemm_mx_static": (
         _i,
         [ctypes.c_void_p, _u8p, _u8p, _u8p, _u8p, _u8p, _i, _i, _i, _ll, _ll, _ll, _ll, _ll, _i, _i, _i],

@@ -21,6 +21,7 @@ SOURCES = {
     "pto_b200_capi.cu": ["capi_shared.cuh", "gemm_tile_loop.cuh", "gemm_tile_loop_2cta.cuh", "gemv.cuh", "gemv_mx.cuh",
                          "ksplit_reduce.cuh", "mx_quantize.cuh", "sm100_ptx.cuh", _ABI],
     "nvfp4_capi.cu": ["capi_shared.cuh", "gemm_tile_loop.cuh", "gemm_nvfp4.cuh", "nvfp4_quantize.cuh", "sm100_ptx.cuh", _ABI],
+    "checkpoint_capi.cu": ["capi_shared.cuh", "gemm_tile_loop.cuh", "gemm_wgrad_mx.cuh", "mx_quantize.cuh", "sm100_ptx.cuh", _ABI],
 }
 
 NVCC_FLAGS = [

@@ -1,0 +1,163 @@
+// C ABI of the operators around activations kept in 8 bits: the quantiser from 16-bit rows and the weight gradient.
+#include "capi_shared.cuh"
+
+#include <atomic>
+
+#include "gemm_wgrad_mx.cuh"
+#include "mx_quantize.cuh"
+
+namespace pto_b200 {
+namespace {
+
+bool misaligned(const void* p, unsigned bytes) { return (reinterpret_cast<uintptr_t>(p) & (bytes - 1u)) != 0; }
+
+template <int ALG, bool F16>
+int launch_quantize16(cudaStream_t s, int sm_count, const uint8_t* src, uint8_t* data, uint8_t* scales, int rows, int k,
+                      long long ld_src, long long ld_data, long long ld_scales)
+{
+    auto kernel = mx_quantize_e4m3_16bit_kernel<ALG, F16>;
+    int per_sm = 0;
+    if (int rc = note_cuda_error(cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per_sm, kernel, kQuantThreads, 0),
+                                 "mx_quantize occupancy")) {
+        return rc;
+    }
+    const long long want = (static_cast<long long>(rows) * (k / 8) + kQuantThreads - 1) / kQuantThreads;
+    const long long cap = static_cast<long long>(sm_count) * (per_sm > 0 ? per_sm : 1); // one resident wave
+    const int grid = static_cast<int>(want < cap ? want : cap);
+    kernel<<<grid, kQuantThreads, 0, s>>>(reinterpret_cast<const uint16_t*>(src), data, scales, rows, k, ld_src, ld_data, ld_scales);
+    count_launches(1);
+    return note_cuda_error(cudaGetLastError(), "mx_quantize (16-bit) launch");
+}
+
+template <bool F16, int OUT>
+int launch_wgrad(cudaStream_t stream, const HostContext& host, const uint8_t* dy, const uint8_t* data, long long ld_dy,
+                 long long ld_data, WgradParams p)
+{
+    auto kernel = gemm_wgrad_mx<F16, OUT>;
+    static std::atomic<int> max_pairs[kMaxDevices];
+    cudaLaunchConfig_t cfg = {};
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = 2;
+    attr[0].val.clusterDim.y = 1;
+    attr[0].val.clusterDim.z = 1;
+    cfg.blockDim = dim3(kWgThreads, 1, 1);
+    cfg.dynamicSmemBytes = WgSmem::kTotal;
+    cfg.stream = stream;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    int pairs = max_pairs[host.device].load(std::memory_order_acquire);
+    if (pairs == 0) {
+        if (int rc = note_cuda_error(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, WgSmem::kTotal),
+                                     "cudaFuncSetAttribute(wgrad)")) {
+            return rc;
+        }
+        cfg.gridDim = dim3(2, 1, 1);
+        if (int rc = note_cuda_error(cudaOccupancyMaxActiveClusters(&pairs, kernel, &cfg), "cudaOccupancyMaxActiveClusters")) {
+            return rc;
+        }
+        pairs = pairs > 0 ? pairs : 1;
+        max_pairs[host.device].store(pairs, std::memory_order_release);
+    }
+    CUtensorMap tdy, tx;
+    int rc = encode_map_2d(&tdy, F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, dy, p.t, p.n, ld_dy * 2,
+                           64, kWgStageTokens, true);
+    rc = rc ? rc : encode_map_2d(&tx, CU_TENSOR_MAP_DATA_TYPE_UINT8, data, p.t, p.k, ld_data, 128, kWgStageTokens, false);
+    if (rc) {
+        return rc;
+    }
+    p.k_tiles = (p.k + 255) / 256;
+    p.n_tiles = (p.n + 255) / 256;
+    p.group = 8;
+    p.stages = (p.t + kWgStageTokens - 1) / kWgStageTokens;
+    // D fp32 (1 at [4,6)), A and B bf16 (1) or fp16 (0), both with the summed index outermost (bits 15 and 16), 256 x 256
+    const uint32_t fmt = F16 ? 0u : 1u;
+    p.idesc = (1u << 4) | (fmt << 7) | (fmt << 10) | (1u << 15) | (1u << 16) | ((256u >> 3) << 17) | ((256u >> 4) << 24);
+    // tokens in parts where the tiles leave pairs idle: up to four pairs (one cluster of eight CTAs) per tile, each with
+    // two stages at least
+    const long long tiles = static_cast<long long>(p.k_tiles) * p.n_tiles;
+    p.splits = 1;
+    while (p.splits < 4 && tiles * p.splits * 2 <= pairs && p.stages >= p.splits * 4) {
+        p.splits *= 2;
+    }
+    attr[0].val.clusterDim.x = static_cast<unsigned>(2 * p.splits);
+    const long long clusters = p.splits > 1 ? tiles : (tiles < pairs ? tiles : pairs);
+    cfg.gridDim = dim3(static_cast<unsigned>(2 * p.splits * clusters), 1, 1);
+    count_launches(1);
+    return note_cuda_error(cudaLaunchKernelEx(&cfg, kernel, tdy, tx, p), "gemm_wgrad_mx launch");
+}
+
+} // namespace
+} // namespace pto_b200
+
+using namespace pto_b200;
+
+extern "C" int pto_b200_mx_quantize_e4m3_src(void* stream, uint8_t* data, uint8_t* scales, const uint8_t* src, int rows, int k,
+                                             long long ld_src, long long ld_data, long long ld_scales, int src_dtype,
+                                             int scale_alg)
+{
+    if (src_dtype == PTO_B200_F32) {
+        return pto_b200_mx_quantize_e4m3_ex(stream, data, scales, src, rows, k, ld_src, ld_data, ld_scales, scale_alg);
+    }
+    if (data == nullptr || scales == nullptr || src == nullptr || rows <= 0 || k <= 0 || k % 32 != 0 || ld_src < k ||
+        ld_data < k || ld_scales < k / 32) {
+        return PTO_B200_EINVAL;
+    }
+    if ((src_dtype != PTO_B200_BF16 && src_dtype != PTO_B200_F16) ||
+        (scale_alg != PTO_B200_SCALE_OCP && scale_alg != PTO_B200_SCALE_NV)) {
+        return PTO_B200_EDTYPE;
+    }
+    if (misaligned(src, 16) || ld_src % 8 != 0 || misaligned(data, 8) || ld_data % 8 != 0) {
+        return PTO_B200_EALIGN;
+    }
+    HostContext host;
+    if (int rc = host_context(&host)) {
+        return rc;
+    }
+    cudaStream_t s = static_cast<cudaStream_t>(stream);
+    const bool f16 = src_dtype == PTO_B200_F16, nv = scale_alg == PTO_B200_SCALE_NV;
+    auto launch = nv ? (f16 ? launch_quantize16<MX_SCALE_NV, true> : launch_quantize16<MX_SCALE_NV, false>)
+                     : (f16 ? launch_quantize16<MX_SCALE_OCP, true> : launch_quantize16<MX_SCALE_OCP, false>);
+    return launch(s, host.sm_count, src, data, scales, rows, k, ld_src, ld_data, ld_scales);
+}
+
+extern "C" int pto_b200_gemm_wgrad_mx(void* stream, uint8_t* out, const uint8_t* dy, const uint8_t* data, const uint8_t* scales,
+                                      const uint8_t* addend, int t, int n, int k, long long ld_dy, long long ld_data,
+                                      long long ld_scales, long long ld_out, long long ld_addend, int dy_dtype, int out_dtype)
+{
+    if ((dy_dtype != PTO_B200_BF16 && dy_dtype != PTO_B200_F16) ||
+        (out_dtype != PTO_B200_F32 && out_dtype != PTO_B200_BF16 && out_dtype != PTO_B200_F16)) {
+        return PTO_B200_EDTYPE;
+    }
+    if (out == nullptr || dy == nullptr || data == nullptr || scales == nullptr || t <= 0 || n <= 0 || k <= 0 || k % 32 != 0 ||
+        ld_dy < n || ld_data < k || ld_scales < k / 32 || ld_out < k || (addend != nullptr && ld_addend < k)) {
+        return PTO_B200_EINVAL;
+    }
+    const unsigned out_es = out_dtype == PTO_B200_F32 ? 4 : 2;
+    if (misaligned(dy, 16) || ld_dy % 8 != 0 || misaligned(data, 16) || ld_data % 16 != 0 || misaligned(out, out_es) ||
+        misaligned(addend, out_es)) {
+        return PTO_B200_EALIGN;
+    }
+    HostContext host;
+    if (int rc = host_context(&host)) {
+        return rc;
+    }
+    WgradParams p = {};
+    p.out = out;
+    p.addend = addend;
+    p.scales = scales;
+    p.ld_out = ld_out;
+    p.ld_addend = ld_addend;
+    p.ld_scales = ld_scales;
+    p.t = t;
+    p.n = n;
+    p.k = k;
+    p.status = host.status;
+    p.wait_limit = host.wait_limit;
+    cudaStream_t s = static_cast<cudaStream_t>(stream);
+    const bool f16 = dy_dtype == PTO_B200_F16;
+    auto launch = out_dtype == PTO_B200_F32    ? (f16 ? launch_wgrad<true, WG_OUT_F32> : launch_wgrad<false, WG_OUT_F32>)
+                  : out_dtype == PTO_B200_BF16 ? (f16 ? launch_wgrad<true, WG_OUT_BF16> : launch_wgrad<false, WG_OUT_BF16>)
+                                               : (f16 ? launch_wgrad<true, WG_OUT_F16> : launch_wgrad<false, WG_OUT_F16>);
+    return launch(s, host, dy, data, ld_dy, ld_data, p);
+}

@@ -1,0 +1,479 @@
+// Weight gradient from an activation kept in 8 bits (MXFP8), on sm_100a:
+//   dW[n][k] = sum_t dy[t][n] * x[t][k] * 2^(e[t][k/32] - 127)   (+ addend[n][k])
+// dy [T][N] bf16 or fp16, x [T][K] e4m3 bytes with one e8m0 scale per 32 elements of a row: the pair the forward pass
+// quantised, read as it is. The sum runs over tokens, so both operands lie with their summed index outermost
+// ("MN-major"): the tensor core takes them in that order from 128-byte swizzled rows and nothing is transposed.
+//
+// x becomes 16-bit on the way: every e4m3 value times a power of two is a bf16 value exactly (below 2^-126 in magnitude
+// the smallest bits are cut off), and an fp16 value where it lies in fp16's range (above it: infinity, below 2^-14:
+// rounded). So dy meets the numbers the checkpoint stands for, at the 16-bit rate of the tensor core, and the 16-bit
+// copy of x exists only in shared memory, tile by tile.
+//
+// A cluster holds `splits` CTA pairs. A pair owns a 256 (k) x 256 (n) tile, or with splits > 1 its part of the
+// tokens of one. Roles per CTA: warp 0 loads (TMA), warp 1 multiplies (even CTA: cta_group::2), warps 2..9 convert x and
+// finish tiles. x is the 256-row side of the product and each CTA converts its own 128: half as many elements per
+// SM as on the 256-column side of a single-CTA tile.
+//
+// Sums: the tensor core adds into its accumulator by cutting off, not by rounding (measured here: 1.9e-5 of the result
+// lost after 16384 terms, 3.8e-5 after 32768). So an accumulator takes kWgFoldStages x 64 = 2048 tokens at most; the
+// converting warps then add it to fp32 sums in their registers, with rounding, while the other accumulator fills.
+// With splits > 1 the parts are added over distributed shared memory in rank order. No atomics: the result does not
+// depend on timing.
+#pragma once
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+#include <cuda_fp8.h>
+
+#include <cstdint>
+
+#include "gemm_tile_loop.cuh"
+#include "sm100_ptx.cuh"
+
+namespace pto_b200 {
+
+constexpr int kWgThreads = 320;
+constexpr int kWgWorkerWarps = 8;
+constexpr int kWgStages = 5;      // ring of dy tiles and converted x tiles
+constexpr int kWgRawStages = 4;   // ring of x tiles as they come
+constexpr int kWgStageTokens = 64;
+constexpr int kWgFoldStages = 32;
+
+constexpr int ST_WG_PRODUCER = 31;
+constexpr int ST_WG_MMA = 32;
+constexpr int ST_WG_WORKER = 33;
+
+enum WgOut : int { WG_OUT_F32 = 0, WG_OUT_BF16 = 1, WG_OUT_F16 = 2 };
+
+struct WgradParams {
+    void* out;
+    const void* addend;   // of out's type, or null; may be out itself
+    const uint8_t* scales;
+    long long ld_out, ld_addend, ld_scales;
+    int t, n, k;
+    int k_tiles, n_tiles, group;
+    int stages;           // 64-token stages of T
+    int splits;
+    uint32_t idesc;
+    int* status;
+    long long wait_limit;
+};
+
+struct WgSmem {
+    static constexpr int kDyBytes = kWgStageTokens * 128 * 2; // this CTA's 128 columns of dy: two blocks of 64 columns
+    static constexpr int kXBytes = kWgStageTokens * 128 * 2;  // converted x: two blocks of 64 columns
+    static constexpr int kRawBytes = kWgStageTokens * 128;
+    static constexpr int kXOff = kWgStages * kDyBytes;
+    static constexpr int kRawOff = kXOff + kWgStages * kXBytes;
+    static constexpr int kBarOff = kRawOff + kWgRawStages * kRawBytes;
+    static constexpr int kNumBars = 2 * kWgStages + 2 * kWgRawStages + 4;
+    static constexpr int kMiscOff = kBarOff + kNumBars * 8;
+    static constexpr int kTotal = kMiscOff + 16 + 1024;
+};
+static_assert(WgSmem::kTotal <= 227 * 1024, "shared memory of the weight-gradient kernel");
+static_assert(256 * 128 * 4 <= WgSmem::kRawOff, "partial sums reuse the ring");
+
+// As bounded_wait, for a barrier that threads of another CTA arrive on after writing shared memory of theirs.
+__device__ __forceinline__ bool bounded_wait_cluster(uint64_t* bar, uint32_t parity, volatile uint32_t* abort_flag, int* status,
+                                                     int code, long long limit)
+{
+    const long long t0 = clock64();
+    uint32_t spins = 0;
+    while (!ptx::mbar_try_wait_cluster(bar, parity)) {
+        if (((++spins) & 0x3Fu) == 0) {
+            if (*abort_flag != 0) {
+                return false;
+            }
+            if (clock64() - t0 > limit) {
+                *abort_flag = 1;
+                atomicCAS(status, 0, code);
+                return false;
+            }
+        }
+    }
+    return true;
+}
+
+// Sixteen e4m3 bytes times one scale -> sixteen 16-bit values.
+template <bool F16>
+__device__ __forceinline__ void wg_convert16(const uint4& raw, float scale, uint32_t (&o)[8])
+{
+    const uint32_t w[4] = {raw.x, raw.y, raw.z, raw.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            const __half2_raw r = __nv_cvt_fp8x2_to_halfraw2(static_cast<__nv_fp8x2_storage_t>((w[i] >> (16 * h)) & 0xFFFFu), __NV_E4M3);
+            const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&r));
+            const float lo = f.x * scale, hi = f.y * scale;
+            if constexpr (F16) {
+                const __half2 v = __floats2half2_rn(lo, hi);
+                o[2 * i + h] = *reinterpret_cast<const uint32_t*>(&v);
+            } else {
+                // at most four significant bits: the upper half of the float is the bf16 value
+                o[2 * i + h] = __byte_perm(__float_as_uint(lo), __float_as_uint(hi), 0x7632);
+            }
+        }
+    }
+}
+
+template <int OUT>
+__device__ __forceinline__ float wg_load(const void* base, long long at)
+{
+    if constexpr (OUT == WG_OUT_F32) {
+        return static_cast<const float*>(base)[at];
+    } else if constexpr (OUT == WG_OUT_BF16) {
+        return __bfloat162float(static_cast<const __nv_bfloat16*>(base)[at]);
+    } else {
+        return __half2float(static_cast<const __half*>(base)[at]);
+    }
+}
+
+// One element of dW: the addend joins in fp32, one rounding to the output's type.
+template <int OUT>
+__device__ __forceinline__ void wg_store(const WgradParams& p, int n, int k, float f)
+{
+    if (p.addend != nullptr) {
+        f += wg_load<OUT>(p.addend, n * p.ld_addend + k);
+    }
+    const long long at = n * p.ld_out + k;
+    if constexpr (OUT == WG_OUT_F32) {
+        static_cast<float*>(p.out)[at] = f;
+    } else if constexpr (OUT == WG_OUT_BF16) {
+        static_cast<__nv_bfloat16*>(p.out)[at] = __float2bfloat16_rn(f);
+    } else {
+        static_cast<__half*>(p.out)[at] = __float2half_rn(f);
+    }
+}
+
+template <bool F16, int OUT>
+__global__ void __launch_bounds__(kWgThreads, 1)
+    gemm_wgrad_mx(const __grid_constant__ CUtensorMap tmap_dy, const __grid_constant__ CUtensorMap tmap_x, const WgradParams p)
+{
+    using L = WgSmem;
+    extern __shared__ uint8_t smem_raw[];
+    uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+    uint64_t* full_bar = reinterpret_cast<uint64_t*>(smem + L::kBarOff); // even CTA: dy landed, x converted, in both CTAs
+    uint64_t* empty_bar = full_bar + kWgStages;                         // each CTA: products have read the stage
+    uint64_t* raw_full_bar = empty_bar + kWgStages;                     // each CTA: x landed
+    uint64_t* raw_empty_bar = raw_full_bar + kWgRawStages;              // each CTA: x read by the converting warps
+    uint64_t* acc_full_bar = raw_empty_bar + kWgRawStages;              // each CTA: an accumulator is finished
+    uint64_t* acc_empty_bar = acc_full_bar + 2;                         // even CTA: sixteen warps have read it
+    uint32_t* tmem_base_slot = reinterpret_cast<uint32_t*>(smem + L::kMiscOff);
+    volatile uint32_t* abort_flag = reinterpret_cast<volatile uint32_t*>(smem + L::kMiscOff + 4);
+
+    const int warp = threadIdx.x >> 5;
+    const int lane = threadIdx.x & 31;
+    const uint32_t cta_rank = ptx::cluster_ctarank();
+    const uint32_t leader_rank = cta_rank & ~1u;
+    const bool leader = (cta_rank == leader_rank);
+    const int side = static_cast<int>(cta_rank & 1u);
+    const int split = static_cast<int>(cta_rank >> 1);
+    const uint16_t pair_mask = static_cast<uint16_t>(3u << leader_rank);
+    const int cluster_ctas = 2 * p.splits;
+    const int cluster = static_cast<int>(blockIdx.x) / cluster_ctas;
+    const int clusters = static_cast<int>(gridDim.x) / cluster_ctas;
+    const int tiles = p.k_tiles * p.n_tiles;
+    const int first_stage = static_cast<int>(static_cast<long long>(p.stages) * split / p.splits);
+    const int last_stage = static_cast<int>(static_cast<long long>(p.stages) * (split + 1) / p.splits);
+
+    if (threadIdx.x == 0) {
+        for (int s = 0; s < kWgStages; ++s) {
+            ptx::mbar_init(&full_bar[s], 1 + 2 * kWgWorkerWarps);
+            ptx::mbar_init(&empty_bar[s], 1);
+        }
+        for (int s = 0; s < kWgRawStages; ++s) {
+            ptx::mbar_init(&raw_full_bar[s], 1);
+            ptx::mbar_init(&raw_empty_bar[s], kWgWorkerWarps);
+        }
+        for (int a = 0; a < 2; ++a) {
+            ptx::mbar_init(&acc_full_bar[a], 1);
+            ptx::mbar_init(&acc_empty_bar[a], 2 * kWgWorkerWarps);
+        }
+        *abort_flag = 0;
+        ptx::fence_mbar_init();
+        ptx::prefetch_tensormap(&tmap_dy);
+        ptx::prefetch_tensormap(&tmap_x);
+    }
+    if (warp == 1) {
+        ptx::tmem_alloc_pair(tmem_base_slot, kTmemCols);
+        ptx::tmem_relinquish_alloc_permit_pair();
+    }
+    ptx::tc_fence_before_sync();
+    __syncthreads();
+    ptx::cluster_arrive(); // the peer's barriers must exist before anything is signalled across the pair
+    ptx::cluster_wait();
+    ptx::tc_fence_after_sync();
+    const uint32_t tmem_base = *tmem_base_slot;
+
+    auto tile_of = [&](int tile, int& ki, int& ni) { // grouped raster: a wave of pairs shares few columns of dy and x
+        const int group_size = p.group * p.n_tiles;
+        const int g = tile / group_size;
+        const int first = g * p.group;
+        const int rows = min(p.k_tiles - first, p.group);
+        const int r = tile - g * group_size;
+        ki = first + r % rows;
+        ni = r / rows;
+    };
+
+    if (warp == 0) {
+        // ---------------------------------------------------------------- loads
+        if (lane == 0) {
+            int stage = 0, raw = 0;
+            uint32_t phase = 0, raw_phase = 0;
+            bool ok = true;
+            for (int tile = cluster; ok && tile < tiles; tile += clusters) {
+                int ki, ni;
+                tile_of(tile, ki, ni);
+                const int k0 = ki * 256 + side * 128;
+                const int n0 = ni * 256 + side * 128;
+                for (int st = first_stage; st < last_stage; ++st) {
+                    const int token = st * kWgStageTokens;
+                    ok = bounded_wait(&raw_empty_bar[raw], raw_phase ^ 1u, abort_flag, p.status, ST_WG_PRODUCER, p.wait_limit);
+                    if (!ok) {
+                        break;
+                    }
+                    ptx::mbar_arrive_expect_tx(&raw_full_bar[raw], L::kRawBytes);
+                    ptx::tma_load_2d(smem + L::kRawOff + raw * L::kRawBytes, &tmap_x, &raw_full_bar[raw], k0, token);
+                    if (++raw == kWgRawStages) {
+                        raw = 0;
+                        raw_phase ^= 1u;
+                    }
+                    ok = bounded_wait(&empty_bar[stage], phase ^ 1u, abort_flag, p.status, ST_WG_PRODUCER, p.wait_limit);
+                    if (!ok) {
+                        break;
+                    }
+                    if (leader) {
+                        ptx::mbar_arrive_expect_tx(&full_bar[stage], 2u * L::kDyBytes);
+                    }
+                    const uint32_t full_addr = ptx::map_to_cta(ptx::smem_u32(&full_bar[stage]), leader_rank);
+                    uint8_t* dst = smem + stage * L::kDyBytes;
+                    ptx::tma_load_2d_pair(dst, &tmap_dy, full_addr, n0, token);
+                    ptx::tma_load_2d_pair(dst + 8192, &tmap_dy, full_addr, n0 + 64, token);
+                    if (++stage == kWgStages) {
+                        stage = 0;
+                        phase ^= 1u;
+                    }
+                }
+            }
+        }
+    } else if (warp == 1) {
+        // ---------------------------------------------------------------- products (even CTA)
+        if (leader && lane == 0) {
+            int stage = 0, acc = 0;
+            uint32_t phase = 0, acc_phase = 0;
+            bool ok = true;
+            for (int tile = cluster; ok && tile < tiles; tile += clusters) {
+                for (int st = first_stage; ok && st < last_stage; ++st) {
+                    const bool fresh = (st - first_stage) % kWgFoldStages == 0;
+                    if (fresh) {
+                        ok = bounded_wait(&acc_empty_bar[acc], acc_phase ^ 1u, abort_flag, p.status, ST_WG_MMA, p.wait_limit);
+                        if (!ok) {
+                            break;
+                        }
+                    }
+                    ok = bounded_wait_cluster(&full_bar[stage], phase, abort_flag, p.status, ST_WG_MMA, p.wait_limit);
+                    if (!ok) {
+                        break;
+                    }
+                    ptx::tc_fence_after_sync();
+                    const uint32_t x_base = ptx::smem_u32(smem + L::kXOff + stage * L::kXBytes);
+                    const uint32_t dy_base = ptx::smem_u32(smem + stage * L::kDyBytes);
+#pragma unroll
+                    for (int kk = 0; kk < kWgStageTokens / 16; ++kk) { // 16 tokens (rows of 128 bytes) per instruction
+                        ptx::umma_f16_pair(tmem_base + 256u * acc, ptx::make_smem_desc(x_base + kk * 2048, 8192, 1024, ptx::kSwizzle128B),
+                                           ptx::make_smem_desc(dy_base + kk * 2048, 8192, 1024, ptx::kSwizzle128B), p.idesc,
+                                           (!fresh || kk > 0) ? 1u : 0u);
+                    }
+                    ptx::umma_commit_pair(&empty_bar[stage], pair_mask);
+                    if (++stage == kWgStages) {
+                        stage = 0;
+                        phase ^= 1u;
+                    }
+                    if ((st - first_stage) % kWgFoldStages == kWgFoldStages - 1 || st == last_stage - 1) {
+                        ptx::umma_commit_pair(&acc_full_bar[acc], pair_mask);
+                        acc ^= 1;
+                        acc_phase ^= (acc == 0) ? 1u : 0u;
+                    }
+                }
+            }
+        }
+    } else {
+        // ---------------------------------------------------------------- conversion, sums, stores
+        const int worker = static_cast<int>(threadIdx.x) - 64; // 0..255
+        const int quarter = warp & 3;
+        const int half = (warp - 2) >> 2; // which 128 columns (n) of the accumulator
+        const int row0 = worker >> 3;     // two 16-byte pieces per stage: rows row0 and row0 + 32 of the tile
+        const int piece = worker & 7;
+        int stage = 0, raw = 0, acc = 0;
+        uint32_t phase = 0, raw_phase = 0, acc_phase = 0;
+        bool ok = true;
+        float sum[128];
+        auto fold = [&]() { // the oldest finished accumulator joins the sums
+            ok = bounded_wait(&acc_full_bar[acc], acc_phase, abort_flag, p.status, ST_WG_WORKER, p.wait_limit);
+            ok = __all_sync(0xFFFFFFFFu, ok);
+            if (!ok) {
+                return;
+            }
+            ptx::tc_fence_after_sync();
+            const uint32_t t_row = tmem_base + 256u * acc + 128u * half + (static_cast<uint32_t>(quarter * 32) << 16);
+#pragma unroll
+            for (int q = 0; q < 4; ++q) {
+                uint32_t v[32];
+                ptx::tmem_ld_32x32b_x32(t_row + 32u * q, v);
+                ptx::tmem_ld_wait();
+#pragma unroll
+                for (int i = 0; i < 32; ++i) {
+                    sum[32 * q + i] += __uint_as_float(v[i]);
+                }
+            }
+            ptx::tc_fence_before_sync();
+            __syncwarp();
+            if (lane == 0) {
+                ptx::mbar_arrive_cluster(ptx::map_to_cta(ptx::smem_u32(&acc_empty_bar[acc]), leader_rank));
+            }
+            acc ^= 1;
+            acc_phase ^= (acc == 0) ? 1u : 0u;
+        };
+        for (int tile = cluster; ok && tile < tiles; tile += clusters) {
+            int ki, ni;
+            tile_of(tile, ki, ni);
+            const int k0 = ki * 256 + side * 128;
+            const int block = (k0 + piece * 16) >> 5; // scale of this thread's pieces
+            const bool block_ok = (k0 + piece * 16) < p.k;
+            auto scale_of = [&](int st, int row) -> uint32_t {
+                const int token = st * kWgStageTokens + row;
+                return (block_ok && token < p.t && st < last_stage) ? p.scales[token * p.ld_scales + block] : 127u;
+            };
+            uint32_t e0 = scale_of(first_stage, row0), e1 = scale_of(first_stage, row0 + 32);
+            bool pending = false;
+            int pending_end = 0;
+#pragma unroll
+            for (int i = 0; i < 128; ++i) {
+                sum[i] = 0.0f;
+            }
+            for (int st = first_stage; ok && st < last_stage; ++st) {
+                const uint32_t next0 = scale_of(st + 1, row0), next1 = scale_of(st + 1, row0 + 32);
+                ok = bounded_wait(&raw_full_bar[raw], raw_phase, abort_flag, p.status, ST_WG_WORKER, p.wait_limit) &&
+                     bounded_wait(&empty_bar[stage], phase ^ 1u, abort_flag, p.status, ST_WG_WORKER, p.wait_limit);
+                ok = __all_sync(0xFFFFFFFFu, ok);
+                if (!ok) {
+                    break;
+                }
+                if (pending && st - pending_end >= kWgStages) { // its last products are known to be done: no waiting
+                    pending = false;
+                    fold();
+                    if (!ok) {
+                        break;
+                    }
+                }
+                const uint8_t* src = smem + L::kRawOff + raw * L::kRawBytes;
+                uint8_t* dst = smem + L::kXOff + stage * L::kXBytes + (piece >> 2) * 8192;
+                uint4 in[2];
+                in[0] = *reinterpret_cast<const uint4*>(src + row0 * 128 + piece * 16);
+                in[1] = *reinterpret_cast<const uint4*>(src + (row0 + 32) * 128 + piece * 16);
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    const int row = row0 + 32 * h;
+                    const uint32_t e = h == 0 ? e0 : e1;
+                    // 2^(e - 127); e = 0 is the subnormal 2^-127, e = 255 a NaN
+                    const float scale = __uint_as_float(e == 0u ? 0x00400000u : e == 255u ? 0x7FC00000u : e << 23);
+                    uint32_t o[8];
+                    wg_convert16<F16>(in[h], scale, o);
+                    // 128-byte swizzle; the two halves of a row go to blocks 8 KiB apart, and the second half writes its
+                    // odd piece first so that the eight lanes of a row hit different banks
+                    uint8_t* line = dst + row * 128;
+                    const int q0 = (piece & 3) * 2;
+                    const uint4 lo = make_uint4(o[0], o[1], o[2], o[3]), hi = make_uint4(o[4], o[5], o[6], o[7]);
+                    const bool odd = piece >= 4;
+                    *reinterpret_cast<uint4*>(line + (((q0 + (odd ? 1 : 0)) ^ (row & 7)) * 16)) = odd ? hi : lo;
+                    *reinterpret_cast<uint4*>(line + (((q0 + (odd ? 0 : 1)) ^ (row & 7)) * 16)) = odd ? lo : hi;
+                }
+                ptx::fence_proxy_async_smem();
+                __syncwarp();
+                if (lane == 0) {
+                    ptx::mbar_arrive(&raw_empty_bar[raw]);
+                    ptx::mbar_arrive_cluster(ptx::map_to_cta(ptx::smem_u32(&full_bar[stage]), leader_rank));
+                }
+                e0 = next0;
+                e1 = next1;
+                if (++raw == kWgRawStages) {
+                    raw = 0;
+                    raw_phase ^= 1u;
+                }
+                if (++stage == kWgStages) {
+                    stage = 0;
+                    phase ^= 1u;
+                }
+                if ((st - first_stage) % kWgFoldStages == kWgFoldStages - 1 || st == last_stage - 1) {
+                    if (pending) {
+                        fold();
+                    }
+                    pending = true;
+                    pending_end = st + 1;
+                }
+            }
+            if (ok && pending) {
+                fold();
+            }
+            if (!ok) {
+                break;
+            }
+            const int in_tile = quarter * 32 + lane;
+            if (p.splits == 1) {
+                const int k = k0 + in_tile;
+                const int n0 = ni * 256 + half * 128;
+                if (k < p.k) {
+#pragma unroll
+                    for (int i = 0; i < 128; ++i) {
+                        if (n0 + i < p.n) {
+                            wg_store<OUT>(p, n0 + i, k, sum[i]);
+                        }
+                    }
+                }
+            } else {
+                float* part = reinterpret_cast<float*>(smem); // [256 n][128 k]: every load and product of the ring is done
+#pragma unroll
+                for (int i = 0; i < 128; ++i) {
+                    part[(half * 128 + i) * 128 + in_tile] = sum[i];
+                }
+            }
+        }
+    }
+
+    ptx::tc_fence_before_sync();
+    __syncthreads();
+    if (*abort_flag != 0) {
+        for (int i = 0; i < 2000; ++i) { // copies and products in flight end before shared and tensor memory go away
+            __nanosleep(1000);
+        }
+    }
+    ptx::cluster_arrive(); // no CTA touches another's tensor memory or barriers any more; partial sums are in place
+    ptx::cluster_wait();
+    if (warp == 1) {
+        ptx::tc_fence_after_sync();
+        ptx::tmem_dealloc_pair(tmem_base, kTmemCols);
+    }
+    if (p.splits > 1) {
+        // one tile per cluster: its parts of the same side, added in rank order
+        int ki, ni;
+        tile_of(cluster, ki, ni);
+        const uint32_t base = ptx::smem_u32(smem);
+        const int first = 256 * 128 * split / p.splits;
+        const int last = 256 * 128 * (split + 1) / p.splits;
+        for (int i = first + static_cast<int>(threadIdx.x); i < last; i += kWgThreads) {
+            const int k = ki * 256 + side * 128 + (i & 127);
+            const int n = ni * 256 + (i >> 7);
+            if (k < p.k && n < p.n) {
+                float f = 0.0f;
+                for (int s = 0; s < p.splits; ++s) {
+                    f += ptx::ld_shared_cluster_f32(ptx::map_to_cta(base + 4u * static_cast<uint32_t>(i), static_cast<uint32_t>(2 * s + side)));
+                }
+                wg_store<OUT>(p, n, k, f);
+            }
+        }
+        ptx::cluster_arrive_relaxed(); // no CTA leaves while another still reads its shared memory
+        ptx::cluster_wait();
+    }
+}
+
+} // namespace pto_b200

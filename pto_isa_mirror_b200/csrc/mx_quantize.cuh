@@ -18,6 +18,7 @@
 // values (one 16-byte load each), share the maximum with three shuffles and store 4 bytes each, so a warp reads 512
 // contiguous bytes and writes 128.
 #pragma once
+#include <cuda_fp16.h>
 #include <cuda_fp8.h>
 
 #include <cstdint>
@@ -47,6 +48,39 @@ constexpr int kQuantItems = 4; // 16-byte loads in flight per thread
 // src: [rows][ld_src] floats (16-byte aligned rows); data: [rows][ld_data] bytes (4-byte aligned rows);
 // scales: [rows][ld_scales] bytes. k % 32 == 0.
 enum MxScaleAlg : int { MX_SCALE_OCP = 0, MX_SCALE_NV = 1 };
+
+// The e8m0 scale of a block from its largest magnitude.
+template <int ALG>
+__device__ __forceinline__ uint32_t mx_e4m3_exponent(float amax)
+{
+    if constexpr (ALG == MX_SCALE_OCP) {
+        const uint32_t exponent = (__float_as_uint(amax) & 0x7F800000u) >> 23;
+        return exponent <= 8u ? 0u : exponent - 8u;
+    } else {
+        const uint32_t bits = __float_as_uint(__fmul_rn(amax, 1.0f / 448.0f));
+        const uint32_t exponent = (bits & 0x7F800000u) >> 23;
+        const uint32_t mantissa = bits & 0x007FFFFFu;
+        const bool round_up = mantissa > 0u && !(exponent == 0u && mantissa <= 0x00400000u);
+        return (amax == 0.0f) ? 0u : exponent + (round_up ? 1u : 0u);
+    }
+}
+
+// Four scaled values -> four codes, the first in the low byte.
+template <int ALG>
+__device__ __forceinline__ uint32_t mx_e4m3_encode4(float y0, float y1, float y2, float y3)
+{
+    uint32_t packed = cvt_e4m3x2(y0, y1) | (cvt_e4m3x2(y2, y3) << 16);
+    if constexpr (ALG == MX_SCALE_OCP) {
+        packed = drop_negative_zero(packed);
+    } else {
+        // values below 2^-10 keep their sign as +-0 (what the conversion gives); a value of exactly -2^-10 is a
+        // tie that the reference's search resolves to +0
+        constexpr float kTie = -0.0009765625f;
+        packed &= ~((y0 == kTie ? 0x80u : 0u) | (y1 == kTie ? 0x8000u : 0u) | (y2 == kTie ? 0x800000u : 0u) |
+                    (y3 == kTie ? 0x80000000u : 0u));
+    }
+    return packed;
+}
 
 template <int ALG>
 __global__ void __launch_bounds__(kQuantThreads) mx_quantize_e4m3_kernel(const float* __restrict__ src,
@@ -96,35 +130,101 @@ __global__ void __launch_bounds__(kQuantThreads) mx_quantize_e4m3_kernel(const f
             amax = fmaxf(amax, __shfl_xor_sync(group_mask, amax, 1));
             amax = fmaxf(amax, __shfl_xor_sync(group_mask, amax, 2));
             amax = fmaxf(amax, __shfl_xor_sync(group_mask, amax, 4));
-            uint32_t e8m0;
-            if constexpr (ALG == MX_SCALE_OCP) {
-                const uint32_t exponent = (__float_as_uint(amax) & 0x7F800000u) >> 23;
-                e8m0 = exponent <= 8u ? 0u : exponent - 8u;
-            } else {
-                const uint32_t bits = __float_as_uint(__fmul_rn(amax, 1.0f / 448.0f));
-                const uint32_t exponent = (bits & 0x7F800000u) >> 23;
-                const uint32_t mantissa = bits & 0x007FFFFFu;
-                const bool round_up = mantissa > 0u && !(exponent == 0u && mantissa <= 0x00400000u);
-                e8m0 = (amax == 0.0f) ? 0u : exponent + (round_up ? 1u : 0u);
-            }
+            const uint32_t e8m0 = mx_e4m3_exponent<ALG>(amax);
             const float scaling = __uint_as_float((254u - e8m0) << 23); // e8m0 <= 246 for finite input: never zero
-            const float y0 = __fmul_rn(v[u].x, scaling), y1 = __fmul_rn(v[u].y, scaling);
-            const float y2 = __fmul_rn(v[u].z, scaling), y3 = __fmul_rn(v[u].w, scaling);
-            const uint32_t lo = cvt_e4m3x2(y0, y1);
-            const uint32_t hi = cvt_e4m3x2(y2, y3);
-            uint32_t packed = lo | (hi << 16);
-            if constexpr (ALG == MX_SCALE_OCP) {
-                packed = drop_negative_zero(packed);
-            } else {
-                // values below 2^-10 keep their sign as +-0 (what the conversion gives); a value of exactly -2^-10 is a
-                // tie that the reference's search resolves to +0
-                constexpr float kTie = -0.0009765625f;
-                packed &= ~((y0 == kTie ? 0x80u : 0u) | (y1 == kTie ? 0x8000u : 0u) | (y2 == kTie ? 0x800000u : 0u) |
-                            (y3 == kTie ? 0x80000000u : 0u));
-            }
+            const uint32_t packed = mx_e4m3_encode4<ALG>(__fmul_rn(v[u].x, scaling), __fmul_rn(v[u].y, scaling),
+                                                         __fmul_rn(v[u].z, scaling), __fmul_rn(v[u].w, scaling));
             *reinterpret_cast<uint32_t*>(data + row[u] * ld_data + static_cast<long long>(c4[u]) * 4) = packed;
             if ((c4[u] & 7) == 0) {
                 scales[row[u] * ld_scales + (c4[u] >> 3)] = static_cast<uint8_t>(e8m0);
+            }
+        }
+    }
+}
+
+// The same from 16-bit rows (bf16, or fp16 with F16): what an activation kept for a backward pass comes as. Every value is
+// a float exactly, so bytes and scales are those of the fp32 kernel on the same numbers. Unlike there, a block with an
+// infinity or a NaN is in the domain: its scale is 255, which e8m0 reads as NaN, and its bytes are zero.
+// Four consecutive lanes own one block of 32 values (16 bytes each) and store 8 bytes each.
+// src: [rows][ld_src] elements (16-byte aligned rows); data: [rows][ld_data] bytes (8-byte aligned rows). k % 32 == 0.
+constexpr int kQuant16Items = 4;
+
+template <int ALG, bool F16>
+__global__ void __launch_bounds__(kQuantThreads) mx_quantize_e4m3_16bit_kernel(const uint16_t* __restrict__ src,
+                                                                                uint8_t* __restrict__ data,
+                                                                                uint8_t* __restrict__ scales, int rows, int k,
+                                                                                long long ld_src, long long ld_data,
+                                                                                long long ld_scales)
+{
+    const int k8 = k / 8;
+    const long long total = static_cast<long long>(rows) * k8; // 16-byte items; a multiple of 4 per row
+    const long long stride = static_cast<long long>(gridDim.x) * blockDim.x;
+    const unsigned group_mask = 0xFu << (threadIdx.x & 28u);
+    const long long row_step = stride / k8;
+    const int col_step = static_cast<int>(stride - row_step * k8);
+    long long i = blockIdx.x * static_cast<long long>(blockDim.x) + threadIdx.x;
+    long long cur_row = i / k8;
+    int cur_c8 = static_cast<int>(i - cur_row * k8);
+    // total and stride are multiples of 4: the four lanes of a group are all in range or all out of range
+    while (i < total) {
+        uint4 v[kQuant16Items];
+        long long row[kQuant16Items];
+        int c8[kQuant16Items];
+#pragma unroll
+        for (int u = 0; u < kQuant16Items; ++u) {
+            row[u] = -1;
+            if (i < total) {
+                row[u] = cur_row;
+                c8[u] = cur_c8;
+                v[u] = __ldcs(reinterpret_cast<const uint4*>(src + cur_row * ld_src) + cur_c8);
+            }
+            i += stride;
+            cur_row += row_step;
+            cur_c8 += col_step;
+            if (cur_c8 >= k8) {
+                cur_c8 -= k8;
+                cur_row += 1;
+            }
+        }
+#pragma unroll
+        for (int u = 0; u < kQuant16Items; ++u) {
+            if (row[u] < 0) {
+                continue;
+            }
+            const uint32_t w[4] = {v[u].x, v[u].y, v[u].z, v[u].w};
+            // the largest magnitude of both halves of the words, as 16-bit patterns: their order is the value order,
+            // infinities and NaN above all numbers
+            uint32_t top = 0u;
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                top = __vmaxu2(top, w[j] & 0x7FFF7FFFu);
+            }
+            top = __vmaxu2(top, __shfl_xor_sync(group_mask, top, 1));
+            top = __vmaxu2(top, __shfl_xor_sync(group_mask, top, 2));
+            top = max(top & 0xFFFFu, top >> 16);
+            const bool finite = top < (F16 ? 0x7C00u : 0x7F80u);
+            const float amax = F16 ? __half2float(__ushort_as_half(static_cast<unsigned short>(top))) : __uint_as_float(top << 16);
+            const uint32_t e8m0 = finite ? mx_e4m3_exponent<ALG>(amax) : 255u;
+            const float scaling = __uint_as_float((254u - (finite ? e8m0 : 0u)) << 23);
+            float y[8];
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                if constexpr (F16) {
+                    const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&w[j]));
+                    y[2 * j] = __fmul_rn(f.x, scaling);
+                    y[2 * j + 1] = __fmul_rn(f.y, scaling);
+                } else {
+                    y[2 * j] = __fmul_rn(__uint_as_float(w[j] << 16), scaling);
+                    y[2 * j + 1] = __fmul_rn(__uint_as_float(w[j] & 0xFFFF0000u), scaling);
+                }
+            }
+            uint2 packed = make_uint2(mx_e4m3_encode4<ALG>(y[0], y[1], y[2], y[3]), mx_e4m3_encode4<ALG>(y[4], y[5], y[6], y[7]));
+            if (!finite) {
+                packed = make_uint2(0u, 0u);
+            }
+            *reinterpret_cast<uint2*>(data + row[u] * ld_data + static_cast<long long>(c8[u]) * 8) = packed;
+            if ((c8[u] & 3) == 0) {
+                scales[row[u] * ld_scales + (c8[u] >> 2)] = static_cast<uint8_t>(e8m0);
             }
         }
     }

@@ -331,14 +331,15 @@ def gemv_mx(x: torch.Tensor, b_dn: torch.Tensor, sfx: torch.Tensor, sfb: torch.T
 def mx_quantize_e4m3(src: torch.Tensor, stream: Optional[torch.cuda.Stream] = None,
                      data: Optional[torch.Tensor] = None, scales: Optional[torch.Tensor] = None,
                      scale_alg: int = _capi.SCALE_OCP):
-    """OCP MX quantisation (TQUANT, MXFP8): float32 src [rows, K] -> (e4m3 bytes [rows, K] uint8, e8m0 scales
-    [rows, K/32] uint8), one scale per 32 elements along K. Finite input only. ``data`` / ``scales``: caller's output
+    """OCP MX quantisation (TQUANT, MXFP8): float32, bfloat16 or float16 src [rows, K] -> (e4m3 bytes [rows, K] uint8, e8m0
+    scales [rows, K/32] uint8), one scale per 32 elements along K. float32: finite input only; a 16-bit block with an
+    infinity or a NaN gets the scale 255, a NaN. ``data`` / ``scales``: caller's output
     buffers of those shapes (allocated when omitted). ``scale_alg``: ``_capi.SCALE_OCP`` (default) or ``_capi.SCALE_NV``,
     the reference's QuantScaleAlg."""
     lib = _capi.load()
     _require_cuda_2d(src, "src")
-    if src.dtype != torch.float32:
-        raise ValueError("src must be float32")
+    if src.dtype not in (torch.float32, torch.bfloat16, torch.float16):
+        raise ValueError("src must be float32, bfloat16 or float16")
     rows, k = src.shape
     if k % 32 != 0:
         raise ValueError("K must be a multiple of 32")
@@ -350,9 +351,10 @@ def mx_quantize_e4m3(src: torch.Tensor, stream: Optional[torch.cuda.Stream] = No
         _require_cuda_2d(t, name)
         if t.dtype != torch.uint8 or tuple(t.shape) != shape:
             raise ValueError(f"{name} must be a uint8 CUDA tensor of shape {shape}")
-    rc = lib.pto_b200_mx_quantize_e4m3_ex(_stream_ptr(stream), data.data_ptr(), scales.data_ptr(), src.data_ptr(), rows,
-                                          k, src.stride(0), data.stride(0), scales.stride(0), scale_alg)
-    _capi.check(rc, "pto_b200_mx_quantize_e4m3_ex")
+    rc = lib.pto_b200_mx_quantize_e4m3_src(_stream_ptr(stream), data.data_ptr(), scales.data_ptr(), src.data_ptr(), rows,
+                                           k, src.stride(0), data.stride(0), scales.stride(0), _TORCH_TO_PTO[src.dtype],
+                                           scale_alg)
+    _capi.check(rc, "pto_b200_mx_quantize_e4m3_src")
     return data, scales
 
 

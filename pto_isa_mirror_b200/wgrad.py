@@ -1,0 +1,59 @@
+"""The backward pass's use of activations kept in 8 bits: a linear layer's weight gradient."""
+from __future__ import annotations
+
+from typing import Optional
+
+import torch
+
+from . import _capi
+from .gemm import _TORCH_TO_PTO, _require_cuda_2d
+from .nvfp4 import _FLOATS, _launching, _ptr
+
+
+def gemm_wgrad_mx(dy: torch.Tensor, data: torch.Tensor, scales: torch.Tensor, out_dtype: torch.dtype = torch.float32,
+                  addend: Optional[torch.Tensor] = None, out: Optional[torch.Tensor] = None,
+                  stream: Optional[torch.cuda.Stream] = None) -> torch.Tensor:
+    """dW [N, K] = dy^T @ x (+ addend) for a layer y = x @ W^T whose input x [T, K] was kept as MXFP8: ``data`` [T, K] e4m3
+    bytes and ``scales`` [T, K / 32] e8m0 bytes, as :func:`mx_quantize_e4m3` returns them (and :func:`gemm_mx` reads them
+    in the forward pass). dy [T, N]: bfloat16 or float16, rows on 16-byte boundaries; K a multiple of 32.
+
+    x enters as the numbers the bytes stand for, in dy's type - exact for bfloat16; float16 has its range. Sums are
+    float32; dW is float32, bfloat16 or float16. ``addend`` [N, K], of dW's type, is added before the rounding; it may be
+    ``out`` itself, which accumulates gradients in place."""
+    lib = _capi.load()
+    for t, name in ((dy, "dy"), (data, "data"), (scales, "scales")):
+        _require_cuda_2d(t, name)
+    if dy.dtype not in (torch.bfloat16, torch.float16):
+        raise ValueError("dy must be bfloat16 or float16")
+    if data.element_size() != 1 or scales.element_size() != 1:
+        raise ValueError("data and scales must have one-byte elements")
+    t, n = dy.shape
+    k = data.shape[1]
+    if data.shape[0] != t:
+        raise ValueError("dy and data must have the same number of rows")
+    if t == 0 or n == 0 or k == 0 or k % 32 != 0 or tuple(scales.shape) != (t, k // 32):
+        raise ValueError("T, N and K must be positive, K a multiple of 32 and scales [T, K / 32]")
+    if out is not None:
+        _require_cuda_2d(out, "out")
+        if out.dtype not in _FLOATS or tuple(out.shape) != (n, k):
+            raise ValueError("out must be [N, K] float32, bfloat16 or float16")
+        out_dtype = out.dtype
+    elif out_dtype not in _FLOATS:
+        raise ValueError("out_dtype must be float32, bfloat16 or float16")
+    if addend is not None:
+        _require_cuda_2d(addend, "addend")
+        if addend.dtype != out_dtype or tuple(addend.shape) != (n, k):
+            raise ValueError("addend must be [N, K] of dW's type")
+    with _launching(stream, dy, data, scales, addend, out) as sp:
+        if out is None:
+            out = torch.empty((n, k), dtype=out_dtype, device=dy.device)
+        ld_dy = dy.stride(0) if t > 1 else (n + 7) // 8 * 8
+        ld_data = data.stride(0) if t > 1 else (k + 15) // 16 * 16
+        ld_scales = scales.stride(0) if t > 1 else k // 32
+        ld_out = out.stride(0) if n > 1 else k
+        ld_addend = 0 if addend is None else addend.stride(0) if n > 1 else k
+        rc = lib.pto_b200_gemm_wgrad_mx(sp, out.data_ptr(), dy.data_ptr(), data.data_ptr(), scales.data_ptr(), _ptr(addend), t, n,
+                                        k, ld_dy, ld_data, ld_scales, ld_out, ld_addend, _TORCH_TO_PTO[dy.dtype],
+                                        _TORCH_TO_PTO[out_dtype])
+        _capi.check(rc, "pto_b200_gemm_wgrad_mx")
+    return out
