@@ -10,9 +10,16 @@
 // copy of x exists only in shared memory, tile by tile.
 //
 // A cluster holds `splits` CTA pairs. A pair owns a 256 (k) x 256 (n) tile, or with splits > 1 its part of the
-// tokens of one. Roles per CTA: warp 0 loads (TMA), warp 1 multiplies (even CTA: cta_group::2), warps 2..9 convert x and
-// finish tiles. x is the 256-row side of the product and each CTA converts its own 128: half as many elements per
-// SM as on the 256-column side of a single-CTA tile.
+// tokens of one. x is the 256-row side of the product and each CTA converts its own 128: half as many elements per SM as
+// on the 256-column side of a single-CTA tile. Roles per CTA:
+//   warp 0, 2    TMA loads of dy and of x
+//   warp 1       products (even CTA: cta_group::2)
+//   warps 4..19  four groups of four, one warp of each per scheduler; a group converts every fourth stage and keeps the
+//                fp32 sums of 64 of the 256 columns
+// What limits such a kernel is issue slots, not bandwidth: the converting warps leave few, and a role with its own warp
+// runs at some eight cycles per instruction beside them. So a group takes a whole stage at a time (waits and counters
+// once per 64 values of a thread), scales are fetched by the threads that use them, and the product warp keeps its
+// descriptors in uniform registers (its issue alone took 800 cycles of a stage's 513 before).
 //
 // Sums: the tensor core adds into its accumulator by cutting off, not by rounding (measured here: 1.9e-5 of the result
 // lost after 16384 terms, 3.8e-5 after 32768). So an accumulator takes kWgFoldStages x 64 = 2048 tokens at most; the
@@ -31,10 +38,15 @@
 
 namespace pto_b200 {
 
-constexpr int kWgThreads = 320;
-constexpr int kWgWorkerWarps = 8;
-constexpr int kWgStages = 5;      // ring of dy tiles and converted x tiles
-constexpr int kWgRawStages = 4;   // ring of x tiles as they come
+constexpr int kWgThreads = 640;
+constexpr int kWgWorkerWarps = 16;
+constexpr int kWgGroups = 4;      // of four converting warps; a group takes every fourth stage
+constexpr int kWgStages = 6;      // ring of dy tiles and converted x tiles
+constexpr int kWgRawStages = 4;   // ring of x tiles as they come: one place per group
+static_assert(kWgRawStages == kWgGroups, "a group reads its own place of the ring of x");
+// registers: 96 at launch; the loading and multiplying warps give back what the sums need
+constexpr int kWgRegsOthers = 56, kWgRegsWorkers = 104;
+static_assert(128 * kWgRegsOthers + 512 * kWgRegsWorkers <= kWgThreads * 96, "register split within the launch's total");
 constexpr int kWgStageTokens = 64;
 constexpr int kWgFoldStages = 32;
 
@@ -72,25 +84,11 @@ struct WgSmem {
 static_assert(WgSmem::kTotal <= 227 * 1024, "shared memory of the weight-gradient kernel");
 static_assert(256 * 128 * 4 <= WgSmem::kRawOff, "partial sums reuse the ring");
 
-// As bounded_wait, for a barrier that threads of another CTA arrive on after writing shared memory of theirs.
-__device__ __forceinline__ bool bounded_wait_cluster(uint64_t* bar, uint32_t parity, volatile uint32_t* abort_flag, int* status,
-                                                     int code, long long limit)
+__device__ __forceinline__ uint64_t wg_pack2(float lo, float hi)
 {
-    const long long t0 = clock64();
-    uint32_t spins = 0;
-    while (!ptx::mbar_try_wait_cluster(bar, parity)) {
-        if (((++spins) & 0x3Fu) == 0) {
-            if (*abort_flag != 0) {
-                return false;
-            }
-            if (clock64() - t0 > limit) {
-                *abort_flag = 1;
-                atomicCAS(status, 0, code);
-                return false;
-            }
-        }
-    }
-    return true;
+    uint64_t r;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(lo), "f"(hi));
+    return r;
 }
 
 // Sixteen e4m3 bytes times one scale -> sixteen 16-bit values.
@@ -98,13 +96,21 @@ template <bool F16>
 __device__ __forceinline__ void wg_convert16(const uint4& raw, float scale, uint32_t (&o)[8])
 {
     const uint32_t w[4] = {raw.x, raw.y, raw.z, raw.w};
+    const uint64_t scale2 = wg_pack2(scale, scale);
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
-            const __half2_raw r = __nv_cvt_fp8x2_to_halfraw2(static_cast<__nv_fp8x2_storage_t>((w[i] >> (16 * h)) & 0xFFFFu), __NV_E4M3);
+            const __half2_raw r = __nv_cvt_fp8x2_to_halfraw2(static_cast<__nv_fp8x2_storage_t>(h == 0 ? w[i] & 0xFFFFu : w[i] >> 16), __NV_E4M3);
             const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&r));
-            const float lo = f.x * scale, hi = f.y * scale;
+            float lo, hi;
+            asm("{\n\t"
+                ".reg .b64 t;\n\t"
+                "mul.rn.f32x2 t, %2, %3;\n\t"
+                "mov.b64 {%0, %1}, t;\n\t"
+                "}"
+                : "=f"(lo), "=f"(hi)
+                : "l"(wg_pack2(f.x, f.y)), "l"(scale2));
             if constexpr (F16) {
                 const __half2 v = __floats2half2_rn(lo, hi);
                 o[2 * i + h] = *reinterpret_cast<const uint32_t*>(&v);
@@ -114,6 +120,12 @@ __device__ __forceinline__ void wg_convert16(const uint4& raw, float scale, uint
             }
         }
     }
+}
+
+// 2^(e - 127): e = 0 is the subnormal 2^-127, e = 255 a NaN.
+__device__ __forceinline__ float wg_scale(uint32_t e)
+{
+    return __uint_as_float(e == 0u ? 0x00400000u : e == 255u ? 0x7FC00000u : e << 23);
 }
 
 template <int OUT>
@@ -178,12 +190,12 @@ __global__ void __launch_bounds__(kWgThreads, 1)
 
     if (threadIdx.x == 0) {
         for (int s = 0; s < kWgStages; ++s) {
-            ptx::mbar_init(&full_bar[s], 1 + 2 * kWgWorkerWarps);
+            ptx::mbar_init(&full_bar[s], 1 + 2 * (kWgWorkerWarps / kWgGroups)); // dy's bytes, and a group in each CTA
             ptx::mbar_init(&empty_bar[s], 1);
         }
         for (int s = 0; s < kWgRawStages; ++s) {
             ptx::mbar_init(&raw_full_bar[s], 1);
-            ptx::mbar_init(&raw_empty_bar[s], kWgWorkerWarps);
+            ptx::mbar_init(&raw_empty_bar[s], kWgWorkerWarps / kWgGroups);
         }
         for (int a = 0; a < 2; ++a) {
             ptx::mbar_init(&acc_full_bar[a], 1);
@@ -215,82 +227,109 @@ __global__ void __launch_bounds__(kWgThreads, 1)
         ni = r / rows;
     };
 
-    if (warp == 0) {
-        // ---------------------------------------------------------------- loads
-        if (lane == 0) {
-            int stage = 0, raw = 0;
-            uint32_t phase = 0, raw_phase = 0;
-            bool ok = true;
-            for (int tile = cluster; ok && tile < tiles; tile += clusters) {
-                int ki, ni;
-                tile_of(tile, ki, ni);
-                const int k0 = ki * 256 + side * 128;
-                const int n0 = ni * 256 + side * 128;
-                for (int st = first_stage; st < last_stage; ++st) {
-                    const int token = st * kWgStageTokens;
-                    ok = bounded_wait(&raw_empty_bar[raw], raw_phase ^ 1u, abort_flag, p.status, ST_WG_PRODUCER, p.wait_limit);
-                    if (!ok) {
-                        break;
-                    }
-                    ptx::mbar_arrive_expect_tx(&raw_full_bar[raw], L::kRawBytes);
-                    ptx::tma_load_2d(smem + L::kRawOff + raw * L::kRawBytes, &tmap_x, &raw_full_bar[raw], k0, token);
-                    if (++raw == kWgRawStages) {
-                        raw = 0;
-                        raw_phase ^= 1u;
-                    }
-                    ok = bounded_wait(&empty_bar[stage], phase ^ 1u, abort_flag, p.status, ST_WG_PRODUCER, p.wait_limit);
-                    if (!ok) {
-                        break;
-                    }
-                    if (leader) {
-                        ptx::mbar_arrive_expect_tx(&full_bar[stage], 2u * L::kDyBytes);
-                    }
-                    const uint32_t full_addr = ptx::map_to_cta(ptx::smem_u32(&full_bar[stage]), leader_rank);
-                    uint8_t* dst = smem + stage * L::kDyBytes;
-                    ptx::tma_load_2d_pair(dst, &tmap_dy, full_addr, n0, token);
-                    ptx::tma_load_2d_pair(dst + 8192, &tmap_dy, full_addr, n0 + 64, token);
-                    if (++stage == kWgStages) {
-                        stage = 0;
-                        phase ^= 1u;
+    if (warp < 4) {
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kWgRegsOthers));
+        if (warp == 0) {
+            // ---------------------------------------------------------------- loads of dy
+            if (lane == 0) {
+                int stage = 0;
+                uint32_t phase = 0;
+                bool ok = true;
+                for (int tile = cluster; ok && tile < tiles; tile += clusters) {
+                    int ki, ni;
+                    tile_of(tile, ki, ni);
+                    const int n0 = ni * 256 + side * 128;
+                    for (int st = first_stage; st < last_stage; ++st) {
+                        const int token = st * kWgStageTokens;
+                        ok = bounded_wait(&empty_bar[stage], phase ^ 1u, abort_flag, p.status, ST_WG_PRODUCER, p.wait_limit);
+                        if (!ok) {
+                            break;
+                        }
+                        if (leader) {
+                            ptx::mbar_arrive_expect_tx(&full_bar[stage], 2u * L::kDyBytes);
+                        }
+                        const uint32_t full_addr = ptx::map_to_cta(ptx::smem_u32(&full_bar[stage]), leader_rank);
+                        uint8_t* dst = smem + stage * L::kDyBytes;
+                        ptx::tma_load_2d_pair(dst, &tmap_dy, full_addr, n0, token);
+                        ptx::tma_load_2d_pair(dst + 8192, &tmap_dy, full_addr, n0 + 64, token);
+                        if (++stage == kWgStages) {
+                            stage = 0;
+                            phase ^= 1u;
+                        }
                     }
                 }
             }
-        }
-    } else if (warp == 1) {
-        // ---------------------------------------------------------------- products (even CTA)
-        if (leader && lane == 0) {
-            int stage = 0, acc = 0;
+        } else if (warp == 2) {
+            // ---------------------------------------------------------------- loads of x, as far ahead as their own ring goes
+            if (lane == 0) {
+                int raw = 0;
+                uint32_t phase = 0;
+                bool ok = true;
+                for (int tile = cluster; ok && tile < tiles; tile += clusters) {
+                    int ki, ni;
+                    tile_of(tile, ki, ni);
+                    const int k0 = ki * 256 + side * 128;
+                    for (int st = first_stage; st < last_stage; ++st) {
+                        ok = bounded_wait(&raw_empty_bar[raw], phase ^ 1u, abort_flag, p.status, ST_WG_PRODUCER, p.wait_limit);
+                        if (!ok) {
+                            break;
+                        }
+                        ptx::mbar_arrive_expect_tx(&raw_full_bar[raw], L::kRawBytes);
+                        ptx::tma_load_2d(smem + L::kRawOff + raw * L::kRawBytes, &tmap_x, &raw_full_bar[raw], k0,
+                                         st * kWgStageTokens);
+                        if (++raw == kWgRawStages) {
+                            raw = 0;
+                            phase ^= 1u;
+                        }
+                    }
+                }
+            }
+        } else if (warp == 1 && leader) {
+            // ---------------------------------------------------------------- products (even CTA)
+            // The whole warp walks the stages and one elected lane issues, so addresses and descriptors stay in uniform
+            // registers: beside the converting warps this warp gets few issue slots, and each instruction it saves counts.
+            int stage = 0, acc = 0, in_part = 0;
             uint32_t phase = 0, acc_phase = 0;
             bool ok = true;
+            const uint64_t x_desc0 = ptx::make_smem_desc(ptx::smem_u32(smem + L::kXOff), 8192, 1024, ptx::kSwizzle128B);
+            const uint64_t dy_desc0 = ptx::make_smem_desc(ptx::smem_u32(smem), 8192, 1024, ptx::kSwizzle128B);
+            const int stages = last_stage - first_stage;
             for (int tile = cluster; ok && tile < tiles; tile += clusters) {
-                for (int st = first_stage; ok && st < last_stage; ++st) {
-                    const bool fresh = (st - first_stage) % kWgFoldStages == 0;
-                    if (fresh) {
+                for (int st = 0; st < stages; ++st) {
+                    if (in_part == 0) {
                         ok = bounded_wait(&acc_empty_bar[acc], acc_phase ^ 1u, abort_flag, p.status, ST_WG_MMA, p.wait_limit);
                         if (!ok) {
                             break;
                         }
                     }
-                    ok = bounded_wait_cluster(&full_bar[stage], phase, abort_flag, p.status, ST_WG_MMA, p.wait_limit);
+                    ok = bounded_wait(&full_bar[stage], phase, abort_flag, p.status, ST_WG_MMA, p.wait_limit);
                     if (!ok) {
                         break;
                     }
                     ptx::tc_fence_after_sync();
-                    const uint32_t x_base = ptx::smem_u32(smem + L::kXOff + stage * L::kXBytes);
-                    const uint32_t dy_base = ptx::smem_u32(smem + stage * L::kDyBytes);
+                    const bool last = in_part == kWgFoldStages - 1 || st == stages - 1;
+                    if (ptx::elect_one()) {
+                        // 16 tokens, 16 rows of 128 bytes, per instruction (descriptor addresses count 16 bytes)
+                        const uint64_t x_desc = x_desc0 + static_cast<uint64_t>(stage * (L::kXBytes / 16));
+                        const uint64_t dy_desc = dy_desc0 + static_cast<uint64_t>(stage * (L::kDyBytes / 16));
+                        ptx::umma_f16_pair(tmem_base + 256u * acc, x_desc, dy_desc, p.idesc, in_part != 0 ? 1u : 0u);
 #pragma unroll
-                    for (int kk = 0; kk < kWgStageTokens / 16; ++kk) { // 16 tokens (rows of 128 bytes) per instruction
-                        ptx::umma_f16_pair(tmem_base + 256u * acc, ptx::make_smem_desc(x_base + kk * 2048, 8192, 1024, ptx::kSwizzle128B),
-                                           ptx::make_smem_desc(dy_base + kk * 2048, 8192, 1024, ptx::kSwizzle128B), p.idesc,
-                                           (!fresh || kk > 0) ? 1u : 0u);
+                        for (int kk = 1; kk < kWgStageTokens / 16; ++kk) {
+                            ptx::umma_f16_pair(tmem_base + 256u * acc, x_desc + kk * 128, dy_desc + kk * 128, p.idesc, 1u);
+                        }
+                        ptx::umma_commit_pair(&empty_bar[stage], pair_mask);
+                        if (last) {
+                            ptx::umma_commit_pair(&acc_full_bar[acc], pair_mask);
+                        }
                     }
-                    ptx::umma_commit_pair(&empty_bar[stage], pair_mask);
+                    __syncwarp();
                     if (++stage == kWgStages) {
                         stage = 0;
                         phase ^= 1u;
                     }
-                    if ((st - first_stage) % kWgFoldStages == kWgFoldStages - 1 || st == last_stage - 1) {
-                        ptx::umma_commit_pair(&acc_full_bar[acc], pair_mask);
+                    ++in_part;
+                    if (last) {
+                        in_part = 0;
                         acc ^= 1;
                         acc_phase ^= (acc == 0) ? 1u : 0u;
                     }
@@ -298,133 +337,144 @@ __global__ void __launch_bounds__(kWgThreads, 1)
             }
         }
     } else {
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kWgRegsWorkers));
         // ---------------------------------------------------------------- conversion, sums, stores
-        const int worker = static_cast<int>(threadIdx.x) - 64; // 0..255
-        const int quarter = warp & 3;
-        const int half = (warp - 2) >> 2; // which 128 columns (n) of the accumulator
-        const int row0 = worker >> 3;     // two 16-byte pieces per stage: rows row0 and row0 + 32 of the tile
-        const int piece = worker & 7;
-        int stage = 0, raw = 0, acc = 0;
+        const int group = (warp - 4) >> 2;         // converts stages group, group + 4, ..; keeps the sums of 64 columns (n)
+        const int quarter = warp & 3;              // and of these 32 tensor-memory lanes (k)
+        const int row = quarter * 4 + (lane >> 3); // four 16-byte pieces of x per stage, rows row + 16 h of the tile
+        const int piece = lane & 7;
+        // where the pieces go: 128-byte swizzle; the halves of a row lie in blocks 8 KiB apart, and the second half writes
+        // its odd piece first so that the eight lanes of a row hit different banks (row + 16 h has the row's swizzle)
+        const bool odd = piece >= 4;
+        const uint32_t line = (piece >> 2) * 8192 + row * 128;
+        const uint32_t at0 = line + ((((piece & 3) * 2 + (odd ? 1 : 0)) ^ (row & 7)) * 16);
+        const uint32_t at1 = line + ((((piece & 3) * 2 + (odd ? 0 : 1)) ^ (row & 7)) * 16);
+        const uint8_t* raw = smem + L::kRawOff + group * L::kRawBytes + row * 128 + piece * 16;
+        int stage = group, acc = 0;
         uint32_t phase = 0, raw_phase = 0, acc_phase = 0;
         bool ok = true;
-        float sum[128];
-        auto fold = [&]() { // the oldest finished accumulator joins the sums
-            ok = bounded_wait(&acc_full_bar[acc], acc_phase, abort_flag, p.status, ST_WG_WORKER, p.wait_limit);
-            ok = __all_sync(0xFFFFFFFFu, ok);
-            if (!ok) {
-                return;
-            }
-            ptx::tc_fence_after_sync();
-            const uint32_t t_row = tmem_base + 256u * acc + 128u * half + (static_cast<uint32_t>(quarter * 32) << 16);
+        int first_of_tile = group; // first stage of the tile that this group converts
+        const int stages = last_stage - first_stage; // of a tile
+        const int parts = (stages + kWgFoldStages - 1) / kWgFoldStages;
+        // Block scales come straight from memory, one visit (four stages) ahead of their use: their rows start on any byte,
+        // so no TMA, and a thread fetches what its own pieces need.
+        const uint8_t* scale_at = nullptr;
+        int token = 0;
+        bool column_ok = false;
+        uint32_t e[4];
+        auto fetch_scales = [&]() {
 #pragma unroll
-            for (int q = 0; q < 4; ++q) {
-                uint32_t v[32];
-                ptx::tmem_ld_32x32b_x32(t_row + 32u * q, v);
-                ptx::tmem_ld_wait();
-#pragma unroll
-                for (int i = 0; i < 32; ++i) {
-                    sum[32 * q + i] += __uint_as_float(v[i]);
-                }
+            for (int h = 0; h < 4; ++h) {
+                e[h] = (column_ok && token + 16 * h < p.t) ? __ldg(scale_at + 16 * h * p.ld_scales) : 127u;
             }
-            ptx::tc_fence_before_sync();
-            __syncwarp();
-            if (lane == 0) {
-                ptx::mbar_arrive_cluster(ptx::map_to_cta(ptx::smem_u32(&acc_empty_bar[acc]), leader_rank));
-            }
-            acc ^= 1;
-            acc_phase ^= (acc == 0) ? 1u : 0u;
+            scale_at += kWgGroups * kWgStageTokens * p.ld_scales;
+            token += kWgGroups * kWgStageTokens;
         };
+        auto start_scales = [&](int tile) { // of the first stage that this group converts of a tile
+            int ki, ni;
+            tile_of(tile, ki, ni);
+            const int column = ki * 256 + side * 128 + piece * 16;
+            token = (first_stage + first_of_tile) * kWgStageTokens + row;
+            column_ok = tile < tiles && column < p.k;
+            scale_at = p.scales + token * p.ld_scales + (column >> 5);
+            fetch_scales();
+        };
+        start_scales(cluster);
         for (int tile = cluster; ok && tile < tiles; tile += clusters) {
             int ki, ni;
             tile_of(tile, ki, ni);
-            const int k0 = ki * 256 + side * 128;
-            const int block = (k0 + piece * 16) >> 5; // scale of this thread's pieces
-            const bool block_ok = (k0 + piece * 16) < p.k;
-            auto scale_of = [&](int st, int row) -> uint32_t {
-                const int token = st * kWgStageTokens + row;
-                return (block_ok && token < p.t && st < last_stage) ? p.scales[token * p.ld_scales + block] : 127u;
-            };
-            uint32_t e0 = scale_of(first_stage, row0), e1 = scale_of(first_stage, row0 + 32);
-            bool pending = false;
-            int pending_end = 0;
+            float sum[64];
 #pragma unroll
-            for (int i = 0; i < 128; ++i) {
+            for (int i = 0; i < 64; ++i) {
                 sum[i] = 0.0f;
             }
-            for (int st = first_stage; ok && st < last_stage; ++st) {
-                const uint32_t next0 = scale_of(st + 1, row0), next1 = scale_of(st + 1, row0 + 32);
-                ok = bounded_wait(&raw_full_bar[raw], raw_phase, abort_flag, p.status, ST_WG_WORKER, p.wait_limit) &&
-                     bounded_wait(&empty_bar[stage], phase ^ 1u, abort_flag, p.status, ST_WG_WORKER, p.wait_limit);
-                ok = __all_sync(0xFFFFFFFFu, ok);
-                if (!ok) {
-                    break;
-                }
-                if (pending && st - pending_end >= kWgStages) { // its last products are known to be done: no waiting
-                    pending = false;
-                    fold();
+            int folded = 0;
+            for (int st = first_of_tile; folded < parts; st += kWgGroups) {
+                if (st < stages) {
+                    float scale[4];
+#pragma unroll
+                    for (int h = 0; h < 4; ++h) {
+                        scale[h] = wg_scale(e[h]);
+                    }
+                    fetch_scales(); // of the next visit; past the tile's last token they are not used
+                    ok = bounded_wait(&raw_full_bar[group], raw_phase, abort_flag, p.status, ST_WG_WORKER, p.wait_limit);
+                    uint4 in[4];
+#pragma unroll
+                    for (int h = 0; h < 4; ++h) {
+                        in[h] = *reinterpret_cast<const uint4*>(raw + h * 16 * 128);
+                    }
+                    ok = ok && bounded_wait(&empty_bar[stage], phase ^ 1u, abort_flag, p.status, ST_WG_WORKER, p.wait_limit);
+                    ok = __all_sync(0xFFFFFFFFu, ok);
                     if (!ok) {
                         break;
                     }
-                }
-                const uint8_t* src = smem + L::kRawOff + raw * L::kRawBytes;
-                uint8_t* dst = smem + L::kXOff + stage * L::kXBytes + (piece >> 2) * 8192;
-                uint4 in[2];
-                in[0] = *reinterpret_cast<const uint4*>(src + row0 * 128 + piece * 16);
-                in[1] = *reinterpret_cast<const uint4*>(src + (row0 + 32) * 128 + piece * 16);
-#pragma unroll
-                for (int h = 0; h < 2; ++h) {
-                    const int row = row0 + 32 * h;
-                    const uint32_t e = h == 0 ? e0 : e1;
-                    // 2^(e - 127); e = 0 is the subnormal 2^-127, e = 255 a NaN
-                    const float scale = __uint_as_float(e == 0u ? 0x00400000u : e == 255u ? 0x7FC00000u : e << 23);
-                    uint32_t o[8];
-                    wg_convert16<F16>(in[h], scale, o);
-                    // 128-byte swizzle; the two halves of a row go to blocks 8 KiB apart, and the second half writes its
-                    // odd piece first so that the eight lanes of a row hit different banks
-                    uint8_t* line = dst + row * 128;
-                    const int q0 = (piece & 3) * 2;
-                    const uint4 lo = make_uint4(o[0], o[1], o[2], o[3]), hi = make_uint4(o[4], o[5], o[6], o[7]);
-                    const bool odd = piece >= 4;
-                    *reinterpret_cast<uint4*>(line + (((q0 + (odd ? 1 : 0)) ^ (row & 7)) * 16)) = odd ? hi : lo;
-                    *reinterpret_cast<uint4*>(line + (((q0 + (odd ? 0 : 1)) ^ (row & 7)) * 16)) = odd ? lo : hi;
-                }
-                ptx::fence_proxy_async_smem();
-                __syncwarp();
-                if (lane == 0) {
-                    ptx::mbar_arrive(&raw_empty_bar[raw]);
-                    ptx::mbar_arrive_cluster(ptx::map_to_cta(ptx::smem_u32(&full_bar[stage]), leader_rank));
-                }
-                e0 = next0;
-                e1 = next1;
-                if (++raw == kWgRawStages) {
-                    raw = 0;
-                    raw_phase ^= 1u;
-                }
-                if (++stage == kWgStages) {
-                    stage = 0;
-                    phase ^= 1u;
-                }
-                if ((st - first_stage) % kWgFoldStages == kWgFoldStages - 1 || st == last_stage - 1) {
-                    if (pending) {
-                        fold();
+                    __syncwarp();
+                    if (lane == 0) {
+                        ptx::mbar_arrive(&raw_empty_bar[group]);
                     }
-                    pending = true;
-                    pending_end = st + 1;
+                    uint8_t* dst = smem + L::kXOff + stage * L::kXBytes;
+#pragma unroll
+                    for (int h = 0; h < 4; ++h) {
+                        uint32_t o[8];
+                        wg_convert16<F16>(in[h], scale[h], o);
+                        const uint4 lo = make_uint4(o[0], o[1], o[2], o[3]), hi = make_uint4(o[4], o[5], o[6], o[7]);
+                        *reinterpret_cast<uint4*>(dst + at0 + h * 16 * 128) = odd ? hi : lo;
+                        *reinterpret_cast<uint4*>(dst + at1 + h * 16 * 128) = odd ? lo : hi;
+                    }
+                    ptx::fence_proxy_async_smem();
+                    __syncwarp();
+                    if (lane == 0) {
+                        ptx::mbar_arrive_pair(ptx::map_to_cta(ptx::smem_u32(&full_bar[stage]), leader_rank));
+                    }
+                    raw_phase ^= 1u;
+                    stage += kWgGroups;
+                    if (stage >= kWgStages) {
+                        stage -= kWgStages;
+                        phase ^= 1u;
+                    }
                 }
-            }
-            if (ok && pending) {
-                fold();
+                // The oldest finished accumulator joins the sums: behind the last stage, or once this group has had a place
+                // in the ring whose last products came after that accumulator's - then nothing is waited for.
+                if (st >= stages || st >= (folded + 1) * kWgFoldStages + kWgStages) {
+                    ok = bounded_wait(&acc_full_bar[acc], acc_phase, abort_flag, p.status, ST_WG_WORKER, p.wait_limit);
+                    ok = __all_sync(0xFFFFFFFFu, ok);
+                    if (!ok) {
+                        break;
+                    }
+                    ptx::tc_fence_after_sync();
+                    const uint32_t t_row = tmem_base + 256u * acc + 64u * group + (static_cast<uint32_t>(quarter * 32) << 16);
+#pragma unroll
+                    for (int q = 0; q < 2; ++q) {
+                        uint32_t v[32];
+                        ptx::tmem_ld_32x32b_x32(t_row + 32u * q, v);
+                        ptx::tmem_ld_wait();
+#pragma unroll
+                        for (int i = 0; i < 32; ++i) {
+                            sum[32 * q + i] += __uint_as_float(v[i]);
+                        }
+                    }
+                    ptx::tc_fence_before_sync();
+                    __syncwarp();
+                    if (lane == 0) {
+                        ptx::mbar_arrive_pair(ptx::map_to_cta(ptx::smem_u32(&acc_empty_bar[acc]), leader_rank));
+                    }
+                    acc ^= 1;
+                    acc_phase ^= (acc == 0) ? 1u : 0u;
+                    ++folded;
+                }
             }
             if (!ok) {
                 break;
             }
+            first_of_tile = (first_of_tile - stages % kWgGroups + kWgGroups) % kWgGroups; // stages go round the groups
+            start_scales(tile + clusters); // come while this tile is stored
             const int in_tile = quarter * 32 + lane;
             if (p.splits == 1) {
-                const int k = k0 + in_tile;
-                const int n0 = ni * 256 + half * 128;
+                const int k = ki * 256 + side * 128 + in_tile;
+                const int n0 = ni * 256 + group * 64;
                 if (k < p.k) {
 #pragma unroll
-                    for (int i = 0; i < 128; ++i) {
+                    for (int i = 0; i < 64; ++i) {
                         if (n0 + i < p.n) {
                             wg_store<OUT>(p, n0 + i, k, sum[i]);
                         }
@@ -433,8 +483,8 @@ __global__ void __launch_bounds__(kWgThreads, 1)
             } else {
                 float* part = reinterpret_cast<float*>(smem); // [256 n][128 k]: every load and product of the ring is done
 #pragma unroll
-                for (int i = 0; i < 128; ++i) {
-                    part[(half * 128 + i) * 128 + in_tile] = sum[i];
+                for (int i = 0; i < 64; ++i) {
+                    part[(group * 64 + i) * 128 + in_tile] = sum[i];
                 }
             }
         }

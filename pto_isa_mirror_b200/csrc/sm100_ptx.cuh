@@ -57,20 +57,18 @@ __device__ __forceinline__ bool mbar_try_wait(uint64_t* bar, uint32_t parity)
     return ok != 0;
 }
 
-// The same for a barrier that other CTAs of the cluster arrive on: acquires what they released at cluster scope.
-__device__ __forceinline__ bool mbar_try_wait_cluster(uint64_t* bar, uint32_t parity)
+// True in one lane of a converged warp.
+__device__ __forceinline__ bool elect_one()
 {
-    uint32_t ok;
+    uint32_t r;
     asm volatile(
         "{\n\t"
         ".reg .pred p;\n\t"
-        "mbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2;\n\t"
+        "elect.sync _|p, 0xFFFFFFFF;\n\t"
         "selp.u32 %0, 1, 0, p;\n\t"
         "}"
-        : "=r"(ok)
-        : "r"(smem_u32(bar)), "r"(parity)
-        : "memory");
-    return ok != 0;
+        : "=r"(r));
+    return r != 0;
 }
 
 // ---------------------------------------------------------------- TMA (no multicast anywhere)
@@ -303,6 +301,14 @@ __device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.w
 __device__ __forceinline__ void mbar_arrive_cluster(uint32_t cluster_addr)
 {
     asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(cluster_addr) : "memory");
+}
+
+// The same without ordering anything at cluster scope, which takes over a thousand cycles: for "my shared memory is ready
+// for the tensor core". Its writers have handed it to the async proxy (fence_proxy_async_smem) before they arrive, and a
+// pair's product reads it on the SM that holds it.
+__device__ __forceinline__ void mbar_arrive_pair(uint32_t cluster_addr)
+{
+    asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(cluster_addr) : "memory");
 }
 
 // TMA load for a CTA pair: data lands in this CTA's shared memory, the transaction bytes complete on an
