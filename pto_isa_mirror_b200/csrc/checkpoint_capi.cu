@@ -130,7 +130,8 @@ extern "C" int pto_b200_gemm_wgrad_mx(void* stream, uint8_t* out, const uint8_t*
         return PTO_B200_EDTYPE;
     }
     if (out == nullptr || dy == nullptr || data == nullptr || scales == nullptr || t <= 0 || n <= 0 || k <= 0 || k % 32 != 0 ||
-        ld_dy < n || ld_data < k || ld_scales < k / 32 || ld_out < k || (addend != nullptr && ld_addend < k)) {
+        ld_dy < n || ld_data < k || ld_scales < k / 32 || ld_scales >= (1 << 26) || ld_out < k ||
+        (addend != nullptr && ld_addend < k)) { // offsets within a stage's scales are 32-bit
         return PTO_B200_EINVAL;
     }
     const unsigned out_es = out_dtype == PTO_B200_F32 ? 4 : 2;

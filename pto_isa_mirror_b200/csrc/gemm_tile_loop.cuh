@@ -134,6 +134,28 @@ __device__ __forceinline__ bool bounded_wait(uint64_t* bar, uint32_t parity, vol
     return true;
 }
 
+// The same wait for kernels whose other warps need the issue slots a polling one takes: suspended in between, 10 us at a
+// time at most, so that the abort flag and the limit are still looked at.
+__device__ __forceinline__ bool bounded_wait_quiet(uint64_t* bar, uint32_t parity, volatile uint32_t* abort_flag, int* status,
+                                                   int code, long long limit)
+{
+    if (ptx::mbar_try_wait(bar, parity)) {
+        return true;
+    }
+    const long long t0 = clock64();
+    while (!ptx::mbar_try_wait_for(bar, parity, 10000u)) {
+        if (*abort_flag != 0) {
+            return false;
+        }
+        if (clock64() - t0 > limit) {
+            *abort_flag = 1;
+            atomicCAS(status, 0, code);
+            return false;
+        }
+    }
+    return true;
+}
+
 // Grouped raster: walk group_m row-tiles down, then step one column-tile right, so a wave of
 // concurrent CTAs shares a small set of A and B panels in L2.
 __device__ __forceinline__ void tile_coords(int t, const GemmParams& p, int& mi, int& ni)

@@ -84,49 +84,107 @@ struct WgSmem {
 static_assert(WgSmem::kTotal <= 227 * 1024, "shared memory of the weight-gradient kernel");
 static_assert(256 * 128 * 4 <= WgSmem::kRawOff, "partial sums reuse the ring");
 
-__device__ __forceinline__ uint64_t wg_pack2(float lo, float hi)
-{
-    uint64_t r;
-    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(lo), "f"(hi));
-    return r;
-}
-
-// Sixteen e4m3 bytes times one scale -> sixteen 16-bit values.
-template <bool F16>
-__device__ __forceinline__ void wg_convert16(const uint4& raw, float scale, uint32_t (&o)[8])
-{
-    const uint32_t w[4] = {raw.x, raw.y, raw.z, raw.w};
-    const uint64_t scale2 = wg_pack2(scale, scale);
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-            const __half2_raw r = __nv_cvt_fp8x2_to_halfraw2(static_cast<__nv_fp8x2_storage_t>(h == 0 ? w[i] & 0xFFFFu : w[i] >> 16), __NV_E4M3);
-            const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&r));
-            float lo, hi;
-            asm("{\n\t"
-                ".reg .b64 t;\n\t"
-                "mul.rn.f32x2 t, %2, %3;\n\t"
-                "mov.b64 {%0, %1}, t;\n\t"
-                "}"
-                : "=f"(lo), "=f"(hi)
-                : "l"(wg_pack2(f.x, f.y)), "l"(scale2));
-            if constexpr (F16) {
-                const __half2 v = __floats2half2_rn(lo, hi);
-                o[2 * i + h] = *reinterpret_cast<const uint32_t*>(&v);
-            } else {
-                // at most four significant bits: the upper half of the float is the bf16 value
-                o[2 * i + h] = __byte_perm(__float_as_uint(lo), __float_as_uint(hi), 0x7632);
-            }
-        }
-    }
-}
-
 // 2^(e - 127): e = 0 is the subnormal 2^-127, e = 255 a NaN.
 __device__ __forceinline__ float wg_scale(uint32_t e)
 {
     return __uint_as_float(e == 0u ? 0x00400000u : e == 255u ? 0x7FC00000u : e << 23);
 }
+
+__device__ __forceinline__ uint32_t wg_e4m3x2_to_f16x2(uint32_t two)
+{
+    const __half2_raw r = __nv_cvt_fp8x2_to_halfraw2(static_cast<__nv_fp8x2_storage_t>(two), __NV_E4M3);
+    return static_cast<uint32_t>(r.x) | (static_cast<uint32_t>(r.y) << 16);
+}
+
+// Sixteen e4m3 bytes times 2^(e - 127) -> sixteen 16-bit values, whatever the bytes and e: through fp32.
+template <bool F16>
+__device__ __forceinline__ void wg_convert16_any(const uint4& raw, uint32_t e, uint32_t (&o)[8])
+{
+    const uint32_t w[4] = {raw.x, raw.y, raw.z, raw.w};
+    const float scale = wg_scale(e);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+        const uint32_t h = wg_e4m3x2_to_f16x2((w[i / 2] >> (16 * (i & 1))) & 0xFFFFu);
+        const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&h));
+        const float lo = f.x * scale, hi = f.y * scale;
+        if constexpr (F16) {
+            const __half2 v = __floats2half2_rn(lo, hi);
+            o[i] = *reinterpret_cast<const uint32_t*>(&v);
+        } else {
+            // at most four significant bits: the upper half of the float is the bf16 value
+            o[i] = __byte_perm(__float_as_uint(lo), __float_as_uint(hi), 0x7632);
+        }
+    }
+}
+
+// The same in the fewest instructions, for the scales and bytes that activations have; wg_needs_any() says where it does
+// not hold. One multiplication per two values, exact but for results below the type's normal range, rounded once.
+// bf16: the byte's fields are put where bf16 has them, sign | 0000 eeee | mmm 0000, which is the value times 2^-120, and
+//       multiplied by 2^(e - 7). High and low bytes are made for four values at a time.
+// fp16: the conversion instruction, then 2^(e - 127) as an fp16 number.
+template <bool F16>
+__device__ __forceinline__ void wg_convert16(const uint4& raw, uint32_t e, uint32_t (&o)[8])
+{
+    const uint32_t w[4] = {raw.x, raw.y, raw.z, raw.w};
+    if constexpr (F16) {
+        const float f = __uint_as_float(e << 23);
+        const __half2 factor = __floats2half2_rn(f, f);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            const uint32_t h = wg_e4m3x2_to_f16x2((i & 1) ? w[i / 2] >> 16 : w[i / 2] & 0xFFFFu);
+            const __half2 v = __hmul2(*reinterpret_cast<const __half2*>(&h), factor);
+            o[i] = *reinterpret_cast<const uint32_t*>(&v);
+        }
+    } else {
+        const uint32_t f = e * 0x00800080u + 0x3C003C00u; // (e - 7 + 127) << 7, twice
+        const __nv_bfloat162 factor = *reinterpret_cast<const __nv_bfloat162*>(&f);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const uint32_t low = (w[i] << 4) & 0xF0F0F0F0u;
+            const uint32_t high = ((w[i] >> 4) & 0x07070707u) | (w[i] & 0x80808080u);
+            const uint32_t a = __byte_perm(low, high, 0x5140), b = __byte_perm(low, high, 0x7362);
+            const __nv_bfloat162 va = __hmul2(*reinterpret_cast<const __nv_bfloat162*>(&a), factor);
+            const __nv_bfloat162 vb = __hmul2(*reinterpret_cast<const __nv_bfloat162*>(&b), factor);
+            o[2 * i] = *reinterpret_cast<const uint32_t*>(&va);
+            o[2 * i + 1] = *reinterpret_cast<const uint32_t*>(&vb);
+        }
+    }
+}
+
+// Whether wg_convert16 does not hold for some of a thread's pieces: a scale whose factor has no number of the type, or
+// (bf16) a NaN among the bytes, 0x7F or 0xFF - the bytes whose top bit an added one flips.
+template <bool F16>
+__device__ __forceinline__ bool wg_needs_any(const uint4 (&in)[4], const uint32_t (&e)[4])
+{
+    const uint32_t top = max(max(e[0], e[1]), max(e[2], e[3]));
+    if constexpr (F16) {
+        const uint32_t low = min(min(e[0], e[1]), min(e[2], e[3]));
+        return top > 142u || low < 103u;
+    } else {
+        uint32_t flips = 0u;
+#pragma unroll
+        for (int h = 0; h < 4; ++h) {
+            flips |= (in[h].x + 0x01010101u) ^ in[h].x;
+            flips |= (in[h].y + 0x01010101u) ^ in[h].y;
+            flips |= (in[h].z + 0x01010101u) ^ in[h].z;
+            flips |= (in[h].w + 0x01010101u) ^ in[h].w;
+        }
+        return top > 134u || (flips & 0x80808080u) != 0u;
+    }
+}
+
+template <int OUT>
+struct WgElem {
+    using type = float;
+};
+template <>
+struct WgElem<WG_OUT_BF16> {
+    using type = __nv_bfloat16;
+};
+template <>
+struct WgElem<WG_OUT_F16> {
+    using type = __half;
+};
 
 template <int OUT>
 __device__ __forceinline__ float wg_load(const void* base, long long at)
@@ -241,7 +299,7 @@ __global__ void __launch_bounds__(kWgThreads, 1)
                     const int n0 = ni * 256 + side * 128;
                     for (int st = first_stage; st < last_stage; ++st) {
                         const int token = st * kWgStageTokens;
-                        ok = bounded_wait(&empty_bar[stage], phase ^ 1u, abort_flag, p.status, ST_WG_PRODUCER, p.wait_limit);
+                        ok = bounded_wait_quiet(&empty_bar[stage], phase ^ 1u, abort_flag, p.status, ST_WG_PRODUCER, p.wait_limit);
                         if (!ok) {
                             break;
                         }
@@ -270,7 +328,7 @@ __global__ void __launch_bounds__(kWgThreads, 1)
                     tile_of(tile, ki, ni);
                     const int k0 = ki * 256 + side * 128;
                     for (int st = first_stage; st < last_stage; ++st) {
-                        ok = bounded_wait(&raw_empty_bar[raw], phase ^ 1u, abort_flag, p.status, ST_WG_PRODUCER, p.wait_limit);
+                        ok = bounded_wait_quiet(&raw_empty_bar[raw], phase ^ 1u, abort_flag, p.status, ST_WG_PRODUCER, p.wait_limit);
                         if (!ok) {
                             break;
                         }
@@ -297,12 +355,12 @@ __global__ void __launch_bounds__(kWgThreads, 1)
             for (int tile = cluster; ok && tile < tiles; tile += clusters) {
                 for (int st = 0; st < stages; ++st) {
                     if (in_part == 0) {
-                        ok = bounded_wait(&acc_empty_bar[acc], acc_phase ^ 1u, abort_flag, p.status, ST_WG_MMA, p.wait_limit);
+                        ok = bounded_wait_quiet(&acc_empty_bar[acc], acc_phase ^ 1u, abort_flag, p.status, ST_WG_MMA, p.wait_limit);
                         if (!ok) {
                             break;
                         }
                     }
-                    ok = bounded_wait(&full_bar[stage], phase, abort_flag, p.status, ST_WG_MMA, p.wait_limit);
+                    ok = bounded_wait_quiet(&full_bar[stage], phase, abort_flag, p.status, ST_WG_MMA, p.wait_limit);
                     if (!ok) {
                         break;
                     }
@@ -341,14 +399,14 @@ __global__ void __launch_bounds__(kWgThreads, 1)
         // ---------------------------------------------------------------- conversion, sums, stores
         const int group = (warp - 4) >> 2;         // converts stages group, group + 4, ..; keeps the sums of 64 columns (n)
         const int quarter = warp & 3;              // and of these 32 tensor-memory lanes (k)
-        const int row = quarter * 4 + (lane >> 3); // four 16-byte pieces of x per stage, rows row + 16 h of the tile
-        const int piece = lane & 7;
-        // where the pieces go: 128-byte swizzle; the halves of a row lie in blocks 8 KiB apart, and the second half writes
-        // its odd piece first so that the eight lanes of a row hit different banks (row + 16 h has the row's swizzle)
-        const bool odd = piece >= 4;
+        // Four 16-byte pieces of x per stage: rows row + 16 h of the tile. Eight lanes read a half of one row and the other
+        // half of the next, 128 bytes on different banks; converted, the halves of a row lie in blocks 8 KiB apart with a
+        // 128-byte swizzle, where the two rows' pieces are on different banks again.
+        const int row = quarter * 4 + (lane >> 4) * 2 + ((lane >> 2) & 1);
+        const int piece = (lane & 3) + 4 * (((lane >> 2) ^ (lane >> 3)) & 1);
         const uint32_t line = (piece >> 2) * 8192 + row * 128;
-        const uint32_t at0 = line + ((((piece & 3) * 2 + (odd ? 1 : 0)) ^ (row & 7)) * 16);
-        const uint32_t at1 = line + ((((piece & 3) * 2 + (odd ? 0 : 1)) ^ (row & 7)) * 16);
+        const uint32_t at0 = line + ((((piece & 3) * 2) ^ (row & 7)) * 16); // row + 16 h has the row's swizzle
+        const uint32_t at1 = line + ((((piece & 3) * 2 + 1) ^ (row & 7)) * 16);
         const uint8_t* raw = smem + L::kRawOff + group * L::kRawBytes + row * 128 + piece * 16;
         int stage = group, acc = 0;
         uint32_t phase = 0, raw_phase = 0, acc_phase = 0;
@@ -357,26 +415,36 @@ __global__ void __launch_bounds__(kWgThreads, 1)
         const int stages = last_stage - first_stage; // of a tile
         const int parts = (stages + kWgFoldStages - 1) / kWgFoldStages;
         // Block scales come straight from memory, one visit (four stages) ahead of their use: their rows start on any byte,
-        // so no TMA, and a thread fetches what its own pieces need.
-        const uint8_t* scale_at = nullptr;
-        int token = 0;
-        bool column_ok = false;
-        uint32_t e[4];
+        // so no TMA, and a thread fetches what its own pieces need. What lies outside takes the nearest scale inside: a
+        // column past K is never stored, and a token past T has zeros in dy and x.
+        int visit_token = 0;      // first token of the stage whose scales come next
+        uint32_t scale_off[4];
+        uint32_t e[4] = {127u, 127u, 127u, 127u};
         auto fetch_scales = [&]() {
+            const uint8_t* base = p.scales + visit_token * p.ld_scales;
+            if (visit_token + kWgStageTokens <= p.t) {
 #pragma unroll
-            for (int h = 0; h < 4; ++h) {
-                e[h] = (column_ok && token + 16 * h < p.t) ? __ldg(scale_at + 16 * h * p.ld_scales) : 127u;
+                for (int h = 0; h < 4; ++h) {
+                    e[h] = __ldg(base + scale_off[h]);
+                }
+            } else if (visit_token < p.t) {
+                const int last_row = p.t - 1 - visit_token;
+#pragma unroll
+                for (int h = 0; h < 4; ++h) {
+                    e[h] = __ldg(base + scale_off[h] - max(row + 16 * h - last_row, 0) * p.ld_scales);
+                }
             }
-            scale_at += kWgGroups * kWgStageTokens * p.ld_scales;
-            token += kWgGroups * kWgStageTokens;
+            visit_token += kWgGroups * kWgStageTokens;
         };
         auto start_scales = [&](int tile) { // of the first stage that this group converts of a tile
             int ki, ni;
-            tile_of(tile, ki, ni);
-            const int column = ki * 256 + side * 128 + piece * 16;
-            token = (first_stage + first_of_tile) * kWgStageTokens + row;
-            column_ok = tile < tiles && column < p.k;
-            scale_at = p.scales + token * p.ld_scales + (column >> 5);
+            tile_of(min(tile, tiles - 1), ki, ni);
+            const int column = min(ki * 256 + side * 128 + piece * 16, p.k - 1) >> 5;
+#pragma unroll
+            for (int h = 0; h < 4; ++h) {
+                scale_off[h] = static_cast<uint32_t>((row + 16 * h) * p.ld_scales + column);
+            }
+            visit_token = (first_stage + first_of_tile) * kWgStageTokens;
             fetch_scales();
         };
         start_scales(cluster);
@@ -391,19 +459,15 @@ __global__ void __launch_bounds__(kWgThreads, 1)
             int folded = 0;
             for (int st = first_of_tile; folded < parts; st += kWgGroups) {
                 if (st < stages) {
-                    float scale[4];
-#pragma unroll
-                    for (int h = 0; h < 4; ++h) {
-                        scale[h] = wg_scale(e[h]);
-                    }
+                    const uint32_t e_now[4] = {e[0], e[1], e[2], e[3]};
                     fetch_scales(); // of the next visit; past the tile's last token they are not used
-                    ok = bounded_wait(&raw_full_bar[group], raw_phase, abort_flag, p.status, ST_WG_WORKER, p.wait_limit);
+                    ok = bounded_wait_quiet(&raw_full_bar[group], raw_phase, abort_flag, p.status, ST_WG_WORKER, p.wait_limit);
                     uint4 in[4];
 #pragma unroll
                     for (int h = 0; h < 4; ++h) {
                         in[h] = *reinterpret_cast<const uint4*>(raw + h * 16 * 128);
                     }
-                    ok = ok && bounded_wait(&empty_bar[stage], phase ^ 1u, abort_flag, p.status, ST_WG_WORKER, p.wait_limit);
+                    ok = ok && bounded_wait_quiet(&empty_bar[stage], phase ^ 1u, abort_flag, p.status, ST_WG_WORKER, p.wait_limit);
                     ok = __all_sync(0xFFFFFFFFu, ok);
                     if (!ok) {
                         break;
@@ -413,13 +477,23 @@ __global__ void __launch_bounds__(kWgThreads, 1)
                         ptx::mbar_arrive(&raw_empty_bar[group]);
                     }
                     uint8_t* dst = smem + L::kXOff + stage * L::kXBytes;
+                    if (!__any_sync(0xFFFFFFFFu, wg_needs_any<F16>(in, e_now))) {
 #pragma unroll
-                    for (int h = 0; h < 4; ++h) {
-                        uint32_t o[8];
-                        wg_convert16<F16>(in[h], scale[h], o);
-                        const uint4 lo = make_uint4(o[0], o[1], o[2], o[3]), hi = make_uint4(o[4], o[5], o[6], o[7]);
-                        *reinterpret_cast<uint4*>(dst + at0 + h * 16 * 128) = odd ? hi : lo;
-                        *reinterpret_cast<uint4*>(dst + at1 + h * 16 * 128) = odd ? lo : hi;
+                        for (int h = 0; h < 4; ++h) {
+                            uint32_t o[8];
+                            wg_convert16<F16>(in[h], e_now[h], o);
+                            *reinterpret_cast<uint4*>(dst + at0 + h * 16 * 128) = make_uint4(o[0], o[1], o[2], o[3]);
+                            *reinterpret_cast<uint4*>(dst + at1 + h * 16 * 128) = make_uint4(o[4], o[5], o[6], o[7]);
+                        }
+                    } else {
+#pragma unroll 1
+                        for (int h = 0; h < 4; ++h) {
+                            uint32_t o[8];
+                            wg_convert16_any<F16>(h == 0 ? in[0] : h == 1 ? in[1] : h == 2 ? in[2] : in[3],
+                                                  h == 0 ? e_now[0] : h == 1 ? e_now[1] : h == 2 ? e_now[2] : e_now[3], o);
+                            *reinterpret_cast<uint4*>(dst + at0 + h * 16 * 128) = make_uint4(o[0], o[1], o[2], o[3]);
+                            *reinterpret_cast<uint4*>(dst + at1 + h * 16 * 128) = make_uint4(o[4], o[5], o[6], o[7]);
+                        }
                     }
                     ptx::fence_proxy_async_smem();
                     __syncwarp();
@@ -436,7 +510,7 @@ __global__ void __launch_bounds__(kWgThreads, 1)
                 // The oldest finished accumulator joins the sums: behind the last stage, or once this group has had a place
                 // in the ring whose last products came after that accumulator's - then nothing is waited for.
                 if (st >= stages || st >= (folded + 1) * kWgFoldStages + kWgStages) {
-                    ok = bounded_wait(&acc_full_bar[acc], acc_phase, abort_flag, p.status, ST_WG_WORKER, p.wait_limit);
+                    ok = bounded_wait_quiet(&acc_full_bar[acc], acc_phase, abort_flag, p.status, ST_WG_WORKER, p.wait_limit);
                     ok = __all_sync(0xFFFFFFFFu, ok);
                     if (!ok) {
                         break;
@@ -473,10 +547,20 @@ __global__ void __launch_bounds__(kWgThreads, 1)
                 const int k = ki * 256 + side * 128 + in_tile;
                 const int n0 = ni * 256 + group * 64;
                 if (k < p.k) {
+                    if (p.addend == nullptr && n0 + 64 <= p.n) {
+                        using T = typename WgElem<OUT>::type;
+                        T* at = static_cast<T*>(p.out) + n0 * p.ld_out + k;
 #pragma unroll
-                    for (int i = 0; i < 64; ++i) {
-                        if (n0 + i < p.n) {
-                            wg_store<OUT>(p, n0 + i, k, sum[i]);
+                        for (int i = 0; i < 64; ++i) {
+                            *at = static_cast<T>(sum[i]);
+                            at += p.ld_out;
+                        }
+                    } else {
+#pragma unroll
+                        for (int i = 0; i < 64; ++i) {
+                            if (n0 + i < p.n) {
+                                wg_store<OUT>(p, n0 + i, k, sum[i]);
+                            }
                         }
                     }
                 }
