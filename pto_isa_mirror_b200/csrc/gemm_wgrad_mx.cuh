@@ -45,7 +45,7 @@ constexpr int kWgStages = 6;      // ring of dy tiles and converted x tiles
 constexpr int kWgRawStages = 4;   // ring of x tiles as they come: one place per group
 static_assert(kWgRawStages == kWgGroups, "a group reads its own place of the ring of x");
 // registers: 96 at launch; the loading and multiplying warps give back what the sums need
-constexpr int kWgRegsOthers = 56, kWgRegsWorkers = 104;
+constexpr int kWgRegsOthers = 32, kWgRegsWorkers = 112;
 static_assert(128 * kWgRegsOthers + 512 * kWgRegsWorkers <= kWgThreads * 96, "register split within the launch's total");
 constexpr int kWgStageTokens = 64;
 constexpr int kWgFoldStages = 32;
@@ -418,20 +418,20 @@ __global__ void __launch_bounds__(kWgThreads, 1)
         // so no TMA, and a thread fetches what its own pieces need. What lies outside takes the nearest scale inside: a
         // column past K is never stored, and a token past T has zeros in dy and x.
         int visit_token = 0;      // first token of the stage whose scales come next
-        uint32_t scale_off[4];
+        uint32_t scale_off = 0;
         uint32_t e[4] = {127u, 127u, 127u, 127u};
         auto fetch_scales = [&]() {
             const uint8_t* base = p.scales + visit_token * p.ld_scales;
             if (visit_token + kWgStageTokens <= p.t) {
 #pragma unroll
                 for (int h = 0; h < 4; ++h) {
-                    e[h] = __ldg(base + scale_off[h]);
+                    e[h] = __ldg(base + 16 * h * p.ld_scales + scale_off);
                 }
             } else if (visit_token < p.t) {
                 const int last_row = p.t - 1 - visit_token;
 #pragma unroll
                 for (int h = 0; h < 4; ++h) {
-                    e[h] = __ldg(base + scale_off[h] - max(row + 16 * h - last_row, 0) * p.ld_scales);
+                    e[h] = __ldg(base + (min(row + 16 * h, last_row) - row) * p.ld_scales + scale_off);
                 }
             }
             visit_token += kWgGroups * kWgStageTokens;
@@ -440,10 +440,7 @@ __global__ void __launch_bounds__(kWgThreads, 1)
             int ki, ni;
             tile_of(min(tile, tiles - 1), ki, ni);
             const int column = min(ki * 256 + side * 128 + piece * 16, p.k - 1) >> 5;
-#pragma unroll
-            for (int h = 0; h < 4; ++h) {
-                scale_off[h] = static_cast<uint32_t>((row + 16 * h) * p.ld_scales + column);
-            }
+            scale_off = static_cast<uint32_t>(row * p.ld_scales + column);
             visit_token = (first_stage + first_of_tile) * kWgStageTokens;
             fetch_scales();
         };
