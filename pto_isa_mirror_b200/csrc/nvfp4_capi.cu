@@ -19,30 +19,39 @@ int size_of(int src) { return src == NV_F32 ? 4 : 2; }
 bool misaligned(const void* p, unsigned bytes) { return (reinterpret_cast<uintptr_t>(p) & (bytes - 1u)) != 0; }
 
 // Blocks for `items` single-thread items: one resident wave that walks them with a grid stride.
-template <typename Kernel>
-int one_wave(Kernel kernel, long long items, int sm_count, int* grid)
+template <auto KERNEL>
+int one_wave(long long items, const HostContext& host, int* grid)
 {
-    int per_sm = 0;
-    if (int rc = note_cuda_error(cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per_sm, kernel, kNvQuantThreads, 0),
-                                 "nvfp4 occupancy")) {
-        return rc;
+    static std::atomic<int> blocks_per_sm[kMaxDevices];
+    int per_sm = blocks_per_sm[host.device].load(std::memory_order_relaxed);
+    if (per_sm == 0) {
+        if (int rc = note_cuda_error(cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per_sm, KERNEL, kNvQuantThreads, 0),
+                                     "nvfp4 occupancy")) {
+            return rc;
+        }
+        per_sm = per_sm > 0 ? per_sm : 1;
+        blocks_per_sm[host.device].store(per_sm, std::memory_order_relaxed);
     }
     const long long want = (items + kNvQuantThreads - 1) / kNvQuantThreads;
-    const long long cap = static_cast<long long>(sm_count) * (per_sm > 0 ? per_sm : 1);
+    const long long cap = static_cast<long long>(host.sm_count) * per_sm;
     *grid = static_cast<int>(want < cap ? want : cap);
     return PTO_B200_OK;
 }
 
 template <int SRC, bool VEC>
-int launch_quantize(cudaStream_t s, int sm_count, const void* src, const float* amax, uint8_t* data, uint8_t* scales,
+int launch_quantize(cudaStream_t s, const HostContext& host, const void* src, const float* amax, uint8_t* data, uint8_t* scales,
                     float* tensor_scale, int rows, int k, long long ld_src, long long ld_data, bool transpose)
 {
     if (transpose) {
         constexpr int kSmem = kNvTransRows / 16 * kNvTransGroupBytes<SRC>;
         auto kernel = nvfp4_quantize_transposed_kernel<SRC, VEC>;
-        if (int rc = note_cuda_error(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem),
-                                     "cudaFuncSetAttribute(nvfp4 transpose)")) {
-            return rc;
+        static std::atomic<int> attr_done[kMaxDevices];
+        if (attr_done[host.device].load(std::memory_order_acquire) == 0) {
+            if (int rc = note_cuda_error(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem),
+                                         "cudaFuncSetAttribute(nvfp4 transpose)")) {
+                return rc;
+            }
+            attr_done[host.device].store(1, std::memory_order_release);
         }
         // whole 128-row tiles of scales: columns past k are quantised as zeros, which fills the tiles' padding
         const dim3 grid(static_cast<unsigned>((rows + kNvTransRows - 1) / kNvTransRows),
@@ -51,7 +60,7 @@ int launch_quantize(cudaStream_t s, int sm_count, const void* src, const float* 
     } else {
         const long long items = (static_cast<long long>(rows) + 127) / 128 * 128 * ((k + 63) / 64 * 4);
         int grid = 0;
-        if (int rc = one_wave(nvfp4_quantize_kernel<SRC, VEC>, items, sm_count, &grid)) {
+        if (int rc = one_wave<nvfp4_quantize_kernel<SRC, VEC>>(items, host, &grid)) {
             return rc;
         }
         nvfp4_quantize_kernel<SRC, VEC>
@@ -62,10 +71,10 @@ int launch_quantize(cudaStream_t s, int sm_count, const void* src, const float* 
 }
 
 template <int SRC, bool VEC>
-int launch_amax(cudaStream_t s, int sm_count, const void* src, float* amax, int rows, int k, long long ld_src)
+int launch_amax(cudaStream_t s, const HostContext& host, const void* src, float* amax, int rows, int k, long long ld_src)
 {
     int grid = 0;
-    if (int rc = one_wave(amax_kernel<SRC, VEC>, static_cast<long long>(rows) * ((k + 15) / 16), sm_count, &grid)) {
+    if (int rc = one_wave<amax_kernel<SRC, VEC>>(static_cast<long long>(rows) * ((k + 15) / 16), host, &grid)) {
         return rc;
     }
     if (int rc = note_cuda_error(cudaMemsetAsync(amax, 0, sizeof(float), s), "amax memset")) {
@@ -77,11 +86,11 @@ int launch_amax(cudaStream_t s, int sm_count, const void* src, float* amax, int 
 }
 
 template <int DST, bool VEC>
-int launch_dequantize(cudaStream_t s, int sm_count, const uint8_t* data, const uint8_t* scales, const float* tensor_scale,
+int launch_dequantize(cudaStream_t s, const HostContext& host, const uint8_t* data, const uint8_t* scales, const float* tensor_scale,
                       void* out, int rows, int k, long long ld_data, long long ld_out)
 {
     int grid = 0;
-    if (int rc = one_wave(nvfp4_dequantize_kernel<DST, VEC>, static_cast<long long>(rows) * ((k + 7) / 8), sm_count, &grid)) {
+    if (int rc = one_wave<nvfp4_dequantize_kernel<DST, VEC>>(static_cast<long long>(rows) * ((k + 7) / 8), host, &grid)) {
         return rc;
     }
     nvfp4_dequantize_kernel<DST, VEC>
@@ -267,7 +276,7 @@ extern "C" int pto_b200_amax(void* stream, float* amax, const uint8_t* src, int 
         return rc;
     }
     const bool vec = !misaligned(src, 16) && (ld_src * es) % 16 == 0;
-    return PTO_NV_DISPATCH(type, vec, launch_amax, static_cast<cudaStream_t>(stream), host.sm_count, src, amax, rows, k, ld_src);
+    return PTO_NV_DISPATCH(type, vec, launch_amax, static_cast<cudaStream_t>(stream), host, src, amax, rows, k, ld_src);
 }
 
 extern "C" int pto_b200_nvfp4_quantize(void* stream, uint8_t* data, uint8_t* scales, float* tensor_scale, const uint8_t* src,
@@ -293,7 +302,7 @@ extern "C" int pto_b200_nvfp4_quantize(void* stream, uint8_t* data, uint8_t* sca
         return rc;
     }
     const bool vec = !misaligned(src, 16) && (ld_src * es) % 16 == 0;
-    return PTO_NV_DISPATCH(type, vec, launch_quantize, static_cast<cudaStream_t>(stream), host.sm_count, src, amax, data,
+    return PTO_NV_DISPATCH(type, vec, launch_quantize, static_cast<cudaStream_t>(stream), host, src, amax, data,
                            scales, tensor_scale, rows, k, ld_src, ld_data, transpose != 0);
 }
 
@@ -318,7 +327,7 @@ extern "C" int pto_b200_nvfp4_dequantize(void* stream, uint8_t* out, const uint8
         return rc;
     }
     const bool vec = !misaligned(out, 16) && (ld_out * es) % 16 == 0;
-    return PTO_NV_DISPATCH(type, vec, launch_dequantize, static_cast<cudaStream_t>(stream), host.sm_count, data, scales,
+    return PTO_NV_DISPATCH(type, vec, launch_dequantize, static_cast<cudaStream_t>(stream), host, data, scales,
                            tensor_scale, out, rows, k, ld_data, ld_out);
 }
 

@@ -29,9 +29,11 @@ if hasattr(torch, "float8_e4m3fn"):
     _TORCH_TO_PTO[torch.float8_e5m2] = E5M2
 
 
+_raw_stream = torch._C._cuda_getCurrentRawStream  # the current stream of a device as a pointer, without a Stream object
+
+
 def _stream_ptr(stream: Optional[torch.cuda.Stream]) -> int:
-    s = stream if stream is not None else torch.cuda.current_stream()
-    return s.cuda_stream
+    return stream.cuda_stream if stream is not None else _raw_stream(torch.cuda.current_device())
 
 
 def _require_cuda_2d(t: torch.Tensor, name: str) -> None:

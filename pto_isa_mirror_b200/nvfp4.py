@@ -9,39 +9,38 @@ tiles by ``s.view(rt, 4, 32, kt, 4).permute(0, 3, 2, 1, 4).reshape(rt, kt, 512)`
 """
 from __future__ import annotations
 
-import contextlib
 from typing import Optional, Tuple
 
 import torch
 
 from . import _capi
-from .gemm import _TORCH_TO_PTO, _require_cuda_2d
+from .gemm import _TORCH_TO_PTO, _raw_stream, _require_cuda_2d
 
 _FLOATS = (torch.float32, torch.bfloat16, torch.float16)
 
 
-@contextlib.contextmanager
-def _launching(stream: Optional[torch.cuda.Stream], *tensors: Optional[torch.Tensor]):
-    """The raw stream to launch on: ``stream``, or the current one of the tensors' device. Their device is current
-    inside, and what is allocated inside belongs to that stream."""
-    given = [t for t in tensors if t is not None]
-    device = given[0].device
-    if any(t.device != device for t in given):
-        raise ValueError("all tensors must be on one device")
-    if stream is not None:
-        if stream.device != device:
-            raise ValueError("stream is on another device than the tensors")
-        with torch.cuda.stream(stream):
-            yield stream.cuda_stream
-    elif device.index != torch.cuda.current_device():
-        with torch.cuda.device(device):
-            yield torch.cuda.current_stream().cuda_stream
-    else:
-        yield torch.cuda.current_stream().cuda_stream
+def _device_of(first: torch.Tensor, *others: Optional[torch.Tensor]) -> int:
+    """The ordinal of the one device that all tensors are on."""
+    device = first.get_device()
+    for t in others:
+        if t is not None and t.get_device() != device:
+            raise ValueError("all tensors must be on one CUDA device")
+    return device
+
+
+def _launch(device: int, stream: Optional[torch.cuda.Stream], call):
+    """``call(raw stream)`` with ``device`` current, on ``stream`` or the device's current one; what it allocates belongs to
+    that stream."""
+    if stream is None and device == torch.cuda.current_device():
+        return call(_raw_stream(device))
+    if stream is not None and stream.device_index != device:
+        raise ValueError("stream is on another device than the tensors")
+    with torch.cuda.device(device) if stream is None else torch.cuda.stream(stream):
+        return call(_raw_stream(device))
 
 
 def _require_float_scalar(t: Optional[torch.Tensor], name: str) -> None:
-    if t is not None and (t.dtype != torch.float32 or not t.is_cuda or t.numel() != 1):
+    if t is not None and (t.dtype is not torch.float32 or not t.is_cuda or t.numel() != 1):
         raise ValueError(f"{name} must be a CUDA float32 tensor with one element")
 
 
@@ -50,7 +49,7 @@ def _tiles(rows: int, k: int) -> Tuple[int, int, int]:
 
 
 def _require_scales(t: torch.Tensor, rows: int, k: int, name: str) -> None:
-    if not t.is_cuda or t.element_size() != 1 or not t.is_contiguous() or tuple(t.shape) != _tiles(rows, k):
+    if not t.is_cuda or t.element_size() != 1 or not t.is_contiguous() or t.shape != _tiles(rows, k):
         raise ValueError(f"{name} must be contiguous scale tiles of shape {_tiles(rows, k)} in one-byte elements")
 
 
@@ -91,25 +90,28 @@ def nvfp4_quantize(src: torch.Tensor, amax: Optional[torch.Tensor] = None, trans
             raise ValueError(f"data must be uint8 of shape {(out_rows, width)}")
     if scales is not None:
         _require_scales(scales, out_rows, length, "scales")
-    with _launching(stream, src, amax, data, scales, tensor_scale) as sp:
-        if data is None:
-            pitch = (width + 15) // 16 * 16  # TMA rows start on 16-byte boundaries
-            data = torch.empty((out_rows, pitch), dtype=torch.uint8, device=src.device)[:, :width]
-        if scales is None:
-            scales = torch.empty(_tiles(out_rows, length), dtype=torch.uint8, device=src.device)
-        if tensor_scale is None:
-            tensor_scale = torch.empty((1,), dtype=torch.float32, device=src.device)
-        ld = src.stride(0) if rows > 1 else max(src.stride(0), k)
-        ld_data = data.stride(0) if out_rows > 1 else max(data.stride(0), (width + 15) // 16 * 16)
-        dtype = _TORCH_TO_PTO[src.dtype]
+    pitch = (width + 15) // 16 * 16  # TMA rows start on 16-byte boundaries
+    src_pitch = src.stride(0) if rows > 1 else k
+    dtype = _TORCH_TO_PTO[src.dtype]
+
+    def call(sp):
+        nonlocal amax
+        d, s, t = data, scales, tensor_scale
+        if d is None:
+            d = torch.empty_strided((out_rows, width), (pitch, 1), dtype=torch.uint8, device=src.device)
+        if s is None:
+            s = torch.empty(_tiles(out_rows, length), dtype=torch.uint8, device=src.device)
+        if t is None:
+            t = torch.empty((1,), dtype=torch.float32, device=src.device)
         if amax is None:
             amax = torch.empty((1,), dtype=torch.float32, device=src.device)
-            rc = lib.pto_b200_amax(sp, amax.data_ptr(), src.data_ptr(), rows, k, ld, dtype)
-            _capi.check(rc, "pto_b200_amax")
-        rc = lib.pto_b200_nvfp4_quantize(sp, data.data_ptr(), scales.data_ptr(), tensor_scale.data_ptr(), src.data_ptr(),
-                                         amax.data_ptr(), rows, k, ld, ld_data, dtype, int(bool(transpose)))
+            _capi.check(lib.pto_b200_amax(sp, amax.data_ptr(), src.data_ptr(), rows, k, src_pitch, dtype), "pto_b200_amax")
+        rc = lib.pto_b200_nvfp4_quantize(sp, d.data_ptr(), s.data_ptr(), t.data_ptr(), src.data_ptr(), amax.data_ptr(), rows, k,
+                                         src_pitch, d.stride(0) if out_rows > 1 else pitch, dtype, int(bool(transpose)))
         _capi.check(rc, "pto_b200_nvfp4_quantize")
-    return data, scales, tensor_scale
+        return d, s, t
+
+    return _launch(_device_of(src, amax, data, scales, tensor_scale), stream, call)
 
 
 def nvfp4_dequantize(data: torch.Tensor, scales: torch.Tensor, tensor_scale: Optional[torch.Tensor] = None,
@@ -133,16 +135,17 @@ def nvfp4_dequantize(data: torch.Tensor, scales: torch.Tensor, tensor_scale: Opt
             raise ValueError("out must be [rows, K] float32, bfloat16 or float16")
     elif out_dtype not in _FLOATS:
         raise ValueError("out_dtype must be float32, bfloat16 or float16")
-    with _launching(stream, data, scales, tensor_scale, out) as sp:
-        if out is None:
-            out = torch.empty((rows, k), dtype=out_dtype, device=data.device)
-        cols = out.shape[1]
-        ld_data = data.stride(0) if rows > 1 else max(data.stride(0), (data.shape[1] + 3) // 4 * 4)
-        ld_out = out.stride(0) if rows > 1 else max(out.stride(0), cols)
-        rc = lib.pto_b200_nvfp4_dequantize(sp, out.data_ptr(), data.data_ptr(), scales.data_ptr(), _ptr(tensor_scale), rows,
-                                           cols, ld_data, ld_out, _TORCH_TO_PTO[out.dtype])
+
+    def call(sp):
+        o = out if out is not None else torch.empty((rows, k), dtype=out_dtype, device=data.device)
+        cols = o.shape[1]
+        rc = lib.pto_b200_nvfp4_dequantize(sp, o.data_ptr(), data.data_ptr(), scales.data_ptr(), _ptr(tensor_scale), rows, cols,
+                                           data.stride(0) if rows > 1 else (k // 2 + 3) // 4 * 4,
+                                           o.stride(0) if rows > 1 else cols, _TORCH_TO_PTO[o.dtype])
         _capi.check(rc, "pto_b200_nvfp4_dequantize")
-    return out
+        return o
+
+    return _launch(_device_of(data, scales, tensor_scale, out), stream, call)
 
 
 def gemm_nvfp4(a: torch.Tensor, b_dn: torch.Tensor, sfa: torch.Tensor, sfb: torch.Tensor, ga: Optional[torch.Tensor] = None,
@@ -176,14 +179,14 @@ def gemm_nvfp4(a: torch.Tensor, b_dn: torch.Tensor, sfa: torch.Tensor, sfb: torc
             raise ValueError("out must be [M, N] float32, bfloat16 or float16")
     elif out_dtype not in _FLOATS:
         raise ValueError("out_dtype must be float32, bfloat16 or float16")
-    with _launching(stream, a, b_dn, sfa, sfb, ga, gb, bias, out) as sp:
-        if out is None:
-            out = torch.empty((m, n), dtype=out_dtype, device=a.device)
-        row = (k // 2 + 15) // 16 * 16
-        lda = (a.stride(0) if m > 1 else max(a.stride(0), row)) * 2
-        ldb = (b_dn.stride(0) if n > 1 else max(b_dn.stride(0), row)) * 2
-        ldc = out.stride(0) if m > 1 else max(out.stride(0), n)
-        rc = lib.pto_b200_gemm_nvfp4(sp, out.data_ptr(), a.data_ptr(), b_dn.data_ptr(), sfa.data_ptr(), sfb.data_ptr(), _ptr(ga),
-                                     _ptr(gb), _ptr(bias), m, n, k, lda, ldb, ldc, _TORCH_TO_PTO[out.dtype])
+
+    def call(sp):
+        o = out if out is not None else torch.empty((m, n), dtype=out_dtype, device=a.device)
+        row = (k // 2 + 15) // 16 * 32  # a single row's pitch, in 4-bit elements
+        rc = lib.pto_b200_gemm_nvfp4(sp, o.data_ptr(), a.data_ptr(), b_dn.data_ptr(), sfa.data_ptr(), sfb.data_ptr(), _ptr(ga),
+                                     _ptr(gb), _ptr(bias), m, n, k, a.stride(0) * 2 if m > 1 else row,
+                                     b_dn.stride(0) * 2 if n > 1 else row, o.stride(0) if m > 1 else n, _TORCH_TO_PTO[o.dtype])
         _capi.check(rc, "pto_b200_gemm_nvfp4")
-    return out
+        return o
+
+    return _launch(_device_of(a, b_dn, sfa, sfb, ga, gb, bias, out), stream, call)

@@ -7,7 +7,7 @@ import torch
 
 from . import _capi
 from .gemm import _TORCH_TO_PTO, _require_cuda_2d
-from .nvfp4 import _FLOATS, _launching, _ptr
+from .nvfp4 import _FLOATS, _device_of, _launch, _ptr
 
 
 def gemm_wgrad_mx(dy: torch.Tensor, data: torch.Tensor, scales: torch.Tensor, out_dtype: torch.dtype = torch.float32,
@@ -44,16 +44,15 @@ def gemm_wgrad_mx(dy: torch.Tensor, data: torch.Tensor, scales: torch.Tensor, ou
         _require_cuda_2d(addend, "addend")
         if addend.dtype != out_dtype or tuple(addend.shape) != (n, k):
             raise ValueError("addend must be [N, K] of dW's type")
-    with _launching(stream, dy, data, scales, addend, out) as sp:
-        if out is None:
-            out = torch.empty((n, k), dtype=out_dtype, device=dy.device)
-        ld_dy = dy.stride(0) if t > 1 else (n + 7) // 8 * 8
-        ld_data = data.stride(0) if t > 1 else (k + 15) // 16 * 16
-        ld_scales = scales.stride(0) if t > 1 else k // 32
-        ld_out = out.stride(0) if n > 1 else k
-        ld_addend = 0 if addend is None else addend.stride(0) if n > 1 else k
-        rc = lib.pto_b200_gemm_wgrad_mx(sp, out.data_ptr(), dy.data_ptr(), data.data_ptr(), scales.data_ptr(), _ptr(addend), t, n,
-                                        k, ld_dy, ld_data, ld_scales, ld_out, ld_addend, _TORCH_TO_PTO[dy.dtype],
+
+    def call(sp):
+        o = out if out is not None else torch.empty((n, k), dtype=out_dtype, device=dy.device)
+        rc = lib.pto_b200_gemm_wgrad_mx(sp, o.data_ptr(), dy.data_ptr(), data.data_ptr(), scales.data_ptr(), _ptr(addend), t, n, k,
+                                        dy.stride(0) if t > 1 else (n + 7) // 8 * 8, data.stride(0) if t > 1 else (k + 15) // 16 * 16,
+                                        scales.stride(0) if t > 1 else k // 32, o.stride(0) if n > 1 else k,
+                                        0 if addend is None else addend.stride(0) if n > 1 else k, _TORCH_TO_PTO[dy.dtype],
                                         _TORCH_TO_PTO[out_dtype])
         _capi.check(rc, "pto_b200_gemm_wgrad_mx")
-    return out
+        return o
+
+    return _launch(_device_of(dy, data, scales, addend, out), stream, call)
