@@ -38,28 +38,31 @@ int one_wave(long long items, const HostContext& host, int* grid)
     return PTO_B200_OK;
 }
 
-template <int SRC, bool VEC>
+template <int SRC, int VEC>
 int launch_quantize(cudaStream_t s, const HostContext& host, const void* src, const float* amax, uint8_t* data, uint8_t* scales,
                     float* tensor_scale, int rows, int k, long long ld_src, long long ld_data, bool transpose)
 {
+    int grid = 0;
     if (transpose) {
-        constexpr int kSmem = kNvTransRows / 16 * kNvTransGroupBytes<SRC>;
-        auto kernel = nvfp4_quantize_transposed_kernel<SRC, VEC>;
-        static std::atomic<int> attr_done[kMaxDevices];
-        if (attr_done[host.device].load(std::memory_order_acquire) == 0) {
-            if (int rc = note_cuda_error(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem),
-                                         "cudaFuncSetAttribute(nvfp4 transpose)")) {
+        // 16-bit columns in pairs where rows start on 4-byte boundaries
+        const bool pairs = SRC != NV_F32 && !misaligned(src, 4) && ld_src % 2 == 0;
+        const long long items = (static_cast<long long>(rows) + 63) / 64 * ((k + 127) / 128 * (pairs ? 64 : 128));
+        if (pairs) {
+            constexpr bool kPairs = SRC != NV_F32;
+            if (int rc = one_wave<nvfp4_quantize_transposed_kernel<SRC, kPairs>>(items, host, &grid)) {
                 return rc;
             }
-            attr_done[host.device].store(1, std::memory_order_release);
+            nvfp4_quantize_transposed_kernel<SRC, kPairs>
+                <<<grid, kNvQuantThreads, 0, s>>>(src, amax, data, scales, tensor_scale, rows, k, ld_src, ld_data);
+        } else {
+            if (int rc = one_wave<nvfp4_quantize_transposed_kernel<SRC, false>>(items, host, &grid)) {
+                return rc;
+            }
+            nvfp4_quantize_transposed_kernel<SRC, false>
+                <<<grid, kNvQuantThreads, 0, s>>>(src, amax, data, scales, tensor_scale, rows, k, ld_src, ld_data);
         }
-        // whole 128-row tiles of scales: columns past k are quantised as zeros, which fills the tiles' padding
-        const dim3 grid(static_cast<unsigned>((rows + kNvTransRows - 1) / kNvTransRows),
-                        static_cast<unsigned>((k + 127) / 128 * (128 / kNvTransCols)));
-        kernel<<<grid, kNvQuantThreads, kSmem, s>>>(src, amax, data, scales, tensor_scale, rows, k, ld_src, ld_data);
     } else {
         const long long items = (static_cast<long long>(rows) + 127) / 128 * 128 * ((k + 63) / 64 * 4);
-        int grid = 0;
         if (int rc = one_wave<nvfp4_quantize_kernel<SRC, VEC>>(items, host, &grid)) {
             return rc;
         }
@@ -70,7 +73,7 @@ int launch_quantize(cudaStream_t s, const HostContext& host, const void* src, co
     return note_cuda_error(cudaGetLastError(), "nvfp4_quantize launch");
 }
 
-template <int SRC, bool VEC>
+template <int SRC, int VEC>
 int launch_amax(cudaStream_t s, const HostContext& host, const void* src, float* amax, int rows, int k, long long ld_src)
 {
     int grid = 0;
@@ -89,8 +92,9 @@ template <int DST, bool VEC>
 int launch_dequantize(cudaStream_t s, const HostContext& host, const uint8_t* data, const uint8_t* scales, const float* tensor_scale,
                       void* out, int rows, int k, long long ld_data, long long ld_out)
 {
+    constexpr int kElems = DST == NV_F32 ? 8 : 16; // per thread
     int grid = 0;
-    if (int rc = one_wave<nvfp4_dequantize_kernel<DST, VEC>>(static_cast<long long>(rows) * ((k + 7) / 8), host, &grid)) {
+    if (int rc = one_wave<nvfp4_dequantize_kernel<DST, VEC>>(static_cast<long long>(rows) * ((k + kElems - 1) / kElems), host, &grid)) {
         return rc;
     }
     nvfp4_dequantize_kernel<DST, VEC>
@@ -99,11 +103,19 @@ int launch_dequantize(cudaStream_t s, const HostContext& host, const uint8_t* da
     return note_cuda_error(cudaGetLastError(), "nvfp4_dequantize launch");
 }
 
-// f(SRC, VEC) as template arguments
-#define PTO_NV_DISPATCH(src, vec, f, ...)                                                            \
-    ((src) == NV_F32 ? ((vec) ? f<NV_F32, true>(__VA_ARGS__) : f<NV_F32, false>(__VA_ARGS__))        \
-     : (src) == NV_BF16 ? ((vec) ? f<NV_BF16, true>(__VA_ARGS__) : f<NV_BF16, false>(__VA_ARGS__))   \
-                        : ((vec) ? f<NV_F16, true>(__VA_ARGS__) : f<NV_F16, false>(__VA_ARGS__)))
+// The widest access that every row of a matrix starts on: 32 or 16 bytes, or 0 for its elements.
+int row_access(const void* base, long long pitch_bytes)
+{
+    return !misaligned(base, 32) && pitch_bytes % 32 == 0 ? 32 : !misaligned(base, 16) && pitch_bytes % 16 == 0 ? 16 : 0;
+}
+
+// f<type, access>
+#define PTO_NV_TYPES(type, access, f, ...)                                                      \
+    ((type) == NV_F32 ? f<NV_F32, access>(__VA_ARGS__)                                          \
+                      : (type) == NV_BF16 ? f<NV_BF16, access>(__VA_ARGS__) : f<NV_F16, access>(__VA_ARGS__))
+#define PTO_NV_DISPATCH(type, access, f, ...)                                                   \
+    ((access) == 32 ? PTO_NV_TYPES(type, 32, f, __VA_ARGS__)                                    \
+                    : (access) == 16 ? PTO_NV_TYPES(type, 16, f, __VA_ARGS__) : PTO_NV_TYPES(type, 0, f, __VA_ARGS__))
 
 // Instruction descriptor of kind::mxf4nvf4: e2m1 is 1 in both format fields ([7,10) and [10,12)), N >> 3 at [17,23),
 // scale format e4m3 (0) at 23, M >> 7 at [27,29), K = 64 (0) at 31; scale ids 0, since an instruction uses all four
@@ -275,8 +287,7 @@ extern "C" int pto_b200_amax(void* stream, float* amax, const uint8_t* src, int 
     if (int rc = host_context(&host)) {
         return rc;
     }
-    const bool vec = !misaligned(src, 16) && (ld_src * es) % 16 == 0;
-    return PTO_NV_DISPATCH(type, vec, launch_amax, static_cast<cudaStream_t>(stream), host, src, amax, rows, k, ld_src);
+    return PTO_NV_DISPATCH(type, row_access(src, ld_src * es), launch_amax, static_cast<cudaStream_t>(stream), host, src, amax, rows, k, ld_src);
 }
 
 extern "C" int pto_b200_nvfp4_quantize(void* stream, uint8_t* data, uint8_t* scales, float* tensor_scale, const uint8_t* src,
@@ -285,7 +296,7 @@ extern "C" int pto_b200_nvfp4_quantize(void* stream, uint8_t* data, uint8_t* sca
 {
     const long long length = transpose ? rows : k; // of the result's rows
     if (data == nullptr || scales == nullptr || tensor_scale == nullptr || src == nullptr || amax == nullptr || rows <= 0 ||
-        k <= 0 || ld_src < k || ld_data < (length + 15) / 16 * 8 || (transpose && (k + 127) / 128 * 2 > 65535)) {
+        k <= 0 || ld_src < k || ld_data < (length + 15) / 16 * 8) {
         return PTO_B200_EINVAL;
     }
     const int type = source_of(src_dtype);
@@ -301,8 +312,7 @@ extern "C" int pto_b200_nvfp4_quantize(void* stream, uint8_t* data, uint8_t* sca
     if (int rc = host_context(&host)) {
         return rc;
     }
-    const bool vec = !misaligned(src, 16) && (ld_src * es) % 16 == 0;
-    return PTO_NV_DISPATCH(type, vec, launch_quantize, static_cast<cudaStream_t>(stream), host, src, amax, data,
+    return PTO_NV_DISPATCH(type, row_access(src, ld_src * es), launch_quantize, static_cast<cudaStream_t>(stream), host, src, amax, data,
                            scales, tensor_scale, rows, k, ld_src, ld_data, transpose != 0);
 }
 
@@ -326,9 +336,11 @@ extern "C" int pto_b200_nvfp4_dequantize(void* stream, uint8_t* out, const uint8
     if (int rc = host_context(&host)) {
         return rc;
     }
-    const bool vec = !misaligned(out, 16) && (ld_out * es) % 16 == 0;
-    return PTO_NV_DISPATCH(type, vec, launch_dequantize, static_cast<cudaStream_t>(stream), host, data, scales,
-                           tensor_scale, out, rows, k, ld_data, ld_out);
+    cudaStream_t s = static_cast<cudaStream_t>(stream);
+    if (row_access(out, ld_out * es) == 32) {
+        return PTO_NV_TYPES(type, true, launch_dequantize, s, host, data, scales, tensor_scale, out, rows, k, ld_data, ld_out);
+    }
+    return PTO_NV_TYPES(type, false, launch_dequantize, s, host, data, scales, tensor_scale, out, rows, k, ld_data, ld_out);
 }
 
 extern "C" int pto_b200_gemm_nvfp4(void* stream, uint8_t* out, const uint8_t* src0, const uint8_t* src1, const uint8_t* src2,

@@ -68,31 +68,109 @@ __device__ __forceinline__ void nv_unpack2(uint32_t w, float& lo, float& hi)
     }
 }
 
-// 16 consecutive elements from a 16-byte aligned address, read once.
-template <int SRC>
-__device__ __forceinline__ void nv_load16(const void* ptr, float (&x)[16])
+// 32 bytes in one access (32-byte aligned): a warp's accesses are then whole lines. With two of 16 bytes each covers
+// half of every sector (dequantising 16384 x 8192 to bf16 took 92 us that way).
+__device__ __forceinline__ void nv_ld32(const void* ptr, uint4& a, uint4& b)
 {
-    const uint4* p = static_cast<const uint4*>(ptr);
-    if constexpr (SRC == NV_F32) {
+    asm volatile("ld.global.nc.L1::no_allocate.v8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
+                 : "=r"(a.x), "=r"(a.y), "=r"(a.z), "=r"(a.w), "=r"(b.x), "=r"(b.y), "=r"(b.z), "=r"(b.w)
+                 : "l"(ptr));
+}
+
+__device__ __forceinline__ void nv_st32(void* ptr, const uint4& a, const uint4& b)
+{
+    asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(ptr), "r"(a.x), "r"(a.y), "r"(a.z),
+                 "r"(a.w), "r"(b.x), "r"(b.y), "r"(b.z), "r"(b.w)
+                 : "memory");
+}
+
+// 16 consecutive elements, read once, as they lie in memory. VEC: what the address is a multiple of, 32 or 16 bytes.
+template <int SRC>
+struct NvRaw16 {
+    static constexpr int kQuads = SRC == NV_F32 ? 4 : 2;
+    uint4 q[kQuads];
+
+    template <int VEC>
+    __device__ __forceinline__ void load(const void* ptr)
+    {
+        if constexpr (VEC == 32) {
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const uint4 v = __ldcs(p + i);
-            x[4 * i + 0] = __uint_as_float(v.x);
-            x[4 * i + 1] = __uint_as_float(v.y);
-            x[4 * i + 2] = __uint_as_float(v.z);
-            x[4 * i + 3] = __uint_as_float(v.w);
-        }
-    } else {
+            for (int i = 0; i < kQuads; i += 2) {
+                nv_ld32(static_cast<const uint4*>(ptr) + i, q[i], q[i + 1]);
+            }
+        } else {
 #pragma unroll
-        for (int i = 0; i < 2; ++i) {
-            const uint4 v = __ldcs(p + i);
-            nv_unpack2<SRC>(v.x, x[8 * i + 0], x[8 * i + 1]);
-            nv_unpack2<SRC>(v.y, x[8 * i + 2], x[8 * i + 3]);
-            nv_unpack2<SRC>(v.z, x[8 * i + 4], x[8 * i + 5]);
-            nv_unpack2<SRC>(v.w, x[8 * i + 6], x[8 * i + 7]);
+            for (int i = 0; i < kQuads; ++i) {
+                q[i] = __ldcs(static_cast<const uint4*>(ptr) + i);
+            }
         }
     }
-}
+    __device__ __forceinline__ void load_some(const typename NvElem<SRC>::type* p, int n) // the first n, zeros behind
+    {
+        __align__(16) typename NvElem<SRC>::type part[16];
+#pragma unroll
+        for (int j = 0; j < 16; ++j) {
+            part[j] = j < n ? p[j] : static_cast<typename NvElem<SRC>::type>(0.0f);
+        }
+#pragma unroll
+        for (int i = 0; i < kQuads; ++i) {
+            q[i] = reinterpret_cast<const uint4*>(part)[i];
+        }
+    }
+    __device__ __forceinline__ void zero()
+    {
+#pragma unroll
+        for (int i = 0; i < kQuads; ++i) {
+            q[i] = make_uint4(0u, 0u, 0u, 0u);
+        }
+    }
+    __device__ __forceinline__ uint32_t word(int i) const
+    {
+        const uint4& v = q[i / 4];
+        return (i & 3) == 0 ? v.x : (i & 3) == 1 ? v.y : (i & 3) == 2 ? v.z : v.w;
+    }
+    __device__ __forceinline__ void unpack(float (&x)[16]) const
+    {
+#pragma unroll
+        for (int i = 0; i < 4 * kQuads; ++i) {
+            if constexpr (SRC == NV_F32) {
+                x[i] = __uint_as_float(word(i));
+            } else {
+                nv_unpack2<SRC>(word(i), x[2 * i], x[2 * i + 1]);
+            }
+        }
+    }
+    // The largest magnitude as an fp32 pattern; an infinity or a NaN among the values gives a pattern of at least 0x7F800000.
+    __device__ __forceinline__ uint32_t top() const
+    {
+        if constexpr (SRC == NV_F32) {
+            uint32_t t = 0u;
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+                t = max(t, word(i) & 0x7FFFFFFFu);
+            }
+            return t;
+        } else if constexpr (SRC == NV_BF16) {
+            __nv_bfloat162 t = __floats2bfloat162_rn(0.0f, 0.0f);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                const uint32_t w = word(i);
+                t = __hmax2_nan(t, __habs2(*reinterpret_cast<const __nv_bfloat162*>(&w)));
+            }
+            const uint32_t w = *reinterpret_cast<const uint32_t*>(&t) & 0x7FFF7FFFu;
+            return max(w << 16, w & 0xFFFF0000u);
+        } else {
+            __half2 t = __floats2half2_rn(0.0f, 0.0f);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                const uint32_t w = word(i);
+                t = __hmax2_nan(t, __habs2(*reinterpret_cast<const __half2*>(&w)));
+            }
+            const float2 f = __half22float2(t);
+            return max(__float_as_uint(f.x) & 0x7FFFFFFFu, __float_as_uint(f.y) & 0x7FFFFFFFu);
+        }
+    }
+};
 
 // Exponent field of g for a tensor maximum: amax / 2688 rounded up to a power of two, 2688 = 1.3125 * 2^11.
 __device__ __forceinline__ uint32_t nv_scale_exponent(float amax)
@@ -128,48 +206,90 @@ __device__ __forceinline__ uint32_t nv_cvt_e2m1x8(const float* q)
     return r;
 }
 
-// One block: its e4m3 scale code and its sixteen codes.
-__device__ __forceinline__ uint32_t nv_quantize_block(float (&x)[16], float inv_g, uint2& codes)
+__device__ __forceinline__ uint64_t nv_pair(float lo, float hi)
 {
-    uint32_t top = 0u; // |x| as bits: the integer order is the value order, infinities and NaN above all numbers
-#pragma unroll
-    for (int i = 0; i < 16; ++i) {
-        top = max(top, __float_as_uint(x[i]) & 0x7FFFFFFFu);
+    uint64_t r;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(lo), "f"(hi));
+    return r;
+}
+
+__device__ __forceinline__ uint64_t nv_fma2(uint64_t a, uint64_t b, uint64_t c)
+{
+    uint64_t r;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+    return r;
+}
+
+__device__ __forceinline__ uint64_t nv_mul2(uint64_t a, uint64_t b)
+{
+    uint64_t r;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
+
+// What every block of a tensor needs of its scale g = 2^(e - 127).
+struct NvTensorScale {
+    uint32_t e;
+    float g, inv_g;
+    bool plain; // s g and 1 / (s g) are normal numbers for every block scale s
+
+    __device__ __forceinline__ explicit NvTensorScale(float amax)
+    {
+        e = nv_scale_exponent(amax);
+        g = __uint_as_float(e << 23);
+        inv_g = __uint_as_float((254u - e) << 23);
+        plain = e >= 24u && e <= 230u;
     }
+};
+
+// One block with its largest magnitude `top` (an fp32 pattern): its e4m3 scale code and its sixteen codes.
+// x / (s g) is rounded correctly: a quotient from the reciprocal, then one correction by its exact remainder. (s g has
+// four significant bits; the product with the reciprocal alone misses ties by one unit, and 1/16 of all bf16 quotients
+// are ties.)
+__device__ __forceinline__ uint32_t nv_quantize_block(float (&x)[16], uint32_t top, const NvTensorScale& t, uint2& codes)
+{
     codes = make_uint2(0u, 0u);
     if (top >= 0x7F800000u) {
         return 0x7Fu;
     }
-    const float y_max = __uint_as_float(top) * inv_g;
-    const uint32_t s_code =
-        __nv_cvt_float_to_fp8(fminf(__fdiv_rn(y_max, 6.0f), 448.0f), __NV_SATFINITE, __NV_E4M3);
+    const float y_max = __uint_as_float(top) * t.inv_g;
+    const uint32_t s_code = __nv_cvt_float_to_fp8(fminf(__fdiv_rn(y_max, 6.0f), 448.0f), __NV_SATFINITE, __NV_E4M3);
     if (s_code == 0u) {
         return 0u;
     }
     const float s = nv_e4m3_to_float(s_code);
     const float r = __frcp_rn(s);
-    if (y_max > 1.0e30f) { // only with a caller's amax far below the data: keeps the quotients finite
+    if (t.plain && y_max <= 1.0e30f) {
+        const float ri = r * t.inv_g, sg = -s * t.g; // powers of two: exact
+        const uint64_t ri2 = nv_pair(ri, ri), sg2 = nv_pair(sg, sg);
+#pragma unroll
+        for (int i = 0; i < 16; i += 2) {
+            const uint64_t v = nv_pair(x[i], x[i + 1]);
+            const uint64_t q0 = nv_mul2(v, ri2);
+            const uint64_t q = nv_fma2(nv_fma2(q0, sg2, v), ri2, q0);
+            asm("mov.b64 {%0, %1}, %2;" : "=f"(x[i]), "=f"(x[i + 1]) : "l"(q));
+        }
+    } else { // a tensor near either end of fp32's range, or a caller's amax far below the data: one step more, clamped
 #pragma unroll
         for (int i = 0; i < 16; ++i) {
-            x[i] = fminf(fmaxf(x[i] * inv_g, -8192.0f), 8192.0f);
+            const float y = fminf(fmaxf(x[i] * t.inv_g, -8192.0f), 8192.0f);
+            const float q0 = __fmul_rn(y, r);
+            x[i] = __fmaf_rn(__fmaf_rn(-q0, s, y), r, q0);
         }
-    } else {
-#pragma unroll
-        for (int i = 0; i < 16; ++i) {
-            x[i] *= inv_g;
-        }
-    }
-    // x / s rounded correctly: a quotient from the reciprocal, then one correction by its exact remainder. (s has four
-    // significant bits; the product alone misses ties by one unit and 1/16 of all bf16 quotients are ties.)
-#pragma unroll
-    for (int i = 0; i < 16; ++i) {
-        const float q0 = __fmul_rn(x[i], r);
-        const float rem = __fmaf_rn(-q0, s, x[i]);
-        x[i] = __fmaf_rn(rem, r, q0);
     }
     codes.x = nv_cvt_e2m1x8(x);
     codes.y = nv_cvt_e2m1x8(x + 8);
     return s_code;
+}
+
+__device__ __forceinline__ uint32_t nv_top(const float (&x)[16])
+{
+    uint32_t t = 0u; // |x| as bits: the integer order is the value order, infinities and NaN above all numbers
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+        t = max(t, __float_as_uint(x[i]) & 0x7FFFFFFFu);
+    }
+    return t;
 }
 
 // Stores a block's codes and, once per four lanes, the scale word of four consecutive blocks. The four lanes of an
@@ -190,8 +310,11 @@ __device__ __forceinline__ void nv_store_block(uint8_t* data, uint8_t* scales, l
     }
 }
 
-// src: [rows][ld_src]; VEC: rows start on 16-byte boundaries. One thread per block of 16 and step.
-template <int SRC, bool VEC>
+// src: [rows][ld_src]; VEC: rows start on 32- or 16-byte boundaries, 0: on any element. One thread per block of 16 and
+// step, two blocks in flight.
+constexpr int kNvItems = 2;
+
+template <int SRC, int VEC>
 __global__ void __launch_bounds__(kNvQuantThreads)
     nvfp4_quantize_kernel(const void* __restrict__ src, const float* __restrict__ amax, uint8_t* __restrict__ data,
                           uint8_t* __restrict__ scales, float* __restrict__ tensor_scale, int rows, int k,
@@ -204,118 +327,142 @@ __global__ void __launch_bounds__(kNvQuantThreads)
     const long long rows_padded = (static_cast<long long>(rows) + 127) / 128 * 128;
     const long long total = rows_padded * row_blocks;  // a multiple of 4, as the stride is: groups of four stay whole
     const long long stride = static_cast<long long>(gridDim.x) * blockDim.x;
-    const uint32_t e = nv_scale_exponent(__ldg(amax));
-    const float inv_g = __uint_as_float((254u - e) << 23);
-    if (blockIdx.x == 0 && threadIdx.x == 0) {
-        *tensor_scale = __uint_as_float(e << 23);
-    }
     long long i = blockIdx.x * static_cast<long long>(blockDim.x) + threadIdx.x;
     const long long row_step = stride / row_blocks;
     const int kb_step = static_cast<int>(stride - row_step * row_blocks);
     long long row = i / row_blocks;
     int kb = static_cast<int>(i - row * row_blocks);
-    for (; i < total; i += stride) {
-        uint32_t s_code = 0u;
-        uint2 codes = make_uint2(0u, 0u);
-        if (row < rows && kb < k_blocks) {
-            float x[16];
-            const T* p = static_cast<const T*>(src) + row * ld_src + static_cast<long long>(kb) * 16;
-            if (VEC && kb * 16 + 16 <= k) {
-                nv_load16<SRC>(p, x);
-            } else {
+    const NvTensorScale t(__ldg(amax));
+    if (blockIdx.x == 0 && threadIdx.x == 0) {
+        *tensor_scale = t.g;
+    }
+    while (i < total) {
+        NvRaw16<SRC> raw[kNvItems];
+        int rows_of[kNvItems], kbs[kNvItems];
 #pragma unroll
-                for (int j = 0; j < 16; ++j) {
-                    x[j] = (kb * 16 + j < k) ? nv_to_float<SRC>(p[j]) : 0.0f;
+        for (int u = 0; u < kNvItems; ++u) {
+            rows_of[u] = i < total ? static_cast<int>(row) : -1;
+            kbs[u] = kb;
+            raw[u].zero();
+            if (i < total && row < rows && kb < k_blocks) {
+                const T* p = static_cast<const T*>(src) + row * ld_src + static_cast<long long>(kb) * 16;
+                if (VEC != 0 && kb * 16 + 16 <= k) {
+                    raw[u].template load<VEC>(p);
+                } else {
+                    raw[u].load_some(p, k - kb * 16);
                 }
             }
-            s_code = nv_quantize_block(x, inv_g, codes);
+            i += stride;
+            row += row_step;
+            kb += kb_step;
+            if (kb >= row_blocks) {
+                kb -= row_blocks;
+                row += 1;
+            }
         }
-        nv_store_block(data, scales, ld_data, rows, k_blocks, k_atoms, static_cast<int>(row), kb, s_code, codes);
-        row += row_step;
-        kb += kb_step;
-        if (kb >= row_blocks) {
-            kb -= row_blocks;
-            row += 1;
+#pragma unroll
+        for (int u = 0; u < kNvItems; ++u) {
+            if (rows_of[u] >= 0) { // the same for the four lanes of a group
+                float x[16];
+                raw[u].unpack(x);
+                uint2 codes;
+                const uint32_t s_code = nv_quantize_block(x, raw[u].top(), t, codes);
+                nv_store_block(data, scales, ld_data, rows, k_blocks, k_atoms, rows_of[u], kbs[u], s_code, codes);
+            }
         }
     }
 }
 
 // The same of the transpose: blocks run down the columns of src [rows][ld_src], row c of the result is column c of src.
-// A thread block takes 256 rows x 64 columns through shared memory; sixteen lanes then hold the sixteen blocks of one
-// column, so a column's codes leave as 128 contiguous bytes. 16-row groups are skewed by two words, which puts the
-// sixteen lanes (16 rows apart) and the two columns of a warp on different banks.
-constexpr int kNvTransRows = 256;
-constexpr int kNvTransCols = 64;
-
-template <int SRC>
-inline constexpr int kNvTransGroupBytes = 16 * kNvTransCols * static_cast<int>(sizeof(typename NvElem<SRC>::type)) + 8;
-
-template <int SRC, bool VEC>
+// A thread takes one column (two for 16-bit types with PAIRS: rows start on 4-byte boundaries) down 64 rows: loads are
+// contiguous across the lanes, the codes of its four blocks are one 32-byte sector and their scales one word of a scale
+// tile, so nothing is exchanged and nothing goes through shared memory. Columns past k fill the padding with zeros.
+// (Through a shared-memory tile of 256 x 64: 118 us for bf16 and 249 us for fp32 on 16384 x 8192.)
+template <int SRC, bool PAIRS>
 __global__ void __launch_bounds__(kNvQuantThreads)
     nvfp4_quantize_transposed_kernel(const void* __restrict__ src, const float* __restrict__ amax,
                                      uint8_t* __restrict__ data, uint8_t* __restrict__ scales,
                                      float* __restrict__ tensor_scale, int rows, int k, long long ld_src, long long ld_data)
 {
     using T = typename NvElem<SRC>::type;
-    extern __shared__ uint2 nv_trans_smem[];
-    uint8_t* tile = reinterpret_cast<uint8_t*>(nv_trans_smem);
-    constexpr int kGroupBytes = kNvTransGroupBytes<SRC>;
-    const int k_blocks = (rows + 15) / 16; // the result's rows run over src's rows
-    const int k_atoms = (k_blocks + 3) / 4;
-    const int row0 = static_cast<int>(blockIdx.x) * kNvTransRows;
-    const int col0 = static_cast<int>(blockIdx.y) * kNvTransCols;
-    const uint32_t e = nv_scale_exponent(__ldg(amax));
-    const float inv_g = __uint_as_float((254u - e) << 23);
-    if (blockIdx.x == 0 && blockIdx.y == 0 && threadIdx.x == 0) {
-        *tensor_scale = __uint_as_float(e << 23);
+    constexpr int kCols = PAIRS ? 2 : 1;
+    const int k_atoms = (rows + 63) / 64; // the result's rows run over src's rows
+    const int col_items = (k + 127) / 128 * (128 / kCols);
+    const long long total = static_cast<long long>(k_atoms) * col_items;
+    const bool wide = (reinterpret_cast<uintptr_t>(data) & 31u) == 0 && (ld_data & 31) == 0;
+    const NvTensorScale t(__ldg(amax));
+    if (blockIdx.x == 0 && threadIdx.x == 0) {
+        *tensor_scale = t.g;
     }
-    const T* base = static_cast<const T*>(src);
-    constexpr int kPer16 = 16 / static_cast<int>(sizeof(T));   // elements of a 16-byte load
-    constexpr int kLoads = kNvTransCols / kPer16;              // of a row
-#pragma unroll 4
-    for (int it = threadIdx.x; it < kNvTransRows * kLoads; it += kNvQuantThreads) {
-        const int r = it / kLoads;
-        const int c = (it % kLoads) * kPer16;
-        uint4 v = make_uint4(0u, 0u, 0u, 0u);
-        if (row0 + r < rows) {
-            const T* p = base + (row0 + r) * ld_src + col0 + c;
-            if (VEC && col0 + c + kPer16 <= k) {
-                v = __ldcs(reinterpret_cast<const uint4*>(p));
-            } else {
-                __align__(16) T part[kPer16];
+    for (long long it = blockIdx.x * static_cast<long long>(blockDim.x) + threadIdx.x; it < total;
+         it += static_cast<long long>(gridDim.x) * blockDim.x) {
+        const int atom = static_cast<int>(it / col_items);
+        const int col = static_cast<int>(it - static_cast<long long>(atom) * col_items) * kCols;
+        const int row0 = atom * 64;
+        const int blocks = min(4, (rows - row0 + 15) / 16);
+        const bool full = row0 + 64 <= rows && col + kCols <= k;
+        uint2 codes[kCols][4];
+        uint32_t word[kCols];
 #pragma unroll
-                for (int j = 0; j < kPer16; ++j) {
-                    part[j] = (col0 + c + j < k) ? p[j] : static_cast<T>(0.0f);
+        for (int c = 0; c < kCols; ++c) {
+            word[c] = 0u;
+        }
+        const T* p = static_cast<const T*>(src) + static_cast<long long>(row0) * ld_src + col;
+#pragma unroll
+        for (int b = 0; b < 4; ++b) {
+            float x[kCols][16];
+            if (full) { // sixteen loads in flight
+#pragma unroll
+                for (int j = 0; j < 16; ++j) {
+                    const T* at = p + static_cast<long long>(b * 16 + j) * ld_src;
+                    if constexpr (PAIRS) {
+                        nv_unpack2<SRC>(__ldcs(reinterpret_cast<const uint32_t*>(at)), x[0][j], x[1][j]);
+                    } else {
+                        x[0][j] = nv_to_float<SRC>(*at);
+                    }
                 }
-                v = *reinterpret_cast<const uint4*>(part);
+            } else {
+#pragma unroll
+                for (int j = 0; j < 16; ++j) {
+#pragma unroll
+                    for (int c = 0; c < kCols; ++c) {
+                        x[c][j] = 0.0f;
+                        if (row0 + b * 16 + j < rows && col + c < k) {
+                            x[c][j] = nv_to_float<SRC>(p[static_cast<long long>(b * 16 + j) * ld_src + c]);
+                        }
+                    }
+                }
+            }
+#pragma unroll
+            for (int c = 0; c < kCols; ++c) {
+                word[c] |= nv_quantize_block(x[c], nv_top(x[c]), t, codes[c][b]) << (8 * b);
             }
         }
-        uint2* dst = reinterpret_cast<uint2*>(tile + (r >> 4) * kGroupBytes +
-                                              ((r & 15) * kNvTransCols + c) * static_cast<int>(sizeof(T)));
-        dst[0] = make_uint2(v.x, v.y);
-        dst[1] = make_uint2(v.z, v.w);
-    }
-    __syncthreads();
-    const int b = threadIdx.x & 15;
-    const int kb = row0 / 16 + b;
-    if (kb >= k_atoms * 4) { // whole groups of four lanes leave together
-        return;
-    }
-    for (int c = threadIdx.x >> 4; c < kNvTransCols; c += kNvQuantThreads / 16) {
-        float x[16];
-        const T* col = reinterpret_cast<const T*>(tile + b * kGroupBytes) + c;
 #pragma unroll
-        for (int j = 0; j < 16; ++j) {
-            x[j] = nv_to_float<SRC>(col[j * kNvTransCols]);
+        for (int c = 0; c < kCols; ++c) {
+            const int out_row = col + c;
+            if (out_row < k) {
+                uint8_t* dst = data + out_row * ld_data + static_cast<long long>(atom) * 32;
+                if (wide && blocks == 4) {
+                    nv_st32(dst, make_uint4(codes[c][0].x, codes[c][0].y, codes[c][1].x, codes[c][1].y),
+                            make_uint4(codes[c][2].x, codes[c][2].y, codes[c][3].x, codes[c][3].y));
+                } else {
+#pragma unroll
+                    for (int b = 0; b < 4; ++b) {
+                        if (b < blocks) {
+                            reinterpret_cast<uint2*>(dst)[b] = codes[c][b];
+                        }
+                    }
+                }
+            }
+            const long long tile = static_cast<long long>(out_row >> 7) * k_atoms + atom;
+            *reinterpret_cast<uint32_t*>(scales + tile * 512 + (out_row & 31) * 16 + ((out_row >> 5) & 3) * 4) = word[c];
         }
-        uint2 codes;
-        const uint32_t s_code = nv_quantize_block(x, inv_g, codes);
-        nv_store_block(data, scales, ld_data, k, k_blocks, k_atoms, col0 + c, kb, s_code, codes);
     }
 }
 
 // Largest finite |x| of a matrix into *out, which the caller has set to zero. The maximum does not depend on the order.
-template <int SRC, bool VEC>
+template <int SRC, int VEC>
 __global__ void __launch_bounds__(kNvQuantThreads)
     amax_kernel(const void* __restrict__ src, uint32_t* __restrict__ out, int rows, int k, long long ld_src)
 {
@@ -331,15 +478,14 @@ __global__ void __launch_bounds__(kNvQuantThreads)
     uint32_t top = 0u;
     for (; i < total; i += stride) {
         const T* p = static_cast<const T*>(src) + row * ld_src + static_cast<long long>(c) * 16;
-        float x[16];
-        if (VEC && c * 16 + 16 <= k) {
-            nv_load16<SRC>(p, x);
+        NvRaw16<SRC> raw;
+        if (VEC != 0 && c * 16 + 16 <= k) {
+            raw.template load<VEC>(p);
         } else {
-#pragma unroll
-            for (int j = 0; j < 16; ++j) {
-                x[j] = (c * 16 + j < k) ? nv_to_float<SRC>(p[j]) : 0.0f;
-            }
+            raw.load_some(p, k - c * 16);
         }
+        float x[16];
+        raw.unpack(x);
 #pragma unroll
         for (int j = 0; j < 16; ++j) {
             const uint32_t bits = __float_as_uint(x[j]) & 0x7FFFFFFFu;
@@ -366,8 +512,8 @@ __global__ void __launch_bounds__(kNvQuantThreads)
     }
 }
 
-// Two e2m1 codes (a byte) -> two floats.
-__device__ __forceinline__ float2 nv_e2m1x2_to_float2(uint32_t byte)
+// Two e2m1 codes (a byte) -> two halves.
+__device__ __forceinline__ __half2 nv_e2m1x2_to_half2(uint32_t byte)
 {
     uint32_t h;
     asm("{\n\t"
@@ -377,11 +523,12 @@ __device__ __forceinline__ float2 nv_e2m1x2_to_float2(uint32_t byte)
         "}"
         : "=r"(h)
         : "r"(byte));
-    return __half22float2(*reinterpret_cast<const __half2*>(&h));
+    return *reinterpret_cast<const __half2*>(&h);
 }
 
-// Back to numbers: (code * s) is exact, one rounding by g (none when g is a power of two), one by the output type.
-// One thread per eight elements: four bytes in, 16 or 32 contiguous bytes out.
+// Back to numbers: code * s is exact in fp16 (six significant bits, at most 2688 and at least 2^-10), then one rounding by
+// g (none when g is a power of two) and one by the output type. One thread per 32 bytes of the result - 8 or 16
+// elements - two of them in flight. VEC: the result's rows start on 32-byte boundaries.
 template <int DST, bool VEC>
 __global__ void __launch_bounds__(kNvQuantThreads)
     nvfp4_dequantize_kernel(const uint8_t* __restrict__ data, const uint8_t* __restrict__ scales,
@@ -389,53 +536,70 @@ __global__ void __launch_bounds__(kNvQuantThreads)
                             long long ld_data, long long ld_out)
 {
     using T = typename NvElem<DST>::type;
-    const int items_per_row = (k + 7) / 8;
+    constexpr int kElems = 32 / static_cast<int>(sizeof(T));
+    constexpr int kWords = kElems / 8;
+    const int row_items = (k + kElems - 1) / kElems;
     const int k_atoms = (k + 63) / 64;
     const float g = tensor_scale != nullptr ? __ldg(tensor_scale) : 1.0f;
-    const long long total = static_cast<long long>(rows) * items_per_row;
+    const long long total = static_cast<long long>(rows) * row_items;
     const long long stride = static_cast<long long>(gridDim.x) * blockDim.x;
     long long i = blockIdx.x * static_cast<long long>(blockDim.x) + threadIdx.x;
-    const long long row_step = stride / items_per_row;
-    const int c_step = static_cast<int>(stride - row_step * items_per_row);
-    long long row = i / items_per_row;
-    int c = static_cast<int>(i - row * items_per_row);
-    for (; i < total; i += stride) {
-        const uint32_t codes = __ldcs(reinterpret_cast<const uint32_t*>(data + row * ld_data + static_cast<long long>(c) * 4));
-        const int kb = c >> 1;
-        const long long tile = (row >> 7) * k_atoms + (kb >> 2);
-        const float s = nv_e4m3_to_float(__ldg(scales + tile * 512 + (row & 31) * 16 + ((row >> 5) & 3) * 4 + (kb & 3)));
-        float v[8];
+    const long long row_step = stride / row_items;
+    const int c_step = static_cast<int>(stride - row_step * row_items);
+    long long row = i / row_items;
+    int c = static_cast<int>(i - row * row_items);
+    while (i < total) {
+        uint32_t codes[kNvItems][kWords], s_code[kNvItems];
+        long long rows_of[kNvItems];
+        int cs[kNvItems];
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            const float2 f = nv_e2m1x2_to_float2((codes >> (8 * j)) & 0xFFu);
-            v[2 * j] = __fmul_rn(__fmul_rn(f.x, s), g);
-            v[2 * j + 1] = __fmul_rn(__fmul_rn(f.y, s), g);
-        }
-        T* dst = static_cast<T*>(out) + row * ld_out + static_cast<long long>(c) * 8;
-        __align__(16) T o[8];
+        for (int u = 0; u < kNvItems; ++u) {
+            rows_of[u] = -1;
+            if (i < total) {
+                rows_of[u] = row;
+                cs[u] = c;
+                const uint32_t* p = reinterpret_cast<const uint32_t*>(data + row * ld_data) + static_cast<long long>(c) * kWords;
 #pragma unroll
-        for (int j = 0; j < 8; ++j) {
-            o[j] = static_cast<T>(v[j]);
-        }
-        if (VEC && c * 8 + 8 <= k) {
-            constexpr int kQuads = 8 * static_cast<int>(sizeof(T)) / 16;
-#pragma unroll
-            for (int j = 0; j < kQuads; ++j) {
-                reinterpret_cast<uint4*>(dst)[j] = reinterpret_cast<const uint4*>(o)[j];
+                for (int w = 0; w < kWords; ++w) {
+                    codes[u][w] = c * kElems + 8 * w < k ? __ldcs(p + w) : 0u;
+                }
+                const int kb = c * kElems / 16;
+                const long long tile = (row >> 7) * k_atoms + (kb >> 2);
+                s_code[u] = __ldg(scales + tile * 512 + (row & 31) * 16 + ((row >> 5) & 3) * 4 + (kb & 3));
             }
-        } else {
+            i += stride;
+            row += row_step;
+            c += c_step;
+            if (c >= row_items) {
+                c -= row_items;
+                row += 1;
+            }
+        }
 #pragma unroll
-            for (int j = 0; j < 8; ++j) {
-                if (c * 8 + j < k) {
-                    dst[j] = o[j];
+        for (int u = 0; u < kNvItems; ++u) {
+            if (rows_of[u] < 0) {
+                continue;
+            }
+            const __half_raw sr = __nv_cvt_fp8_to_halfraw(static_cast<__nv_fp8_storage_t>(s_code[u]), __NV_E4M3);
+            const __half2 s = __half2half2(*reinterpret_cast<const __half*>(&sr));
+            __align__(16) T o[kElems];
+#pragma unroll
+            for (int j = 0; j < kElems / 2; ++j) {
+                const float2 f = __half22float2(__hmul2(nv_e2m1x2_to_half2((codes[u][j / 4] >> (8 * (j & 3))) & 0xFFu), s));
+                o[2 * j] = static_cast<T>(__fmul_rn(f.x, g));
+                o[2 * j + 1] = static_cast<T>(__fmul_rn(f.y, g));
+            }
+            T* dst = static_cast<T*>(out) + rows_of[u] * ld_out + static_cast<long long>(cs[u]) * kElems;
+            if (VEC && cs[u] * kElems + kElems <= k) {
+                nv_st32(dst, reinterpret_cast<const uint4*>(o)[0], reinterpret_cast<const uint4*>(o)[1]);
+            } else {
+#pragma unroll
+                for (int j = 0; j < kElems; ++j) {
+                    if (cs[u] * kElems + j < k) {
+                        dst[j] = o[j];
+                    }
                 }
             }
-        }
-        row += row_step;
-        c += c_step;
-        if (c >= items_per_row) {
-            c -= items_per_row;
-            row += 1;
         }
     }
 }
