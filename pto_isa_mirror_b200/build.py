@@ -19,9 +19,11 @@ _ABI = os.path.join("..", "..", "include", "pto_b200.h")
 # source -> the headers it includes
 SOURCES = {
     "pto_b200_capi.cu": ["capi_shared.cuh", "gemm_tile_loop.cuh", "gemm_tile_loop_2cta.cuh", "gemv.cuh", "gemv_mx.cuh",
-                         "ksplit_reduce.cuh", "mx_quantize.cuh", "sm100_ptx.cuh", _ABI],
-    "nvfp4_capi.cu": ["capi_shared.cuh", "gemm_tile_loop.cuh", "gemm_nvfp4.cuh", "nvfp4_quantize.cuh", "sm100_ptx.cuh", _ABI],
-    "checkpoint_capi.cu": ["capi_shared.cuh", "gemm_tile_loop.cuh", "gemm_wgrad_mx.cuh", "mx_quantize.cuh", "sm100_ptx.cuh", _ABI],
+                         "ksplit_reduce.cuh", "mx_quantize.cuh", "row_elements.cuh", "sm100_ptx.cuh", _ABI],
+    "nvfp4_capi.cu": ["capi_shared.cuh", "gemm_tile_loop.cuh", "gemm_nvfp4.cuh", "nvfp4_quantize.cuh", "row_elements.cuh", "sm100_ptx.cuh",
+                       _ABI],
+    "checkpoint_capi.cu": ["capi_shared.cuh", "gemm_tile_loop.cuh", "gemm_wgrad_mx.cuh", "mx_quantize.cuh",
+                           "row_elements.cuh", "sm100_ptx.cuh", _ABI],
 }
 
 NVCC_FLAGS = [

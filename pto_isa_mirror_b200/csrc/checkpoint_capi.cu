@@ -11,22 +11,36 @@ namespace {
 
 bool misaligned(const void* p, unsigned bytes) { return (reinterpret_cast<uintptr_t>(p) & (bytes - 1u)) != 0; }
 
-template <int ALG, bool F16>
-int launch_quantize16(cudaStream_t s, int sm_count, const uint8_t* src, uint8_t* data, uint8_t* scales, int rows, int k,
-                      long long ld_src, long long ld_data, long long ld_scales)
+template <int ALG, int SRC, int VEC>
+int launch_quantize16(cudaStream_t s, const HostContext& host, const uint8_t* src, uint8_t* data, uint8_t* scales, int rows,
+                      int k, long long ld_src, long long ld_data, long long ld_scales)
 {
-    auto kernel = mx_quantize_e4m3_16bit_kernel<ALG, F16>;
-    int per_sm = 0;
-    if (int rc = note_cuda_error(cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per_sm, kernel, kQuantThreads, 0),
-                                 "mx_quantize occupancy")) {
-        return rc;
+    auto kernel = mx_quantize_e4m3_16bit_kernel<ALG, SRC, VEC>;
+    static std::atomic<int> blocks_per_sm[kMaxDevices];
+    int per_sm = blocks_per_sm[host.device].load(std::memory_order_relaxed);
+    if (per_sm == 0) {
+        if (int rc = note_cuda_error(cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per_sm, kernel, kQuantThreads, 0),
+                                     "mx_quantize occupancy")) {
+            return rc;
+        }
+        per_sm = per_sm > 0 ? per_sm : 1;
+        blocks_per_sm[host.device].store(per_sm, std::memory_order_relaxed);
     }
-    const long long want = (static_cast<long long>(rows) * (k / 8) + kQuantThreads - 1) / kQuantThreads;
-    const long long cap = static_cast<long long>(sm_count) * (per_sm > 0 ? per_sm : 1); // one resident wave
+    const long long want = (static_cast<long long>(rows) * (k / 16) + kQuantThreads - 1) / kQuantThreads;
+    const long long cap = static_cast<long long>(host.sm_count) * per_sm; // one resident wave
     const int grid = static_cast<int>(want < cap ? want : cap);
     kernel<<<grid, kQuantThreads, 0, s>>>(reinterpret_cast<const uint16_t*>(src), data, scales, rows, k, ld_src, ld_data, ld_scales);
     count_launches(1);
     return note_cuda_error(cudaGetLastError(), "mx_quantize (16-bit) launch");
+}
+
+template <int ALG, int SRC>
+int launch_quantize16_any(cudaStream_t s, const HostContext& host, const uint8_t* src, uint8_t* data, uint8_t* scales, int rows,
+                          int k, long long ld_src, long long ld_data, long long ld_scales)
+{
+    return !misaligned(src, 32) && ld_src % 16 == 0
+               ? launch_quantize16<ALG, SRC, 32>(s, host, src, data, scales, rows, k, ld_src, ld_data, ld_scales)
+               : launch_quantize16<ALG, SRC, 16>(s, host, src, data, scales, rows, k, ld_src, ld_data, ld_scales);
 }
 
 template <bool F16, int OUT>
@@ -116,9 +130,9 @@ extern "C" int pto_b200_mx_quantize_e4m3_src(void* stream, uint8_t* data, uint8_
     }
     cudaStream_t s = static_cast<cudaStream_t>(stream);
     const bool f16 = src_dtype == PTO_B200_F16, nv = scale_alg == PTO_B200_SCALE_NV;
-    auto launch = nv ? (f16 ? launch_quantize16<MX_SCALE_NV, true> : launch_quantize16<MX_SCALE_NV, false>)
-                     : (f16 ? launch_quantize16<MX_SCALE_OCP, true> : launch_quantize16<MX_SCALE_OCP, false>);
-    return launch(s, host.sm_count, src, data, scales, rows, k, ld_src, ld_data, ld_scales);
+    auto launch = nv ? (f16 ? launch_quantize16_any<MX_SCALE_NV, NV_F16> : launch_quantize16_any<MX_SCALE_NV, NV_BF16>)
+                     : (f16 ? launch_quantize16_any<MX_SCALE_OCP, NV_F16> : launch_quantize16_any<MX_SCALE_OCP, NV_BF16>);
+    return launch(s, host, src, data, scales, rows, k, ld_src, ld_data, ld_scales);
 }
 
 extern "C" int pto_b200_gemm_wgrad_mx(void* stream, uint8_t* out, const uint8_t* dy, const uint8_t* data, const uint8_t* scales,

@@ -23,6 +23,8 @@
 
 #include <cstdint>
 
+#include "row_elements.cuh"
+
 namespace pto_b200 {
 
 constexpr int kQuantThreads = 256;
@@ -142,89 +144,77 @@ __global__ void __launch_bounds__(kQuantThreads) mx_quantize_e4m3_kernel(const f
     }
 }
 
-// The same from 16-bit rows (bf16, or fp16 with F16): what an activation kept for a backward pass comes as. Every value is
-// a float exactly, so bytes and scales are those of the fp32 kernel on the same numbers. Unlike there, a block with an
+// The same from 16-bit rows (SRC: NV_BF16 or NV_F16): what an activation kept for a backward pass comes as. Every value is a
+// float exactly, so bytes and scales are those of the fp32 kernel on the same numbers. Unlike there, a block with an
 // infinity or a NaN is in the domain: its scale is 255, which e8m0 reads as NaN, and its bytes are zero.
-// Four consecutive lanes own one block of 32 values (16 bytes each) and store 8 bytes each.
-// src: [rows][ld_src] elements (16-byte aligned rows); data: [rows][ld_data] bytes (8-byte aligned rows). k % 32 == 0.
-constexpr int kQuant16Items = 4;
+// Two neighbouring lanes own one block of 32 values, 16 each. HBM-bound: 2 bytes read and 1 + 1/32 written per element.
+// src: [rows][ld_src] elements, rows on VEC = 32- or 16-byte boundaries; data: [rows][ld_data] bytes, rows on 8-byte ones.
+// k % 32 == 0.
+constexpr int kQuant16Items = 2;
 
-template <int ALG, bool F16>
+template <int ALG, int SRC, int VEC>
 __global__ void __launch_bounds__(kQuantThreads) mx_quantize_e4m3_16bit_kernel(const uint16_t* __restrict__ src,
                                                                                 uint8_t* __restrict__ data,
                                                                                 uint8_t* __restrict__ scales, int rows, int k,
                                                                                 long long ld_src, long long ld_data,
                                                                                 long long ld_scales)
 {
-    const int k8 = k / 8;
-    const long long total = static_cast<long long>(rows) * k8; // 16-byte items; a multiple of 4 per row
+    const int row_items = k / 16;
+    const long long total = static_cast<long long>(rows) * row_items; // a multiple of 2 per row, as the stride is
     const long long stride = static_cast<long long>(gridDim.x) * blockDim.x;
-    const unsigned group_mask = 0xFu << (threadIdx.x & 28u);
-    const long long row_step = stride / k8;
-    const int col_step = static_cast<int>(stride - row_step * k8);
+    const bool wide = (reinterpret_cast<uintptr_t>(data) & 15u) == 0 && (ld_data & 15) == 0;
     long long i = blockIdx.x * static_cast<long long>(blockDim.x) + threadIdx.x;
-    long long cur_row = i / k8;
-    int cur_c8 = static_cast<int>(i - cur_row * k8);
-    // total and stride are multiples of 4: the four lanes of a group are all in range or all out of range
-    while (i < total) {
-        uint4 v[kQuant16Items];
+    const long long row_step = stride / row_items;
+    const int c_step = static_cast<int>(stride - row_step * row_items);
+    long long cur_row = i / row_items;
+    int cur_c = static_cast<int>(i - cur_row * row_items);
+    while (i - static_cast<int>(threadIdx.x & 31u) < total) { // the warp goes on together
+        NvRaw16<SRC> raw[kQuant16Items];
         long long row[kQuant16Items];
-        int c8[kQuant16Items];
+        int c[kQuant16Items];
 #pragma unroll
         for (int u = 0; u < kQuant16Items; ++u) {
-            row[u] = -1;
+            row[u] = i < total ? cur_row : -1;
+            c[u] = cur_c;
+            raw[u].zero();
             if (i < total) {
-                row[u] = cur_row;
-                c8[u] = cur_c8;
-                v[u] = __ldcs(reinterpret_cast<const uint4*>(src + cur_row * ld_src) + cur_c8);
+                raw[u].template load<VEC>(src + cur_row * ld_src + static_cast<long long>(cur_c) * 16);
             }
             i += stride;
             cur_row += row_step;
-            cur_c8 += col_step;
-            if (cur_c8 >= k8) {
-                cur_c8 -= k8;
+            cur_c += c_step;
+            if (cur_c >= row_items) {
+                cur_c -= row_items;
                 cur_row += 1;
             }
         }
 #pragma unroll
         for (int u = 0; u < kQuant16Items; ++u) {
-            if (row[u] < 0) {
-                continue;
-            }
-            const uint32_t w[4] = {v[u].x, v[u].y, v[u].z, v[u].w};
-            // the largest magnitude of both halves of the words, as 16-bit patterns: their order is the value order,
-            // infinities and NaN above all numbers
-            uint32_t top = 0u;
-#pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                top = __vmaxu2(top, w[j] & 0x7FFF7FFFu);
-            }
-            top = __vmaxu2(top, __shfl_xor_sync(group_mask, top, 1));
-            top = __vmaxu2(top, __shfl_xor_sync(group_mask, top, 2));
-            top = max(top & 0xFFFFu, top >> 16);
-            const bool finite = top < (F16 ? 0x7C00u : 0x7F80u);
-            const float amax = F16 ? __half2float(__ushort_as_half(static_cast<unsigned short>(top))) : __uint_as_float(top << 16);
-            const uint32_t e8m0 = finite ? mx_e4m3_exponent<ALG>(amax) : 255u;
+            uint32_t top = raw[u].top();
+            top = max(top, __shfl_xor_sync(0xFFFFFFFFu, top, 1));
+            const bool finite = top < 0x7F800000u;
+            const uint32_t e8m0 = finite ? mx_e4m3_exponent<ALG>(__uint_as_float(top)) : 255u;
             const float scaling = __uint_as_float((254u - (finite ? e8m0 : 0u)) << 23);
-            float y[8];
+            float x[16];
+            raw[u].unpack(x);
+            uint32_t o[4];
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
-                if constexpr (F16) {
-                    const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&w[j]));
-                    y[2 * j] = __fmul_rn(f.x, scaling);
-                    y[2 * j + 1] = __fmul_rn(f.y, scaling);
+                o[j] = mx_e4m3_encode4<ALG>(__fmul_rn(x[4 * j], scaling), __fmul_rn(x[4 * j + 1], scaling),
+                                            __fmul_rn(x[4 * j + 2], scaling), __fmul_rn(x[4 * j + 3], scaling));
+                o[j] = finite ? o[j] : 0u;
+            }
+            if (row[u] >= 0) {
+                uint8_t* dst = data + row[u] * ld_data + static_cast<long long>(c[u]) * 16;
+                if (wide) {
+                    *reinterpret_cast<uint4*>(dst) = make_uint4(o[0], o[1], o[2], o[3]);
                 } else {
-                    y[2 * j] = __fmul_rn(__uint_as_float(w[j] << 16), scaling);
-                    y[2 * j + 1] = __fmul_rn(__uint_as_float(w[j] & 0xFFFF0000u), scaling);
+                    reinterpret_cast<uint2*>(dst)[0] = make_uint2(o[0], o[1]);
+                    reinterpret_cast<uint2*>(dst)[1] = make_uint2(o[2], o[3]);
                 }
-            }
-            uint2 packed = make_uint2(mx_e4m3_encode4<ALG>(y[0], y[1], y[2], y[3]), mx_e4m3_encode4<ALG>(y[4], y[5], y[6], y[7]));
-            if (!finite) {
-                packed = make_uint2(0u, 0u);
-            }
-            *reinterpret_cast<uint2*>(data + row[u] * ld_data + static_cast<long long>(c8[u]) * 8) = packed;
-            if ((c8[u] & 3) == 0) {
-                scales[row[u] * ld_scales + (c8[u] >> 2)] = static_cast<uint8_t>(e8m0);
+                if ((c[u] & 1) == 0) {
+                    scales[row[u] * ld_scales + (c[u] >> 1)] = static_cast<uint8_t>(e8m0);
+                }
             }
         }
     }

@@ -24,153 +24,11 @@
 
 #include <cstdint>
 
+#include "row_elements.cuh"
+
 namespace pto_b200 {
 
 constexpr int kNvQuantThreads = 256;
-
-enum NvSrc : int { NV_F32 = 0, NV_BF16 = 1, NV_F16 = 2 };
-
-template <int SRC>
-struct NvElem {
-    using type = float;
-};
-template <>
-struct NvElem<NV_BF16> {
-    using type = __nv_bfloat16;
-};
-template <>
-struct NvElem<NV_F16> {
-    using type = __half;
-};
-
-template <int SRC>
-__device__ __forceinline__ float nv_to_float(typename NvElem<SRC>::type v)
-{
-    if constexpr (SRC == NV_F32) {
-        return v;
-    } else if constexpr (SRC == NV_BF16) {
-        return __bfloat162float(v);
-    } else {
-        return __half2float(v);
-    }
-}
-
-template <int SRC>
-__device__ __forceinline__ void nv_unpack2(uint32_t w, float& lo, float& hi)
-{
-    if constexpr (SRC == NV_BF16) {
-        lo = __uint_as_float(w << 16);
-        hi = __uint_as_float(w & 0xFFFF0000u);
-    } else {
-        const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&w));
-        lo = f.x;
-        hi = f.y;
-    }
-}
-
-// 32 bytes in one access (32-byte aligned): a warp's accesses are then whole lines. With two of 16 bytes each covers
-// half of every sector (dequantising 16384 x 8192 to bf16 took 92 us that way).
-__device__ __forceinline__ void nv_ld32(const void* ptr, uint4& a, uint4& b)
-{
-    asm volatile("ld.global.nc.L1::no_allocate.v8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
-                 : "=r"(a.x), "=r"(a.y), "=r"(a.z), "=r"(a.w), "=r"(b.x), "=r"(b.y), "=r"(b.z), "=r"(b.w)
-                 : "l"(ptr));
-}
-
-__device__ __forceinline__ void nv_st32(void* ptr, const uint4& a, const uint4& b)
-{
-    asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(ptr), "r"(a.x), "r"(a.y), "r"(a.z),
-                 "r"(a.w), "r"(b.x), "r"(b.y), "r"(b.z), "r"(b.w)
-                 : "memory");
-}
-
-// 16 consecutive elements, read once, as they lie in memory. VEC: what the address is a multiple of, 32 or 16 bytes.
-template <int SRC>
-struct NvRaw16 {
-    static constexpr int kQuads = SRC == NV_F32 ? 4 : 2;
-    uint4 q[kQuads];
-
-    template <int VEC>
-    __device__ __forceinline__ void load(const void* ptr)
-    {
-        if constexpr (VEC == 32) {
-#pragma unroll
-            for (int i = 0; i < kQuads; i += 2) {
-                nv_ld32(static_cast<const uint4*>(ptr) + i, q[i], q[i + 1]);
-            }
-        } else {
-#pragma unroll
-            for (int i = 0; i < kQuads; ++i) {
-                q[i] = __ldcs(static_cast<const uint4*>(ptr) + i);
-            }
-        }
-    }
-    __device__ __forceinline__ void load_some(const typename NvElem<SRC>::type* p, int n) // the first n, zeros behind
-    {
-        __align__(16) typename NvElem<SRC>::type part[16];
-#pragma unroll
-        for (int j = 0; j < 16; ++j) {
-            part[j] = j < n ? p[j] : static_cast<typename NvElem<SRC>::type>(0.0f);
-        }
-#pragma unroll
-        for (int i = 0; i < kQuads; ++i) {
-            q[i] = reinterpret_cast<const uint4*>(part)[i];
-        }
-    }
-    __device__ __forceinline__ void zero()
-    {
-#pragma unroll
-        for (int i = 0; i < kQuads; ++i) {
-            q[i] = make_uint4(0u, 0u, 0u, 0u);
-        }
-    }
-    __device__ __forceinline__ uint32_t word(int i) const
-    {
-        const uint4& v = q[i / 4];
-        return (i & 3) == 0 ? v.x : (i & 3) == 1 ? v.y : (i & 3) == 2 ? v.z : v.w;
-    }
-    __device__ __forceinline__ void unpack(float (&x)[16]) const
-    {
-#pragma unroll
-        for (int i = 0; i < 4 * kQuads; ++i) {
-            if constexpr (SRC == NV_F32) {
-                x[i] = __uint_as_float(word(i));
-            } else {
-                nv_unpack2<SRC>(word(i), x[2 * i], x[2 * i + 1]);
-            }
-        }
-    }
-    // The largest magnitude as an fp32 pattern; an infinity or a NaN among the values gives a pattern of at least 0x7F800000.
-    __device__ __forceinline__ uint32_t top() const
-    {
-        if constexpr (SRC == NV_F32) {
-            uint32_t t = 0u;
-#pragma unroll
-            for (int i = 0; i < 16; ++i) {
-                t = max(t, word(i) & 0x7FFFFFFFu);
-            }
-            return t;
-        } else if constexpr (SRC == NV_BF16) {
-            __nv_bfloat162 t = __floats2bfloat162_rn(0.0f, 0.0f);
-#pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                const uint32_t w = word(i);
-                t = __hmax2_nan(t, __habs2(*reinterpret_cast<const __nv_bfloat162*>(&w)));
-            }
-            const uint32_t w = *reinterpret_cast<const uint32_t*>(&t) & 0x7FFF7FFFu;
-            return max(w << 16, w & 0xFFFF0000u);
-        } else {
-            __half2 t = __floats2half2_rn(0.0f, 0.0f);
-#pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                const uint32_t w = word(i);
-                t = __hmax2_nan(t, __habs2(*reinterpret_cast<const __half2*>(&w)));
-            }
-            const float2 f = __half22float2(t);
-            return max(__float_as_uint(f.x) & 0x7FFFFFFFu, __float_as_uint(f.y) & 0x7FFFFFFFu);
-        }
-    }
-};
 
 // Exponent field of g for a tensor maximum: amax / 2688 rounded up to a power of two, 2688 = 1.3125 * 2^11.
 __device__ __forceinline__ uint32_t nv_scale_exponent(float amax)
@@ -292,19 +150,19 @@ __device__ __forceinline__ uint32_t nv_top(const float (&x)[16])
     return t;
 }
 
-// Stores a block's codes and, once per four lanes, the scale word of four consecutive blocks. The four lanes of an
-// aligned group hold blocks kb, kb + 1, .. kb + 3 of one row and call this together.
+// Stores a block's codes and, once per four lanes, the scale word of four consecutive blocks. Every lane of the warp calls
+// it; the four lanes of an aligned group hold blocks kb .. kb + 3 of one row, or none (row < 0). (With a mask per group
+// the shuffles cost a synchronisation each: the address unit was busy 31 % of the time.)
 __device__ __forceinline__ void nv_store_block(uint8_t* data, uint8_t* scales, long long ld_data, int rows, int k_blocks,
                                                int k_atoms, int row, int kb, uint32_t s_code, const uint2& codes)
 {
-    if (row < rows && kb < k_blocks) {
+    if (row >= 0 && row < rows && kb < k_blocks) {
         *reinterpret_cast<uint2*>(data + row * ld_data + static_cast<long long>(kb) * 8) = codes;
     }
-    const unsigned mask = 0xFu << (threadIdx.x & 28u);
     uint32_t word = s_code << (8 * (threadIdx.x & 3u));
-    word |= __shfl_xor_sync(mask, word, 1);
-    word |= __shfl_xor_sync(mask, word, 2);
-    if ((threadIdx.x & 3u) == 0u) {
+    word |= __shfl_xor_sync(0xFFFFFFFFu, word, 1);
+    word |= __shfl_xor_sync(0xFFFFFFFFu, word, 2);
+    if ((threadIdx.x & 3u) == 0u && row >= 0) {
         const long long tile = static_cast<long long>(row >> 7) * k_atoms + (kb >> 2);
         *reinterpret_cast<uint32_t*>(scales + tile * 512 + (row & 31) * 16 + ((row >> 5) & 3) * 4) = word;
     }
@@ -336,7 +194,7 @@ __global__ void __launch_bounds__(kNvQuantThreads)
     if (blockIdx.x == 0 && threadIdx.x == 0) {
         *tensor_scale = t.g;
     }
-    while (i < total) {
+    while (i - static_cast<int>(threadIdx.x & 31u) < total) { // the warp goes on together
         NvRaw16<SRC> raw[kNvItems];
         int rows_of[kNvItems], kbs[kNvItems];
 #pragma unroll
@@ -362,13 +220,11 @@ __global__ void __launch_bounds__(kNvQuantThreads)
         }
 #pragma unroll
         for (int u = 0; u < kNvItems; ++u) {
-            if (rows_of[u] >= 0) { // the same for the four lanes of a group
-                float x[16];
-                raw[u].unpack(x);
-                uint2 codes;
-                const uint32_t s_code = nv_quantize_block(x, raw[u].top(), t, codes);
-                nv_store_block(data, scales, ld_data, rows, k_blocks, k_atoms, rows_of[u], kbs[u], s_code, codes);
-            }
+            float x[16];
+            raw[u].unpack(x);
+            uint2 codes;
+            const uint32_t s_code = nv_quantize_block(x, raw[u].top(), t, codes);
+            nv_store_block(data, scales, ld_data, rows, k_blocks, k_atoms, rows_of[u], kbs[u], s_code, codes);
         }
     }
 }
