@@ -76,14 +76,21 @@ int launch_quantize(cudaStream_t s, const HostContext& host, const void* src, co
 template <int SRC, int VEC>
 int launch_amax(cudaStream_t s, const HostContext& host, const void* src, float* amax, int rows, int k, long long ld_src)
 {
-    int grid = 0;
-    if (int rc = one_wave<amax_kernel<SRC, VEC>>(static_cast<long long>(rows) * ((k + 15) / 16), host, &grid)) {
-        return rc;
+    const long long items = static_cast<long long>(rows) * ((k + 15) / 16);
+    if (items * 16 <= kAmaxSingleElems) { // small: one block stores the result, nothing to clear first
+        amax_kernel<SRC, VEC>
+            <<<1, kAmaxSingleThreads, 0, s>>>(src, reinterpret_cast<uint32_t*>(amax), rows, k, ld_src);
+    } else {
+        int grid = 0;
+        if (int rc = one_wave<amax_kernel<SRC, VEC>>(items, host, &grid)) {
+            return rc;
+        }
+        if (int rc = note_cuda_error(cudaMemsetAsync(amax, 0, sizeof(float), s), "amax memset")) {
+            return rc;
+        }
+        amax_kernel<SRC, VEC>
+            <<<grid, kNvQuantThreads, 0, s>>>(src, reinterpret_cast<uint32_t*>(amax), rows, k, ld_src);
     }
-    if (int rc = note_cuda_error(cudaMemsetAsync(amax, 0, sizeof(float), s), "amax memset")) {
-        return rc;
-    }
-    amax_kernel<SRC, VEC><<<grid, kNvQuantThreads, 0, s>>>(src, reinterpret_cast<uint32_t*>(amax), rows, k, ld_src);
     count_launches(1);
     return note_cuda_error(cudaGetLastError(), "amax launch");
 }

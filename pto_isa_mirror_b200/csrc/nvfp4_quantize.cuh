@@ -101,9 +101,9 @@ struct NvTensorScale {
 };
 
 // One block with its largest magnitude `top` (an fp32 pattern): its e4m3 scale code and its sixteen codes.
-// x / (s g) is rounded correctly: a quotient from the reciprocal, then one correction by its exact remainder. (s g has
-// four significant bits; the product with the reciprocal alone misses ties by one unit, and 1/16 of all bf16 quotients
-// are ties.)
+// x / (s g) is rounded correctly: a quotient from the nearest reciprocal, then one correction by its exact remainder
+// (Markstein's theorem). s g has four significant bits; the product with the reciprocal alone misses ties by one unit, and
+// 1/16 of all bf16 quotients are ties.
 __device__ __forceinline__ uint32_t nv_quantize_block(float (&x)[16], uint32_t top, const NvTensorScale& t, uint2& codes)
 {
     codes = make_uint2(0u, 0u);
@@ -111,12 +111,19 @@ __device__ __forceinline__ uint32_t nv_quantize_block(float (&x)[16], uint32_t t
         return 0x7Fu;
     }
     const float y_max = __uint_as_float(top) * t.inv_g;
-    const uint32_t s_code = __nv_cvt_float_to_fp8(fminf(__fdiv_rn(y_max, 6.0f), 448.0f), __NV_SATFINITE, __NV_E4M3);
+    constexpr float kSixth = 1.0f / 6.0f;
+    const float sixth = __fmul_rn(y_max, kSixth); // corrected as below; a NaN from an infinite y_max ends at 448 too
+    const float m = __fmaf_rn(__fmaf_rn(-6.0f, sixth, y_max), kSixth, sixth);
+    const uint32_t s_code = __nv_cvt_float_to_fp8(fminf(m, 448.0f), __NV_SATFINITE, __NV_E4M3);
     if (s_code == 0u) {
         return 0u;
     }
     const float s = nv_e4m3_to_float(s_code);
-    const float r = __frcp_rn(s);
+    // 1 / s to the nearest float: an approximation and one step of Newton's iteration. s has four significant bits, so no
+    // 1 / s lies near the middle of two floats and the step's error cannot decide.
+    float r;
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(s));
+    r = __fmaf_rn(r, __fmaf_rn(-s, r, 1.0f), r);
     if (t.plain && y_max <= 1.0e30f) {
         const float ri = r * t.inv_g, sg = -s * t.g; // powers of two: exact
         const uint64_t ri2 = nv_pair(ri, ri), sg2 = nv_pair(sg, sg);
@@ -317,53 +324,77 @@ __global__ void __launch_bounds__(kNvQuantThreads)
     }
 }
 
-// Largest finite |x| of a matrix into *out, which the caller has set to zero. The maximum does not depend on the order.
+// Largest finite |x| of a matrix into *out: by a maximum with what the caller has set to zero, or (a single block) stored.
+// The maximum does not depend on the order.
+constexpr int kAmaxSingleThreads = 1024;
+constexpr int kAmaxSingleElems = 65536; // what one block of that many threads is given at most
+
 template <int SRC, int VEC>
-__global__ void __launch_bounds__(kNvQuantThreads)
+__global__ void __launch_bounds__(kAmaxSingleThreads)
     amax_kernel(const void* __restrict__ src, uint32_t* __restrict__ out, int rows, int k, long long ld_src)
 {
     using T = typename NvElem<SRC>::type;
-    const int items_per_row = (k + 15) / 16;
-    const long long total = static_cast<long long>(rows) * items_per_row;
+    constexpr int kAmaxItems = SRC == NV_F32 ? 2 : 4; // 128 bytes in flight per thread
+    const int row_items = (k + 15) / 16;
+    const long long total = static_cast<long long>(rows) * row_items;
     const long long stride = static_cast<long long>(gridDim.x) * blockDim.x;
     long long i = blockIdx.x * static_cast<long long>(blockDim.x) + threadIdx.x;
-    const long long row_step = stride / items_per_row;
-    const int c_step = static_cast<int>(stride - row_step * items_per_row);
-    long long row = i / items_per_row;
-    int c = static_cast<int>(i - row * items_per_row);
+    const long long row_step = stride / row_items;
+    const int c_step = static_cast<int>(stride - row_step * row_items);
+    long long row = i / row_items;
+    int c = static_cast<int>(i - row * row_items);
     uint32_t top = 0u;
-    for (; i < total; i += stride) {
-        const T* p = static_cast<const T*>(src) + row * ld_src + static_cast<long long>(c) * 16;
-        NvRaw16<SRC> raw;
-        if (VEC != 0 && c * 16 + 16 <= k) {
-            raw.template load<VEC>(p);
-        } else {
-            raw.load_some(p, k - c * 16);
-        }
-        float x[16];
-        raw.unpack(x);
+    while (i < total) {
+        NvRaw16<SRC> raw[kAmaxItems];
 #pragma unroll
-        for (int j = 0; j < 16; ++j) {
-            const uint32_t bits = __float_as_uint(x[j]) & 0x7FFFFFFFu;
-            top = max(top, bits < 0x7F800000u ? bits : 0u);
+        for (int u = 0; u < kAmaxItems; ++u) {
+            raw[u].zero();
+            if (i < total) {
+                const T* p = static_cast<const T*>(src) + row * ld_src + static_cast<long long>(c) * 16;
+                if (VEC != 0 && c * 16 + 16 <= k) {
+                    raw[u].template load<VEC>(p);
+                } else {
+                    raw[u].load_some(p, k - c * 16);
+                }
+            }
+            i += stride;
+            row += row_step;
+            c += c_step;
+            if (c >= row_items) {
+                c -= row_items;
+                row += 1;
+            }
         }
-        row += row_step;
-        c += c_step;
-        if (c >= items_per_row) {
-            c -= items_per_row;
-            row += 1;
+#pragma unroll
+        for (int u = 0; u < kAmaxItems; ++u) {
+            const uint32_t t = raw[u].top();
+            if (t < 0x7F800000u) {
+                top = max(top, t);
+            } else { // an infinity or a NaN among them: the others one by one
+                float x[16];
+                raw[u].unpack(x);
+#pragma unroll
+                for (int j = 0; j < 16; ++j) {
+                    const uint32_t bits = __float_as_uint(x[j]) & 0x7FFFFFFFu;
+                    top = max(top, bits < 0x7F800000u ? bits : 0u);
+                }
+            }
         }
     }
     top = __reduce_max_sync(0xFFFFFFFFu, top);
-    __shared__ uint32_t part[kNvQuantThreads / 32];
+    __shared__ uint32_t part[kAmaxSingleThreads / 32];
     if ((threadIdx.x & 31) == 0) {
         part[threadIdx.x >> 5] = top;
     }
     __syncthreads();
-    if (threadIdx.x < kNvQuantThreads / 32) {
-        top = __reduce_max_sync((1u << (kNvQuantThreads / 32)) - 1u, part[threadIdx.x]);
-        if (threadIdx.x == 0 && top != 0u) {
-            atomicMax(out, top);
+    if (threadIdx.x < 32) {
+        top = __reduce_max_sync(0xFFFFFFFFu, threadIdx.x < blockDim.x / 32 ? part[threadIdx.x] : 0u);
+        if (threadIdx.x == 0) {
+            if (gridDim.x == 1) {
+                *out = top;
+            } else if (top != 0u) {
+                atomicMax(out, top);
+            }
         }
     }
 }
