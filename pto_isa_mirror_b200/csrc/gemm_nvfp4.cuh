@@ -43,9 +43,8 @@ struct NvGemmParams {
 
 // status codes of bounded waits that gave up
 constexpr int ST_NV_PRODUCER = 21;
-constexpr int ST_NV_SCALES = 22;
-constexpr int ST_NV_MMA = 23;
-constexpr int ST_NV_EPILOGUE = 24;
+constexpr int ST_NV_MMA = 22;
+constexpr int ST_NV_EPILOGUE = 23;
 
 constexpr int kNvStageK = 256;       // elements of K per stage
 constexpr int kNvAtomBytes = 512;    // scales of 128 rows x 64 elements
@@ -71,11 +70,15 @@ __device__ __forceinline__ uint32_t nv_pack2(float lo, float hi)
 
 // ---------------------------------------------------------------- many rows: CTA pairs, 256 x 256 tiles
 //
-// Roles per CTA: warp 0 loads (TMA), warp 1 multiplies (leader CTA) or copies scales to tensor memory (second CTA, whose
-// MMA warp has nothing else to do), warps 2..9 store. A 256-column accumulator and the scale columns of five stages
-// fill tensor memory, so there is one accumulator: the store warps - eight of them, so that a thread owns 128 columns
-// of its row - move it to registers in one go and hand it back before they convert and store, and the next tile's
-// products start some hundred cycles after the last one's end instead of after its stores.
+// Roles per CTA: warp 0 loads (TMA), warp 1 copies scales to tensor memory and multiplies (leader CTA), warps 2..9 store.
+// A 256-column accumulator and the scale columns of five stages fill tensor memory, so there is one accumulator: the
+// store warps - eight of them, so that a thread owns 128 columns of its row - move it to registers in one go and hand it
+// back before they convert and store, and the next tile's products start some hundred cycles after the last one's end
+// instead of after its stores.
+//
+// The issuing warps walk their loops as whole warps and one elected lane issues: addresses and descriptors then stay in
+// uniform registers. Measured per 256-element stage: twelve scale copies and four products 513 cycles, which is the
+// products' own time; issued by a lane that branched off, 1176, and with the copies on the other CTA still 844.
 constexpr int kNvPairStages = 5;
 constexpr int kNvPairThreads = 320;
 constexpr int kNvStoreWarps = 8; // per CTA
@@ -92,7 +95,8 @@ struct NvPairSmem {
     static constexpr int kSfaOff = kEpiOff + kNvStoreWarps * kEpiBufBytes;
     static constexpr int kSfbOff = kSfaOff + kNvPairStages * kSfaBytes;
     static constexpr int kBarOff = kSfbOff + kNvPairStages * kSfbBytes;
-    static constexpr int kNumBars = 4 * kNvPairStages + 2;
+    static constexpr int kStageBytes = kABytes + kBBytes + kSfaBytes + kSfbBytes; // per CTA, on the leader's barrier
+    static constexpr int kNumBars = 2 * kNvPairStages + 2;
     static constexpr int kMiscOff = kBarOff + kNumBars * 8;
     static constexpr int kTotal = kMiscOff + 16 + 1024;
 };
@@ -123,11 +127,9 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kNvPairThreads, 1)
 
     extern __shared__ uint8_t smem_raw[];
     uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-    uint64_t* full_bar = reinterpret_cast<uint64_t*>(smem + L::kBarOff); // leader: both CTAs' operands landed
+    uint64_t* full_bar = reinterpret_cast<uint64_t*>(smem + L::kBarOff); // leader: both CTAs' operands and scales landed
     uint64_t* empty_bar = full_bar + STAGES;                            // each CTA
-    uint64_t* sf_landed_bar = empty_bar + STAGES;                       // second CTA: both CTAs' scales landed
-    uint64_t* sf_full_bar = sf_landed_bar + STAGES;                     // leader: scales are in tensor memory
-    uint64_t* acc_full_bar = sf_full_bar + STAGES;                      // each CTA
+    uint64_t* acc_full_bar = empty_bar + STAGES;                        // each CTA
     uint64_t* acc_empty_bar = acc_full_bar + 1;                         // leader: sixteen store warps
     uint32_t* tmem_base_slot = reinterpret_cast<uint32_t*>(smem + L::kMiscOff);
     volatile uint32_t* abort_flag = reinterpret_cast<volatile uint32_t*>(smem + L::kMiscOff + 4);
@@ -144,8 +146,6 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kNvPairThreads, 1)
         for (int s = 0; s < STAGES; ++s) {
             ptx::mbar_init(&full_bar[s], 1);
             ptx::mbar_init(&empty_bar[s], 1);
-            ptx::mbar_init(&sf_landed_bar[s], 1);
-            ptx::mbar_init(&sf_full_bar[s], 1);
         }
         ptx::mbar_init(acc_full_bar, 1);
         ptx::mbar_init(acc_empty_bar, 2 * kNvStoreWarps);
@@ -172,84 +172,55 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kNvPairThreads, 1)
 
     if (warp == 0) {
         // ---------------------------------------------------------------- loads (both CTAs)
-        if (lane == 0) {
-            int stage = 0;
-            uint32_t phase = 0;
-            bool ok = true;
-            for (int t = pair; ok && t < tiles; t += num_pairs) {
-                int mi, ni;
-                nv_tile_coords(t, p, mi, ni);
-                const int row_a = mi * 256 + static_cast<int>(cta_rank) * 128;
-                const int row_b = ni * 256 + static_cast<int>(cta_rank) * 128;
-                // scale tiles as rows of 256 bytes, two per 512-byte tile; tiles past the last row read as zero
-                const int sfa_row = (2 * mi + static_cast<int>(cta_rank)) * p.k_atoms * 2;
-                const int sfb_row = 2 * ni * p.k_atoms * 2;
-                for (int ks = 0; ks < p.k_stages; ++ks) {
-                    ok = bounded_wait(&empty_bar[stage], phase ^ 1u, abort_flag, p.status, ST_NV_PRODUCER, p.wait_limit);
-                    if (!ok) {
-                        break;
-                    }
+        int stage = 0;
+        uint32_t phase = 0;
+        bool ok = true;
+        for (int t = pair; ok && t < tiles; t += num_pairs) {
+            int mi, ni;
+            nv_tile_coords(t, p, mi, ni);
+            const int row_a = mi * 256 + static_cast<int>(cta_rank) * 128;
+            const int row_b = ni * 256 + static_cast<int>(cta_rank) * 128;
+            // scale tiles as rows of 256 bytes, two per 512-byte tile; tiles past the last row read as zero
+            const int sfa_row = (2 * mi + static_cast<int>(cta_rank)) * p.k_atoms * 2;
+            const int sfb_row = 2 * ni * p.k_atoms * 2;
+            for (int ks = 0; ks < p.k_stages; ++ks) {
+                ok = bounded_wait(&empty_bar[stage], phase ^ 1u, abort_flag, p.status, ST_NV_PRODUCER, p.wait_limit);
+                if (!ok) {
+                    break;
+                }
+                if (ptx::elect_one()) {
                     if (leader) {
-                        ptx::mbar_arrive_expect_tx(&full_bar[stage], 2u * (L::kABytes + L::kBBytes));
-                    } else {
-                        ptx::mbar_arrive_expect_tx(&sf_landed_bar[stage], 2u * (L::kSfaBytes + L::kSfbBytes));
+                        ptx::mbar_arrive_expect_tx(&full_bar[stage], 2u * L::kStageBytes);
                     }
                     const uint32_t full_addr = ptx::map_to_cta(ptx::smem_u32(&full_bar[stage]), 0);
-                    const uint32_t landed_addr = ptx::map_to_cta(ptx::smem_u32(&sf_landed_bar[stage]), 1);
                     uint8_t* sfa = smem + L::kSfaOff + stage * L::kSfaBytes;
                     uint8_t* sfb = smem + L::kSfbOff + stage * L::kSfbBytes;
-                    ptx::tma_load_2d_pair(sfa, &tmap_sfa, landed_addr, 0, sfa_row + ks * 8);
-                    ptx::tma_load_2d_pair(sfb, &tmap_sfb, landed_addr, 0, sfb_row + ks * 8);
-                    ptx::tma_load_2d_pair(sfb + 4 * kNvAtomBytes, &tmap_sfb, landed_addr, 0, sfb_row + p.k_atoms * 2 + ks * 8);
                     ptx::tma_load_2d_pair(smem + L::kAOff + stage * L::kABytes, &tmap_a, full_addr, ks * 128, row_a);
                     ptx::tma_load_2d_pair(smem + L::kBOff + stage * L::kBBytes, &tmap_b, full_addr, ks * 128, row_b);
-                    if (++stage == STAGES) {
-                        stage = 0;
-                        phase ^= 1u;
-                    }
+                    ptx::tma_load_2d_pair(sfa, &tmap_sfa, full_addr, 0, sfa_row + ks * 8);
+                    ptx::tma_load_2d_pair(sfb, &tmap_sfb, full_addr, 0, sfb_row + ks * 8);
+                    ptx::tma_load_2d_pair(sfb + 4 * kNvAtomBytes, &tmap_sfb, full_addr, 0, sfb_row + p.k_atoms * 2 + ks * 8);
                 }
-            }
-        }
-    } else if (warp == 1 && !leader) {
-        // ---------------------------------------------------------------- scales to tensor memory (second CTA)
-        // cta_group::2 copies the same shared-memory offsets of both CTAs into both CTAs' tensor memory
-        if (lane == 0) {
-            int stage = 0;
-            uint32_t phase = 0;
-            bool ok = true;
-            for (int t = pair; ok && t < tiles; t += num_pairs) {
-                for (int ks = 0; ks < p.k_stages; ++ks) {
-                    ok = bounded_wait(&sf_landed_bar[stage], phase, abort_flag, p.status, ST_NV_SCALES, p.wait_limit);
-                    if (!ok) {
-                        break;
-                    }
-                    ptx::tc_fence_after_sync();
-                    const uint32_t sfa = ptx::smem_u32(smem + L::kSfaOff + stage * L::kSfaBytes);
-                    const uint32_t sfb = ptx::smem_u32(smem + L::kSfbOff + stage * L::kSfbBytes);
-                    const uint32_t sf = tmem_base + kSfCol0 + kSfColsPerStage * static_cast<uint32_t>(stage);
-#pragma unroll
-                    for (uint32_t g = 0; g < 4; ++g) {
-                        ptx::tmem_cp_32x128b_warpx4_pair(sf + 4u * g, ptx::make_smem_desc(sfa + 512u * g, 0, 128, ptx::kSwizzleNone));
-                        ptx::tmem_cp_32x128b_warpx4_pair(sf + 16u + 8u * g,
-                                                         ptx::make_smem_desc(sfb + 512u * g, 0, 128, ptx::kSwizzleNone));
-                        ptx::tmem_cp_32x128b_warpx4_pair(sf + 20u + 8u * g,
-                                                         ptx::make_smem_desc(sfb + 2048u + 512u * g, 0, 128, ptx::kSwizzleNone));
-                    }
-                    ptx::umma_commit_pair(&sf_full_bar[stage], 0x1);
-                    if (++stage == STAGES) {
-                        stage = 0;
-                        phase ^= 1u;
-                    }
+                __syncwarp();
+                if (++stage == STAGES) {
+                    stage = 0;
+                    phase ^= 1u;
                 }
             }
         }
     } else if (warp == 1) {
-        // ---------------------------------------------------------------- products (leader)
-        if (lane == 0) {
+        // ---------------------------------------------------------------- scale copies and products (leader)
+        // cta_group::2 copies the same shared-memory offsets of both CTAs into both CTAs' tensor memory; a thread's copies
+        // and products run in order
+        if (leader) {
             int stage = 0;
             uint32_t phase = 0;
             uint32_t acc_phase = 0;
             bool ok = true;
+            const uint64_t a_desc0 = ptx::make_smem_desc(ptx::smem_u32(smem + L::kAOff), 16, 1024, ptx::kSwizzle128B);
+            const uint64_t b_desc0 = ptx::make_smem_desc(ptx::smem_u32(smem + L::kBOff), 16, 1024, ptx::kSwizzle128B);
+            const uint64_t sfa_desc0 = ptx::make_smem_desc(ptx::smem_u32(smem + L::kSfaOff), 0, 128, ptx::kSwizzleNone);
+            const uint64_t sfb_desc0 = ptx::make_smem_desc(ptx::smem_u32(smem + L::kSfbOff), 0, 128, ptx::kSwizzleNone);
             for (int t = pair; ok && t < tiles; t += num_pairs) {
                 ok = bounded_wait(acc_empty_bar, acc_phase ^ 1u, abort_flag, p.status, ST_NV_MMA, p.wait_limit);
                 if (!ok) {
@@ -257,34 +228,45 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kNvPairThreads, 1)
                 }
                 ptx::tc_fence_after_sync();
                 for (int ks = 0; ks < p.k_stages; ++ks) {
-                    ok = bounded_wait(&full_bar[stage], phase, abort_flag, p.status, ST_NV_MMA, p.wait_limit) &&
-                         bounded_wait(&sf_full_bar[stage], phase, abort_flag, p.status, ST_NV_MMA, p.wait_limit);
+                    ok = bounded_wait(&full_bar[stage], phase, abort_flag, p.status, ST_NV_MMA, p.wait_limit);
                     if (!ok) {
                         break;
                     }
                     ptx::tc_fence_after_sync();
-                    const uint32_t a_base = ptx::smem_u32(smem + L::kAOff + stage * L::kABytes);
-                    const uint32_t b_base = ptx::smem_u32(smem + L::kBOff + stage * L::kBBytes);
-                    const uint32_t sf = tmem_base + kSfCol0 + kSfColsPerStage * static_cast<uint32_t>(stage);
-                    const int groups = min(4, p.k_atoms - 4 * ks);
+                    if (ptx::elect_one()) {
+                        // descriptor addresses count 16 bytes
+                        const uint64_t a_desc = a_desc0 + static_cast<uint64_t>(stage * (L::kABytes / 16));
+                        const uint64_t b_desc = b_desc0 + static_cast<uint64_t>(stage * (L::kBBytes / 16));
+                        const uint64_t sfa_desc = sfa_desc0 + static_cast<uint64_t>(stage * (L::kSfaBytes / 16));
+                        const uint64_t sfb_desc = sfb_desc0 + static_cast<uint64_t>(stage * (L::kSfbBytes / 16));
+                        const uint32_t sf = tmem_base + kSfCol0 + kSfColsPerStage * static_cast<uint32_t>(stage);
+                        const int groups = p.k_atoms - 4 * ks; // 64-element groups left
 #pragma unroll
-                    for (int g = 0; g < 4; ++g) {
-                        if (g < groups) {
-                            ptx::umma_nvf4_pair(tmem_base, ptx::make_smem_desc(a_base + g * 32, 16, 1024, ptx::kSwizzle128B),
-                                                ptx::make_smem_desc(b_base + g * 32, 16, 1024, ptx::kSwizzle128B), p.idesc,
-                                                sf + 4u * g, sf + 16u + 8u * g, (ks > 0 || g > 0) ? 1u : 0u);
+                        for (int g = 0; g < 4; ++g) {
+                            if (g < groups) {
+                                ptx::tmem_cp_32x128b_warpx4_pair(sf + 4u * g, sfa_desc + 32 * g);
+                                ptx::tmem_cp_32x128b_warpx4_pair(sf + 16u + 8u * g, sfb_desc + 32 * g);
+                                ptx::tmem_cp_32x128b_warpx4_pair(sf + 20u + 8u * g, sfb_desc + 128 + 32 * g);
+                            }
+                        }
+#pragma unroll
+                        for (int g = 0; g < 4; ++g) {
+                            if (g < groups) {
+                                ptx::umma_nvf4_pair(tmem_base, a_desc + 2 * g, b_desc + 2 * g, p.idesc, sf + 4u * g,
+                                                    sf + 16u + 8u * g, (ks > 0 || g > 0) ? 1u : 0u);
+                            }
+                        }
+                        ptx::umma_commit_pair(&empty_bar[stage], 0x3);
+                        if (ks == p.k_stages - 1) {
+                            ptx::umma_commit_pair(acc_full_bar, 0x3);
                         }
                     }
-                    ptx::umma_commit_pair(&empty_bar[stage], 0x3);
+                    __syncwarp();
                     if (++stage == STAGES) {
                         stage = 0;
                         phase ^= 1u;
                     }
                 }
-                if (!ok) {
-                    break;
-                }
-                ptx::umma_commit_pair(acc_full_bar, 0x3);
                 acc_phase ^= 1u;
             }
         }
@@ -509,15 +491,15 @@ __global__ void __launch_bounds__(kNvFewThreads, 2)
     const uint32_t tmem_base = *tmem_base_slot;
 
     if (warp == 0) {
-        if (lane == 0) {
-            int stage = 0;
-            uint32_t phase = 0;
-            const uint8_t* sfw = p.sfb + static_cast<size_t>(ni) * p.k_atoms * kNvAtomBytes;
-            const uint8_t* sfx = p.sfa + static_cast<size_t>(ti) * p.k_atoms * kNvAtomBytes;
-            for (int ks = ks0; ks < ks1; ++ks) {
-                if (!bounded_wait(&empty_bar[stage], phase ^ 1u, abort_flag, p.status, ST_NV_PRODUCER, p.wait_limit)) {
-                    break;
-                }
+        int stage = 0;
+        uint32_t phase = 0;
+        const uint8_t* sfw = p.sfb + static_cast<size_t>(ni) * p.k_atoms * kNvAtomBytes;
+        const uint8_t* sfx = p.sfa + static_cast<size_t>(ti) * p.k_atoms * kNvAtomBytes;
+        for (int ks = ks0; ks < ks1; ++ks) {
+            if (!bounded_wait(&empty_bar[stage], phase ^ 1u, abort_flag, p.status, ST_NV_PRODUCER, p.wait_limit)) {
+                break;
+            }
+            if (ptx::elect_one()) {
                 const uint32_t sf_bytes = static_cast<uint32_t>(min(4, p.k_atoms - 4 * ks)) * kNvAtomBytes;
                 ptx::mbar_arrive_expect_tx(&full_bar[stage], L::kWBytes + L::kXBytes + 2u * sf_bytes);
                 ptx::tma_load_2d(smem + stage * L::kWBytes, &tmap_w, &full_bar[stage], ks * 128, ni * 128);
@@ -525,54 +507,58 @@ __global__ void __launch_bounds__(kNvFewThreads, 2)
                 const size_t at = static_cast<size_t>(ks) * 4 * kNvAtomBytes;
                 ptx::bulk_load_1d(smem + L::kSfwOff + stage * L::kSfBytes, sfw + at, sf_bytes, &full_bar[stage]);
                 ptx::bulk_load_1d(smem + L::kSfxOff + stage * L::kSfBytes, sfx + at, sf_bytes, &full_bar[stage]);
-                if (++stage == STAGES) {
-                    stage = 0;
-                    phase ^= 1u;
-                }
+            }
+            __syncwarp();
+            if (++stage == STAGES) {
+                stage = 0;
+                phase ^= 1u;
             }
         }
     } else if (warp == 1) {
-        if (lane == 0) {
-            int stage = 0;
-            uint32_t phase = 0;
-            bool ok = true;
-            for (int ks = ks0; ks < ks1; ++ks) {
-                ok = bounded_wait(&full_bar[stage], phase, abort_flag, p.status, ST_NV_MMA, p.wait_limit);
-                if (!ok) {
-                    break;
-                }
-                ptx::tc_fence_after_sync();
-                const uint32_t w_base = ptx::smem_u32(smem + stage * L::kWBytes);
-                const uint32_t x_base = ptx::smem_u32(smem + L::kXOff + stage * L::kXBytes);
-                const uint32_t sfw = ptx::smem_u32(smem + L::kSfwOff + stage * L::kSfBytes);
-                const uint32_t sfx = ptx::smem_u32(smem + L::kSfxOff + stage * L::kSfBytes);
+        int stage = 0;
+        uint32_t phase = 0;
+        bool ok = true;
+        const uint64_t w_desc0 = ptx::make_smem_desc(ptx::smem_u32(smem), 16, 1024, ptx::kSwizzle128B);
+        const uint64_t x_desc0 = ptx::make_smem_desc(ptx::smem_u32(smem + L::kXOff), 16, 1024, ptx::kSwizzle128B);
+        const uint64_t sfw_desc0 = ptx::make_smem_desc(ptx::smem_u32(smem + L::kSfwOff), 0, 128, ptx::kSwizzleNone);
+        const uint64_t sfx_desc0 = ptx::make_smem_desc(ptx::smem_u32(smem + L::kSfxOff), 0, 128, ptx::kSwizzleNone);
+        for (int ks = ks0; ks < ks1; ++ks) {
+            ok = bounded_wait(&full_bar[stage], phase, abort_flag, p.status, ST_NV_MMA, p.wait_limit);
+            if (!ok) {
+                break;
+            }
+            ptx::tc_fence_after_sync();
+            if (ptx::elect_one()) {
+                const uint64_t w_desc = w_desc0 + static_cast<uint64_t>(stage * (L::kWBytes / 16));
+                const uint64_t x_desc = x_desc0 + static_cast<uint64_t>(stage * (L::kXBytes / 16));
+                const uint64_t sfw_desc = sfw_desc0 + static_cast<uint64_t>(stage * (L::kSfBytes / 16));
+                const uint64_t sfx_desc = sfx_desc0 + static_cast<uint64_t>(stage * (L::kSfBytes / 16));
                 // every stage has its own scale columns: a copy never meets a product that still reads them
                 const uint32_t sf = tmem_base + L::kSfCol + 32u * static_cast<uint32_t>(stage);
-                const int groups = min(4, p.k_atoms - 4 * ks);
+                const int groups = p.k_atoms - 4 * ks;
 #pragma unroll
                 for (int g = 0; g < 4; ++g) {
                     if (g < groups) {
-                        ptx::tmem_cp_32x128b_warpx4(sf + 4u * g, ptx::make_smem_desc(sfw + 512u * g, 0, 128, ptx::kSwizzleNone));
-                        ptx::tmem_cp_32x128b_warpx4(sf + 16u + 4u * g,
-                                                    ptx::make_smem_desc(sfx + 512u * g, 0, 128, ptx::kSwizzleNone));
+                        ptx::tmem_cp_32x128b_warpx4(sf + 4u * g, sfw_desc + 32 * g);
+                        ptx::tmem_cp_32x128b_warpx4(sf + 16u + 4u * g, sfx_desc + 32 * g);
                     }
                 }
 #pragma unroll
                 for (int g = 0; g < 4; ++g) {
                     if (g < groups) {
-                        ptx::umma_nvf4(tmem_base, ptx::make_smem_desc(w_base + g * 32, 16, 1024, ptx::kSwizzle128B),
-                                       ptx::make_smem_desc(x_base + g * 32, 16, 1024, ptx::kSwizzle128B), p.idesc, sf + 4u * g,
-                                       sf + 16u + 4u * g, (ks > ks0 || g > 0) ? 1u : 0u);
+                        ptx::umma_nvf4(tmem_base, w_desc + 2 * g, x_desc + 2 * g, p.idesc, sf + 4u * g, sf + 16u + 4u * g,
+                                       (ks > ks0 || g > 0) ? 1u : 0u);
                     }
                 }
                 ptx::umma_commit(&empty_bar[stage]);
-                if (++stage == STAGES) {
-                    stage = 0;
-                    phase ^= 1u;
+                if (ks == ks1 - 1) {
+                    ptx::umma_commit(acc_bar);
                 }
             }
-            if (ok) {
-                ptx::umma_commit(acc_bar);
+            __syncwarp();
+            if (++stage == STAGES) {
+                stage = 0;
+                phase ^= 1u;
             }
         }
     } else {
