@@ -470,6 +470,17 @@ __global__ void __launch_bounds__(kNvFewThreads, 2)
     const int ks0 = static_cast<int>(static_cast<long long>(p.k_stages) * rank / splits);
     const int ks1 = static_cast<int>(static_cast<long long>(p.k_stages) * (rank + 1) / splits);
 
+    auto load_stage = [&](int ks, int stage) {
+        const uint32_t sf_bytes = static_cast<uint32_t>(min(4, p.k_atoms - 4 * ks)) * kNvAtomBytes;
+        const size_t at = static_cast<size_t>(ks) * 4 * kNvAtomBytes;
+        ptx::mbar_arrive_expect_tx(&full_bar[stage], L::kWBytes + L::kXBytes + 2u * sf_bytes);
+        ptx::tma_load_2d(smem + stage * L::kWBytes, &tmap_w, &full_bar[stage], ks * 128, ni * 128);
+        ptx::bulk_load_1d(smem + L::kSfwOff + stage * L::kSfBytes,
+                          p.sfb + static_cast<size_t>(ni) * p.k_atoms * kNvAtomBytes + at, sf_bytes, &full_bar[stage]);
+        ptx::tma_load_2d(smem + L::kXOff + stage * L::kXBytes, &tmap_x, &full_bar[stage], ks * 128, ti * BLOCK_T);
+        ptx::bulk_load_1d(smem + L::kSfxOff + stage * L::kSfBytes,
+                          p.sfa + static_cast<size_t>(ti) * p.k_atoms * kNvAtomBytes + at, sf_bytes, &full_bar[stage]);
+    };
     if (threadIdx.x == 0) {
         for (int s = 0; s < STAGES; ++s) {
             ptx::mbar_init(&full_bar[s], 1);
@@ -478,8 +489,10 @@ __global__ void __launch_bounds__(kNvFewThreads, 2)
         ptx::mbar_init(acc_bar, 1);
         *abort_flag = 0;
         ptx::fence_mbar_init();
-        ptx::prefetch_tensormap(&tmap_w);
-        ptx::prefetch_tensormap(&tmap_x);
+        // the first stages are on their way while tensor memory is set up
+        for (int ks = ks0; ks < min(ks1, ks0 + STAGES); ++ks) {
+            load_stage(ks, ks - ks0);
+        }
     }
     if (warp == 1) {
         ptx::tmem_alloc(tmem_base_slot, L::kTmem);
@@ -492,21 +505,13 @@ __global__ void __launch_bounds__(kNvFewThreads, 2)
 
     if (warp == 0) {
         int stage = 0;
-        uint32_t phase = 0;
-        const uint8_t* sfw = p.sfb + static_cast<size_t>(ni) * p.k_atoms * kNvAtomBytes;
-        const uint8_t* sfx = p.sfa + static_cast<size_t>(ti) * p.k_atoms * kNvAtomBytes;
-        for (int ks = ks0; ks < ks1; ++ks) {
+        uint32_t phase = 1; // the first round of the ring is loaded above
+        for (int ks = ks0 + STAGES; ks < ks1; ++ks) {
             if (!bounded_wait(&empty_bar[stage], phase ^ 1u, abort_flag, p.status, ST_NV_PRODUCER, p.wait_limit)) {
                 break;
             }
             if (ptx::elect_one()) {
-                const uint32_t sf_bytes = static_cast<uint32_t>(min(4, p.k_atoms - 4 * ks)) * kNvAtomBytes;
-                ptx::mbar_arrive_expect_tx(&full_bar[stage], L::kWBytes + L::kXBytes + 2u * sf_bytes);
-                ptx::tma_load_2d(smem + stage * L::kWBytes, &tmap_w, &full_bar[stage], ks * 128, ni * 128);
-                ptx::tma_load_2d(smem + L::kXOff + stage * L::kXBytes, &tmap_x, &full_bar[stage], ks * 128, ti * BLOCK_T);
-                const size_t at = static_cast<size_t>(ks) * 4 * kNvAtomBytes;
-                ptx::bulk_load_1d(smem + L::kSfwOff + stage * L::kSfBytes, sfw + at, sf_bytes, &full_bar[stage]);
-                ptx::bulk_load_1d(smem + L::kSfxOff + stage * L::kSfBytes, sfx + at, sf_bytes, &full_bar[stage]);
+                load_stage(ks, stage);
             }
             __syncwarp();
             if (++stage == STAGES) {
@@ -617,24 +622,40 @@ __global__ void __launch_bounds__(kNvFewThreads, 2)
     if (splits > 1) {
         ptx::cluster_arrive(); // every CTA's partial sums are in its shared memory
         ptx::cluster_wait();
+        // Four columns per thread and step; the reads of all ranks are in flight together (one value at a time this took
+        // 12000 cycles for 48 rows).
         const int rows = min(BLOCK_T, p.m - ti * BLOCK_T);
-        const int items = rows * 128;
+        const int items = rows * 32;
         const int first = static_cast<int>(static_cast<long long>(items) * rank / splits);
         const int last = static_cast<int>(static_cast<long long>(items) * (rank + 1) / splits);
         const float alpha = nv_alpha(p);
         const uint32_t base = ptx::smem_u32(smem);
         for (int i = first + static_cast<int>(threadIdx.x); i < last; i += kNvFewThreads) {
-            const int col = ni * 128 + (i & 127);
-            if (col < p.n) {
-                float sum = 0.0f;
-                for (int r = 0; r < splits; ++r) {
-                    sum += ptx::ld_shared_cluster_f32(ptx::map_to_cta(base + 4u * static_cast<uint32_t>(i), static_cast<uint32_t>(r)));
+            float4 part[8];
+#pragma unroll
+            for (int r = 0; r < 8; ++r) {
+                if (r < splits) {
+                    part[r] = ptx::ld_shared_cluster_f32x4(ptx::map_to_cta(base + 16u * static_cast<uint32_t>(i), static_cast<uint32_t>(r)));
                 }
-                sum *= alpha;
-                if (p.bias != nullptr) {
-                    sum += __ldg(p.bias + col);
+            }
+            float4 sum = part[0];
+#pragma unroll
+            for (int r = 1; r < 8; ++r) {
+                if (r < splits) {
+                    sum.x += part[r].x;
+                    sum.y += part[r].y;
+                    sum.z += part[r].z;
+                    sum.w += part[r].w;
                 }
-                nv_store_one<OUT>(p, static_cast<long long>(ti) * BLOCK_T + (i >> 7), col, sum);
+            }
+            const int col = ni * 128 + (i & 31) * 4;
+            const long long row = static_cast<long long>(ti) * BLOCK_T + (i >> 5);
+            const float f[4] = {sum.x * alpha, sum.y * alpha, sum.z * alpha, sum.w * alpha};
+#pragma unroll
+            for (int c = 0; c < 4; ++c) {
+                if (col + c < p.n) {
+                    nv_store_one<OUT>(p, row, col + c, f[c] + (p.bias != nullptr ? __ldg(p.bias + col + c) : 0.0f));
+                }
             }
         }
         ptx::cluster_arrive_relaxed(); // no CTA leaves while another still reads its shared memory

@@ -589,17 +589,34 @@ __global__ void __launch_bounds__(kWgThreads, 1)
         int ki, ni;
         tile_of(cluster, ki, ni);
         const uint32_t base = ptx::smem_u32(smem);
-        const int first = 256 * 128 * split / p.splits;
-        const int last = 256 * 128 * (split + 1) / p.splits;
+        const int first = 256 * 32 * split / p.splits; // four k per thread and step
+        const int last = 256 * 32 * (split + 1) / p.splits;
         for (int i = first + static_cast<int>(threadIdx.x); i < last; i += kWgThreads) {
-            const int k = ki * 256 + side * 128 + (i & 127);
-            const int n = ni * 256 + (i >> 7);
-            if (k < p.k && n < p.n) {
-                float f = 0.0f;
-                for (int s = 0; s < p.splits; ++s) {
-                    f += ptx::ld_shared_cluster_f32(ptx::map_to_cta(base + 4u * static_cast<uint32_t>(i), static_cast<uint32_t>(2 * s + side)));
+            const int k = ki * 256 + side * 128 + (i & 31) * 4;
+            const int n = ni * 256 + (i >> 5);
+            if (k < p.k && n < p.n) { // p.k is a multiple of 32
+                float4 part[4];
+#pragma unroll
+                for (int s = 0; s < 4; ++s) {
+                    if (s < p.splits) {
+                        part[s] = ptx::ld_shared_cluster_f32x4(
+                            ptx::map_to_cta(base + 16u * static_cast<uint32_t>(i), static_cast<uint32_t>(2 * s + side)));
+                    }
                 }
-                wg_store<OUT>(p, n, k, f);
+                float4 f = part[0];
+#pragma unroll
+                for (int s = 1; s < 4; ++s) {
+                    if (s < p.splits) {
+                        f.x += part[s].x;
+                        f.y += part[s].y;
+                        f.z += part[s].z;
+                        f.w += part[s].w;
+                    }
+                }
+                wg_store<OUT>(p, n, k, f.x);
+                wg_store<OUT>(p, n, k + 1, f.y);
+                wg_store<OUT>(p, n, k + 2, f.z);
+                wg_store<OUT>(p, n, k + 3, f.w);
             }
         }
         ptx::cluster_arrive_relaxed(); // no CTA leaves while another still reads its shared memory

@@ -419,11 +419,14 @@ __device__ __forceinline__ void umma_nvf4_pair(uint32_t d_tmem, uint64_t a_desc,
         : "memory");
 }
 
-// 32-bit word of another CTA's shared memory (address from map_to_cta).
-__device__ __forceinline__ float ld_shared_cluster_f32(uint32_t cluster_addr)
+// Four floats of another CTA's shared memory (16-byte aligned address from map_to_cta).
+__device__ __forceinline__ float4 ld_shared_cluster_f32x4(uint32_t cluster_addr)
 {
-    float v;
-    asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(cluster_addr) : "memory");
+    float4 v;
+    asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];"
+                 : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w)
+                 : "r"(cluster_addr)
+                 : "memory");
     return v;
 }
 
