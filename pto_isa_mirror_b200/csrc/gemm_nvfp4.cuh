@@ -445,6 +445,54 @@ __device__ __forceinline__ void nv_store_one(const NvGemmParams& p, long long ro
     }
 }
 
+// This CTA's share of a tile whose K was cut over SPLITS CTAs: their partial sums [rows][128] lie at the same place of each
+// CTA's shared memory and are added in rank order. Four columns per thread and item, UNROLL items at a time, all reads in
+// flight together (a read from another SM takes about a thousand cycles: one value at a time this took 12000 cycles for
+// 48 rows, one item at a time 4300).
+template <int SPLITS, int UNROLL, int OUT>
+__device__ __forceinline__ void nv_add_parts(const NvGemmParams& p, uint32_t base, int rank, int ni, int row0, int rows)
+{
+    const int items = rows * 32;
+    const int first = items * rank / SPLITS;
+    const int last = items * (rank + 1) / SPLITS;
+    const float alpha = nv_alpha(p);
+    for (int i0 = first + static_cast<int>(threadIdx.x); i0 < last; i0 += UNROLL * kNvFewThreads) {
+        float4 part[UNROLL][SPLITS];
+#pragma unroll
+        for (int u = 0; u < UNROLL; ++u) {
+            const int i = min(i0 + u * kNvFewThreads, last - 1);
+#pragma unroll
+            for (int r = 0; r < SPLITS; ++r) {
+                part[u][r] = ptx::ld_shared_cluster_f32x4(ptx::map_to_cta(base + 16u * static_cast<uint32_t>(i), r));
+            }
+        }
+#pragma unroll
+        for (int u = 0; u < UNROLL; ++u) {
+            const int i = i0 + u * kNvFewThreads;
+            if (i >= last) {
+                break;
+            }
+            float4 sum = part[u][0];
+#pragma unroll
+            for (int r = 1; r < SPLITS; ++r) {
+                sum.x += part[u][r].x;
+                sum.y += part[u][r].y;
+                sum.z += part[u][r].z;
+                sum.w += part[u][r].w;
+            }
+            const int col = ni * 128 + (i & 31) * 4;
+            const long long row = row0 + (i >> 5);
+            const float f[4] = {sum.x * alpha, sum.y * alpha, sum.z * alpha, sum.w * alpha};
+#pragma unroll
+            for (int c = 0; c < 4; ++c) {
+                if (col + c < p.n) {
+                    nv_store_one<OUT>(p, row, col + c, f[c] + (p.bias != nullptr ? __ldg(p.bias + col + c) : 0.0f));
+                }
+            }
+        }
+    }
+}
+
 // grid: splits (the cluster) x 128-column tiles x BLOCK_T-row tiles
 template <int BLOCK_T, int OUT>
 __global__ void __launch_bounds__(kNvFewThreads, 2)
@@ -622,41 +670,13 @@ __global__ void __launch_bounds__(kNvFewThreads, 2)
     if (splits > 1) {
         ptx::cluster_arrive(); // every CTA's partial sums are in its shared memory
         ptx::cluster_wait();
-        // Four columns per thread and step; the reads of all ranks are in flight together (one value at a time this took
-        // 12000 cycles for 48 rows).
         const int rows = min(BLOCK_T, p.m - ti * BLOCK_T);
-        const int items = rows * 32;
-        const int first = static_cast<int>(static_cast<long long>(items) * rank / splits);
-        const int last = static_cast<int>(static_cast<long long>(items) * (rank + 1) / splits);
-        const float alpha = nv_alpha(p);
-        const uint32_t base = ptx::smem_u32(smem);
-        for (int i = first + static_cast<int>(threadIdx.x); i < last; i += kNvFewThreads) {
-            float4 part[8];
-#pragma unroll
-            for (int r = 0; r < 8; ++r) {
-                if (r < splits) {
-                    part[r] = ptx::ld_shared_cluster_f32x4(ptx::map_to_cta(base + 16u * static_cast<uint32_t>(i), static_cast<uint32_t>(r)));
-                }
-            }
-            float4 sum = part[0];
-#pragma unroll
-            for (int r = 1; r < 8; ++r) {
-                if (r < splits) {
-                    sum.x += part[r].x;
-                    sum.y += part[r].y;
-                    sum.z += part[r].z;
-                    sum.w += part[r].w;
-                }
-            }
-            const int col = ni * 128 + (i & 31) * 4;
-            const long long row = static_cast<long long>(ti) * BLOCK_T + (i >> 5);
-            const float f[4] = {sum.x * alpha, sum.y * alpha, sum.z * alpha, sum.w * alpha};
-#pragma unroll
-            for (int c = 0; c < 4; ++c) {
-                if (col + c < p.n) {
-                    nv_store_one<OUT>(p, row, col + c, f[c] + (p.bias != nullptr ? __ldg(p.bias + col + c) : 0.0f));
-                }
-            }
+        if (splits == 2) {
+            nv_add_parts<2, 4, OUT>(p, ptx::smem_u32(smem), rank, ni, ti * BLOCK_T, rows);
+        } else if (splits == 4) {
+            nv_add_parts<4, 2, OUT>(p, ptx::smem_u32(smem), rank, ni, ti * BLOCK_T, rows);
+        } else {
+            nv_add_parts<8, 1, OUT>(p, ptx::smem_u32(smem), rank, ni, ti * BLOCK_T, rows);
         }
         ptx::cluster_arrive_relaxed(); // no CTA leaves while another still reads its shared memory
         ptx::cluster_wait();
