@@ -17,6 +17,7 @@
 #include <cstdint>
 
 #include "gemm_tile_loop.cuh"
+#include "row_elements.cuh"
 #include "sm100_ptx.cuh"
 
 namespace pto_b200 {
@@ -38,7 +39,7 @@ struct NvGemmParams {
     const uint8_t* sfb;
     int* status;
     long long wait_limit;
-    int tma_store;      // pair kernel: C leaves through TMA stores
+    int row_access;     // C's rows start on 32- or 16-byte boundaries, or on any element (0)
 };
 
 // status codes of bounded waits that gave up
@@ -117,7 +118,7 @@ template <int OUT>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kNvPairThreads, 1)
     gemm_nvfp4_2cta(const __grid_constant__ CUtensorMap tmap_a, const __grid_constant__ CUtensorMap tmap_b,
                     const __grid_constant__ CUtensorMap tmap_sfa, const __grid_constant__ CUtensorMap tmap_sfb,
-                    const __grid_constant__ CUtensorMap tmap_c, const NvGemmParams p)
+                    const NvGemmParams p)
 {
     using L = NvPairSmem;
     constexpr int STAGES = kNvPairStages;
@@ -155,9 +156,6 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kNvPairThreads, 1)
         ptx::prefetch_tensormap(&tmap_b);
         ptx::prefetch_tensormap(&tmap_sfa);
         ptx::prefetch_tensormap(&tmap_sfb);
-        if (p.tma_store != 0) {
-            ptx::prefetch_tensormap(&tmap_c);
-        }
     }
     if (warp == 1) {
         ptx::tmem_alloc_pair(tmem_base_slot, kTmemCols);
@@ -273,12 +271,16 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kNvPairThreads, 1)
     } else {
         // ---------------------------------------------------------------- stores (both CTAs)
         constexpr bool kOut32 = (OUT == NV_OUT_F32);
-        constexpr int kBoxCols = kOut32 ? 32 : 64; // a box is 32 rows x 128 bytes
+        constexpr int kBoxCols = kOut32 ? 32 : 64; // 128 bytes
         constexpr int kBoxes = 128 / kBoxCols;
         const int quarter = warp & 3;
         const int half = (warp - 2) >> 2; // which 128 columns
         uint8_t* box = smem + L::kEpiOff + (warp - 2) * L::kEpiBufBytes;
         const float alpha = nv_alpha(p);
+        auto finish = [&](uint32_t acc, int col) {
+            const float f = __uint_as_float(acc) * alpha;
+            return p.bias != nullptr && col < p.n ? f + __ldg(p.bias + col) : f;
+        };
         uint32_t acc_phase = 0;
         bool ok = true;
         for (int t = pair; ok && t < tiles; t += num_pairs) {
@@ -301,63 +303,58 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kNvPairThreads, 1)
             ptx::tc_fence_before_sync();
             __syncwarp();
             if (lane == 0) {
-                if (leader) {
-                    ptx::mbar_arrive(acc_empty_bar);
-                } else {
-                    ptx::mbar_arrive_cluster(ptx::map_to_cta(ptx::smem_u32(acc_empty_bar), 0));
-                }
+                ptx::mbar_arrive_pair(ptx::map_to_cta(ptx::smem_u32(acc_empty_bar), 0));
             }
             const int row0 = mi * 256 + static_cast<int>(cta_rank) * 128 + quarter * 32;
             const int col0 = ni * 256 + half * 128;
 #pragma unroll
-            for (int b = 0; b < kBoxes; ++b) {
+            for (int b = 0; b < kBoxes; ++b) { // 128 bytes of this thread's row at a time
                 const int bc = col0 + b * kBoxCols;
                 if (bc >= p.n || row0 >= p.m) {
                     break;
                 }
-                if (p.tma_store != 0 && lane == 0) {
-                    ptx::bulk_wait_group_read<0>(); // the box's last store has left shared memory
+                uint32_t o[32];
+#pragma unroll
+                for (int q = 0; q < 32; ++q) {
+                    if constexpr (kOut32) {
+                        o[q] = __float_as_uint(finish(v[b][q], bc + q));
+                    } else {
+                        const int c = 2 * q;
+                        o[q] = nv_pack2<OUT>(finish(v[2 * b + c / 32][c % 32], bc + c), finish(v[2 * b + c / 32][c % 32 + 1], bc + c + 1));
+                    }
                 }
-                __syncwarp();
+                if (p.row_access == 32 && bc + kBoxCols <= p.n) {
+                    // straight from registers: whole 32-byte sectors, nothing to wait for
+                    if (row0 + lane < p.m) {
+                        uint8_t* dst = static_cast<uint8_t*>(p.c) + ((row0 + lane) * p.ldc + bc) * (kOut32 ? 4 : 2);
+#pragma unroll
+                        for (int q = 0; q < 32; q += 8) {
+                            nv_st32(dst + q * 4, make_uint4(o[q], o[q + 1], o[q + 2], o[q + 3]),
+                                    make_uint4(o[q + 4], o[q + 5], o[q + 6], o[q + 7]));
+                        }
+                    }
+                    continue;
+                }
+                // other rows through shared memory (128-byte swizzle), so that a warp's stores lie along rows: with half
+                // sectors from registers 2040x8100x8192 to fp32 (rows on 16-byte boundaries) took 70 us instead of 60
                 uint8_t* line = box + lane * 128;
 #pragma unroll
-                for (int q = 0; q < 8; ++q) { // 16-byte pieces of this thread's row, 128-byte swizzle
-                    uint32_t o[4];
-                    if constexpr (kOut32) {
-#pragma unroll
-                        for (int j = 0; j < 4; ++j) {
-                            const int col = q * 4 + j;
-                            float f = __uint_as_float(v[b][col]) * alpha;
-                            if (p.bias != nullptr && bc + col < p.n) {
-                                f += __ldg(p.bias + bc + col);
-                            }
-                            o[j] = __float_as_uint(f);
-                        }
-                    } else {
-#pragma unroll
-                        for (int j = 0; j < 4; ++j) {
-                            const int col = q * 8 + 2 * j;
-                            float lo = __uint_as_float(v[2 * b + col / 32][col % 32]) * alpha;
-                            float hi = __uint_as_float(v[2 * b + col / 32][col % 32 + 1]) * alpha;
-                            if (p.bias != nullptr) {
-                                lo += bc + col < p.n ? __ldg(p.bias + bc + col) : 0.0f;
-                                hi += bc + col + 1 < p.n ? __ldg(p.bias + bc + col + 1) : 0.0f;
-                            }
-                            o[j] = nv_pack2<OUT>(lo, hi);
-                        }
-                    }
-                    *reinterpret_cast<uint4*>(line + ((q ^ (lane & 7)) * 16)) = make_uint4(o[0], o[1], o[2], o[3]);
+                for (int q = 0; q < 8; ++q) {
+                    *reinterpret_cast<uint4*>(line + ((q ^ (lane & 7)) * 16)) =
+                        make_uint4(o[4 * q], o[4 * q + 1], o[4 * q + 2], o[4 * q + 3]);
                 }
-                if (p.tma_store != 0) {
-                    ptx::fence_proxy_async_smem();
-                    __syncwarp();
-                    if (lane == 0) {
-                        ptx::tma_store_2d(&tmap_c, box, bc, row0);
-                        ptx::bulk_commit_group();
+                __syncwarp();
+                if (p.row_access != 0 && bc + kBoxCols <= p.n) {
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) {
+                        const int r = i * 4 + (lane >> 3);
+                        if (row0 + r < p.m) {
+                            uint8_t* dst = static_cast<uint8_t*>(p.c) + ((row0 + r) * p.ldc + bc) * (kOut32 ? 4 : 2);
+                            reinterpret_cast<uint4*>(dst)[lane & 7] =
+                                *reinterpret_cast<const uint4*>(box + r * 128 + (((lane & 7) ^ (r & 7)) * 16));
+                        }
                     }
                 } else {
-                    // C or its rows off the TMA's 16-byte grid: element by element, a warp along one row at a time
-                    __syncwarp();
                     const int rows_here = min(32, p.m - row0);
                     for (int r = 0; r < rows_here; ++r) {
                         const uint8_t* src = box + r * 128;
@@ -378,12 +375,9 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kNvPairThreads, 1)
                             }
                         }
                     }
-                    __syncwarp();
                 }
+                __syncwarp();
             }
-        }
-        if (lane == 0) {
-            ptx::bulk_wait_group_read<0>(); // shared memory outlives the reads of the last boxes
         }
     }
 

@@ -172,7 +172,7 @@ int launch_nv_pair(cudaStream_t stream, const HostContext& host, const NvProblem
     p.n_tiles = (q.n + 255) / 256;
     p.group_m = 8;
     p.idesc = nv_idesc(256, 256);
-    CUtensorMap ta, tb, tsa, tsb, tc;
+    CUtensorMap ta, tb, tsa, tsb;
     const long long sf_rows_a = (static_cast<long long>(q.m) + 127) / 128 * p.k_atoms * 2;
     const long long sf_rows_b = (static_cast<long long>(q.n) + 127) / 128 * p.k_atoms * 2;
     const CUtensorMapDataType u8 = CU_TENSOR_MAP_DATA_TYPE_UINT8;
@@ -180,22 +180,15 @@ int launch_nv_pair(cudaStream_t stream, const HostContext& host, const NvProblem
     rc = rc ? rc : encode_map_2d(&tb, u8, q.b, q.n, q.k / 2, q.ldb / 2, 128, 128, true);
     rc = rc ? rc : encode_map_2d(&tsa, u8, p.sfa, sf_rows_a, 256, 256, 256, 8, false);
     rc = rc ? rc : encode_map_2d(&tsb, u8, p.sfb, sf_rows_b, 256, 256, 256, 8, false);
-    // C leaves through TMA stores when its base, its row pitch and the end of its rows lie on 16-byte boundaries (at a
-    // ragged end the store unit is a whole 16-byte piece)
     constexpr int esize = OUT == NV_OUT_F32 ? 4 : 2;
-    p.tma_store = !misaligned(p.c, 16) && (p.ldc * esize) % 16 == 0 && (static_cast<long long>(q.n) * esize) % 16 == 0;
-    tc = ta;
-    if (p.tma_store) {
-        const CUtensorMapDataType type = OUT == NV_OUT_F32 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32 : CU_TENSOR_MAP_DATA_TYPE_UINT16;
-        rc = rc ? rc : encode_map_2d(&tc, type, p.c, q.m, q.n, p.ldc * esize, 128 / esize, 32, true);
-    }
+    p.row_access = row_access(p.c, p.ldc * esize);
     if (rc) {
         return rc;
     }
     const long long tiles = static_cast<long long>(p.m_tiles) * p.n_tiles;
     cfg.gridDim = dim3(static_cast<unsigned>(2 * (tiles < clusters ? tiles : clusters)), 1, 1);
     count_launches(1);
-    return note_cuda_error(cudaLaunchKernelEx(&cfg, kernel, ta, tb, tsa, tsb, tc, p), "gemm_nvfp4_2cta launch");
+    return note_cuda_error(cudaLaunchKernelEx(&cfg, kernel, ta, tb, tsa, tsb, p), "gemm_nvfp4_2cta launch");
 }
 
 template <int BLOCK_T, int OUT>
@@ -248,8 +241,12 @@ int launch_nv_few(cudaStream_t stream, const HostContext& host, const NvProblem&
 template <int OUT>
 int launch_nv(cudaStream_t stream, const HostContext& host, const NvProblem& q, const NvGemmParams& p)
 {
+    // CTA pairs once the other kernel's 128 x 128 tiles outnumber the SMs: two of its CTAs then share an SM's tensor core.
+    // Measured, few rows / pairs, us: 256x8192x8192 (32 tiles of 256 x 256) 19.0 / 19.3, 1500x2000x1000 (48) 10.3 / 9.5,
+    // 512x8192x8192 (64) 24.7 / 20.1, 1024x4096x4096 (64) 16.6 / 14.2. With at most 128 rows half of a pair's rows would be
+    // empty: 128x8192x8192 15.8 / 18.7, 48x14336x4096 12.0 / 14.2.
     const long long tiles256 = ((static_cast<long long>(q.m) + 255) / 256) * ((static_cast<long long>(q.n) + 255) / 256);
-    if (q.m > 128 && tiles256 >= host.sm_count / 2) {
+    if (q.m > 128 && 4 * tiles256 > host.sm_count) {
         return launch_nv_pair<OUT>(stream, host, q, p);
     }
     if (q.m <= 16) {
