@@ -29,9 +29,11 @@ struct NvGemmParams {
     long long ldc;      // elements
     int m, n;
     int m_tiles, n_tiles, group_m;
+    int full_units, units; // pair kernel: whole tiles first, then halves (256 x 128) of the last, partly filled wave's
     int k_stages;       // 256-element stages of K
     int k_atoms;        // 64-element groups of K
     uint32_t idesc;
+    uint32_t idesc_half; // pair kernel: of a 256 x 128 half tile
     const float* ga;    // tensor scales, or null for 1
     const float* gb;
     const float* bias;  // n values, or null
@@ -103,22 +105,30 @@ struct NvPairSmem {
 };
 static_assert(NvPairSmem::kTotal <= 227 * 1024, "shared memory of the pair kernel");
 
-__device__ __forceinline__ void nv_tile_coords(int t, const NvGemmParams& p, int& mi, int& ni)
+// A pair's unit of work: a whole 256 x 256 tile, or where the last wave would leave half of the pairs or more without a
+// tile, one 256 x 128 half of a tile (2040x8100x8192, 256 tiles on 74 pairs: four waves become three and a half).
+struct NvUnit {
+    int row, col; // first row and column of C
+    bool half;
+};
+
+__device__ __forceinline__ NvUnit nv_unit(int u, const NvGemmParams& p)
 {
+    const bool half = u >= p.full_units;
+    const int t = half ? p.full_units + ((u - p.full_units) >> 1) : u;
     const int group_size = p.group_m * p.n_tiles;
     const int g = t / group_size;
     const int first_m = g * p.group_m;
     const int gm = min(p.m_tiles - first_m, p.group_m);
     const int r = t - g * group_size;
-    mi = first_m + r % gm;
-    ni = r / gm;
+    return {(first_m + r % gm) * 256, r / gm * 256 + (half ? ((u - p.full_units) & 1) * 128 : 0), half};
 }
 
 template <int OUT>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kNvPairThreads, 1)
     gemm_nvfp4_2cta(const __grid_constant__ CUtensorMap tmap_a, const __grid_constant__ CUtensorMap tmap_b,
-                    const __grid_constant__ CUtensorMap tmap_sfa, const __grid_constant__ CUtensorMap tmap_sfb,
-                    const NvGemmParams p)
+                    const __grid_constant__ CUtensorMap tmap_b_half, const __grid_constant__ CUtensorMap tmap_sfa,
+                    const __grid_constant__ CUtensorMap tmap_sfb, const NvGemmParams p)
 {
     using L = NvPairSmem;
     constexpr int STAGES = kNvPairStages;
@@ -141,8 +151,6 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kNvPairThreads, 1)
     const bool leader = (cta_rank == 0);
     const int pair = blockIdx.x >> 1;
     const int num_pairs = gridDim.x >> 1;
-    const int tiles = p.m_tiles * p.n_tiles;
-
     if (threadIdx.x == 0) {
         for (int s = 0; s < STAGES; ++s) {
             ptx::mbar_init(&full_bar[s], 1);
@@ -173,14 +181,15 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kNvPairThreads, 1)
         int stage = 0;
         uint32_t phase = 0;
         bool ok = true;
-        for (int t = pair; ok && t < tiles; t += num_pairs) {
-            int mi, ni;
-            nv_tile_coords(t, p, mi, ni);
-            const int row_a = mi * 256 + static_cast<int>(cta_rank) * 128;
-            const int row_b = ni * 256 + static_cast<int>(cta_rank) * 128;
+        for (int u = pair; ok && u < p.units; u += num_pairs) {
+            const NvUnit w = nv_unit(u, p);
+            const int row_a = w.row + static_cast<int>(cta_rank) * 128;
+            const int row_b = w.col + static_cast<int>(cta_rank) * (w.half ? 64 : 128);
             // scale tiles as rows of 256 bytes, two per 512-byte tile; tiles past the last row read as zero
-            const int sfa_row = (2 * mi + static_cast<int>(cta_rank)) * p.k_atoms * 2;
-            const int sfb_row = 2 * ni * p.k_atoms * 2;
+            const int sfa_row = row_a / 128 * p.k_atoms * 2;
+            const int sfb_row = w.col / 128 * p.k_atoms * 2;
+            const CUtensorMap* map_b = w.half ? &tmap_b_half : &tmap_b; // of a half tile 64 rows and one tile of scales
+            const uint32_t stage_bytes = 2u * L::kStageBytes - (w.half ? L::kBBytes + L::kSfbBytes : 0u);
             for (int ks = 0; ks < p.k_stages; ++ks) {
                 ok = bounded_wait(&empty_bar[stage], phase ^ 1u, abort_flag, p.status, ST_NV_PRODUCER, p.wait_limit);
                 if (!ok) {
@@ -188,16 +197,19 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kNvPairThreads, 1)
                 }
                 if (ptx::elect_one()) {
                     if (leader) {
-                        ptx::mbar_arrive_expect_tx(&full_bar[stage], 2u * L::kStageBytes);
+                        ptx::mbar_arrive_expect_tx(&full_bar[stage], stage_bytes);
                     }
                     const uint32_t full_addr = ptx::map_to_cta(ptx::smem_u32(&full_bar[stage]), 0);
                     uint8_t* sfa = smem + L::kSfaOff + stage * L::kSfaBytes;
                     uint8_t* sfb = smem + L::kSfbOff + stage * L::kSfbBytes;
                     ptx::tma_load_2d_pair(smem + L::kAOff + stage * L::kABytes, &tmap_a, full_addr, ks * 128, row_a);
-                    ptx::tma_load_2d_pair(smem + L::kBOff + stage * L::kBBytes, &tmap_b, full_addr, ks * 128, row_b);
+                    ptx::tma_load_2d_pair(smem + L::kBOff + stage * L::kBBytes, map_b, full_addr, ks * 128, row_b);
                     ptx::tma_load_2d_pair(sfa, &tmap_sfa, full_addr, 0, sfa_row + ks * 8);
                     ptx::tma_load_2d_pair(sfb, &tmap_sfb, full_addr, 0, sfb_row + ks * 8);
-                    ptx::tma_load_2d_pair(sfb + 4 * kNvAtomBytes, &tmap_sfb, full_addr, 0, sfb_row + p.k_atoms * 2 + ks * 8);
+                    if (!w.half) {
+                        ptx::tma_load_2d_pair(sfb + 4 * kNvAtomBytes, &tmap_sfb, full_addr, 0,
+                                              sfb_row + p.k_atoms * 2 + ks * 8);
+                    }
                 }
                 __syncwarp();
                 if (++stage == STAGES) {
@@ -219,12 +231,13 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kNvPairThreads, 1)
             const uint64_t b_desc0 = ptx::make_smem_desc(ptx::smem_u32(smem + L::kBOff), 16, 1024, ptx::kSwizzle128B);
             const uint64_t sfa_desc0 = ptx::make_smem_desc(ptx::smem_u32(smem + L::kSfaOff), 0, 128, ptx::kSwizzleNone);
             const uint64_t sfb_desc0 = ptx::make_smem_desc(ptx::smem_u32(smem + L::kSfbOff), 0, 128, ptx::kSwizzleNone);
-            for (int t = pair; ok && t < tiles; t += num_pairs) {
+            for (int u = pair; ok && u < p.units; u += num_pairs) {
                 ok = bounded_wait(acc_empty_bar, acc_phase ^ 1u, abort_flag, p.status, ST_NV_MMA, p.wait_limit);
                 if (!ok) {
                     break;
                 }
                 ptx::tc_fence_after_sync();
+                const uint32_t idesc = u < p.full_units ? p.idesc : p.idesc_half;
                 for (int ks = 0; ks < p.k_stages; ++ks) {
                     ok = bounded_wait(&full_bar[stage], phase, abort_flag, p.status, ST_NV_MMA, p.wait_limit);
                     if (!ok) {
@@ -244,13 +257,14 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kNvPairThreads, 1)
                             if (g < groups) {
                                 ptx::tmem_cp_32x128b_warpx4_pair(sf + 4u * g, sfa_desc + 32 * g);
                                 ptx::tmem_cp_32x128b_warpx4_pair(sf + 16u + 8u * g, sfb_desc + 32 * g);
+                                // (of a half tile what the buffer last held: its columns are not read)
                                 ptx::tmem_cp_32x128b_warpx4_pair(sf + 20u + 8u * g, sfb_desc + 128 + 32 * g);
                             }
                         }
 #pragma unroll
                         for (int g = 0; g < 4; ++g) {
                             if (g < groups) {
-                                ptx::umma_nvf4_pair(tmem_base, a_desc + 2 * g, b_desc + 2 * g, p.idesc, sf + 4u * g,
+                                ptx::umma_nvf4_pair(tmem_base, a_desc + 2 * g, b_desc + 2 * g, idesc, sf + 4u * g,
                                                     sf + 16u + 8u * g, (ks > 0 || g > 0) ? 1u : 0u);
                             }
                         }
@@ -283,9 +297,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kNvPairThreads, 1)
         };
         uint32_t acc_phase = 0;
         bool ok = true;
-        for (int t = pair; ok && t < tiles; t += num_pairs) {
-            int mi, ni;
-            nv_tile_coords(t, p, mi, ni);
+        for (int u = pair; ok && u < p.units; u += num_pairs) {
+            const NvUnit w = nv_unit(u, p);
             ok = bounded_wait(acc_full_bar, acc_phase, abort_flag, p.status, ST_NV_EPILOGUE, p.wait_limit);
             ok = __all_sync(0xFFFFFFFFu, ok);
             if (!ok) {
@@ -305,8 +318,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kNvPairThreads, 1)
             if (lane == 0) {
                 ptx::mbar_arrive_pair(ptx::map_to_cta(ptx::smem_u32(acc_empty_bar), 0));
             }
-            const int row0 = mi * 256 + static_cast<int>(cta_rank) * 128 + quarter * 32;
-            const int col0 = ni * 256 + half * 128;
+            const int row0 = w.row + static_cast<int>(cta_rank) * 128 + quarter * 32;
+            const int col0 = w.half && half != 0 ? p.n : w.col + half * 128; // a half tile has no second 128 columns
 #pragma unroll
             for (int b = 0; b < kBoxes; ++b) { // 128 bytes of this thread's row at a time
                 const int bc = col0 + b * kBoxCols;

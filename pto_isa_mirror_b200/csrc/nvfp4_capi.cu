@@ -172,12 +172,22 @@ int launch_nv_pair(cudaStream_t stream, const HostContext& host, const NvProblem
     p.n_tiles = (q.n + 255) / 256;
     p.group_m = 8;
     p.idesc = nv_idesc(256, 256);
-    CUtensorMap ta, tb, tsa, tsb;
+    p.idesc_half = nv_idesc(256, 128);
+    const long long tiles = static_cast<long long>(p.m_tiles) * p.n_tiles;
+    if (tiles > 1 << 29) {
+        return PTO_B200_EINVAL;
+    }
+    const int leftover = static_cast<int>(tiles % clusters);
+    const bool halves = leftover > 0 && 2 * leftover <= clusters;
+    p.full_units = static_cast<int>(tiles) - (halves ? leftover : 0);
+    p.units = static_cast<int>(tiles) + (halves ? leftover : 0);
+    CUtensorMap ta, tb, tb_half, tsa, tsb;
     const long long sf_rows_a = (static_cast<long long>(q.m) + 127) / 128 * p.k_atoms * 2;
     const long long sf_rows_b = (static_cast<long long>(q.n) + 127) / 128 * p.k_atoms * 2;
     const CUtensorMapDataType u8 = CU_TENSOR_MAP_DATA_TYPE_UINT8;
     int rc = encode_map_2d(&ta, u8, q.a, q.m, q.k / 2, q.lda / 2, 128, 128, true);
     rc = rc ? rc : encode_map_2d(&tb, u8, q.b, q.n, q.k / 2, q.ldb / 2, 128, 128, true);
+    rc = rc ? rc : encode_map_2d(&tb_half, u8, q.b, q.n, q.k / 2, q.ldb / 2, 128, 64, true);
     rc = rc ? rc : encode_map_2d(&tsa, u8, p.sfa, sf_rows_a, 256, 256, 256, 8, false);
     rc = rc ? rc : encode_map_2d(&tsb, u8, p.sfb, sf_rows_b, 256, 256, 256, 8, false);
     constexpr int esize = OUT == NV_OUT_F32 ? 4 : 2;
@@ -185,10 +195,9 @@ int launch_nv_pair(cudaStream_t stream, const HostContext& host, const NvProblem
     if (rc) {
         return rc;
     }
-    const long long tiles = static_cast<long long>(p.m_tiles) * p.n_tiles;
-    cfg.gridDim = dim3(static_cast<unsigned>(2 * (tiles < clusters ? tiles : clusters)), 1, 1);
+    cfg.gridDim = dim3(static_cast<unsigned>(2 * (p.units < clusters ? p.units : clusters)), 1, 1);
     count_launches(1);
-    return note_cuda_error(cudaLaunchKernelEx(&cfg, kernel, ta, tb, tsa, tsb, p), "gemm_nvfp4_2cta launch");
+    return note_cuda_error(cudaLaunchKernelEx(&cfg, kernel, ta, tb, tb_half, tsa, tsb, p), "gemm_nvfp4_2cta launch");
 }
 
 template <int BLOCK_T, int OUT>
