@@ -226,9 +226,10 @@ int launch_nv_few(cudaStream_t stream, const HostContext& host, const NvProblem&
     if (n_tiles > 65535 || t_tiles > 65535) {
         return PTO_B200_EINVAL;
     }
-    // K parts: as many as keep all of them resident at two CTAs per SM, each with two stages of K at least
+    // K parts: as many as keep all of them resident at two CTAs per SM, each with four stages of K at least (with two,
+    // 128x4096x4096 took 11.9 us instead of 9.9)
     int splits = 1;
-    while (splits < 8 && n_tiles * t_tiles * splits * 2 <= 2ll * host.sm_count && p.k_stages >= splits * 4) {
+    while (splits < 8 && n_tiles * t_tiles * splits * 2 <= 2ll * host.sm_count && p.k_stages >= splits * 8) {
         splits *= 2;
     }
     cudaLaunchConfig_t cfg = {};
@@ -250,12 +251,13 @@ int launch_nv_few(cudaStream_t stream, const HostContext& host, const NvProblem&
 template <int OUT>
 int launch_nv(cudaStream_t stream, const HostContext& host, const NvProblem& q, const NvGemmParams& p)
 {
-    // CTA pairs once the other kernel's 128 x 128 tiles outnumber the SMs: two of its CTAs then share an SM's tensor core.
-    // Measured, few rows / pairs, us: 256x8192x8192 (32 tiles of 256 x 256) 19.0 / 19.3, 1500x2000x1000 (48) 10.3 / 9.5,
-    // 512x8192x8192 (64) 24.7 / 20.1, 1024x4096x4096 (64) 16.6 / 14.2. With at most 128 rows half of a pair's rows would be
-    // empty: 128x8192x8192 15.8 / 18.7, 48x14336x4096 12.0 / 14.2.
+    // More than 128 rows: CTA pairs, unless the tiles are so few that the other kernel cuts K into four parts or more and K
+    // is long enough to gain by it (beyond eight 256-element stages). Measured, few rows / pairs, us: 512x8192x8192 (64
+    // tiles of 256 x 256) 24.4 / 19.5, 200x8192x4096 (32) 13.8 / 12.0, 200x4096x8192 (16) 13.7 / 16.1, 256x512x8192 (2)
+    // 8.8 / 15.5, 144x512x1024 (2, four stages) 7.4 / 6.5. At most 128 rows: half of a pair's rows would be empty,
+    // 128x8192x8192 15.8 / 17.0, 48x14336x4096 11.6 / 13.5.
     const long long tiles256 = ((static_cast<long long>(q.m) + 255) / 256) * ((static_cast<long long>(q.n) + 255) / 256);
-    if (q.m > 128 && 4 * tiles256 > host.sm_count) {
+    if (q.m > 128 && (8 * tiles256 > host.sm_count || p.k_stages <= 8)) {
         return launch_nv_pair<OUT>(stream, host, q, p);
     }
     if (q.m <= 16) {
