@@ -544,6 +544,11 @@ __global__ void __launch_bounds__(kNvFewThreads, 2)
         ptx::mbar_init(acc_bar, 1);
         *abort_flag = 0;
         ptx::fence_mbar_init();
+    }
+    // The launch may overlap the end of the kernel before it in the stream (programmatic serialisation, 0.6 us of a graph's
+    // step): nothing above touches global memory, and here every thread waits until that kernel's writes can be seen.
+    ptx::grid_dependency_wait();
+    if (threadIdx.x == 0) {
         // the first stages are on their way while tensor memory is set up
         for (int ks = ks0; ks < min(ks1, ks0 + STAGES); ++ks) {
             load_stage(ks, ks - ks0);

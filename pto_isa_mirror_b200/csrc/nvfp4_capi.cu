@@ -233,17 +233,19 @@ int launch_nv_few(cudaStream_t stream, const HostContext& host, const NvProblem&
         splits *= 2;
     }
     cudaLaunchConfig_t cfg = {};
-    cudaLaunchAttribute attr[1];
+    cudaLaunchAttribute attr[2];
     attr[0].id = cudaLaunchAttributeClusterDimension;
     attr[0].val.clusterDim.x = static_cast<unsigned>(splits);
     attr[0].val.clusterDim.y = 1;
     attr[0].val.clusterDim.z = 1;
+    attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization; // the kernel waits for what comes before it itself
+    attr[1].val.programmaticStreamSerializationAllowed = 1;
     cfg.gridDim = dim3(static_cast<unsigned>(splits), static_cast<unsigned>(n_tiles), static_cast<unsigned>(t_tiles));
     cfg.blockDim = dim3(kNvFewThreads, 1, 1);
     cfg.dynamicSmemBytes = L::kTotal;
     cfg.stream = stream;
     cfg.attrs = attr;
-    cfg.numAttrs = 1;
+    cfg.numAttrs = 2;
     count_launches(1);
     return note_cuda_error(cudaLaunchKernelEx(&cfg, kernel, tw, tx, p), "gemm_nvfp4_few_rows launch");
 }

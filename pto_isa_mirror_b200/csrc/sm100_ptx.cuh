@@ -73,6 +73,9 @@ __device__ __forceinline__ bool mbar_try_wait_for(uint64_t* bar, uint32_t parity
     return ok != 0;
 }
 
+// Until the kernels this launch depends on have finished and their memory can be seen.
+__device__ __forceinline__ void grid_dependency_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+
 // True in one lane of a converged warp.
 __device__ __forceinline__ bool elect_one()
 {
