@@ -346,9 +346,9 @@ def mx_quantize_e4m3(src: torch.Tensor, stream: Optional[torch.cuda.Stream] = No
     if k % 32 != 0:
         raise ValueError("K must be a multiple of 32")
     if data is None:
-        data = torch.empty((rows, k), dtype=torch.uint8, device=src.device)
+        data = torch.empty_strided((rows, k), (k, 1), dtype=torch.uint8, device=src.device)
     if scales is None:
-        scales = torch.empty((rows, k // 32), dtype=torch.uint8, device=src.device)
+        scales = torch.empty_strided((rows, k // 32), (k // 32, 1), dtype=torch.uint8, device=src.device)
     for t, shape, name in ((data, (rows, k), "data"), (scales, (rows, k // 32), "scales")):
         _require_cuda_2d(t, name)
         if t.dtype != torch.uint8 or tuple(t.shape) != shape:

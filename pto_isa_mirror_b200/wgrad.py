@@ -7,7 +7,7 @@ import torch
 
 from . import _capi
 from .gemm import _TORCH_TO_PTO, _require_cuda_2d
-from .nvfp4 import _FLOATS, _device_of, _launch, _ptr
+from .nvfp4 import _FLOATS, _device_of, _launch, _new, _ptr
 
 
 def gemm_wgrad_mx(dy: torch.Tensor, data: torch.Tensor, scales: torch.Tensor, out_dtype: torch.dtype = torch.float32,
@@ -46,7 +46,7 @@ def gemm_wgrad_mx(dy: torch.Tensor, data: torch.Tensor, scales: torch.Tensor, ou
             raise ValueError("addend must be [N, K] of dW's type")
 
     def call(sp):
-        o = out if out is not None else torch.empty((n, k), dtype=out_dtype, device=dy.device)
+        o = out if out is not None else _new((n, k), (k, 1), out_dtype, dy)
         rc = lib.pto_b200_gemm_wgrad_mx(sp, o.data_ptr(), dy.data_ptr(), data.data_ptr(), scales.data_ptr(), _ptr(addend), t, n, k,
                                         dy.stride(0) if t > 1 else (n + 7) // 8 * 8, data.stride(0) if t > 1 else (k + 15) // 16 * 16,
                                         scales.stride(0) if t > 1 else k // 32, o.stride(0) if n > 1 else k,
