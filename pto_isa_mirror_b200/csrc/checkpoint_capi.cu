@@ -48,7 +48,7 @@ int launch_wgrad(cudaStream_t stream, const HostContext& host, const uint8_t* dy
                  long long ld_data, WgradParams p)
 {
     auto kernel = gemm_wgrad_mx<F16, OUT>;
-    static std::atomic<int> max_pairs[kMaxDevices];
+    static std::atomic<int> resident[kMaxDevices][3]; // clusters of 2, 4 and 8 CTAs that the device holds at once
     cudaLaunchConfig_t cfg = {};
     cudaLaunchAttribute attr[1];
     attr[0].id = cudaLaunchAttributeClusterDimension;
@@ -60,18 +60,25 @@ int launch_wgrad(cudaStream_t stream, const HostContext& host, const uint8_t* dy
     cfg.stream = stream;
     cfg.attrs = attr;
     cfg.numAttrs = 1;
-    int pairs = max_pairs[host.device].load(std::memory_order_acquire);
-    if (pairs == 0) {
+    int clusters_of[3];
+    for (int i = 2; i >= 0; --i) { // [0], looked at last here and first above, is stored last: it says that all are known
+        clusters_of[i] = resident[host.device][i].load(std::memory_order_acquire);
+    }
+    if (clusters_of[0] == 0) {
         if (int rc = note_cuda_error(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, WgSmem::kTotal),
                                      "cudaFuncSetAttribute(wgrad)")) {
             return rc;
         }
-        cfg.gridDim = dim3(2, 1, 1);
-        if (int rc = note_cuda_error(cudaOccupancyMaxActiveClusters(&pairs, kernel, &cfg), "cudaOccupancyMaxActiveClusters")) {
-            return rc;
+        for (int i = 2; i >= 0; --i) {
+            attr[0].val.clusterDim.x = 2u << i;
+            cfg.gridDim = dim3(2u << i, 1, 1);
+            if (int rc = note_cuda_error(cudaOccupancyMaxActiveClusters(&clusters_of[i], kernel, &cfg),
+                                         "cudaOccupancyMaxActiveClusters")) {
+                return rc;
+            }
+            clusters_of[i] = clusters_of[i] > 0 ? clusters_of[i] : (i == 0 ? 1 : -1);
+            resident[host.device][i].store(clusters_of[i], std::memory_order_release);
         }
-        pairs = pairs > 0 ? pairs : 1;
-        max_pairs[host.device].store(pairs, std::memory_order_release);
     }
     CUtensorMap tdy, tx;
     int rc = encode_map_2d(&tdy, F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, dy, p.t, p.n, ld_dy * 2,
@@ -87,15 +94,29 @@ int launch_wgrad(cudaStream_t stream, const HostContext& host, const uint8_t* dy
     // D fp32 (1 at [4,6)), A and B bf16 (1) or fp16 (0), both with the summed index outermost (bits 15 and 16), 256 x 256
     const uint32_t fmt = F16 ? 0u : 1u;
     p.idesc = (1u << 4) | (fmt << 7) | (fmt << 10) | (1u << 15) | (1u << 16) | ((256u >> 3) << 17) | ((256u >> 4) << 24);
-    // tokens in parts where the tiles leave pairs idle: up to four pairs (one cluster of eight CTAs) per tile, each with
-    // two stages at least
+    // Tokens in parts where that ends sooner: waves of tiles times a part's stages, and what a tile costs besides (filling
+    // the rings, the stores, some 16 stages; the parts' exchange another 8). Fewer clusters of eight CTAs fit the device than
+    // its SMs would hold - 16 tiles in four parts can take two waves - so the waves go by what the device says it holds.
     const long long tiles = static_cast<long long>(p.k_tiles) * p.n_tiles;
     p.splits = 1;
-    while (p.splits < 4 && tiles * p.splits * 2 <= pairs && p.stages >= p.splits * 4) {
-        p.splits *= 2;
+    long long best = 0;
+    for (int i = 0; i < 3; ++i) {
+        const int splits = 1 << i;
+        if (clusters_of[i] <= 0 || (i > 0 && p.stages < 2 * splits)) {
+            continue;
+        }
+        const long long waves = (tiles + clusters_of[i] - 1) / clusters_of[i];
+        const long long cost = waves * ((p.stages + splits - 1) / splits + 16 + (i > 0 ? 8 : 0));
+        if (i == 0 || cost < best) {
+            best = cost;
+            p.splits = splits;
+        }
     }
     attr[0].val.clusterDim.x = static_cast<unsigned>(2 * p.splits);
-    const long long clusters = p.splits > 1 ? tiles : (tiles < pairs ? tiles : pairs);
+    const long long clusters = p.splits > 1 ? tiles : (tiles < clusters_of[0] ? tiles : clusters_of[0]);
+    if (clusters * 2 * p.splits > 0x7FFFFFFFll) {
+        return PTO_B200_EINVAL;
+    }
     cfg.gridDim = dim3(static_cast<unsigned>(2 * p.splits * clusters), 1, 1);
     count_launches(1);
     return note_cuda_error(cudaLaunchKernelEx(&cfg, kernel, tdy, tx, p), "gemm_wgrad_mx launch");

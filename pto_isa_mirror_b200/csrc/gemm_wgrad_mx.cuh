@@ -186,35 +186,6 @@ struct WgElem<WG_OUT_F16> {
     using type = __half;
 };
 
-template <int OUT>
-__device__ __forceinline__ float wg_load(const void* base, long long at)
-{
-    if constexpr (OUT == WG_OUT_F32) {
-        return static_cast<const float*>(base)[at];
-    } else if constexpr (OUT == WG_OUT_BF16) {
-        return __bfloat162float(static_cast<const __nv_bfloat16*>(base)[at]);
-    } else {
-        return __half2float(static_cast<const __half*>(base)[at]);
-    }
-}
-
-// One element of dW: the addend joins in fp32, one rounding to the output's type.
-template <int OUT>
-__device__ __forceinline__ void wg_store(const WgradParams& p, int n, int k, float f)
-{
-    if (p.addend != nullptr) {
-        f += wg_load<OUT>(p.addend, n * p.ld_addend + k);
-    }
-    const long long at = n * p.ld_out + k;
-    if constexpr (OUT == WG_OUT_F32) {
-        static_cast<float*>(p.out)[at] = f;
-    } else if constexpr (OUT == WG_OUT_BF16) {
-        static_cast<__nv_bfloat16*>(p.out)[at] = __float2bfloat16_rn(f);
-    } else {
-        static_cast<__half*>(p.out)[at] = __float2half_rn(f);
-    }
-}
-
 template <bool F16, int OUT>
 __global__ void __launch_bounds__(kWgThreads, 1)
     gemm_wgrad_mx(const __grid_constant__ CUtensorMap tmap_dy, const __grid_constant__ CUtensorMap tmap_x, const WgradParams p)
@@ -544,20 +515,28 @@ __global__ void __launch_bounds__(kWgThreads, 1)
                 const int k = ki * 256 + side * 128 + in_tile;
                 const int n0 = ni * 256 + group * 64;
                 if (k < p.k) {
-                    if (p.addend == nullptr && n0 + 64 <= p.n) {
-                        using T = typename WgElem<OUT>::type;
-                        T* at = static_cast<T*>(p.out) + n0 * p.ld_out + k;
+                    using T = typename WgElem<OUT>::type;
+                    T* at = static_cast<T*>(p.out) + n0 * p.ld_out + k;
+                    const T* add = static_cast<const T*>(p.addend) + (p.addend != nullptr ? n0 * p.ld_addend + k : 0);
 #pragma unroll
-                        for (int i = 0; i < 64; ++i) {
-                            *at = static_cast<T>(sum[i]);
-                            at += p.ld_out;
-                        }
-                    } else {
+                    for (int i0 = 0; i0 < 64; i0 += 16) {
+                        if (p.addend != nullptr) { // sixteen reads in flight, before the stores: addend may be out
+                            T v[16];
 #pragma unroll
-                        for (int i = 0; i < 64; ++i) {
-                            if (n0 + i < p.n) {
-                                wg_store<OUT>(p, n0 + i, k, sum[i]);
+                            for (int i = 0; i < 16; ++i) {
+                                v[i] = n0 + i0 + i < p.n ? add[(i0 + i) * p.ld_addend] : static_cast<T>(0.0f);
                             }
+#pragma unroll
+                            for (int i = 0; i < 16; ++i) {
+                                sum[i0 + i] += static_cast<float>(v[i]);
+                            }
+                        }
+#pragma unroll
+                        for (int i = 0; i < 16; ++i) {
+                            if (n0 + i0 + i < p.n) {
+                                *at = static_cast<T>(sum[i0 + i]); // one rounding to the output's type
+                            }
+                            at += p.ld_out;
                         }
                     }
                 }
@@ -613,10 +592,20 @@ __global__ void __launch_bounds__(kWgThreads, 1)
                         f.w += part[s].w;
                     }
                 }
-                wg_store<OUT>(p, n, k, f.x);
-                wg_store<OUT>(p, n, k + 1, f.y);
-                wg_store<OUT>(p, n, k + 2, f.z);
-                wg_store<OUT>(p, n, k + 3, f.w);
+                using T = typename WgElem<OUT>::type;
+                if (p.addend != nullptr) {
+                    const T* add = static_cast<const T*>(p.addend) + n * p.ld_addend + k;
+                    const T v[4] = {add[0], add[1], add[2], add[3]};
+                    f.x += static_cast<float>(v[0]);
+                    f.y += static_cast<float>(v[1]);
+                    f.z += static_cast<float>(v[2]);
+                    f.w += static_cast<float>(v[3]);
+                }
+                T* at = static_cast<T*>(p.out) + n * p.ld_out + k;
+                at[0] = static_cast<T>(f.x);
+                at[1] = static_cast<T>(f.y);
+                at[2] = static_cast<T>(f.z);
+                at[3] = static_cast<T>(f.w);
             }
         }
         ptx::cluster_arrive_relaxed(); // no CTA leaves while another still reads its shared memory
