@@ -9,6 +9,8 @@ namespace pto_b200 {
 
 constexpr int kMaxDevices = 64;
 
+constexpr int kMaxExtent = 0x7FFFF000; // of a matrix: kernels count past it in steps of a tile
+
 struct HostContext {
     int device;           // ordinal of the current device, below kMaxDevices
     int sm_count;

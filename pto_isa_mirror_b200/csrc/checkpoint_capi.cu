@@ -134,7 +134,8 @@ extern "C" int pto_b200_mx_quantize_e4m3_src(void* stream, uint8_t* data, uint8_
     if (src_dtype == PTO_B200_F32) {
         return pto_b200_mx_quantize_e4m3_ex(stream, data, scales, src, rows, k, ld_src, ld_data, ld_scales, scale_alg);
     }
-    if (data == nullptr || scales == nullptr || src == nullptr || rows <= 0 || k <= 0 || k % 32 != 0 || ld_src < k ||
+    if (data == nullptr || scales == nullptr || src == nullptr || rows <= 0 || k <= 0 || rows > kMaxExtent || k > kMaxExtent ||
+        k % 32 != 0 || ld_src < k ||
         ld_data < k || ld_scales < k / 32) {
         return PTO_B200_EINVAL;
     }
@@ -164,7 +165,8 @@ extern "C" int pto_b200_gemm_wgrad_mx(void* stream, uint8_t* out, const uint8_t*
         (out_dtype != PTO_B200_F32 && out_dtype != PTO_B200_BF16 && out_dtype != PTO_B200_F16)) {
         return PTO_B200_EDTYPE;
     }
-    if (out == nullptr || dy == nullptr || data == nullptr || scales == nullptr || t <= 0 || n <= 0 || k <= 0 || k % 32 != 0 ||
+    if (out == nullptr || dy == nullptr || data == nullptr || scales == nullptr || t <= 0 || n <= 0 || k <= 0 || t > kMaxExtent ||
+        n > kMaxExtent || k > kMaxExtent || k % 32 != 0 ||
         ld_dy < n || ld_data < k || ld_scales < k / 32 || ld_scales >= (1 << 26) || ld_out < k ||
         (addend != nullptr && ld_addend < k)) { // offsets within a stage's scales are 32-bit
         return PTO_B200_EINVAL;

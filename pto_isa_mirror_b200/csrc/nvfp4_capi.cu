@@ -289,7 +289,8 @@ extern "C" size_t pto_b200_nvfp4_scale_bytes(int rows, int k)
 
 extern "C" int pto_b200_amax(void* stream, float* amax, const uint8_t* src, int rows, int k, long long ld_src, int src_dtype)
 {
-    if (amax == nullptr || src == nullptr || rows <= 0 || k <= 0 || ld_src < k) {
+    if (amax == nullptr || src == nullptr || rows <= 0 || k <= 0 || rows > kMaxExtent ||
+        k > kMaxExtent || ld_src < k) {
         return PTO_B200_EINVAL;
     }
     const int type = source_of(src_dtype);
@@ -313,7 +314,7 @@ extern "C" int pto_b200_nvfp4_quantize(void* stream, uint8_t* data, uint8_t* sca
 {
     const long long length = transpose ? rows : k; // of the result's rows
     if (data == nullptr || scales == nullptr || tensor_scale == nullptr || src == nullptr || amax == nullptr || rows <= 0 ||
-        k <= 0 || ld_src < k || ld_data < (length + 15) / 16 * 8) {
+        k <= 0 || rows > kMaxExtent || k > kMaxExtent || ld_src < k || ld_data < (length + 15) / 16 * 8) {
         return PTO_B200_EINVAL;
     }
     const int type = source_of(src_dtype);
@@ -338,7 +339,7 @@ extern "C" int pto_b200_nvfp4_dequantize(void* stream, uint8_t* out, const uint8
                                          int out_dtype)
 {
     if (out == nullptr || data == nullptr || scales == nullptr || rows <= 0 || k <= 0 ||
-        ld_data < (static_cast<long long>(k) + 7) / 8 * 4 || ld_out < k) {
+        rows > kMaxExtent || k > kMaxExtent || ld_data < (static_cast<long long>(k) + 7) / 8 * 4 || ld_out < k) {
         return PTO_B200_EINVAL;
     }
     const int type = source_of(out_dtype);
@@ -368,7 +369,7 @@ extern "C" int pto_b200_gemm_nvfp4(void* stream, uint8_t* out, const uint8_t* sr
         return PTO_B200_EDTYPE;
     }
     if (out == nullptr || src0 == nullptr || src1 == nullptr || src2 == nullptr || src3 == nullptr || m <= 0 || n <= 0 ||
-        k <= 0 || k % 16 != 0 || lda < k || ldb < k || ldc < n) {
+        k <= 0 || m > kMaxExtent || n > kMaxExtent || k > kMaxExtent || k % 16 != 0 || lda < k || ldb < k || ldc < n) {
         return PTO_B200_EINVAL;
     }
     if (misaligned(src0, 16) || misaligned(src1, 16) || lda % 32 != 0 || ldb % 32 != 0 || misaligned(src2, 16) ||

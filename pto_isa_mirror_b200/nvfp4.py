@@ -17,6 +17,9 @@ from . import _capi
 from .gemm import _TORCH_TO_PTO, _raw_stream, _require_cuda_2d
 
 _FLOATS = (torch.float32, torch.bfloat16, torch.float16)
+# what packed codes and scale bytes may come as
+_CODES = (torch.uint8, torch.int8) + ((torch.float4_e2m1fn_x2,) if hasattr(torch, "float4_e2m1fn_x2") else ())
+_E4M3_BYTES = (torch.uint8, torch.float8_e4m3fn)
 
 
 def _device_of(first: torch.Tensor, *others: Optional[torch.Tensor]) -> int:
@@ -49,8 +52,8 @@ def _tiles(rows: int, k: int) -> Tuple[int, int, int]:
 
 
 def _require_scales(t: torch.Tensor, rows: int, k: int, name: str) -> None:
-    if not t.is_cuda or t.element_size() != 1 or not t.is_contiguous() or t.shape != _tiles(rows, k):
-        raise ValueError(f"{name} must be contiguous scale tiles of shape {_tiles(rows, k)} in one-byte elements")
+    if not t.is_cuda or t.dtype not in _E4M3_BYTES or not t.is_contiguous() or t.shape != _tiles(rows, k):
+        raise ValueError(f"{name} must be contiguous CUDA scale tiles of shape {_tiles(rows, k)}, uint8 or float8_e4m3fn")
 
 
 def _new(size, stride, dtype: torch.dtype, like: torch.Tensor) -> torch.Tensor:
@@ -125,11 +128,11 @@ def nvfp4_dequantize(data: torch.Tensor, scales: torch.Tensor, tensor_scale: Opt
                      stream: Optional[torch.cuda.Stream] = None) -> torch.Tensor:
     """The numbers [rows, K] that packed codes data [rows, K / 2] with their scale tiles stand for: code * scale *
     tensor_scale (None: 1), float32, bfloat16 or float16. Exact before the output's own rounding when tensor_scale is a
-    power of two. ``out`` may be narrower than K: the first columns are written."""
+    power of two. ``out`` may lack up to 15 of the last columns, those that filled up the last block."""
     lib = _capi.load()
     _require_cuda_2d(data, "data")
-    if data.element_size() != 1:
-        raise ValueError("data must have one-byte elements")
+    if data.dtype not in _CODES:
+        raise ValueError("data must be packed codes, uint8")
     rows, k = data.shape[0], data.shape[1] * 2
     if rows == 0 or k == 0:
         raise ValueError("data must not be empty")
@@ -137,8 +140,8 @@ def nvfp4_dequantize(data: torch.Tensor, scales: torch.Tensor, tensor_scale: Opt
     _require_float_scalar(tensor_scale, "tensor_scale")
     if out is not None:
         _require_cuda_2d(out, "out")
-        if out.dtype not in _FLOATS or out.shape[0] != rows or not 0 < out.shape[1] <= k or _tiles(rows, out.shape[1]) != _tiles(rows, k):
-            raise ValueError("out must be [rows, K] float32, bfloat16 or float16")
+        if out.dtype not in _FLOATS or out.shape[0] != rows or not k - 16 < out.shape[1] <= k:
+            raise ValueError("out must be [rows, K] float32, bfloat16 or float16, K less at most the last 15 columns")
     elif out_dtype not in _FLOATS:
         raise ValueError("out_dtype must be float32, bfloat16 or float16")
 
@@ -166,8 +169,8 @@ def gemm_nvfp4(a: torch.Tensor, b_dn: torch.Tensor, sfa: torch.Tensor, sfb: torc
     lib = _capi.load()
     for t, name in ((a, "a"), (b_dn, "b_dn")):
         _require_cuda_2d(t, name)
-        if t.element_size() != 1:
-            raise ValueError(f"{name} must have one-byte elements")
+        if t.dtype not in _CODES:
+            raise ValueError(f"{name} must be packed codes, uint8")
     m, n, k = a.shape[0], b_dn.shape[0], a.shape[1] * 2
     if b_dn.shape[1] * 2 != k:
         raise ValueError("inner dimensions differ")

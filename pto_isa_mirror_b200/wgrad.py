@@ -25,8 +25,8 @@ def gemm_wgrad_mx(dy: torch.Tensor, data: torch.Tensor, scales: torch.Tensor, ou
         _require_cuda_2d(t, name)
     if dy.dtype not in (torch.bfloat16, torch.float16):
         raise ValueError("dy must be bfloat16 or float16")
-    if data.element_size() != 1 or scales.element_size() != 1:
-        raise ValueError("data and scales must have one-byte elements")
+    if data.dtype not in (torch.uint8, torch.float8_e4m3fn) or scales.element_size() != 1:
+        raise ValueError("data must be e4m3 bytes (uint8 or float8_e4m3fn) and scales e8m0 bytes")
     t, n = dy.shape
     k = data.shape[1]
     if data.shape[0] != t:

@@ -182,3 +182,98 @@ def test_captured_and_replayed():
     graph.replay()
     torch.cuda.synchronize()
     assert torch.equal(out.double(), dy.double().t() @ x)
+
+
+def test_python_refusals():
+    data, scales, _ = kept(64, 64, 3, True)
+    dy = torch.zeros((64, 48), dtype=torch.bfloat16, device=DEV)
+    out = torch.zeros((48, 64), device=DEV)
+    bad = [
+        lambda: pto.gemm_wgrad_mx(dy.float(), data, scales), lambda: pto.gemm_wgrad_mx(dy[:63], data, scales),
+        lambda: pto.gemm_wgrad_mx(dy.t(), data, scales), lambda: pto.gemm_wgrad_mx(dy, data[:, :48], scales),
+        lambda: pto.gemm_wgrad_mx(dy, data, scales[:, :1]), lambda: pto.gemm_wgrad_mx(dy, data.float(), scales),
+        lambda: pto.gemm_wgrad_mx(dy, data.view(torch.float8_e5m2), scales), lambda: pto.gemm_wgrad_mx(dy[:, :0], data, scales),
+        lambda: pto.gemm_wgrad_mx(dy, data, scales, out_dtype=torch.float64), lambda: pto.gemm_wgrad_mx(dy, data, scales, out=out.t()),
+        lambda: pto.gemm_wgrad_mx(dy, data, scales, out=out[:, :32]), lambda: pto.gemm_wgrad_mx(dy, data, scales, addend=out.half()),
+        lambda: pto.gemm_wgrad_mx(dy, data, scales, addend=out[:40]),
+        lambda: pto.mx_quantize_e4m3(dy.double()), lambda: pto.mx_quantize_e4m3(dy[:, :40]),
+    ]
+    for call in bad:
+        with pytest.raises(ValueError):
+            call()
+    for call in (lambda: pto.gemm_wgrad_mx(dy[:, 1:], data, scales), lambda: pto.gemm_wgrad_mx(dy, data[:, :32].as_strided((64, 32), (72, 1)), scales[:, :1])):
+        with pytest.raises(pto.PtoB200Error) as e:
+            call()
+        assert e.value.code == 2
+
+
+def test_rows_of_nan_and_infinity_stay_theirs():
+    data, scales, x = kept(700, 96, 4, True)
+    dy = pitched(torch.randint(-2, 3, (700, 70), generator=gen(5)).to(torch.bfloat16), 8, 0)
+    dy[100, 3] = float("nan")
+    dy[650, 60] = float("inf")
+    scales[:, :1][300] = 255
+    got = pto.gemm_wgrad_mx(dy, data, scales).cpu()
+    bad = torch.zeros((70, 96), dtype=torch.bool)
+    bad[3] = bad[60] = True
+    bad[:, :32] = True
+    assert not torch.isfinite(got[3]).any() and not torch.isfinite(got[:, :32]).any()
+    assert torch.isfinite(got[~bad].view(-1)).all()
+
+
+def test_past_two_to_the_31_elements():
+    t, k, n = 66000, 32768, 16
+    data = torch.zeros((t, k), dtype=torch.uint8, device=DEV)
+    scales = torch.full((t, k // 32), 127, dtype=torch.uint8, device=DEV)
+    data[-3:] = torch.randint(0, 0x7F, (3, k), generator=gen(1), dtype=torch.uint8).to(DEV)
+    scales[-1, -1] = 129
+    dy = torch.zeros((t, n), dtype=torch.bfloat16, device=DEV)
+    dy[-3:] = torch.randint(-2, 3, (3, n), generator=gen(2)).to(torch.bfloat16).to(DEV)
+    got = pto.gemm_wgrad_mx(dy, data, scales)
+    x = data[-3:].view(torch.float8_e4m3fn).double()
+    x[-1, -32:] *= 4
+    assert torch.equal(got.double(), dy[-3:].double().t() @ x)  # at most 3 * 2 * 1792 in steps of 2^-9: exact
+
+
+# ------------------------------------------------------------------ together: one linear layer, forward and backward
+
+@pytest.mark.parametrize("t,n,k", [(1, 48, 96), (37, 200, 160), (700, 520, 1056), (2500, 768, 512)])
+def test_a_linear_layers_step(t, n, k):
+    """y = x W^T in 4 bits, x kept in 8, dx in 4 bits from the transposed weight, dW from what was kept - each against
+    64 bits on the numbers that were quantised, and dW against differences of the layer's own (linear) loss."""
+    import nvfp4_reference as ref
+
+    x = torch.randn((t, k), generator=gen(1)).to(torch.bfloat16).to(DEV)
+    w = (torch.randn((n, k), generator=gen(2)) * 0.05).to(torch.bfloat16).to(DEV)
+    dy = (torch.randn((t, n), generator=gen(3)) * 0.1).to(torch.bfloat16).to(DEV)
+
+    xq, wq = pto.nvfp4_quantize(x), pto.nvfp4_quantize(w)
+    y = pto.gemm_nvfp4(xq[0], wq[0], xq[1], wq[1], xq[2], wq[2], out_dtype=torch.float32)
+    kept_data, kept_scales = pto.mx_quantize_e4m3(x)
+
+    wtq, dyq = pto.nvfp4_quantize(w, transpose=True), pto.nvfp4_quantize(dy)
+    dx = pto.gemm_nvfp4(dyq[0], wtq[0], dyq[1], wtq[1], dyq[2], wtq[2], out_dtype=torch.float32)
+    dw = pto.gemm_wgrad_mx(dy, kept_data, kept_scales)
+
+    def number(q):
+        return ref.values(q[0].cpu(), q[1].cpu()).to(DEV) * q[2].double()
+
+    def near(got, a, b, steps):
+        size = a.abs() @ b.abs().t()
+        assert ((got.double() - a @ b.t()).abs() <= size * ((steps + 4) * 2.0 ** -22)).all()
+
+    near(y, number(xq), number(wq), (k + 63) // 64)
+    near(dx, number(dyq), number(wtq), (n + 63) // 64)
+    x8 = kept_data.view(torch.float8_e4m3fn).double().view(t, -1, 32) * torch.exp2(kept_scales.double() - 127)[:, :, None]
+    x8 = x8.view(t, k)
+    near(dw, dy.double().t(), x8.t(), min(t, 2048) // 16 + 1 + t // 2048)
+    # the loss sum(dy * (x8 W^T)) is linear in W: its difference along any direction is dW's product with it
+    direction = torch.randn((n, k), generator=gen(4)).double().to(DEV)
+    wd = w.double()
+    rise = ((dy.double() * (x8 @ (wd + direction).t())).sum() - (dy.double() * (x8 @ wd.t())).sum())
+    spread = (dy.double().abs().t() @ x8.abs() * direction.abs()).sum()
+    assert abs(float(rise - (dw.double() * direction).sum())) <= float(spread) * (min(t, 2048) / 16 + t // 2048 + 6) * 2.0 ** -22
+    # the numbers themselves lie where four and eight bits put them: half a step of e2m1 (1/4 of a value's octave or a
+    # sixth of the block's largest) and of e4m3
+    assert float((number(xq) - x.double()).norm() / x.double().norm()) < 0.25
+    assert float((x8 - x.double()).norm() / x.double().norm()) < 2.0 ** -4

@@ -153,8 +153,10 @@ def check_product(m, n, k, out_dtype, bias, seed, out=None, extra=0):
     return got
 
 
-FEW = [(1, 16, 16), (1, 8, 4096), (7, 130, 48), (16, 256, 64), (17, 100, 272), (32, 1000, 512), (33, 384, 1040), (64, 129, 4096),
-       (65, 640, 336), (128, 128, 8192), (129, 200, 256), (200, 1111, 768), (1000, 300, 1312), (3, 20000, 256)]
+# up to 128 rows, and more of them where K is long beside few tiles; K cut over up to eight CTAs, or not at all
+FEW = [(1, 16, 16), (1, 1, 16), (1, 8, 4096), (7, 130, 48), (16, 256, 64), (17, 100, 272), (32, 1000, 512), (33, 384, 1040),
+       (64, 129, 4096), (65, 640, 336), (128, 128, 8192), (128, 1300, 6160), (129, 200, 2320), (300, 500, 4112), (1000, 300, 2576),
+       (3, 20000, 256)]
 
 
 @pytest.mark.parametrize("m,n,k", FEW)
@@ -163,10 +165,137 @@ def test_product_few_rows(m, n, k, out_dtype, bias):
     check_product(m, n, k, out_dtype, bias, m + n + k)
 
 
-MANY = [(2304, 2304, 256), (2049, 2561, 272), (4000, 1801, 1040), (300, 20001, 80), (2560, 2312, 1808)]
+# pairs of CTAs: less than one wave (halves of tiles), whole waves and ragged last ones, rows of C on 32, 16 and fewer bytes
+MANY = [(129, 200, 256), (144, 512, 1024), (200, 1111, 768), (2304, 2304, 256), (2049, 2561, 272), (4000, 1801, 1040),
+        (300, 20001, 80), (2560, 2312, 1808), (1000, 2004, 2320), (6000, 5000, 16)]
 
 
 @pytest.mark.parametrize("m,n,k", MANY)
 @pytest.mark.parametrize("out_dtype,bias", [(torch.float32, False), (torch.bfloat16, True), (torch.float16, False)])
 def test_product_many_rows(m, n, k, out_dtype, bias):
     check_product(m, n, k, out_dtype, bias, m + n + k)
+
+
+@pytest.mark.parametrize("m,n,k", [(5, 333, 304), (300, 333, 304), (2600, 2900, 304)])
+@pytest.mark.parametrize("offset", [0, 1, 4])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_product_into_a_part_of_a_buffer(m, n, k, offset, dtype):
+    # operands with rows 48 bytes further apart than they need; C anywhere in a buffer whose rest stays as it was
+    buf = torch.full((m + 2, n + 11), 5.0, dtype=dtype, device=DEV)
+    out = buf[1:m + 1, offset:offset + n]
+    assert check_product(m, n, k, dtype, True, m + offset, out=out, extra=48) is out
+    assert (buf[0] == 5).all() and (buf[m + 1] == 5).all() and (buf[:, :offset] == 5).all() and (buf[:, offset + n:] == 5).all()
+
+
+def test_quantize_into_given_buffers():
+    x, host = wide(70, 90, torch.bfloat16, 1)
+    data = torch.full((70, 64), 0xAB, dtype=torch.uint8, device=DEV)
+    scales = torch.full((1, 2, 512), 0xCD, dtype=torch.uint8, device=DEV)
+    g = torch.full((1,), -1.0, device=DEV)
+    got = pto.nvfp4_quantize(x, data=data[:, :48], scales=scales, tensor_scale=g)
+    assert got[1] is scales and got[2] is g
+    check_quantized(got, *ref.quantize(host), 70)
+    assert (data[:, 48:] == 0xAB).all()
+
+
+def test_scales_of_zero_and_masked_rows():
+    # a row of zeros beside others: its scales and codes are zero, and so is its row of the product
+    host = torch.randn((20, 64), generator=torch.Generator().manual_seed(9))
+    host[7] = 0.0
+    a = pto.nvfp4_quantize(host.to(DEV))
+    w = pto.nvfp4_quantize(torch.randn((33, 64), generator=torch.Generator().manual_seed(10)).to(DEV))
+    out = pto.gemm_nvfp4(a[0], w[0], a[1], w[1], a[2], w[2], out_dtype=torch.float32)
+    assert (out[7] == 0).all() and (out[[6, 8]] != 0).any(1).all()
+    zero = pto.nvfp4_quantize(torch.zeros((3, 32), device=DEV))
+    assert float(zero[2]) == 1.0 and (zero[0] == 0).all() and (zero[1] == 0).all()
+
+
+def test_results_do_not_depend_on_the_stream_or_the_call():
+    side = torch.cuda.Stream()
+    for m, n, k in ((48, 700, 4096), (600, 3000, 1024)):
+        x, w = torch.randn((m, k), device=DEV, dtype=torch.bfloat16), torch.randn((n, k), device=DEV, dtype=torch.bfloat16)
+        side.wait_stream(torch.cuda.current_stream())
+        outs = []
+        for i in range(6):
+            s = side if i % 2 else None
+            a, b = pto.nvfp4_quantize(x, stream=s), pto.nvfp4_quantize(w, stream=s)
+            outs.append(pto.gemm_nvfp4(a[0], b[0], a[1], b[1], a[2], b[2], stream=s))
+        torch.cuda.synchronize()
+        assert all(torch.equal(outs[0], o) for o in outs)
+
+
+@pytest.mark.parametrize("m", [1, 40, 700])
+def test_captured_and_replayed(m):
+    k, n = 768, 900
+    x = torch.randn((m, k), device=DEV, dtype=torch.bfloat16)
+    w = pto.nvfp4_quantize(torch.randn((n, k), device=DEV))
+    out, again = torch.empty((m, n), device=DEV), torch.empty((m, n), device=DEV)
+
+    def step(into):
+        a = pto.nvfp4_quantize(x)
+        pto.gemm_nvfp4(a[0], w[0], a[1], w[1], a[2], w[2], out=into)
+
+    step(out)  # warm: what is set up once per device
+    graphs = []
+    for into in (out, again):  # two graphs alive at once
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            step(into)
+        graphs.append(g)
+    x.mul_(-3.0)
+    for _ in range(3):
+        for g in graphs:
+            g.replay()
+    want = torch.empty((m, n), device=DEV)
+    step(want)
+    torch.cuda.synchronize()
+    assert torch.equal(out, want) and torch.equal(again, want)
+
+
+def test_python_refusals():
+    x = torch.randn((8, 64), device=DEV)
+    data, scales, g = pto.nvfp4_quantize(x)
+    bad = [
+        lambda: pto.nvfp4_quantize(x.double()), lambda: pto.nvfp4_quantize(x[:, ::2]), lambda: pto.nvfp4_quantize(x[0]),
+        lambda: pto.nvfp4_quantize(x[:0]), lambda: pto.nvfp4_quantize(x, amax=torch.ones(2, device=DEV)),
+        lambda: pto.nvfp4_quantize(x, amax=torch.ones(1)), lambda: pto.nvfp4_quantize(x, data=data[:, :16]),
+        lambda: pto.nvfp4_quantize(x, scales=scales[:, :, :256]), lambda: pto.nvfp4_quantize(x, tensor_scale=g.double()),
+        lambda: pto.nvfp4_dequantize(data, scales[:, :0]), lambda: pto.nvfp4_dequantize(data, scales, out_dtype=torch.int32),
+        lambda: pto.nvfp4_dequantize(data, scales, out=x[:, :40]), lambda: pto.nvfp4_dequantize(x, scales),
+        lambda: pto.gemm_nvfp4(data, data[:, :24], scales, scales), lambda: pto.gemm_nvfp4(data, data, scales, scales.view(1, 512, 1)),
+        lambda: pto.gemm_nvfp4(data.view(torch.float8_e4m3fn), data, scales, scales),
+        lambda: pto.gemm_nvfp4(data[:, :4], data[:, :4], scales, scales),
+        lambda: pto.gemm_nvfp4(data, data, scales, scales, ga=torch.ones(2, device=DEV)),
+        lambda: pto.gemm_nvfp4(data, data, scales, scales, bias=torch.ones(7, device=DEV)),
+        lambda: pto.gemm_nvfp4(data, data, scales, scales, bias=torch.ones(8, device=DEV).half()),
+        lambda: pto.gemm_nvfp4(data, data, scales, scales, out=x), lambda: pto.gemm_nvfp4(data, data, scales, scales, out_dtype=torch.int8),
+    ]
+    for call in bad:
+        with pytest.raises(ValueError):
+            call()
+    shifted = torch.zeros(8 * 32 + 8, dtype=torch.uint8, device=DEV)[8:].view(8, 32)  # off the 16-byte boundary
+    with pytest.raises(pto.PtoB200Error) as e:
+        pto.gemm_nvfp4(shifted, data, scales, scales)
+    assert e.value.code == 2
+
+
+def test_past_two_to_the_31_elements():
+    rows, k = 65664, 32832  # 2^31 + 8e6 elements
+    x = torch.empty((rows, k), dtype=torch.bfloat16, device=DEV)
+    for r in range(0, rows, 4104):
+        x[r:r + 4104].normal_(generator=torch.Generator(DEV).manual_seed(r))
+    amax = torch.tensor([6.0], device=DEV)
+    data, scales, g = pto.nvfp4_quantize(x, amax=amax)
+    tail = pto.nvfp4_quantize(x[-128:], amax=amax)
+    assert torch.equal(data[-128:], tail[0]) and torch.equal(scales[-1], tail[1][0])
+    back = pto.nvfp4_dequantize(data, scales, g)
+    assert torch.equal(back[-128:], pto.nvfp4_dequantize(tail[0], tail[1], g))
+    del back
+    turned = pto.nvfp4_quantize(x, amax=amax, transpose=True)
+    assert torch.equal(turned[0][:, -32:], pto.nvfp4_quantize(x[-64:], amax=amax, transpose=True)[0])
+    del x, turned
+    # a product with as many results
+    a, b = (data[:, :32], scales[:, :1].contiguous()), (data[:k, 32:64], scales[:(k + 127) // 128, 1:2].contiguous())
+    c = pto.gemm_nvfp4(a[0], b[0], a[1], b[1][:(k + 127) // 128])
+    want = pto.gemm_nvfp4(a[0][-128:], b[0], a[1][-1:], b[1][:(k + 127) // 128])
+    assert torch.equal(c[-128:], want)
