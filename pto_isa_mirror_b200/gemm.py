@@ -345,14 +345,15 @@ def mx_quantize_e4m3(src: torch.Tensor, stream: Optional[torch.cuda.Stream] = No
     rows, k = src.shape
     if k % 32 != 0:
         raise ValueError("K must be a multiple of 32")
+    for t, shape, name in ((data, (rows, k), "data"), (scales, (rows, k // 32), "scales")):
+        if t is not None:
+            _require_cuda_2d(t, name)
+            if t.dtype != torch.uint8 or tuple(t.shape) != shape:
+                raise ValueError(f"{name} must be a uint8 CUDA tensor of shape {shape}")
     if data is None:
         data = torch.empty_strided((rows, k), (k, 1), dtype=torch.uint8, device=src.device)
     if scales is None:
         scales = torch.empty_strided((rows, k // 32), (k // 32, 1), dtype=torch.uint8, device=src.device)
-    for t, shape, name in ((data, (rows, k), "data"), (scales, (rows, k // 32), "scales")):
-        _require_cuda_2d(t, name)
-        if t.dtype != torch.uint8 or tuple(t.shape) != shape:
-            raise ValueError(f"{name} must be a uint8 CUDA tensor of shape {shape}")
     rc = lib.pto_b200_mx_quantize_e4m3_src(_stream_ptr(stream), data.data_ptr(), scales.data_ptr(), src.data_ptr(), rows,
                                            k, src.stride(0), data.stride(0), scales.stride(0), _TORCH_TO_PTO[src.dtype],
                                            scale_alg)

@@ -31,15 +31,14 @@ def _device_of(first: torch.Tensor, *others: Optional[torch.Tensor]) -> int:
     return device
 
 
-def _launch(device: int, stream: Optional[torch.cuda.Stream], call):
-    """``call(raw stream)`` with ``device`` current, on ``stream`` or the device's current one; what it allocates belongs to
-    that stream."""
-    if stream is None and device == torch.cuda.current_device():
-        return call(_raw_stream(device))
-    if stream is not None and stream.device_index != device:
+def _elsewhere(device: int, stream: Optional[torch.cuda.Stream]):
+    """None when launches go to the current stream of the current device, which is ``device``; otherwise a context in which
+    they do, ``stream`` being that stream when one is given - and in which what is allocated belongs to it."""
+    if stream is None:
+        return None if device == torch.cuda.current_device() else torch.cuda.device(device)
+    if stream.device_index != device:
         raise ValueError("stream is on another device than the tensors")
-    with torch.cuda.device(device) if stream is None else torch.cuda.stream(stream):
-        return call(_raw_stream(device))
+    return torch.cuda.stream(stream)
 
 
 def _require_float_scalar(t: Optional[torch.Tensor], name: str) -> None:
@@ -98,29 +97,30 @@ def nvfp4_quantize(src: torch.Tensor, amax: Optional[torch.Tensor] = None, trans
             raise ValueError(f"data must be uint8 of shape {(out_rows, width)}")
     if scales is not None:
         _require_scales(scales, out_rows, length, "scales")
+    device = _device_of(src, amax, data, scales, tensor_scale)
+    there = _elsewhere(device, stream)
+    if there is not None:
+        with there:
+            return nvfp4_quantize(src, amax, transpose, data, scales, tensor_scale)
+    sp = _raw_stream(device)
     pitch = (width + 15) // 16 * 16  # TMA rows start on 16-byte boundaries
     src_pitch = src.stride(0) if rows > 1 else k
     dtype = _TORCH_TO_PTO[src.dtype]
-
-    def call(sp):
-        nonlocal amax
-        d, s, t = data, scales, tensor_scale
-        if d is None:
-            d = _new((out_rows, width), (pitch, 1), torch.uint8, src)
-        if s is None:
-            tiles = _tiles(out_rows, length)
-            s = _new(tiles, (tiles[1] * 512, 512, 1), torch.uint8, src)
-        if t is None:
-            t = _new((1,), (1,), torch.float32, src)
-        if amax is None:
-            amax = _new((1,), (1,), torch.float32, src)
-            _capi.check(lib.pto_b200_amax(sp, amax.data_ptr(), src.data_ptr(), rows, k, src_pitch, dtype), "pto_b200_amax")
-        rc = lib.pto_b200_nvfp4_quantize(sp, d.data_ptr(), s.data_ptr(), t.data_ptr(), src.data_ptr(), amax.data_ptr(), rows, k,
-                                         src_pitch, d.stride(0) if out_rows > 1 else pitch, dtype, int(bool(transpose)))
-        _capi.check(rc, "pto_b200_nvfp4_quantize")
-        return d, s, t
-
-    return _launch(_device_of(src, amax, data, scales, tensor_scale), stream, call)
+    if data is None:
+        data = _new((out_rows, width), (pitch, 1), torch.uint8, src)
+    if scales is None:
+        tiles = _tiles(out_rows, length)
+        scales = _new(tiles, (tiles[1] * 512, 512, 1), torch.uint8, src)
+    if tensor_scale is None:
+        tensor_scale = _new((1,), (1,), torch.float32, src)
+    if amax is None:
+        amax = _new((1,), (1,), torch.float32, src)
+        _capi.check(lib.pto_b200_amax(sp, amax.data_ptr(), src.data_ptr(), rows, k, src_pitch, dtype), "pto_b200_amax")
+    rc = lib.pto_b200_nvfp4_quantize(sp, data.data_ptr(), scales.data_ptr(), tensor_scale.data_ptr(), src.data_ptr(),
+                                     amax.data_ptr(), rows, k, src_pitch, data.stride(0) if out_rows > 1 else pitch, dtype,
+                                     1 if transpose else 0)
+    _capi.check(rc, "pto_b200_nvfp4_quantize")
+    return data, scales, tensor_scale
 
 
 def nvfp4_dequantize(data: torch.Tensor, scales: torch.Tensor, tensor_scale: Optional[torch.Tensor] = None,
@@ -144,17 +144,20 @@ def nvfp4_dequantize(data: torch.Tensor, scales: torch.Tensor, tensor_scale: Opt
             raise ValueError("out must be [rows, K] float32, bfloat16 or float16, K less at most the last 15 columns")
     elif out_dtype not in _FLOATS:
         raise ValueError("out_dtype must be float32, bfloat16 or float16")
-
-    def call(sp):
-        o = out if out is not None else _new((rows, k), (k, 1), out_dtype, data)
-        cols = o.shape[1]
-        rc = lib.pto_b200_nvfp4_dequantize(sp, o.data_ptr(), data.data_ptr(), scales.data_ptr(), _ptr(tensor_scale), rows, cols,
-                                           data.stride(0) if rows > 1 else (k // 2 + 3) // 4 * 4,
-                                           o.stride(0) if rows > 1 else cols, _TORCH_TO_PTO[o.dtype])
-        _capi.check(rc, "pto_b200_nvfp4_dequantize")
-        return o
-
-    return _launch(_device_of(data, scales, tensor_scale, out), stream, call)
+    device = _device_of(data, scales, tensor_scale, out)
+    there = _elsewhere(device, stream)
+    if there is not None:
+        with there:
+            return nvfp4_dequantize(data, scales, tensor_scale, out_dtype, out)
+    if out is None:
+        out = _new((rows, k), (k, 1), out_dtype, data)
+    cols = out.shape[1]
+    rc = lib.pto_b200_nvfp4_dequantize(_raw_stream(device), out.data_ptr(), data.data_ptr(), scales.data_ptr(),
+                                       _ptr(tensor_scale), rows, cols,
+                                       data.stride(0) if rows > 1 else (k // 2 + 3) // 4 * 4,
+                                       out.stride(0) if rows > 1 else cols, _TORCH_TO_PTO[out.dtype])
+    _capi.check(rc, "pto_b200_nvfp4_dequantize")
+    return out
 
 
 def gemm_nvfp4(a: torch.Tensor, b_dn: torch.Tensor, sfa: torch.Tensor, sfb: torch.Tensor, ga: Optional[torch.Tensor] = None,
@@ -188,14 +191,17 @@ def gemm_nvfp4(a: torch.Tensor, b_dn: torch.Tensor, sfa: torch.Tensor, sfb: torc
             raise ValueError("out must be [M, N] float32, bfloat16 or float16")
     elif out_dtype not in _FLOATS:
         raise ValueError("out_dtype must be float32, bfloat16 or float16")
-
-    def call(sp):
-        o = out if out is not None else _new((m, n), (n, 1), out_dtype, a)
-        row = (k // 2 + 15) // 16 * 32  # a single row's pitch, in 4-bit elements
-        rc = lib.pto_b200_gemm_nvfp4(sp, o.data_ptr(), a.data_ptr(), b_dn.data_ptr(), sfa.data_ptr(), sfb.data_ptr(), _ptr(ga),
-                                     _ptr(gb), _ptr(bias), m, n, k, a.stride(0) * 2 if m > 1 else row,
-                                     b_dn.stride(0) * 2 if n > 1 else row, o.stride(0) if m > 1 else n, _TORCH_TO_PTO[o.dtype])
-        _capi.check(rc, "pto_b200_gemm_nvfp4")
-        return o
-
-    return _launch(_device_of(a, b_dn, sfa, sfb, ga, gb, bias, out), stream, call)
+    device = _device_of(a, b_dn, sfa, sfb, ga, gb, bias, out)
+    there = _elsewhere(device, stream)
+    if there is not None:
+        with there:
+            return gemm_nvfp4(a, b_dn, sfa, sfb, ga, gb, out_dtype, bias, out)
+    if out is None:
+        out = _new((m, n), (n, 1), out_dtype, a)
+    row = (k // 2 + 15) // 16 * 32  # a single row's pitch, in 4-bit elements
+    rc = lib.pto_b200_gemm_nvfp4(_raw_stream(device), out.data_ptr(), a.data_ptr(), b_dn.data_ptr(), sfa.data_ptr(),
+                                 sfb.data_ptr(), _ptr(ga), _ptr(gb), _ptr(bias), m, n, k,
+                                 a.stride(0) * 2 if m > 1 else row, b_dn.stride(0) * 2 if n > 1 else row,
+                                 out.stride(0) if m > 1 else n, _TORCH_TO_PTO[out.dtype])
+    _capi.check(rc, "pto_b200_gemm_nvfp4")
+    return out

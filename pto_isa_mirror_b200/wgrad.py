@@ -6,8 +6,8 @@ from typing import Optional
 import torch
 
 from . import _capi
-from .gemm import _TORCH_TO_PTO, _require_cuda_2d
-from .nvfp4 import _FLOATS, _device_of, _launch, _new, _ptr
+from .gemm import _TORCH_TO_PTO, _raw_stream, _require_cuda_2d
+from .nvfp4 import _FLOATS, _device_of, _elsewhere, _new, _ptr
 
 
 def gemm_wgrad_mx(dy: torch.Tensor, data: torch.Tensor, scales: torch.Tensor, out_dtype: torch.dtype = torch.float32,
@@ -44,15 +44,18 @@ def gemm_wgrad_mx(dy: torch.Tensor, data: torch.Tensor, scales: torch.Tensor, ou
         _require_cuda_2d(addend, "addend")
         if addend.dtype != out_dtype or tuple(addend.shape) != (n, k):
             raise ValueError("addend must be [N, K] of dW's type")
-
-    def call(sp):
-        o = out if out is not None else _new((n, k), (k, 1), out_dtype, dy)
-        rc = lib.pto_b200_gemm_wgrad_mx(sp, o.data_ptr(), dy.data_ptr(), data.data_ptr(), scales.data_ptr(), _ptr(addend), t, n, k,
-                                        dy.stride(0) if t > 1 else (n + 7) // 8 * 8, data.stride(0) if t > 1 else (k + 15) // 16 * 16,
-                                        scales.stride(0) if t > 1 else k // 32, o.stride(0) if n > 1 else k,
-                                        0 if addend is None else addend.stride(0) if n > 1 else k, _TORCH_TO_PTO[dy.dtype],
-                                        _TORCH_TO_PTO[out_dtype])
-        _capi.check(rc, "pto_b200_gemm_wgrad_mx")
-        return o
-
-    return _launch(_device_of(dy, data, scales, addend, out), stream, call)
+    device = _device_of(dy, data, scales, addend, out)
+    there = _elsewhere(device, stream)
+    if there is not None:
+        with there:
+            return gemm_wgrad_mx(dy, data, scales, out_dtype, addend, out)
+    if out is None:
+        out = _new((n, k), (k, 1), out_dtype, dy)
+    rc = lib.pto_b200_gemm_wgrad_mx(_raw_stream(device), out.data_ptr(), dy.data_ptr(), data.data_ptr(), scales.data_ptr(),
+                                    _ptr(addend), t, n, k, dy.stride(0) if t > 1 else (n + 7) // 8 * 8,
+                                    data.stride(0) if t > 1 else (k + 15) // 16 * 16, scales.stride(0) if t > 1 else k // 32,
+                                    out.stride(0) if n > 1 else k,
+                                    0 if addend is None else addend.stride(0) if n > 1 else k, _TORCH_TO_PTO[dy.dtype],
+                                    _TORCH_TO_PTO[out_dtype])
+    _capi.check(rc, "pto_b200_gemm_wgrad_mx")
+    return out
