@@ -295,13 +295,16 @@ int pto_b200_mx_quantize_e4m3_src(void* stream, uint8_t* data, uint8_t* scales, 
  *   scales : t x k/32 e8m0 bytes, leading dimension ld_scales (what pto_b200_mx_quantize_e4m3* writes)
  *   addend : n x k of out's type or null; may be out itself (gradient accumulation)
  *   out    : n x k, F32, BF16 or F16
+ *   workspace : null, or t * k * 2 bytes, 32-byte aligned: the activations are then converted to dy's type once, into it,
+ *               instead of tile by tile for every 256 columns of dy; the result is the same to the bit
  * The activations are multiplied as the numbers they stand for, in dy's type: exact for BF16 down to 2^-126; for F16 what
  * lies above 65504 becomes infinite and what lies below 2^-14 is rounded. Sums are fp32, rounded at least every 2048
- * tokens where the tensor core's own sum cuts off. The result does not depend on timing; no workspace is needed.
+ * tokens where the tensor core's own sum cuts off. The result does not depend on timing.
  */
 int pto_b200_gemm_wgrad_mx(void* stream, uint8_t* out, const uint8_t* dy, const uint8_t* data, const uint8_t* scales,
-                           const uint8_t* addend, int t, int n, int k, long long ld_dy, long long ld_data,
-                           long long ld_scales, long long ld_out, long long ld_addend, int dy_dtype, int out_dtype);
+                           const uint8_t* addend, uint8_t* workspace, size_t workspace_bytes, int t, int n, int k,
+                           long long ld_dy, long long ld_data, long long ld_scales, long long ld_out, long long ld_addend,
+                           int dy_dtype, int out_dtype);
 
 /*
  * fp32 -> bf16 cast (round to nearest even) of `count` contiguous elements: the TSTORE cast applied to the

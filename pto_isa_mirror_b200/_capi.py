@@ -77,7 +77,7 @@ SYMBOLS = {
     "pto_b200_mx_quantize_e4m3_src": (_i, [ctypes.c_void_p, _u8p, _u8p, _u8p, _i, _i, _ll, _ll, _ll, _i, _i]),
     "pto_b200_gemm_wgrad_mx": (
         _i,
-        [ctypes.c_void_p, _u8p, _u8p, _u8p, _u8p, _u8p, _i, _i, _i, _ll, _ll, _ll, _ll, _ll, _i, _i],
+        [ctypes.c_void_p, _u8p, _u8p, _u8p, _u8p, _u8p, _u8p, ctypes.c_size_t, _i, _i, _i, _ll, _ll, _ll, _ll, _ll, _i, _i],
     ),
     "pto_b200_gemm_mx_static": (
         _i,

@@ -2,6 +2,7 @@
 #include "capi_shared.cuh"
 
 #include <atomic>
+#include <type_traits>
 
 #include "gemm_wgrad_mx.cuh"
 #include "mx_quantize.cuh"
@@ -43,11 +44,35 @@ int launch_quantize16_any(cudaStream_t s, const HostContext& host, const uint8_t
                : launch_quantize16<ALG, SRC, 16>(s, host, src, data, scales, rows, k, ld_src, ld_data, ld_scales);
 }
 
-template <bool F16, int OUT>
-int launch_wgrad(cudaStream_t stream, const HostContext& host, const uint8_t* dy, const uint8_t* data, long long ld_dy,
-                 long long ld_data, WgradParams p)
+// x [t][k] as 16-bit values into scratch memory: one resident wave.
+template <bool F16>
+int launch_convert(cudaStream_t s, const HostContext& host, const uint8_t* data, long long ld_data, uint8_t* scratch,
+                   const WgradParams& p)
 {
-    auto kernel = gemm_wgrad_mx<F16, OUT>;
+    auto kernel = mx_to_16bit_kernel<F16>;
+    static std::atomic<int> blocks_per_sm[kMaxDevices];
+    int per_sm = blocks_per_sm[host.device].load(std::memory_order_relaxed);
+    if (per_sm == 0) {
+        if (int rc = note_cuda_error(cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per_sm, kernel, kWgConvertThreads, 0),
+                                     "mx_to_16bit occupancy")) {
+            return rc;
+        }
+        per_sm = per_sm > 0 ? per_sm : 1;
+        blocks_per_sm[host.device].store(per_sm, std::memory_order_relaxed);
+    }
+    const long long want = (static_cast<long long>(p.t) * (p.k / 16) + kWgConvertThreads - 1) / kWgConvertThreads;
+    const long long cap = static_cast<long long>(host.sm_count) * per_sm;
+    kernel<<<static_cast<int>(want < cap ? want : cap), kWgConvertThreads, 0, s>>>(
+        data, p.scales, reinterpret_cast<uint16_t*>(scratch), p.t, p.k, ld_data, p.ld_scales);
+    count_launches(1);
+    return note_cuda_error(cudaGetLastError(), "mx_to_16bit launch");
+}
+
+template <bool F16, int OUT, bool SCRATCH>
+int launch_wgrad(cudaStream_t stream, const HostContext& host, const uint8_t* dy, const uint8_t* data, long long ld_dy,
+                 long long ld_data, uint8_t* scratch, WgradParams p)
+{
+    auto kernel = gemm_wgrad_mx<F16, OUT, SCRATCH>;
     static std::atomic<int> resident[kMaxDevices][3]; // clusters of 2, 4 and 8 CTAs that the device holds at once
     cudaLaunchConfig_t cfg = {};
     cudaLaunchAttribute attr[1];
@@ -83,7 +108,13 @@ int launch_wgrad(cudaStream_t stream, const HostContext& host, const uint8_t* dy
     CUtensorMap tdy, tx;
     int rc = encode_map_2d(&tdy, F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, dy, p.t, p.n, ld_dy * 2,
                            64, kWgStageTokens, true);
-    rc = rc ? rc : encode_map_2d(&tx, CU_TENSOR_MAP_DATA_TYPE_UINT8, data, p.t, p.k, ld_data, 128, kWgStageTokens, false);
+    if constexpr (SCRATCH) {
+        rc = rc ? rc : launch_convert<F16>(stream, host, data, ld_data, scratch, p);
+        rc = rc ? rc : encode_map_2d(&tx, F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, scratch, p.t,
+                                     p.k, p.k * 2ll, 64, kWgStageTokens, true);
+    } else {
+        rc = rc ? rc : encode_map_2d(&tx, CU_TENSOR_MAP_DATA_TYPE_UINT8, data, p.t, p.k, ld_data, 128, kWgStageTokens, false);
+    }
     if (rc) {
         return rc;
     }
@@ -158,8 +189,9 @@ extern "C" int pto_b200_mx_quantize_e4m3_src(void* stream, uint8_t* data, uint8_
 }
 
 extern "C" int pto_b200_gemm_wgrad_mx(void* stream, uint8_t* out, const uint8_t* dy, const uint8_t* data, const uint8_t* scales,
-                                      const uint8_t* addend, int t, int n, int k, long long ld_dy, long long ld_data,
-                                      long long ld_scales, long long ld_out, long long ld_addend, int dy_dtype, int out_dtype)
+                                      const uint8_t* addend, uint8_t* workspace, size_t workspace_bytes, int t, int n, int k,
+                                      long long ld_dy, long long ld_data, long long ld_scales, long long ld_out,
+                                      long long ld_addend, int dy_dtype, int out_dtype)
 {
     if ((dy_dtype != PTO_B200_BF16 && dy_dtype != PTO_B200_F16) ||
         (out_dtype != PTO_B200_F32 && out_dtype != PTO_B200_BF16 && out_dtype != PTO_B200_F16)) {
@@ -175,6 +207,10 @@ extern "C" int pto_b200_gemm_wgrad_mx(void* stream, uint8_t* out, const uint8_t*
     if (misaligned(dy, 16) || ld_dy % 8 != 0 || misaligned(data, 16) || ld_data % 16 != 0 || misaligned(out, out_es) ||
         misaligned(addend, out_es)) {
         return PTO_B200_EALIGN;
+    }
+    if (workspace != nullptr &&
+        (misaligned(workspace, 32) || workspace_bytes < static_cast<size_t>(t) * static_cast<size_t>(k) * 2)) {
+        return PTO_B200_EWORKSPACE;
     }
     HostContext host;
     if (int rc = host_context(&host)) {
@@ -194,8 +230,14 @@ extern "C" int pto_b200_gemm_wgrad_mx(void* stream, uint8_t* out, const uint8_t*
     p.wait_limit = host.wait_limit;
     cudaStream_t s = static_cast<cudaStream_t>(stream);
     const bool f16 = dy_dtype == PTO_B200_F16;
-    auto launch = out_dtype == PTO_B200_F32    ? (f16 ? launch_wgrad<true, WG_OUT_F32> : launch_wgrad<false, WG_OUT_F32>)
-                  : out_dtype == PTO_B200_BF16 ? (f16 ? launch_wgrad<true, WG_OUT_BF16> : launch_wgrad<false, WG_OUT_BF16>)
-                                               : (f16 ? launch_wgrad<true, WG_OUT_F16> : launch_wgrad<false, WG_OUT_F16>);
-    return launch(s, host, dy, data, ld_dy, ld_data, p);
+    auto launch = [&](auto scratch) {
+        constexpr bool kScratch = decltype(scratch)::value;
+        auto of_type = out_dtype == PTO_B200_F32
+                           ? (f16 ? launch_wgrad<true, WG_OUT_F32, kScratch> : launch_wgrad<false, WG_OUT_F32, kScratch>)
+                       : out_dtype == PTO_B200_BF16
+                           ? (f16 ? launch_wgrad<true, WG_OUT_BF16, kScratch> : launch_wgrad<false, WG_OUT_BF16, kScratch>)
+                           : (f16 ? launch_wgrad<true, WG_OUT_F16, kScratch> : launch_wgrad<false, WG_OUT_F16, kScratch>);
+        return of_type(s, host, dy, data, ld_dy, ld_data, workspace, p);
+    };
+    return workspace != nullptr ? launch(std::true_type{}) : launch(std::false_type{});
 }

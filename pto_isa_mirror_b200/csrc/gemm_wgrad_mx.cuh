@@ -6,8 +6,12 @@
 //
 // x becomes 16-bit on the way: every e4m3 value times a power of two is a bf16 value exactly (below 2^-126 in magnitude
 // the smallest bits are cut off), and an fp16 value where it lies in fp16's range (above it: infinity, below 2^-14:
-// rounded). So dy meets the numbers the checkpoint stands for, at the 16-bit rate of the tensor core, and the 16-bit
-// copy of x exists only in shared memory, tile by tile.
+// rounded). So dy meets the numbers the checkpoint stands for, at the 16-bit rate of the tensor core.
+//
+// Two ways to the same bits. Without scratch memory x is converted tile by tile in shared memory, beside the products
+// (SCRATCH = false); every tile of x then is converted once for each 256 columns of dy. With scratch for T x K 16-bit
+// values x is converted once, by mx_to_16bit_kernel, and both operands come by TMA (SCRATCH = true): at 16384x8192x8192
+// 60 us more traffic, but the products run at nearly the rate of a 16-bit GEMM.
 //
 // A cluster holds `splits` CTA pairs. A pair owns a 256 (k) x 256 (n) tile, or with splits > 1 its part of the
 // tokens of one. x is the 256-row side of the product and each CTA converts its own 128: half as many elements per SM as
@@ -34,6 +38,7 @@
 #include <cstdint>
 
 #include "gemm_tile_loop.cuh"
+#include "row_elements.cuh"
 #include "sm100_ptx.cuh"
 
 namespace pto_b200 {
@@ -186,7 +191,62 @@ struct WgElem<WG_OUT_F16> {
     using type = __half;
 };
 
-template <bool F16, int OUT>
+// x [rows][k] as 16-bit values, contiguous rows on 32-byte boundaries: 16 values per thread and step.
+constexpr int kWgConvertThreads = 256;
+
+template <bool F16>
+__global__ void __launch_bounds__(kWgConvertThreads) mx_to_16bit_kernel(const uint8_t* __restrict__ data,
+                                                                         const uint8_t* __restrict__ scales,
+                                                                         uint16_t* __restrict__ out, int rows, int k,
+                                                                         long long ld_data, long long ld_scales)
+{
+    const int row_items = k / 16;
+    const long long total = static_cast<long long>(rows) * row_items;
+    const long long stride = static_cast<long long>(gridDim.x) * blockDim.x;
+    long long i = blockIdx.x * static_cast<long long>(blockDim.x) + threadIdx.x;
+    const long long row_step = stride / row_items;
+    const int c_step = static_cast<int>(stride - row_step * row_items);
+    long long row = i / row_items;
+    int c = static_cast<int>(i - row * row_items);
+    constexpr int kItems = 4;
+    while (i < total) {
+        uint4 in[kItems];
+        uint32_t e[kItems];
+        long long at[kItems];
+#pragma unroll
+        for (int u = 0; u < kItems; ++u) {
+            at[u] = i < total ? i : -1;
+            in[u] = make_uint4(0u, 0u, 0u, 0u);
+            e[u] = 127u;
+            if (i < total) {
+                in[u] = __ldcs(reinterpret_cast<const uint4*>(data + row * ld_data) + c);
+                e[u] = __ldg(scales + row * ld_scales + (c >> 1));
+            }
+            i += stride;
+            row += row_step;
+            c += c_step;
+            if (c >= row_items) {
+                c -= row_items;
+                row += 1;
+            }
+        }
+        const bool any = wg_needs_any<F16>(in, e);
+#pragma unroll
+        for (int u = 0; u < kItems; ++u) {
+            uint32_t o[8];
+            if (!any) {
+                wg_convert16<F16>(in[u], e[u], o);
+            } else {
+                wg_convert16_any<F16>(in[u], e[u], o);
+            }
+            if (at[u] >= 0) {
+                nv_st32(out + at[u] * 16, make_uint4(o[0], o[1], o[2], o[3]), make_uint4(o[4], o[5], o[6], o[7]));
+            }
+        }
+    }
+}
+
+template <bool F16, int OUT, bool SCRATCH>
 __global__ void __launch_bounds__(kWgThreads, 1)
     gemm_wgrad_mx(const __grid_constant__ CUtensorMap tmap_dy, const __grid_constant__ CUtensorMap tmap_x, const WgradParams p)
 {
@@ -219,7 +279,8 @@ __global__ void __launch_bounds__(kWgThreads, 1)
 
     if (threadIdx.x == 0) {
         for (int s = 0; s < kWgStages; ++s) {
-            ptx::mbar_init(&full_bar[s], 1 + 2 * (kWgWorkerWarps / kWgGroups)); // dy's bytes, and a group in each CTA
+            // dy's bytes (with SCRATCH x's too), and a converting group in each CTA
+            ptx::mbar_init(&full_bar[s], SCRATCH ? 1 : 1 + 2 * (kWgWorkerWarps / kWgGroups));
             ptx::mbar_init(&empty_bar[s], 1);
         }
         for (int s = 0; s < kWgRawStages; ++s) {
@@ -259,38 +320,45 @@ __global__ void __launch_bounds__(kWgThreads, 1)
     if (warp < 4) {
         asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kWgRegsOthers));
         if (warp == 0) {
-            // ---------------------------------------------------------------- loads of dy
-            if (lane == 0) {
-                int stage = 0;
-                uint32_t phase = 0;
-                bool ok = true;
-                for (int tile = cluster; ok && tile < tiles; tile += clusters) {
-                    int ki, ni;
-                    tile_of(tile, ki, ni);
-                    const int n0 = ni * 256 + side * 128;
-                    for (int st = first_stage; st < last_stage; ++st) {
-                        const int token = st * kWgStageTokens;
-                        ok = bounded_wait_quiet(&empty_bar[stage], phase ^ 1u, abort_flag, p.status, ST_WG_PRODUCER, p.wait_limit);
-                        if (!ok) {
-                            break;
-                        }
+            // ---------------------------------------------------------------- loads of dy (with SCRATCH of x, too)
+            int stage = 0;
+            uint32_t phase = 0;
+            bool ok = true;
+            for (int tile = cluster; ok && tile < tiles; tile += clusters) {
+                int ki, ni;
+                tile_of(tile, ki, ni);
+                const int k0 = ki * 256 + side * 128;
+                const int n0 = ni * 256 + side * 128;
+                for (int st = first_stage; st < last_stage; ++st) {
+                    const int token = st * kWgStageTokens;
+                    ok = bounded_wait_quiet(&empty_bar[stage], phase ^ 1u, abort_flag, p.status, ST_WG_PRODUCER, p.wait_limit);
+                    if (!ok) {
+                        break;
+                    }
+                    if (ptx::elect_one()) {
                         if (leader) {
-                            ptx::mbar_arrive_expect_tx(&full_bar[stage], 2u * L::kDyBytes);
+                            ptx::mbar_arrive_expect_tx(&full_bar[stage], 2u * (L::kDyBytes + (SCRATCH ? L::kXBytes : 0)));
                         }
                         const uint32_t full_addr = ptx::map_to_cta(ptx::smem_u32(&full_bar[stage]), leader_rank);
                         uint8_t* dst = smem + stage * L::kDyBytes;
                         ptx::tma_load_2d_pair(dst, &tmap_dy, full_addr, n0, token);
                         ptx::tma_load_2d_pair(dst + 8192, &tmap_dy, full_addr, n0 + 64, token);
-                        if (++stage == kWgStages) {
-                            stage = 0;
-                            phase ^= 1u;
+                        if constexpr (SCRATCH) {
+                            uint8_t* x = smem + L::kXOff + stage * L::kXBytes;
+                            ptx::tma_load_2d_pair(x, &tmap_x, full_addr, k0, token);
+                            ptx::tma_load_2d_pair(x + 8192, &tmap_x, full_addr, k0 + 64, token);
                         }
+                    }
+                    __syncwarp();
+                    if (++stage == kWgStages) {
+                        stage = 0;
+                        phase ^= 1u;
                     }
                 }
             }
         } else if (warp == 2) {
             // ---------------------------------------------------------------- loads of x, as far ahead as their own ring goes
-            if (lane == 0) {
+            if (!SCRATCH && lane == 0) {
                 int raw = 0;
                 uint32_t phase = 0;
                 bool ok = true;
@@ -415,7 +483,9 @@ __global__ void __launch_bounds__(kWgThreads, 1)
             visit_token = (first_stage + first_of_tile) * kWgStageTokens;
             fetch_scales();
         };
-        start_scales(cluster);
+        if constexpr (!SCRATCH) {
+            start_scales(cluster);
+        }
         for (int tile = cluster; ok && tile < tiles; tile += clusters) {
             int ki, ni;
             tile_of(tile, ki, ni);
@@ -425,8 +495,8 @@ __global__ void __launch_bounds__(kWgThreads, 1)
                 sum[i] = 0.0f;
             }
             int folded = 0;
-            for (int st = first_of_tile; folded < parts; st += kWgGroups) {
-                if (st < stages) {
+            for (int st = SCRATCH ? stages : first_of_tile; folded < parts; st += kWgGroups) {
+                if (!SCRATCH && st < stages) {
                     const uint32_t e_now[4] = {e[0], e[1], e[2], e[3]};
                     fetch_scales(); // of the next visit; past the tile's last token they are not used
                     ok = bounded_wait_quiet(&raw_full_bar[group], raw_phase, abort_flag, p.status, ST_WG_WORKER, p.wait_limit);
@@ -509,7 +579,9 @@ __global__ void __launch_bounds__(kWgThreads, 1)
                 break;
             }
             first_of_tile = (first_of_tile - stages % kWgGroups + kWgGroups) % kWgGroups; // stages go round the groups
-            start_scales(tile + clusters); // come while this tile is stored
+            if constexpr (!SCRATCH) {
+                start_scales(tile + clusters); // come while this tile is stored
+            }
             const int in_tile = quarter * 32 + lane;
             if (p.splits == 1) {
                 const int k = ki * 256 + side * 128 + in_tile;

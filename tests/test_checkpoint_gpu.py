@@ -158,6 +158,30 @@ def test_every_byte_and_scale():
             assert torch.equal(got.double(), want) if e > 9 else ((got.double() - want).abs() <= 2.0 ** -133).all()
 
 
+@pytest.mark.parametrize("t,n,k", [(1, 8, 32), (130, 257, 96), (515, 1000, 1056), (4500, 264, 160), (640, 9000, 1056), (3000, 2304, 2560)])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+def test_scratch_memory_changes_no_bit(t, n, k, dtype):
+    data, scales, _ = kept(t, k, t + n, False, spread=40)  # scales past what the short conversion holds for
+    scales[:: 7] = torch.randint(100, 150, scales[:: 7].shape, generator=gen(1), dtype=torch.uint8).to(DEV)
+    dy = pitched((torch.randn((t, n), generator=gen(n)) * 0.01).to(dtype), 8, 8)
+    scratch = torch.full((2 * t * k + 64,), 0xFF, dtype=torch.uint8, device=DEV)
+    without = pto.gemm_wgrad_mx(dy, data, scales, workspace=False)
+    assert torch.equal(without.view(torch.int32), pto.gemm_wgrad_mx(dy, data, scales, workspace=scratch[:2 * t * k]).view(torch.int32))
+    assert torch.equal(without.view(torch.int32), pto.gemm_wgrad_mx(dy, data, scales).view(torch.int32))
+    assert (scratch[2 * t * k:] == 0xFF).all()
+
+
+def test_scratch_memory_carries_nan_and_every_byte():
+    data = torch.arange(256, dtype=torch.int32).to(torch.uint8)[:, None].repeat(1, 64).to(DEV)
+    eye = torch.eye(256, device=DEV)
+    for e in (0, 3, 102, 103, 127, 134, 135, 142, 143, 254, 255):
+        scales = torch.full((256, 2), e, dtype=torch.uint8, device=DEV)
+        for dtype in (torch.bfloat16, torch.float16):
+            one = pto.gemm_wgrad_mx(eye.to(dtype), data, scales, workspace=False)
+            two = pto.gemm_wgrad_mx(eye.to(dtype), data, scales, workspace=torch.empty(256 * 128, dtype=torch.uint8, device=DEV))
+            assert torch.equal(torch.isnan(one), torch.isnan(two)) and torch.equal(torch.nan_to_num(one), torch.nan_to_num(two))
+
+
 def test_splits_and_streams_agree_bit_for_bit():
     data, scales, _ = kept(3000, 512, 9, False)
     dy = torch.randn((3000, 512), generator=gen(8)).to(torch.bfloat16).to(DEV)
@@ -196,6 +220,7 @@ def test_python_refusals():
         lambda: pto.gemm_wgrad_mx(dy, data, scales, out_dtype=torch.float64), lambda: pto.gemm_wgrad_mx(dy, data, scales, out=out.t()),
         lambda: pto.gemm_wgrad_mx(dy, data, scales, out=out[:, :32]), lambda: pto.gemm_wgrad_mx(dy, data, scales, addend=out.half()),
         lambda: pto.gemm_wgrad_mx(dy, data, scales, addend=out[:40]),
+        lambda: pto.gemm_wgrad_mx(dy, data, scales, workspace=True), lambda: pto.gemm_wgrad_mx(dy, data, scales, workspace=out),
         lambda: pto.mx_quantize_e4m3(dy.double()), lambda: pto.mx_quantize_e4m3(dy[:, :40]),
     ]
     for call in bad:
@@ -205,6 +230,9 @@ def test_python_refusals():
         with pytest.raises(pto.PtoB200Error) as e:
             call()
         assert e.value.code == 2
+    with pytest.raises(pto.PtoB200Error) as e:
+        pto.gemm_wgrad_mx(dy, data, scales, workspace=torch.empty(2 * 64 * 64 - 1, dtype=torch.uint8, device=DEV))
+    assert e.value.code == 4
 
 
 def test_rows_of_nan_and_infinity_stay_theirs():

@@ -82,7 +82,7 @@ def test_checkpoint_refusals(lib, p):
         (dict(k=48), EINVAL), (dict(ld_src=32), EINVAL), (dict(ld_data=32), EINVAL), (dict(ld_scales=1), EINVAL),
         (dict(dtype=S8), EDTYPE), (dict(alg=2), EDTYPE), (dict(src=p + 8), EALIGN), (dict(ld_src=68), EALIGN),
         (dict(data=p + 4), EALIGN), (dict(ld_data=68), EALIGN), (dict(dtype=F32, src=p + 8), EALIGN)])
-    good = dict(stream=None, out=p, dy=p, data=p, scales=p, addend=None, t=4, n=16, k=64, ld_dy=16, ld_data=64, ld_scales=2,
+    good = dict(stream=None, out=p, dy=p, data=p, scales=p, addend=None, workspace=None, workspace_bytes=0, t=4, n=16, k=64, ld_dy=16, ld_data=64, ld_scales=2,
                 ld_out=64, ld_addend=0, dy_dtype=BF16, out_dtype=F32)
     refused(lib.pto_b200_gemm_wgrad_mx, good, [
         (dict(out=None), EINVAL), (dict(dy=None), EINVAL), (dict(data=None), EINVAL), (dict(scales=None), EINVAL),
@@ -90,7 +90,8 @@ def test_checkpoint_refusals(lib, p):
         (dict(ld_data=48), EINVAL), (dict(ld_scales=1), EINVAL), (dict(ld_scales=1 << 26), EINVAL), (dict(ld_out=63), EINVAL),
         (dict(addend=p, ld_addend=32), EINVAL), (dict(dy_dtype=F32), EDTYPE), (dict(dy_dtype=E4M3), EDTYPE),
         (dict(out_dtype=S8), EDTYPE), (dict(dy=p + 8), EALIGN), (dict(ld_dy=20), EALIGN), (dict(data=p + 8), EALIGN),
-        (dict(ld_data=72), EALIGN), (dict(out=p + 2), EALIGN), (dict(addend=p + 2, ld_addend=64), EALIGN)])
+        (dict(ld_data=72), EALIGN), (dict(out=p + 2), EALIGN), (dict(addend=p + 2, ld_addend=64), EALIGN),
+        (dict(workspace=p, workspace_bytes=511), _capi.EWORKSPACE), (dict(workspace=p + 16, workspace_bytes=4096), _capi.EWORKSPACE)])
     assert lib.pto_b200_launch_count() == before
 
 
