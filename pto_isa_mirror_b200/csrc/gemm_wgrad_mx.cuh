@@ -26,8 +26,14 @@
 // descriptors in uniform registers (its issue alone took 800 cycles of a stage's 513 before).
 //
 // Sums: the tensor core adds into its accumulator by cutting off, not by rounding (measured here: 1.9e-5 of the result
-// lost after 16384 terms, 3.8e-5 after 32768). So an accumulator takes kWgFoldStages x 64 = 2048 tokens at most; the
+// lost after 16384 terms, 3.8e-5 after 32768). So an accumulator takes kWgFoldStages x 64 = 1024 tokens at most; the
 // converting warps then add it to fp32 sums in their registers, with rounding, while the other accumulator fills.
+// Relative error of 16384 tokens, and time of 16384x8192x8192 with and without scratch, by tokens per accumulator:
+//   2048   6.3e-7 (terms of one sign 2.4e-6)   1456 / 1739 us
+//   1024   2.8e-7 (9.4e-7)                     1440 / 1778 us
+//    512   1.5e-7 (3.6e-7)                     1470 / 1863 us
+//    256   1.1e-7 (1.5e-7)                     1515 / 2595 us
+// A plain fp32 matrix product of the same numbers has 5.7e-7 there.
 // With splits > 1 the parts are added over distributed shared memory in rank order. No atomics: the result does not
 // depend on timing.
 #pragma once
@@ -53,7 +59,8 @@ static_assert(kWgRawStages == kWgGroups, "a group reads its own place of the rin
 constexpr int kWgRegsOthers = 32, kWgRegsWorkers = 112;
 static_assert(128 * kWgRegsOthers + 512 * kWgRegsWorkers <= kWgThreads * 96, "register split within the launch's total");
 constexpr int kWgStageTokens = 64;
-constexpr int kWgFoldStages = 32;
+constexpr int kWgFoldStages = 16;
+static_assert(kWgFoldStages >= kWgStages + kWgGroups, "an accumulator is read before its second successor needs it");
 
 constexpr int ST_WG_PRODUCER = 31;
 constexpr int ST_WG_MMA = 32;

@@ -3,7 +3,7 @@
 The 16-bit quantiser has to give the bytes of the fp32 one for the same numbers, which is checked against the reference
 elsewhere. Weight gradients over small whole numbers are exact in fp32 and compared for equality; over real ones the
 products are exact (8 + 4 significant bits), each 16-token step of the tensor core is off by at most two units (2^-22)
-of the magnitudes summed in its 2048-token part, and each part's joining by half a unit of the whole."""
+of the magnitudes summed in its 1024-token part, and each part's joining by half a unit of the whole."""
 import pytest
 import torch
 
