@@ -261,6 +261,14 @@ int pto_b200_nvfp4_quantize(void* stream, uint8_t* data, uint8_t* scales, float*
                             int transpose);
 
 /*
+ * pto_b200_amax and pto_b200_nvfp4_quantize in one call: *amax receives the largest finite magnitude of src, which sets
+ * *tensor_scale. Without transpose up to 16384 blocks of 16 elements (rows filled up to 64) take a single launch.
+ */
+int pto_b200_nvfp4_quantize_dynamic(void* stream, uint8_t* data, uint8_t* scales, float* tensor_scale, float* amax,
+                                    const uint8_t* src, int rows, int k, long long ld_src, long long ld_data, int src_dtype,
+                                    int transpose);
+
+/*
  * Back to numbers: out[r][i] = code * scale * g for the first k elements of each row (tensor_scale null: g = 1), F32, BF16
  * or F16. data: leading dimension ld_data bytes (a multiple of 4, at least ceil(k / 8) * 4), 4-byte aligned.
  */

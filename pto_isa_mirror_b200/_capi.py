@@ -69,6 +69,7 @@ SYMBOLS = {
     "pto_b200_nvfp4_scale_bytes": (ctypes.c_size_t, [_i, _i]),
     "pto_b200_amax": (_i, [ctypes.c_void_p, _u8p, _u8p, _i, _i, _ll, _i]),
     "pto_b200_nvfp4_quantize": (_i, [ctypes.c_void_p, _u8p, _u8p, _u8p, _u8p, _u8p, _i, _i, _ll, _ll, _i, _i]),
+    "pto_b200_nvfp4_quantize_dynamic": (_i, [ctypes.c_void_p, _u8p, _u8p, _u8p, _u8p, _u8p, _i, _i, _ll, _ll, _i, _i]),
     "pto_b200_nvfp4_dequantize": (_i, [ctypes.c_void_p, _u8p, _u8p, _u8p, _u8p, _i, _i, _ll, _ll, _i]),
     "pto_b200_gemm_nvfp4": (
         _i,

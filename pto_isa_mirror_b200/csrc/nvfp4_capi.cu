@@ -95,6 +95,44 @@ int launch_amax(cudaStream_t s, const HostContext& host, const void* src, float*
     return note_cuda_error(cudaGetLastError(), "amax launch");
 }
 
+// Largest magnitude and codes in one launch; total = blocks of 16 in rows filled up to 64 elements, at most kNvOneBlocks.
+template <int SRC, int VEC, int THREADS>
+int launch_quantize_one_of(cudaStream_t s, const void* src, float* amax, uint8_t* data, uint8_t* scales, float* tensor_scale,
+                           int rows, int k, long long ld_src, long long ld_data, int total)
+{
+    int ctas = 1;
+    while (ctas < kNvOneCtas && ctas * THREADS < total) {
+        ctas *= 2;
+    }
+    cudaLaunchConfig_t cfg = {};
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = static_cast<unsigned>(ctas);
+    attr[0].val.clusterDim.y = 1;
+    attr[0].val.clusterDim.z = 1;
+    cfg.gridDim = dim3(static_cast<unsigned>(ctas), 1, 1);
+    cfg.blockDim = dim3(THREADS, 1, 1);
+    cfg.stream = s;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    count_launches(1);
+    return note_cuda_error(cudaLaunchKernelEx(&cfg, nvfp4_quantize_one_kernel<SRC, VEC, THREADS>, src, amax, data, scales,
+                                              tensor_scale, rows, k, ld_src, ld_data),
+                           "nvfp4_quantize launch");
+}
+
+template <int SRC, int VEC>
+int launch_quantize_one(cudaStream_t s, const void* src, float* amax, uint8_t* data, uint8_t* scales, float* tensor_scale,
+                        int rows, int k, long long ld_src, long long ld_data, int total)
+{
+    constexpr int kPerThread = kNvOneCtas * kNvItems;
+    return total <= 256 * kPerThread
+               ? launch_quantize_one_of<SRC, VEC, 256>(s, src, amax, data, scales, tensor_scale, rows, k, ld_src, ld_data, total)
+           : total <= 512 * kPerThread
+               ? launch_quantize_one_of<SRC, VEC, 512>(s, src, amax, data, scales, tensor_scale, rows, k, ld_src, ld_data, total)
+               : launch_quantize_one_of<SRC, VEC, 1024>(s, src, amax, data, scales, tensor_scale, rows, k, ld_src, ld_data, total);
+}
+
 template <int DST, bool VEC>
 int launch_dequantize(cudaStream_t s, const HostContext& host, const uint8_t* data, const uint8_t* scales, const float* tensor_scale,
                       void* out, int rows, int k, long long ld_data, long long ld_out)
@@ -274,6 +312,25 @@ int launch_nv(cudaStream_t stream, const HostContext& host, const NvProblem& q, 
     return launch_nv_few<128, OUT>(stream, host, q, p);
 }
 
+int check_quantize(const void* data, const void* scales, const void* tensor_scale, const void* src, const void* amax, int rows,
+                   int k, long long ld_src, long long ld_data, int src_dtype, int transpose)
+{
+    const long long length = transpose ? rows : k; // of the result's rows
+    if (data == nullptr || scales == nullptr || tensor_scale == nullptr || src == nullptr || amax == nullptr || rows <= 0 ||
+        k <= 0 || rows > kMaxExtent || k > kMaxExtent || ld_src < k || ld_data < (length + 15) / 16 * 8) {
+        return PTO_B200_EINVAL;
+    }
+    const int type = source_of(src_dtype);
+    if (type < 0) {
+        return PTO_B200_EDTYPE;
+    }
+    if (misaligned(src, size_of(type)) || misaligned(data, 8) || ld_data % 8 != 0 || misaligned(scales, 4) ||
+        misaligned(tensor_scale, 4) || misaligned(amax, 4)) {
+        return PTO_B200_EALIGN;
+    }
+    return PTO_B200_OK;
+}
+
 } // namespace
 } // namespace pto_b200
 
@@ -312,26 +369,39 @@ extern "C" int pto_b200_nvfp4_quantize(void* stream, uint8_t* data, uint8_t* sca
                                        const float* amax, int rows, int k, long long ld_src, long long ld_data,
                                        int src_dtype, int transpose)
 {
-    const long long length = transpose ? rows : k; // of the result's rows
-    if (data == nullptr || scales == nullptr || tensor_scale == nullptr || src == nullptr || amax == nullptr || rows <= 0 ||
-        k <= 0 || rows > kMaxExtent || k > kMaxExtent || ld_src < k || ld_data < (length + 15) / 16 * 8) {
-        return PTO_B200_EINVAL;
+    if (int rc = check_quantize(data, scales, tensor_scale, src, amax, rows, k, ld_src, ld_data, src_dtype, transpose)) {
+        return rc;
     }
     const int type = source_of(src_dtype);
-    if (type < 0) {
-        return PTO_B200_EDTYPE;
+    HostContext host;
+    if (int rc = host_context(&host)) {
+        return rc;
     }
-    const int es = size_of(type);
-    if (misaligned(src, es) || misaligned(data, 8) || ld_data % 8 != 0 || misaligned(scales, 4) || misaligned(tensor_scale, 4) ||
-        misaligned(amax, 4)) {
-        return PTO_B200_EALIGN;
+    return PTO_NV_DISPATCH(type, row_access(src, ld_src * size_of(type)), launch_quantize, static_cast<cudaStream_t>(stream), host, src, amax, data,
+                           scales, tensor_scale, rows, k, ld_src, ld_data, transpose != 0);
+}
+
+extern "C" int pto_b200_nvfp4_quantize_dynamic(void* stream, uint8_t* data, uint8_t* scales, float* tensor_scale, float* amax,
+                                               const uint8_t* src, int rows, int k, long long ld_src, long long ld_data,
+                                               int src_dtype, int transpose)
+{
+    if (int rc = check_quantize(data, scales, tensor_scale, src, amax, rows, k, ld_src, ld_data, src_dtype, transpose)) {
+        return rc;
+    }
+    const long long total = static_cast<long long>(rows) * ((k + 63LL) / 64 * 4);
+    if (transpose || total > kNvOneBlocks) {
+        if (int rc = pto_b200_amax(stream, amax, src, rows, k, ld_src, src_dtype)) {
+            return rc;
+        }
+        return pto_b200_nvfp4_quantize(stream, data, scales, tensor_scale, src, amax, rows, k, ld_src, ld_data, src_dtype, transpose);
     }
     HostContext host;
     if (int rc = host_context(&host)) {
         return rc;
     }
-    return PTO_NV_DISPATCH(type, row_access(src, ld_src * es), launch_quantize, static_cast<cudaStream_t>(stream), host, src, amax, data,
-                           scales, tensor_scale, rows, k, ld_src, ld_data, transpose != 0);
+    const int type = source_of(src_dtype);
+    return PTO_NV_DISPATCH(type, row_access(src, ld_src * size_of(type)), launch_quantize_one, static_cast<cudaStream_t>(stream), src,
+                           amax, data, scales, tensor_scale, rows, k, ld_src, ld_data, static_cast<int>(total));
 }
 
 extern "C" int pto_b200_nvfp4_dequantize(void* stream, uint8_t* out, const uint8_t* data, const uint8_t* scales,

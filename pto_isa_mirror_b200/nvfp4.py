@@ -56,8 +56,8 @@ def _require_scales(t: torch.Tensor, rows: int, k: int, name: str) -> None:
 
 
 def _new(size, stride, dtype: torch.dtype, like: torch.Tensor) -> torch.Tensor:
-    """An uninitialised tensor on ``like``'s device (this form takes 1.5 us, ``torch.empty`` 2.3)."""
-    return torch.empty_strided(size, stride, dtype=dtype, device=like.device)
+    """An uninitialised tensor on ``like``'s device (half the time of ``torch.empty``)."""
+    return like.new_empty_strided(size, stride, dtype=dtype)
 
 
 def _ptr(t: Optional[torch.Tensor]):
@@ -73,7 +73,7 @@ def nvfp4_quantize(src: torch.Tensor, amax: Optional[torch.Tensor] = None, trans
 
     tensor_scale: the smallest power of two >= amax / 2688 (1 for amax = 0). ``amax``: one float32 on the device, finite
     and not negative, for a largest magnitude known from calibration (what exceeds it saturates); without it the largest
-    finite magnitude of src is found first, in a pass of its own. Block scale: the e4m3 value nearest to
+    finite magnitude of src is found first: in the same launch for small sources, in a pass of its own for others. Block scale: the e4m3 value nearest to
     max|x| / (6 tensor_scale), at most 448; code: the e2m1 value nearest to x / (scale tensor_scale), ties to the even
     code, at most 6 in magnitude. A block with an infinity or a NaN gets the scale NaN.
 
@@ -104,7 +104,7 @@ def nvfp4_quantize(src: torch.Tensor, amax: Optional[torch.Tensor] = None, trans
             return nvfp4_quantize(src, amax, transpose, data, scales, tensor_scale)
     sp = _raw_stream(device)
     pitch = (width + 15) // 16 * 16  # TMA rows start on 16-byte boundaries
-    src_pitch = src.stride(0) if rows > 1 else k
+    src_pitch = src.stride()[0] if rows > 1 else k
     dtype = _TORCH_TO_PTO[src.dtype]
     if data is None:
         data = _new((out_rows, width), (pitch, 1), torch.uint8, src)
@@ -113,12 +113,16 @@ def nvfp4_quantize(src: torch.Tensor, amax: Optional[torch.Tensor] = None, trans
         scales = _new(tiles, (tiles[1] * 512, 512, 1), torch.uint8, src)
     if tensor_scale is None:
         tensor_scale = _new((1,), (1,), torch.float32, src)
+    out_pitch = data.stride()[0] if out_rows > 1 else pitch
     if amax is None:
         amax = _new((1,), (1,), torch.float32, src)
-        _capi.check(lib.pto_b200_amax(sp, amax.data_ptr(), src.data_ptr(), rows, k, src_pitch, dtype), "pto_b200_amax")
+        rc = lib.pto_b200_nvfp4_quantize_dynamic(sp, data.data_ptr(), scales.data_ptr(), tensor_scale.data_ptr(),
+                                                 amax.data_ptr(), src.data_ptr(), rows, k, src_pitch, out_pitch, dtype,
+                                                 1 if transpose else 0)
+        _capi.check(rc, "pto_b200_nvfp4_quantize_dynamic")
+        return data, scales, tensor_scale
     rc = lib.pto_b200_nvfp4_quantize(sp, data.data_ptr(), scales.data_ptr(), tensor_scale.data_ptr(), src.data_ptr(),
-                                     amax.data_ptr(), rows, k, src_pitch, data.stride(0) if out_rows > 1 else pitch, dtype,
-                                     1 if transpose else 0)
+                                     amax.data_ptr(), rows, k, src_pitch, out_pitch, dtype, 1 if transpose else 0)
     _capi.check(rc, "pto_b200_nvfp4_quantize")
     return data, scales, tensor_scale
 
@@ -154,8 +158,8 @@ def nvfp4_dequantize(data: torch.Tensor, scales: torch.Tensor, tensor_scale: Opt
     cols = out.shape[1]
     rc = lib.pto_b200_nvfp4_dequantize(_raw_stream(device), out.data_ptr(), data.data_ptr(), scales.data_ptr(),
                                        _ptr(tensor_scale), rows, cols,
-                                       data.stride(0) if rows > 1 else (k // 2 + 3) // 4 * 4,
-                                       out.stride(0) if rows > 1 else cols, _TORCH_TO_PTO[out.dtype])
+                                       data.stride()[0] if rows > 1 else (k // 2 + 3) // 4 * 4,
+                                       out.stride()[0] if rows > 1 else cols, _TORCH_TO_PTO[out.dtype])
     _capi.check(rc, "pto_b200_nvfp4_dequantize")
     return out
 
@@ -201,7 +205,7 @@ def gemm_nvfp4(a: torch.Tensor, b_dn: torch.Tensor, sfa: torch.Tensor, sfb: torc
     row = (k // 2 + 15) // 16 * 32  # a single row's pitch, in 4-bit elements
     rc = lib.pto_b200_gemm_nvfp4(_raw_stream(device), out.data_ptr(), a.data_ptr(), b_dn.data_ptr(), sfa.data_ptr(),
                                  sfb.data_ptr(), _ptr(ga), _ptr(gb), _ptr(bias), m, n, k,
-                                 a.stride(0) * 2 if m > 1 else row, b_dn.stride(0) * 2 if n > 1 else row,
-                                 out.stride(0) if m > 1 else n, _TORCH_TO_PTO[out.dtype])
+                                 a.stride()[0] * 2 if m > 1 else row, b_dn.stride()[0] * 2 if n > 1 else row,
+                                 out.stride()[0] if m > 1 else n, _TORCH_TO_PTO[out.dtype])
     _capi.check(rc, "pto_b200_gemm_nvfp4")
     return out

@@ -47,6 +47,14 @@ def test_quantize_refusals(lib, p):
         (dict(src=p + 1), EALIGN), (dict(data=p + 4), EALIGN), (dict(ld_data=36), EALIGN), (dict(scales=p + 2), EALIGN),
         (dict(tensor_scale=p + 2), EALIGN), (dict(amax=p + 1), EALIGN), (dict(dtype=F32, src=p + 2), EALIGN),
     ])
+    good = dict(stream=None, data=p, scales=p, tensor_scale=p, amax=p, src=p, rows=4, k=64, ld_src=64, ld_data=32, dtype=BF16,
+                transpose=0)
+    refused(lib.pto_b200_nvfp4_quantize_dynamic, good, [
+        (dict(data=None), EINVAL), (dict(scales=None), EINVAL), (dict(tensor_scale=None), EINVAL), (dict(src=None), EINVAL),
+        (dict(amax=None), EINVAL), (dict(rows=0), EINVAL), (dict(k=-1), EINVAL), (dict(ld_src=63), EINVAL),
+        (dict(ld_data=24), EINVAL), (dict(rows=1 << 20, ld_data=24), EINVAL), (dict(transpose=1, rows=65), EINVAL),
+        (dict(dtype=S8), EDTYPE), (dict(src=p + 1), EALIGN), (dict(data=p + 4), EALIGN), (dict(scales=p + 2), EALIGN),
+        (dict(tensor_scale=p + 2), EALIGN), (dict(amax=p + 1), EALIGN), (dict(rows=1 << 20, amax=p + 2), EALIGN)])
     good = dict(stream=None, amax=p, src=p, rows=4, k=64, ld_src=64, dtype=F32)
     refused(lib.pto_b200_amax, good, [(dict(amax=None), EINVAL), (dict(src=None), EINVAL), (dict(rows=-1), EINVAL),
                                       (dict(ld_src=8), EINVAL), (dict(dtype=S8), EDTYPE), (dict(src=p + 2), EALIGN),

@@ -65,6 +65,23 @@ def test_quantize_is_exact(rows, cols, pitch, offset, transpose, dtype):
     check_quantized(pto.nvfp4_quantize(x, transpose=transpose), *want, rows)
 
 
+# blocks of 16 in one launch: within CTAs of 256 to 1024 threads, one to eight of them, once and twice over, and one more than fits
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("rows,cols", [(16, 1024), (17, 1024), (1, 20000), (33, 1009), (64, 4096), (3, 65536), (128, 2048), (1024, 255),
+                                       (1025, 256), (1, 262144), (1, 262208), (4096, 3), (4097, 3)])
+def test_one_launch_and_two_agree(rows, cols, dtype):
+    x, host = wide(rows, cols, dtype, rows + cols)
+    x[rows // 2, cols // 2] = float("inf")  # its block only
+    x[rows - 1, cols - 1] = -100.0 if rows * cols > 3 else 1.0
+    amax = x.float().abs()
+    amax = amax[torch.isfinite(amax)].max().reshape(1)
+    before = pto.launch_count()
+    got = pto.nvfp4_quantize(x)
+    assert pto.launch_count() - before == (1 if rows * ((cols + 63) // 64) * 4 <= 16384 else 2)
+    for a, b in zip(got, pto.nvfp4_quantize(x, amax=amax)):
+        assert torch.equal(a, b)
+
+
 @pytest.mark.parametrize("transpose", [False, True])
 def test_quantize_ties_and_borders(transpose):
     # every border of the 4-bit grid and its fp32 neighbours, times scales of every significand
