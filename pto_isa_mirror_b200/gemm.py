@@ -36,6 +36,25 @@ def _stream_ptr(stream: Optional[torch.cuda.Stream]) -> int:
     return stream.cuda_stream if stream is not None else _raw_stream(torch.cuda.current_device())
 
 
+def _device_of(first: torch.Tensor, *others: Optional[torch.Tensor]) -> int:
+    """The ordinal of the one device that all tensors are on."""
+    device = first.get_device()
+    for t in others:
+        if t is not None and t.get_device() != device:
+            raise ValueError("all tensors must be on one CUDA device")
+    return device
+
+
+def _elsewhere(device: int, stream: Optional[torch.cuda.Stream]):
+    """None when launches go to the current stream of the current device, which is ``device``; otherwise a context in which
+    they do, ``stream`` being that stream when one is given - and in which what is allocated belongs to it."""
+    if stream is None:
+        return None if device == torch.cuda.current_device() else torch.cuda.device(device)
+    if stream.device_index != device:
+        raise ValueError("stream is on another device than the tensors")
+    return torch.cuda.stream(stream)
+
+
 def _require_cuda_2d(t: torch.Tensor, name: str) -> None:
     if not t.is_cuda:
         raise ValueError(f"{name} must be a CUDA tensor")
@@ -350,12 +369,17 @@ def mx_quantize_e4m3(src: torch.Tensor, stream: Optional[torch.cuda.Stream] = No
             _require_cuda_2d(t, name)
             if t.dtype != torch.uint8 or tuple(t.shape) != shape:
                 raise ValueError(f"{name} must be a uint8 CUDA tensor of shape {shape}")
+    device = _device_of(src, data, scales)
+    if device != torch.cuda.current_device():
+        with torch.cuda.device(device):
+            return mx_quantize_e4m3(src, stream, data, scales, scale_alg)
     if data is None:
         data = src.new_empty_strided((rows, k), (k, 1), dtype=torch.uint8)
     if scales is None:
         scales = src.new_empty_strided((rows, k // 32), (k // 32, 1), dtype=torch.uint8)
-    rc = lib.pto_b200_mx_quantize_e4m3_src(_stream_ptr(stream), data.data_ptr(), scales.data_ptr(), src.data_ptr(), rows,
-                                           k, src.stride()[0], data.stride()[0], scales.stride()[0], _TORCH_TO_PTO[src.dtype],
+    rc = lib.pto_b200_mx_quantize_e4m3_src(_stream_ptr(stream), data.data_ptr(), scales.data_ptr(), src.data_ptr(), rows, k,
+                                           src.stride()[0] if rows > 1 else k, data.stride()[0] if rows > 1 else k,
+                                           scales.stride()[0] if rows > 1 else k // 32, _TORCH_TO_PTO[src.dtype],
                                            scale_alg)
     _capi.check(rc, "pto_b200_mx_quantize_e4m3_src")
     return data, scales

@@ -14,31 +14,12 @@ from typing import Optional, Tuple
 import torch
 
 from . import _capi
-from .gemm import _TORCH_TO_PTO, _raw_stream, _require_cuda_2d
+from .gemm import _TORCH_TO_PTO, _device_of, _elsewhere, _raw_stream, _require_cuda_2d
 
 _FLOATS = (torch.float32, torch.bfloat16, torch.float16)
 # what packed codes and scale bytes may come as
 _CODES = (torch.uint8, torch.int8) + ((torch.float4_e2m1fn_x2,) if hasattr(torch, "float4_e2m1fn_x2") else ())
 _E4M3_BYTES = (torch.uint8, torch.float8_e4m3fn)
-
-
-def _device_of(first: torch.Tensor, *others: Optional[torch.Tensor]) -> int:
-    """The ordinal of the one device that all tensors are on."""
-    device = first.get_device()
-    for t in others:
-        if t is not None and t.get_device() != device:
-            raise ValueError("all tensors must be on one CUDA device")
-    return device
-
-
-def _elsewhere(device: int, stream: Optional[torch.cuda.Stream]):
-    """None when launches go to the current stream of the current device, which is ``device``; otherwise a context in which
-    they do, ``stream`` being that stream when one is given - and in which what is allocated belongs to it."""
-    if stream is None:
-        return None if device == torch.cuda.current_device() else torch.cuda.device(device)
-    if stream.device_index != device:
-        raise ValueError("stream is on another device than the tensors")
-    return torch.cuda.stream(stream)
 
 
 def _require_float_scalar(t: Optional[torch.Tensor], name: str) -> None:

@@ -6,8 +6,8 @@ from typing import Optional
 import torch
 
 from . import _capi
-from .gemm import _TORCH_TO_PTO, _raw_stream, _require_cuda_2d
-from .nvfp4 import _FLOATS, _device_of, _elsewhere, _new, _ptr
+from .gemm import _TORCH_TO_PTO, _device_of, _elsewhere, _raw_stream, _require_cuda_2d
+from .nvfp4 import _FLOATS, _new, _ptr
 
 
 def _scratch_pays(t: int, n: int, k: int) -> bool:
@@ -72,7 +72,8 @@ def gemm_wgrad_mx(dy: torch.Tensor, data: torch.Tensor, scales: torch.Tensor, ou
     if workspace is None and _scratch_pays(t, n, k):
         given = _new((2 * t * k,), (1,), torch.uint8, dy)
     rc = lib.pto_b200_gemm_wgrad_mx(_raw_stream(device), out.data_ptr(), dy.data_ptr(), data.data_ptr(), scales.data_ptr(),
-                                    _ptr(addend), _ptr(given), 0 if given is None else given.numel(), t, n, k, dy.stride()[0] if t > 1 else (n + 7) // 8 * 8,
+                                    _ptr(addend), _ptr(given), 0 if given is None else given.numel(), t, n, k,
+                                    dy.stride()[0] if t > 1 else (n + 7) // 8 * 8,
                                     data.stride()[0] if t > 1 else (k + 15) // 16 * 16, scales.stride()[0] if t > 1 else k // 32,
                                     out.stride()[0] if n > 1 else k,
                                     0 if addend is None else addend.stride()[0] if n > 1 else k, _TORCH_TO_PTO[dy.dtype],

@@ -42,6 +42,17 @@ def test_16bit_source_gives_the_bytes_of_float32(rows, k, pitch, alg, dtype):
     assert torch.equal(data, want_data) and torch.equal(scales, want_scales)
 
 
+@pytest.mark.parametrize("dtype", FLOATS)
+def test_one_row_of_any_pitch(dtype):
+    column = torch.randn((96, 1), generator=gen(3)).to(dtype).to(DEV)
+    row = column.t()  # one row whose stride says nothing
+    assert row.stride() == (1, 1)
+    got, want = pto.mx_quantize_e4m3(row), pto.mx_quantize_e4m3(column.reshape(1, 96))
+    assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+    for a, b in zip(pto.nvfp4_quantize(row), pto.nvfp4_quantize(column.reshape(1, 96))):
+        assert torch.equal(a, b)
+
+
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
 def test_16bit_extremes(dtype):
     every = torch.arange(0, 65536, dtype=torch.int32).to(torch.int16).view(dtype)  # every pattern there is
