@@ -75,7 +75,7 @@ int launch_wgrad(cudaStream_t stream, const HostContext& host, const uint8_t* dy
     auto kernel = gemm_wgrad_mx<F16, OUT, SCRATCH>;
     static std::atomic<int> resident[kMaxDevices][3]; // clusters of 2, 4 and 8 CTAs that the device holds at once
     cudaLaunchConfig_t cfg = {};
-    cudaLaunchAttribute attr[1];
+    cudaLaunchAttribute attr[2];
     attr[0].id = cudaLaunchAttributeClusterDimension;
     attr[0].val.clusterDim.x = 2;
     attr[0].val.clusterDim.y = 1;
@@ -149,6 +149,9 @@ int launch_wgrad(cudaStream_t stream, const HostContext& host, const uint8_t* dy
         return PTO_B200_EINVAL;
     }
     cfg.gridDim = dim3(static_cast<unsigned>(2 * p.splits * clusters), 1, 1);
+    attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization; // the kernel waits for what comes before it itself
+    attr[1].val.programmaticStreamSerializationAllowed = 1;
+    cfg.numAttrs = 2;
     count_launches(1);
     return note_cuda_error(cudaLaunchKernelEx(&cfg, kernel, tdy, tx, p), "gemm_wgrad_mx launch");
 }

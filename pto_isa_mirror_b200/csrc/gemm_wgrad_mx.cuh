@@ -309,10 +309,10 @@ __global__ void __launch_bounds__(kWgThreads, 1)
     }
     ptx::tc_fence_before_sync();
     __syncthreads();
-    ptx::cluster_arrive(); // the peer's barriers must exist before anything is signalled across the pair
-    ptx::cluster_wait();
+    ptx::cluster_arrive(); // the peer's barriers must exist before anything is signalled across the pair: cluster_wait below
     ptx::tc_fence_after_sync();
     const uint32_t tmem_base = *tmem_base_slot;
+    ptx::grid_dependency_wait(); // nothing of an earlier launch's is read or overwritten before it has ended
 
     auto tile_of = [&](int tile, int& ki, int& ni) { // grouped raster: a wave of pairs shares few columns of dy and x
         const int group_size = p.group * p.n_tiles;
@@ -326,6 +326,7 @@ __global__ void __launch_bounds__(kWgThreads, 1)
 
     if (warp < 4) {
         asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kWgRegsOthers));
+        ptx::cluster_wait();
         if (warp == 0) {
             // ---------------------------------------------------------------- loads of dy (with SCRATCH of x, too)
             int stage = 0;
@@ -484,7 +485,7 @@ __global__ void __launch_bounds__(kWgThreads, 1)
         };
         auto start_scales = [&](int tile) { // of the first stage that this group converts of a tile
             int ki, ni;
-            tile_of(min(tile, tiles - 1), ki, ni);
+            tile_of(tile, ki, ni);
             const int column = min(ki * 256 + side * 128 + piece * 16, p.k - 1) >> 5;
             scale_off = static_cast<uint32_t>(row * p.ld_scales + column);
             visit_token = (first_stage + first_of_tile) * kWgStageTokens;
@@ -493,6 +494,7 @@ __global__ void __launch_bounds__(kWgThreads, 1)
         if constexpr (!SCRATCH) {
             start_scales(cluster);
         }
+        ptx::cluster_wait();
         for (int tile = cluster; ok && tile < tiles; tile += clusters) {
             int ki, ni;
             tile_of(tile, ki, ni);
@@ -586,7 +588,7 @@ __global__ void __launch_bounds__(kWgThreads, 1)
                 break;
             }
             first_of_tile = (first_of_tile - stages % kWgGroups + kWgGroups) % kWgGroups; // stages go round the groups
-            if constexpr (!SCRATCH) {
+            if (!SCRATCH && tile + clusters < tiles) {
                 start_scales(tile + clusters); // come while this tile is stored
             }
             const int in_tile = quarter * 32 + lane;
@@ -636,7 +638,13 @@ __global__ void __launch_bounds__(kWgThreads, 1)
             __nanosleep(1000);
         }
     }
-    ptx::cluster_arrive(); // no CTA touches another's tensor memory or barriers any more; partial sums are in place
+    // No CTA touches another's tensor memory or barriers any more. Partial sums, where there are some, are in place; without
+    // them the arrival orders nothing (the other form waits for the tile's stores).
+    if (p.splits > 1) {
+        ptx::cluster_arrive();
+    } else {
+        ptx::cluster_arrive_relaxed();
+    }
     ptx::cluster_wait();
     if (warp == 1) {
         ptx::tc_fence_after_sync();
