@@ -276,7 +276,7 @@ int pto_b200_nvfp4_dequantize(void* stream, uint8_t* out, const uint8_t* data, c
                               const float* tensor_scale, int rows, int k, long long ld_data, long long ld_out, int out_dtype);
 
 /*
- * C = scale_a scale_b (A * B) (+ bias) of NVFP4 matrices, fp32 accumulation.
+ * C = scale_a scale_b (A * B) (+ bias) of NVFP4 matrices, fp32 accumulation; scale_a scale_b is formed first, in fp32.
  *   src0 / src1 : A (m x k) and B column-major (n x k) codes, 16-byte aligned; lda, ldb in 4-bit elements, multiples of 32
  *   src2 / src3 : their scale tiles, 16-byte aligned; scale_a, scale_b: their tensor scales on the device, or null for 1
  *   bias        : n floats or null, added before the store cast; out_dtype F32, BF16 or F16; k % 16 == 0.

@@ -175,6 +175,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kNvPairThreads, 1)
     ptx::cluster_wait();
     ptx::tc_fence_after_sync();
     const uint32_t tmem_base = *tmem_base_slot;
+    ptx::grid_dependency_wait(); // as in the kernel for few rows
 
     if (warp == 0) {
         // ---------------------------------------------------------------- loads (both CTAs)

@@ -105,7 +105,7 @@ int launch_quantize_one_of(cudaStream_t s, const void* src, float* amax, uint8_t
         ctas *= 2;
     }
     cudaLaunchConfig_t cfg = {};
-    cudaLaunchAttribute attr[1];
+    cudaLaunchAttribute attr[2];
     attr[0].id = cudaLaunchAttributeClusterDimension;
     attr[0].val.clusterDim.x = static_cast<unsigned>(ctas);
     attr[0].val.clusterDim.y = 1;
@@ -114,7 +114,9 @@ int launch_quantize_one_of(cudaStream_t s, const void* src, float* amax, uint8_t
     cfg.blockDim = dim3(THREADS, 1, 1);
     cfg.stream = s;
     cfg.attrs = attr;
-    cfg.numAttrs = 1;
+    attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization; // the kernel waits for what comes before it itself
+    attr[1].val.programmaticStreamSerializationAllowed = 1;
+    cfg.numAttrs = 2;
     count_launches(1);
     return note_cuda_error(cudaLaunchKernelEx(&cfg, nvfp4_quantize_one_kernel<SRC, VEC, THREADS>, src, amax, data, scales,
                                               tensor_scale, rows, k, ld_src, ld_data),
@@ -183,7 +185,7 @@ int launch_nv_pair(cudaStream_t stream, const HostContext& host, const NvProblem
     auto kernel = gemm_nvfp4_2cta<OUT>;
     static std::atomic<int> max_clusters[kMaxDevices];
     cudaLaunchConfig_t cfg = {};
-    cudaLaunchAttribute attr[1];
+    cudaLaunchAttribute attr[2];
     attr[0].id = cudaLaunchAttributeClusterDimension;
     attr[0].val.clusterDim.x = 2;
     attr[0].val.clusterDim.y = 1;
@@ -233,6 +235,9 @@ int launch_nv_pair(cudaStream_t stream, const HostContext& host, const NvProblem
     if (rc) {
         return rc;
     }
+    attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization; // the kernel waits for what comes before it itself
+    attr[1].val.programmaticStreamSerializationAllowed = 1;
+    cfg.numAttrs = 2;
     cfg.gridDim = dim3(static_cast<unsigned>(2 * (p.units < clusters ? p.units : clusters)), 1, 1);
     count_launches(1);
     return note_cuda_error(cudaLaunchKernelEx(&cfg, kernel, ta, tb, tb_half, tsa, tsb, p), "gemm_nvfp4_2cta launch");

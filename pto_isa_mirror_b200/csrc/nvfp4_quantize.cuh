@@ -427,6 +427,7 @@ __global__ void __launch_bounds__(THREADS)
     const int total = rows * row_blocks; // at most 16 THREADS, and a multiple of 4: the groups of nv_store_block stay whole
     const int ctas = static_cast<int>(gridDim.x); // the cluster
     const int first = static_cast<int>(blockIdx.x * THREADS + threadIdx.x);
+    ptx::grid_dependency_wait(); // the launch may overlap the end of the one before (programmatic serialisation)
     NvRaw16<SRC> raw[kNvItems];
     int rows_of[kNvItems], kbs[kNvItems];
 #pragma unroll

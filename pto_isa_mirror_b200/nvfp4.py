@@ -151,7 +151,8 @@ def gemm_nvfp4(a: torch.Tensor, b_dn: torch.Tensor, sfa: torch.Tensor, sfb: torc
                stream: Optional[torch.cuda.Stream] = None) -> torch.Tensor:
     """C = ga gb (A @ B) (+ bias) of NVFP4 matrices: a [M, K / 2] and b_dn [N, K / 2] packed codes, sfa and sfb their scale
     tiles, ga and gb their tensor scales (one float32 each on the device; None: 1), as :func:`nvfp4_quantize` returns
-    them. K is a multiple of 16; rows start on 16-byte boundaries. fp32 accumulation; C is float32, bfloat16 or float16.
+    them. K is a multiple of 16; rows start on 16-byte boundaries. fp32 accumulation, then times ga gb, which is
+    formed first, in fp32; C is float32, bfloat16 or float16.
     ``bias``: n float32 values added per column before the store's rounding. Any M: few rows take a kernel that reads B at
     memory speed, many rows one of 256 x 256 tiles on pairs of SMs."""
     lib = _capi.load()
