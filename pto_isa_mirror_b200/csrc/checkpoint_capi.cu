@@ -30,9 +30,10 @@ int launch_quantize16(cudaStream_t s, const HostContext& host, const uint8_t* sr
     const long long want = (static_cast<long long>(rows) * (k / 16) + kQuantThreads - 1) / kQuantThreads;
     const long long cap = static_cast<long long>(host.sm_count) * per_sm; // one resident wave
     const int grid = static_cast<int>(want < cap ? want : cap);
-    kernel<<<grid, kQuantThreads, 0, s>>>(reinterpret_cast<const uint16_t*>(src), data, scales, rows, k, ld_src, ld_data, ld_scales);
     count_launches(1);
-    return note_cuda_error(cudaGetLastError(), "mx_quantize (16-bit) launch");
+    return note_cuda_error(launch_rows(host, kernel, grid, kQuantThreads, s, reinterpret_cast<const uint16_t*>(src), data, scales,
+                                              rows, k, ld_src, ld_data, ld_scales),
+                           "mx_quantize (16-bit) launch");
 }
 
 template <int ALG, int SRC>
@@ -62,10 +63,10 @@ int launch_convert(cudaStream_t s, const HostContext& host, const uint8_t* data,
     }
     const long long want = (static_cast<long long>(p.t) * (p.k / 16) + kWgConvertThreads - 1) / kWgConvertThreads;
     const long long cap = static_cast<long long>(host.sm_count) * per_sm;
-    kernel<<<static_cast<int>(want < cap ? want : cap), kWgConvertThreads, 0, s>>>(
-        data, p.scales, reinterpret_cast<uint16_t*>(scratch), p.t, p.k, ld_data, p.ld_scales);
     count_launches(1);
-    return note_cuda_error(cudaGetLastError(), "mx_to_16bit launch");
+    return note_cuda_error(launch_rows(host, kernel, static_cast<int>(want < cap ? want : cap), kWgConvertThreads, s, data, p.scales,
+                                              reinterpret_cast<uint16_t*>(scratch), p.t, p.k, ld_data, p.ld_scales),
+                           "mx_to_16bit launch");
 }
 
 template <bool F16, int OUT, bool SCRATCH>

@@ -216,6 +216,7 @@ __global__ void __launch_bounds__(kWgConvertThreads) mx_to_16bit_kernel(const ui
     long long row = i / row_items;
     int c = static_cast<int>(i - row * row_items);
     constexpr int kItems = 4;
+    ptx::grid_dependency_wait();
     while (i < total) {
         uint4 in[kItems];
         uint32_t e[kItems];

@@ -24,6 +24,7 @@
 #include <cstdint>
 
 #include "row_elements.cuh"
+#include "sm100_ptx.cuh"
 
 namespace pto_b200 {
 
@@ -168,6 +169,7 @@ __global__ void __launch_bounds__(kQuantThreads) mx_quantize_e4m3_16bit_kernel(c
     const int c_step = static_cast<int>(stride - row_step * row_items);
     long long cur_row = i / row_items;
     int cur_c = static_cast<int>(i - cur_row * row_items);
+    ptx::grid_dependency_wait();
     while (i - static_cast<int>(threadIdx.x & 31u) < total) { // the warp goes on together
         NvRaw16<SRC> raw[kQuant16Items];
         long long row[kQuant16Items];

@@ -43,6 +43,7 @@ int launch_quantize(cudaStream_t s, const HostContext& host, const void* src, co
                     float* tensor_scale, int rows, int k, long long ld_src, long long ld_data, bool transpose)
 {
     int grid = 0;
+    cudaError_t launched;
     if (transpose) {
         // 16-bit columns in pairs where rows start on 4-byte boundaries
         const bool pairs = SRC != NV_F32 && !misaligned(src, 4) && ld_src % 2 == 0;
@@ -52,25 +53,25 @@ int launch_quantize(cudaStream_t s, const HostContext& host, const void* src, co
             if (int rc = one_wave<nvfp4_quantize_transposed_kernel<SRC, kPairs>>(items, host, &grid)) {
                 return rc;
             }
-            nvfp4_quantize_transposed_kernel<SRC, kPairs>
-                <<<grid, kNvQuantThreads, 0, s>>>(src, amax, data, scales, tensor_scale, rows, k, ld_src, ld_data);
+            launched = launch_rows(host, nvfp4_quantize_transposed_kernel<SRC, kPairs>, grid, kNvQuantThreads, s, src, amax, data,
+                                          scales, tensor_scale, rows, k, ld_src, ld_data);
         } else {
             if (int rc = one_wave<nvfp4_quantize_transposed_kernel<SRC, false>>(items, host, &grid)) {
                 return rc;
             }
-            nvfp4_quantize_transposed_kernel<SRC, false>
-                <<<grid, kNvQuantThreads, 0, s>>>(src, amax, data, scales, tensor_scale, rows, k, ld_src, ld_data);
+            launched = launch_rows(host, nvfp4_quantize_transposed_kernel<SRC, false>, grid, kNvQuantThreads, s, src, amax, data,
+                                          scales, tensor_scale, rows, k, ld_src, ld_data);
         }
     } else {
         const long long items = (static_cast<long long>(rows) + 127) / 128 * 128 * ((k + 63) / 64 * 4);
         if (int rc = one_wave<nvfp4_quantize_kernel<SRC, VEC>>(items, host, &grid)) {
             return rc;
         }
-        nvfp4_quantize_kernel<SRC, VEC>
-            <<<grid, kNvQuantThreads, 0, s>>>(src, amax, data, scales, tensor_scale, rows, k, ld_src, ld_data);
+        launched = launch_rows(host, nvfp4_quantize_kernel<SRC, VEC>, grid, kNvQuantThreads, s, src, amax, data, scales,
+                                      tensor_scale, rows, k, ld_src, ld_data);
     }
     count_launches(1);
-    return note_cuda_error(cudaGetLastError(), "nvfp4_quantize launch");
+    return note_cuda_error(launched, "nvfp4_quantize launch");
 }
 
 template <int SRC, int VEC>
@@ -144,10 +145,10 @@ int launch_dequantize(cudaStream_t s, const HostContext& host, const uint8_t* da
     if (int rc = one_wave<nvfp4_dequantize_kernel<DST, VEC>>(static_cast<long long>(rows) * ((k + kElems - 1) / kElems), host, &grid)) {
         return rc;
     }
-    nvfp4_dequantize_kernel<DST, VEC>
-        <<<grid, kNvQuantThreads, 0, s>>>(data, scales, tensor_scale, out, rows, k, ld_data, ld_out);
     count_launches(1);
-    return note_cuda_error(cudaGetLastError(), "nvfp4_dequantize launch");
+    return note_cuda_error(launch_rows(host, nvfp4_dequantize_kernel<DST, VEC>, grid, kNvQuantThreads, s, data, scales, tensor_scale,
+                                              out, rows, k, ld_data, ld_out),
+                           "nvfp4_dequantize launch");
 }
 
 // The widest access that every row of a matrix starts on: 32 or 16 bytes, or 0 for its elements.

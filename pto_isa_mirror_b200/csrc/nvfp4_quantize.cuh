@@ -198,7 +198,8 @@ __global__ void __launch_bounds__(kNvQuantThreads)
     const int kb_step = static_cast<int>(stride - row_step * row_blocks);
     long long row = i / row_blocks;
     int kb = static_cast<int>(i - row * row_blocks);
-    const NvTensorScale t(__ldg(amax));
+    ptx::grid_dependency_wait();
+    const NvTensorScale t(*static_cast<const volatile float*>(amax)); // volatile: stays behind the wait
     if (blockIdx.x == 0 && threadIdx.x == 0) {
         *tensor_scale = t.g;
     }
@@ -254,7 +255,8 @@ __global__ void __launch_bounds__(kNvQuantThreads)
     const int col_items = (k + 127) / 128 * (128 / kCols);
     const long long total = static_cast<long long>(k_atoms) * col_items;
     const bool wide = (reinterpret_cast<uintptr_t>(data) & 31u) == 0 && (ld_data & 31) == 0;
-    const NvTensorScale t(__ldg(amax));
+    ptx::grid_dependency_wait();
+    const NvTensorScale t(*static_cast<const volatile float*>(amax)); // volatile: stays behind the wait
     if (blockIdx.x == 0 && threadIdx.x == 0) {
         *tensor_scale = t.g;
     }
@@ -533,7 +535,8 @@ __global__ void __launch_bounds__(kNvQuantThreads)
     constexpr int kWords = kElems / 8;
     const int row_items = (k + kElems - 1) / kElems;
     const int k_atoms = (k + 63) / 64;
-    const float g = tensor_scale != nullptr ? __ldg(tensor_scale) : 1.0f;
+    ptx::grid_dependency_wait();
+    const float g = tensor_scale != nullptr ? *static_cast<const volatile float*>(tensor_scale) : 1.0f; // behind the wait
     const long long total = static_cast<long long>(rows) * row_items;
     const long long stride = static_cast<long long>(gridDim.x) * blockDim.x;
     long long i = blockIdx.x * static_cast<long long>(blockDim.x) + threadIdx.x;
