@@ -299,9 +299,9 @@ int launch_nv(cudaStream_t stream, const HostContext& host, const NvProblem& q, 
 {
     // More than 128 rows: CTA pairs, unless the tiles are so few that the other kernel cuts K into four parts or more and K
     // is long enough to gain by it (beyond eight 256-element stages). Measured, few rows / pairs, us: 512x8192x8192 (64
-    // tiles of 256 x 256) 24.4 / 19.5, 200x8192x4096 (32) 13.8 / 12.0, 200x4096x8192 (16) 13.7 / 16.1, 256x512x8192 (2)
-    // 8.8 / 15.5, 144x512x1024 (2, four stages) 7.4 / 6.5. At most 128 rows: half of a pair's rows would be empty,
-    // 128x8192x8192 15.8 / 17.0, 48x14336x4096 11.6 / 13.5.
+    // tiles of 256 x 256) 23.1 / 16.9, 200x8192x4096 (32) 11.6 / 10.3, 200x4096x8192 (16) 11.2 / 14.6, 256x512x8192 (2)
+    // 7.6 / 14.2, 144x512x1024 (2, four stages) 7.8 / 6.1. At most 128 rows: half of a pair's rows would be empty,
+    // 128x8192x8192 12.2 / 15.5, 48x14336x4096 9.2 / 10.7.
     const long long tiles256 = ((static_cast<long long>(q.m) + 255) / 256) * ((static_cast<long long>(q.n) + 255) / 256);
     if (q.m > 128 && (8 * tiles256 > host.sm_count || p.k_stages <= 8)) {
         return launch_nv_pair<OUT>(stream, host, q, p);

@@ -199,7 +199,7 @@ __global__ void __launch_bounds__(kNvQuantThreads)
     long long row = i / row_blocks;
     int kb = static_cast<int>(i - row * row_blocks);
     ptx::grid_dependency_wait();
-    const NvTensorScale t(*static_cast<const volatile float*>(amax)); // volatile: stays behind the wait
+    const NvTensorScale t(nv_ld_common(amax));
     if (blockIdx.x == 0 && threadIdx.x == 0) {
         *tensor_scale = t.g;
     }
@@ -256,7 +256,7 @@ __global__ void __launch_bounds__(kNvQuantThreads)
     const long long total = static_cast<long long>(k_atoms) * col_items;
     const bool wide = (reinterpret_cast<uintptr_t>(data) & 31u) == 0 && (ld_data & 31) == 0;
     ptx::grid_dependency_wait();
-    const NvTensorScale t(*static_cast<const volatile float*>(amax)); // volatile: stays behind the wait
+    const NvTensorScale t(nv_ld_common(amax));
     if (blockIdx.x == 0 && threadIdx.x == 0) {
         *tensor_scale = t.g;
     }
@@ -411,7 +411,7 @@ __global__ void __launch_bounds__(kAmaxSingleThreads)
 // Few rows: the largest magnitude and the codes in one launch. A cluster of up to eight CTAs holds the matrix in registers
 // between the two, kNvItems blocks of 16 per thread, and exchanges its maxima over distributed shared memory. The CTAs have
 // 256, 512 or 1024 threads, the fewest that hold it, since large ones start and meet slowly: 8x4096 bf16 2.9 us with 256,
-// 4.1 with 1024. Two launches take 5.0 us there, 3.9 against 2.3 at 1x4096, 8.2 against 5.2 at 64x4096.
+// 4.1 with 1024 (2.5 as it is launched now). In two launches / in one: 1x4096 4.0 / 2.6, 8x4096 4.6 / 2.5, 64x4096 7.8 / 4.5.
 constexpr int kNvOneCtas = 8;
 constexpr int kNvOneBlocks = kNvOneCtas * 1024 * kNvItems; // of 16 elements, a row's filled up to 64
 
@@ -536,7 +536,7 @@ __global__ void __launch_bounds__(kNvQuantThreads)
     const int row_items = (k + kElems - 1) / kElems;
     const int k_atoms = (k + 63) / 64;
     ptx::grid_dependency_wait();
-    const float g = tensor_scale != nullptr ? *static_cast<const volatile float*>(tensor_scale) : 1.0f; // behind the wait
+    const float g = tensor_scale != nullptr ? nv_ld_common(tensor_scale) : 1.0f;
     const long long total = static_cast<long long>(rows) * row_items;
     const long long stride = static_cast<long long>(gridDim.x) * blockDim.x;
     long long i = blockIdx.x * static_cast<long long>(blockDim.x) + threadIdx.x;

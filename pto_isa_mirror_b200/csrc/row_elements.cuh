@@ -47,6 +47,16 @@ __device__ __forceinline__ void nv_unpack2(uint32_t w, float& lo, float& hi)
     }
 }
 
+// One float that every thread of a grid reads, kept behind what stands before it in the program (a wait for an earlier
+// launch), which a load of constant data need not be. (A volatile load passes the first-level cache by: 2 us more for a
+// cast of 4093x2904 and back.)
+__device__ __forceinline__ float nv_ld_common(const float* ptr)
+{
+    float f;
+    asm volatile("ld.global.ca.f32 %0, [%1];" : "=f"(f) : "l"(ptr) : "memory");
+    return f;
+}
+
 // 32 bytes in one access (32-byte aligned): a warp's accesses are then whole lines. With two of 16 bytes each covers
 // half of every sector (dequantising 16384 x 8192 to bf16 took 92 us that way).
 __device__ __forceinline__ void nv_ld32(const void* ptr, uint4& a, uint4& b)
