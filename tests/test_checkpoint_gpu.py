@@ -316,3 +316,37 @@ def test_a_linear_layers_step(t, n, k):
     # sixth of the block's largest) and of e4m3
     assert float((number(xq) - x.double()).norm() / x.double().norm()) < 0.25
     assert float((x8 - x.double()).norm() / x.double().norm()) < 2.0 ** -4
+
+
+@pytest.mark.parametrize("t,n,k", [(16, 256, 512), (300, 128, 64), (200, 2048, 640)])
+def test_launches_that_overlap_keep_their_order(t, n, k):
+    # the same buffers written and read by one call after the other, no waiting between them; every step's results have to
+    # be those of the step computed alone
+    g = torch.Generator(device=DEV).manual_seed(t)
+    xs = [(torch.randn((t, k), generator=g, device=DEV) * 2.0 ** i).to(torch.bfloat16) for i in range(-6, 6)]
+    dys = [(torch.randn((t, n), generator=g, device=DEV) * 2.0 ** -i).to(torch.bfloat16) for i in range(-6, 6)]
+    w = pto.nvfp4_quantize(torch.randn((n, k), generator=g, device=DEV))
+
+    def step(x, dy, buffers):
+        q = pto.nvfp4_quantize(x, data=buffers[0], scales=buffers[1], tensor_scale=buffers[2])
+        kept = pto.mx_quantize_e4m3(x, data=buffers[3], scales=buffers[4])
+        y = pto.gemm_nvfp4(q[0], w[0], q[1], w[1], q[2], w[2], out=buffers[5], out_dtype=torch.float32)
+        dw = pto.gemm_wgrad_mx(dy, *kept, out=buffers[6], workspace=buffers[7])
+        back = pto.nvfp4_dequantize(*q, out=buffers[8], out_dtype=torch.float32)
+        return [*q, *kept, y, dw, back]
+
+    alone = []
+    for x, dy in zip(xs, dys):
+        alone.append(step(x, dy, [None] * 7 + [False, None]))
+        torch.cuda.synchronize()
+    buffers = [v.clone() for v in alone[0]]
+    buffers = buffers[:7] + [torch.empty(2 * t * k, dtype=torch.uint8, device=DEV), buffers[7]]
+    x, dy = torch.empty_like(xs[0]), torch.empty_like(dys[0])
+    seen = []
+    for i in range(len(xs)):
+        x.copy_(xs[i])
+        dy.copy_(dys[i])
+        seen.append([v.clone() for v in step(x, dy, buffers)])
+    torch.cuda.synchronize()
+    for got, want in zip(seen, alone):
+        assert all(torch.equal(a, b) for a, b in zip(got, want))

@@ -316,3 +316,42 @@ def test_past_two_to_the_31_elements():
     c = pto.gemm_nvfp4(a[0], b[0], a[1], b[1][:(k + 127) // 128])
     want = pto.gemm_nvfp4(a[0][-128:], b[0], a[1][-1:], b[1][:(k + 127) // 128])
     assert torch.equal(c[-128:], want)
+
+
+@pytest.mark.parametrize("m,n,k", [(5, 256, 512), (300, 512, 4096)])
+def test_captured_with_copies_and_two_streams(m, n, k):
+    # launches that may overlap what comes before them, behind a copy, behind a memory set and where two streams join
+    g = torch.Generator().manual_seed(m)
+    x, w = torch.zeros((m, k), device=DEV), torch.zeros((n, k), device=DEV)
+    source = torch.zeros((m, k), device=DEV)
+    side = torch.cuda.Stream()
+    out = torch.zeros((m, n), device=DEV)
+
+    def step():
+        main = torch.cuda.current_stream()
+        side.wait_stream(main)
+        with torch.cuda.stream(side):
+            qw = pto.nvfp4_quantize(w)
+        x.copy_(source)
+        qx = pto.nvfp4_quantize(x)
+        main.wait_stream(side)
+        pto.gemm_nvfp4(qx[0], qw[0], qx[1], qw[1], qx[2], qw[2], out=out)
+        out.add_(0)
+        back = pto.nvfp4_dequantize(*qx, out_dtype=torch.float32)
+        x.zero_()
+        return qx, qw, back
+
+    step()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        qx, qw, back = step()
+    for _ in range(3):
+        source.copy_(torch.randn((m, k), generator=g))
+        w.copy_(torch.randn((n, k), generator=g))
+        graph.replay()
+        torch.cuda.synchronize()
+        a, b = pto.nvfp4_quantize(source), pto.nvfp4_quantize(w)
+        for got, want in zip((*qx, *qw, back), (*a, *b, pto.nvfp4_dequantize(*a, out_dtype=torch.float32))):
+            assert torch.equal(got, want)
+        assert torch.equal(out, pto.gemm_nvfp4(a[0], b[0], a[1], b[1], a[2], b[2], out_dtype=torch.float32))
