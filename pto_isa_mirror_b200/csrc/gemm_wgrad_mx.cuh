@@ -254,6 +254,62 @@ __global__ void __launch_bounds__(kWgConvertThreads) mx_to_16bit_kernel(const ui
     }
 }
 
+// A tile whose tokens were cut over SPLITS pairs: their partial sums [256 n][128 k] lie at the same place of each CTA's
+// shared memory, and CTA `split` of a side adds its share of them in rank order, four k per thread and step. The arrival
+// that lets the other CTAs leave comes behind the last step's reads, in the releasing form, behind which no read is under
+// way, and in front of that step's stores. By the 512 threads of the converting warps.
+template <int SPLITS, int OUT>
+__device__ __forceinline__ void wg_add_parts(const WgradParams& p, uint32_t base, int split, int side, int k0, int n0, int thread)
+{
+    constexpr int kThreads = kWgWorkerWarps * 32;
+    constexpr int kSteps = 256 * 32 / SPLITS / kThreads;
+    using T = typename WgElem<OUT>::type;
+    const int first = split * kSteps * kThreads + thread;
+    const int k = k0 + (first & 31) * 4; // of every step
+#pragma unroll 1
+    for (int j = 0; j < kSteps; ++j) {
+        const int i = first + j * kThreads;
+        const int n = n0 + (i >> 5);
+        const bool mine = k < p.k && n < p.n; // p.k is a multiple of 32
+        float4 part[SPLITS];
+#pragma unroll
+        for (int s = 0; s < SPLITS; ++s) {
+            part[s] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+            if (mine) {
+                part[s] = ptx::ld_shared_cluster_f32x4(
+                    ptx::map_to_cta(base + 16u * static_cast<uint32_t>(i), static_cast<uint32_t>(2 * s + side)));
+            }
+        }
+        float4 f = part[0];
+#pragma unroll
+        for (int s = 1; s < SPLITS; ++s) {
+            f.x += part[s].x;
+            f.y += part[s].y;
+            f.z += part[s].z;
+            f.w += part[s].w;
+        }
+        if (j == kSteps - 1) {
+            __syncwarp();
+            ptx::cluster_arrive();
+        }
+        if (mine) {
+            if (p.addend != nullptr) {
+                const T* add = static_cast<const T*>(p.addend) + n * p.ld_addend + k;
+                const T v[4] = {add[0], add[1], add[2], add[3]};
+                f.x += static_cast<float>(v[0]);
+                f.y += static_cast<float>(v[1]);
+                f.z += static_cast<float>(v[2]);
+                f.w += static_cast<float>(v[3]);
+            }
+            T* at = static_cast<T*>(p.out) + n * p.ld_out + k;
+            at[0] = static_cast<T>(f.x);
+            at[1] = static_cast<T>(f.y);
+            at[2] = static_cast<T>(f.z);
+            at[3] = static_cast<T>(f.w);
+        }
+    }
+}
+
 template <bool F16, int OUT, bool SCRATCH>
 __global__ void __launch_bounds__(kWgThreads, 1)
     gemm_wgrad_mx(const __grid_constant__ CUtensorMap tmap_dy, const __grid_constant__ CUtensorMap tmap_x, const WgradParams p)
@@ -653,53 +709,21 @@ __global__ void __launch_bounds__(kWgThreads, 1)
         ptx::tc_fence_after_sync();
         ptx::tmem_dealloc_pair(tmem_base, kTmemCols);
     }
-    if (p.splits > 1) {
-        // one tile per cluster: its parts of the same side, added in rank order
-        int ki, ni;
-        tile_of(cluster, ki, ni);
-        const uint32_t base = ptx::smem_u32(smem);
-        const int first = 256 * 32 * split / p.splits; // four k per thread and step
-        const int last = 256 * 32 * (split + 1) / p.splits;
-        for (int i = first + static_cast<int>(threadIdx.x); i < last; i += kWgThreads) {
-            const int k = ki * 256 + side * 128 + (i & 31) * 4;
-            const int n = ni * 256 + (i >> 5);
-            if (k < p.k && n < p.n) { // p.k is a multiple of 32
-                float4 part[4];
-#pragma unroll
-                for (int s = 0; s < 4; ++s) {
-                    if (s < p.splits) {
-                        part[s] = ptx::ld_shared_cluster_f32x4(
-                            ptx::map_to_cta(base + 16u * static_cast<uint32_t>(i), static_cast<uint32_t>(2 * s + side)));
-                    }
-                }
-                float4 f = part[0];
-#pragma unroll
-                for (int s = 1; s < 4; ++s) {
-                    if (s < p.splits) {
-                        f.x += part[s].x;
-                        f.y += part[s].y;
-                        f.z += part[s].z;
-                        f.w += part[s].w;
-                    }
-                }
-                using T = typename WgElem<OUT>::type;
-                if (p.addend != nullptr) {
-                    const T* add = static_cast<const T*>(p.addend) + n * p.ld_addend + k;
-                    const T v[4] = {add[0], add[1], add[2], add[3]};
-                    f.x += static_cast<float>(v[0]);
-                    f.y += static_cast<float>(v[1]);
-                    f.z += static_cast<float>(v[2]);
-                    f.w += static_cast<float>(v[3]);
-                }
-                T* at = static_cast<T*>(p.out) + n * p.ld_out + k;
-                at[0] = static_cast<T>(f.x);
-                at[1] = static_cast<T>(f.y);
-                at[2] = static_cast<T>(f.z);
-                at[3] = static_cast<T>(f.w);
+    if (p.splits > 1) { // one tile per cluster
+        if (warp < 4) { // these have given their registers back
+            ptx::cluster_arrive();
+        } else {
+            int ki, ni;
+            tile_of(cluster, ki, ni);
+            const uint32_t base = ptx::smem_u32(smem);
+            const int thread = static_cast<int>(threadIdx.x) - 128;
+            if (p.splits == 2) {
+                wg_add_parts<2, OUT>(p, base, split, side, ki * 256 + side * 128, ni * 256, thread);
+            } else {
+                wg_add_parts<4, OUT>(p, base, split, side, ki * 256 + side * 128, ni * 256, thread);
             }
         }
-        ptx::cluster_arrive_relaxed(); // no CTA leaves while another still reads its shared memory
-        ptx::cluster_wait();
+        ptx::cluster_wait(); // no CTA leaves while another still reads its shared memory
     }
 }
 

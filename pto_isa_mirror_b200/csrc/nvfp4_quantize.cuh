@@ -482,9 +482,8 @@ __global__ void __launch_bounds__(THREADS)
                           max(__float_as_uint(v.z), __float_as_uint(v.w)));
             }
         }
-        __syncwarp();
-        ptx::cluster_arrive_relaxed(); // has read
         top = __reduce_max_sync(0xFFFFFFFFu, top);
+        ptx::cluster_arrive(); // has read: the releasing form, behind which no read of another CTA is under way any more
     } else {
         __syncthreads();
         top = __reduce_max_sync(0xFFFFFFFFu, part[lane]);
