@@ -125,7 +125,7 @@ __device__ __forceinline__ NvUnit nv_unit(int u, const NvGemmParams& p)
 }
 
 template <int OUT>
-__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kNvPairThreads, 1)
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kNvPairThreads)
     gemm_nvfp4_2cta(const __grid_constant__ CUtensorMap tmap_a, const __grid_constant__ CUtensorMap tmap_b,
                     const __grid_constant__ CUtensorMap tmap_b_half, const __grid_constant__ CUtensorMap tmap_sfa,
                     const __grid_constant__ CUtensorMap tmap_sfb, const NvGemmParams p)
@@ -192,7 +192,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kNvPairThreads, 1)
             const CUtensorMap* map_b = w.half ? &tmap_b_half : &tmap_b; // of a half tile 64 rows and one tile of scales
             const uint32_t stage_bytes = 2u * L::kStageBytes - (w.half ? L::kBBytes + L::kSfbBytes : 0u);
             for (int ks = 0; ks < p.k_stages; ++ks) {
-                ok = bounded_wait(&empty_bar[stage], phase ^ 1u, abort_flag, p.status, ST_NV_PRODUCER, p.wait_limit);
+                ok = bounded_wait_warp(&empty_bar[stage], phase ^ 1u, abort_flag, p.status, ST_NV_PRODUCER, p.wait_limit);
                 if (!ok) {
                     break;
                 }
@@ -233,14 +233,14 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kNvPairThreads, 1)
             const uint64_t sfa_desc0 = ptx::make_smem_desc(ptx::smem_u32(smem + L::kSfaOff), 0, 128, ptx::kSwizzleNone);
             const uint64_t sfb_desc0 = ptx::make_smem_desc(ptx::smem_u32(smem + L::kSfbOff), 0, 128, ptx::kSwizzleNone);
             for (int u = pair; ok && u < p.units; u += num_pairs) {
-                ok = bounded_wait(acc_empty_bar, acc_phase ^ 1u, abort_flag, p.status, ST_NV_MMA, p.wait_limit);
+                ok = bounded_wait_warp(acc_empty_bar, acc_phase ^ 1u, abort_flag, p.status, ST_NV_MMA, p.wait_limit);
                 if (!ok) {
                     break;
                 }
                 ptx::tc_fence_after_sync();
                 const uint32_t idesc = u < p.full_units ? p.idesc : p.idesc_half;
                 for (int ks = 0; ks < p.k_stages; ++ks) {
-                    ok = bounded_wait(&full_bar[stage], phase, abort_flag, p.status, ST_NV_MMA, p.wait_limit);
+                    ok = bounded_wait_warp(&full_bar[stage], phase, abort_flag, p.status, ST_NV_MMA, p.wait_limit);
                     if (!ok) {
                         break;
                     }
@@ -587,7 +587,7 @@ __global__ void __launch_bounds__(kNvFewThreads, 2)
         int stage = 0;
         uint32_t phase = 1; // the first round of the ring is loaded above
         for (int ks = ks0 + STAGES; ks < ks1; ++ks) {
-            if (!bounded_wait(&empty_bar[stage], phase ^ 1u, abort_flag, p.status, ST_NV_PRODUCER, p.wait_limit)) {
+            if (!bounded_wait_warp(&empty_bar[stage], phase ^ 1u, abort_flag, p.status, ST_NV_PRODUCER, p.wait_limit)) {
                 break;
             }
             if (ptx::elect_one()) {
@@ -608,7 +608,7 @@ __global__ void __launch_bounds__(kNvFewThreads, 2)
         const uint64_t sfw_desc0 = ptx::make_smem_desc(ptx::smem_u32(smem + L::kSfwOff), 0, 128, ptx::kSwizzleNone);
         const uint64_t sfx_desc0 = ptx::make_smem_desc(ptx::smem_u32(smem + L::kSfxOff), 0, 128, ptx::kSwizzleNone);
         for (int ks = ks0; ks < ks1; ++ks) {
-            ok = bounded_wait(&full_bar[stage], phase, abort_flag, p.status, ST_NV_MMA, p.wait_limit);
+            ok = bounded_wait_warp(&full_bar[stage], phase, abort_flag, p.status, ST_NV_MMA, p.wait_limit);
             if (!ok) {
                 break;
             }

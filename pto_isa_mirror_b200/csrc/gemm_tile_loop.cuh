@@ -156,6 +156,22 @@ __device__ __forceinline__ bool bounded_wait_quiet(uint64_t* bar, uint32_t parit
     return true;
 }
 
+// The same waits for a role that a whole warp walks, one elected lane issuing. The limit can run out in some lanes while the
+// barrier completes for others, which would then wait in the election for ever: the warp agrees on the answer.
+__device__ __forceinline__ bool bounded_wait_warp(uint64_t* bar, uint32_t parity, volatile uint32_t* abort_flag, int* status,
+                                                  int code, long long limit)
+{
+    return __all_sync(0xFFFFFFFFu, ptx::mbar_try_wait(bar, parity)) ||
+           __all_sync(0xFFFFFFFFu, bounded_wait(bar, parity, abort_flag, status, code, limit));
+}
+
+__device__ __forceinline__ bool bounded_wait_quiet_warp(uint64_t* bar, uint32_t parity, volatile uint32_t* abort_flag,
+                                                        int* status, int code, long long limit)
+{
+    return __all_sync(0xFFFFFFFFu, ptx::mbar_try_wait(bar, parity)) ||
+           __all_sync(0xFFFFFFFFu, bounded_wait_quiet(bar, parity, abort_flag, status, code, limit));
+}
+
 // Grouped raster: walk group_m row-tiles down, then step one column-tile right, so a wave of
 // concurrent CTAs shares a small set of A and B panels in L2.
 __device__ __forceinline__ void tile_coords(int t, const GemmParams& p, int& mi, int& ni)

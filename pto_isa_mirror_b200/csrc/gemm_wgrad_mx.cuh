@@ -398,7 +398,7 @@ __global__ void __launch_bounds__(kWgThreads, 1)
                 const int n0 = ni * 256 + side * 128;
                 for (int st = first_stage; st < last_stage; ++st) {
                     const int token = st * kWgStageTokens;
-                    ok = bounded_wait_quiet(&empty_bar[stage], phase ^ 1u, abort_flag, p.status, ST_WG_PRODUCER, p.wait_limit);
+                    ok = bounded_wait_quiet_warp(&empty_bar[stage], phase ^ 1u, abort_flag, p.status, ST_WG_PRODUCER, p.wait_limit);
                     if (!ok) {
                         break;
                     }
@@ -461,12 +461,12 @@ __global__ void __launch_bounds__(kWgThreads, 1)
             for (int tile = cluster; ok && tile < tiles; tile += clusters) {
                 for (int st = 0; st < stages; ++st) {
                     if (in_part == 0) {
-                        ok = bounded_wait_quiet(&acc_empty_bar[acc], acc_phase ^ 1u, abort_flag, p.status, ST_WG_MMA, p.wait_limit);
+                        ok = bounded_wait_quiet_warp(&acc_empty_bar[acc], acc_phase ^ 1u, abort_flag, p.status, ST_WG_MMA, p.wait_limit);
                         if (!ok) {
                             break;
                         }
                     }
-                    ok = bounded_wait_quiet(&full_bar[stage], phase, abort_flag, p.status, ST_WG_MMA, p.wait_limit);
+                    ok = bounded_wait_quiet_warp(&full_bar[stage], phase, abort_flag, p.status, ST_WG_MMA, p.wait_limit);
                     if (!ok) {
                         break;
                     }

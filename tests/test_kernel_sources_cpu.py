@@ -31,3 +31,20 @@ def test_reads_of_another_ctas_shared_memory_are_ordered_before_it_may_leave(nam
         if "add_parts" not in reads:  # which arrives itself
             assert arrival, text[at - 200:at]
         assert arrival is None or arrival.group() == "ptx::cluster_arrive()", text[at - 200:at]
+
+
+@pytest.mark.parametrize("name", ["gemm_nvfp4.cuh", "gemm_wgrad_mx.cuh"])
+def test_a_warp_that_elects_a_lane_agrees_on_its_waits(name):
+    # lanes for which a wait has run out must not leave a loop in which the others still elect a lane among all 32
+    text = source(name)
+    assert "elect_one()" in text
+    bare = list(re.finditer(r"bounded_wait(_quiet)?\((.*?), p\.wait_limit\);", text, re.S))
+    assert len(bare) == len(re.findall(r"bounded_wait(?:_quiet)?\(", text))
+    for m in bare:
+        if re.search(r"ST_\w+_(EPILOGUE|WORKER)$", m.group(2)):  # these roles elect nobody; they agree behind the wait
+            assert "ok = __all_sync(0xFFFFFFFFu, ok);" in text[m.end():m.end() + 700], m.group()
+        else:
+            assert "raw_empty_bar" in m.group(2) and "lane == 0)" in text[m.start() - 900:m.start()], m.group()  # a loop of one lane
+    for form in ("bounded_wait_warp", "bounded_wait_quiet_warp"):  # which answer by votes alone
+        body = source("gemm_tile_loop.cuh").split(f"bool {form}(")[1].split("}")[0].split("return ")[1]
+        assert all(term.strip().startswith("__all_sync(0xFFFFFFFFu, ") for term in body.split("||"))
