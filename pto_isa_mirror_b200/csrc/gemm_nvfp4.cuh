@@ -219,6 +219,14 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kNvPairThreads)
                 }
             }
         }
+#pragma unroll 1
+        for (int i = 0; ok && i < STAGES; ++i) { // the leader's last signals have come before this CTA may leave
+            ok = bounded_wait_warp(&empty_bar[stage], phase ^ 1u, abort_flag, p.status, ST_NV_PRODUCER, p.wait_limit);
+            if (++stage == STAGES) {
+                stage = 0;
+                phase ^= 1u;
+            }
+        }
     } else if (warp == 1) {
         // ---------------------------------------------------------------- scale copies and products (leader)
         // cta_group::2 copies the same shared-memory offsets of both CTAs into both CTAs' tensor memory; a thread's copies
@@ -281,6 +289,9 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kNvPairThreads)
                     }
                 }
                 acc_phase ^= 1u;
+            }
+            if (ok) { // the other CTA's last signals have come before this one may leave
+                bounded_wait_warp(acc_empty_bar, acc_phase ^ 1u, abort_flag, p.status, ST_NV_MMA, p.wait_limit);
             }
         }
     } else {

@@ -423,6 +423,14 @@ __global__ void __launch_bounds__(kWgThreads, 1)
                     }
                 }
             }
+#pragma unroll 1
+            for (int i = 0; ok && i < kWgStages; ++i) { // the even CTA's last signals have come before this CTA may leave
+                ok = bounded_wait_quiet_warp(&empty_bar[stage], phase ^ 1u, abort_flag, p.status, ST_WG_PRODUCER, p.wait_limit);
+                if (++stage == kWgStages) {
+                    stage = 0;
+                    phase ^= 1u;
+                }
+            }
         } else if (warp == 2) {
             // ---------------------------------------------------------------- loads of x, as far ahead as their own ring goes
             if (!SCRATCH && lane == 0) {
@@ -498,6 +506,11 @@ __global__ void __launch_bounds__(kWgThreads, 1)
                         acc_phase ^= (acc == 0) ? 1u : 0u;
                     }
                 }
+            }
+            for (int i = 0; ok && i < 2; ++i) { // the other CTA's last signals have come before this one may leave
+                ok = bounded_wait_quiet_warp(&acc_empty_bar[acc], acc_phase ^ 1u, abort_flag, p.status, ST_WG_MMA, p.wait_limit);
+                acc ^= 1;
+                acc_phase ^= (acc == 0) ? 1u : 0u;
             }
         }
     } else {

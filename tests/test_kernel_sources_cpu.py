@@ -48,3 +48,15 @@ def test_a_warp_that_elects_a_lane_agrees_on_its_waits(name):
     for form in ("bounded_wait_warp", "bounded_wait_quiet_warp"):  # which answer by votes alone
         body = source("gemm_tile_loop.cuh").split(f"bool {form}(")[1].split("}")[0].split("return ")[1]
         assert all(term.strip().startswith("__all_sync(0xFFFFFFFFu, ") for term in body.split("||"))
+
+
+@pytest.mark.parametrize("name,stages,wait", [("gemm_nvfp4.cuh", "STAGES", "bounded_wait_warp"),
+                                              ("gemm_wgrad_mx.cuh", "kWgStages", "bounded_wait_quiet_warp")])
+def test_no_signal_reaches_a_cta_of_the_pair_after_it_has_left(name, stages, wait):
+    text = source(name)
+    # from the even CTA: the loading warp waits once more for every stage of its ring behind its last load
+    assert re.search(r"for \(int i = 0; ok && i < " + stages + r"; \+\+i\) {\s*ok = " + wait + r"\(&empty_bar\[stage\], phase \^ 1u", text)
+    # to it: its product warp waits once more for every accumulator to be handed back
+    issue = text.index("umma_commit_pair(")
+    waits = [m.start() for m in re.finditer(wait + r"\(&?acc_empty_bar", text)]
+    assert len(waits) == 2 and waits[0] < issue < waits[1]
