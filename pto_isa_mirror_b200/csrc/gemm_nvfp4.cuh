@@ -54,8 +54,8 @@ constexpr int kNvAtomBytes = 512;    // scales of 128 rows x 64 elements
 
 __device__ __forceinline__ float nv_alpha(const NvGemmParams& p)
 {
-    const float a = p.ga != nullptr ? __ldg(p.ga) : 1.0f;
-    const float b = p.gb != nullptr ? __ldg(p.gb) : 1.0f;
+    const float a = p.ga != nullptr ? nv_ld_common(p.ga) : 1.0f;
+    const float b = p.gb != nullptr ? nv_ld_common(p.gb) : 1.0f;
     return a * b;
 }
 
@@ -305,7 +305,11 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kNvPairThreads)
         const float alpha = nv_alpha(p);
         auto finish = [&](uint32_t acc, int col) {
             const float f = __uint_as_float(acc) * alpha;
-            return p.bias != nullptr && col < p.n ? f + __ldg(p.bias + col) : f;
+            float add = -0.0f; // changes no number; as a branch around the sum the 16-bit forms spill
+            if (p.bias != nullptr && col < p.n) {
+                add = nv_ld_common(p.bias + col);
+            }
+            return f + add;
         };
         uint32_t acc_phase = 0;
         bool ok = true;
@@ -479,7 +483,14 @@ __device__ __forceinline__ void nv_add_parts(const NvGemmParams& p, uint32_t bas
     const int items = rows * 32;
     const int first = items * rank / SPLITS + static_cast<int>(threadIdx.x);
     const int last = items * (rank + 1) / SPLITS;
+    static_assert(kNvFewThreads % 32 == 0, "a thread's steps lie in the same columns");
+    const int col = ni * 128 + (first & 31) * 4;
     const float alpha = nv_alpha(p);
+    float bias[4];
+#pragma unroll
+    for (int c = 0; c < 4; ++c) {
+        bias[c] = p.bias != nullptr && col + c < p.n ? p.bias[col + c] : 0.0f;
+    }
 #pragma unroll
     for (int k0 = 0; k0 < kSteps; k0 += kKept) {
         float4 sum[kKept];
@@ -492,7 +503,7 @@ __device__ __forceinline__ void nv_add_parts(const NvGemmParams& p, uint32_t bas
 #pragma unroll
                 for (int r = 0; r < SPLITS; ++r) {
                     part[u][r] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-                    if (i < last && ni * 128 + (i & 31) * 4 < p.n) { // nothing is read that is not used
+                    if (i < last && col < p.n) { // nothing is read that is not used
                         part[u][r] = ptx::ld_shared_cluster_f32x4(ptx::map_to_cta(base + 16u * static_cast<uint32_t>(i), r));
                     }
                 }
@@ -516,14 +527,13 @@ __device__ __forceinline__ void nv_add_parts(const NvGemmParams& p, uint32_t bas
 #pragma unroll
         for (int u = 0; u < kKept; ++u) {
             const int i = first + (k0 + u) * kNvFewThreads;
-            const int col = ni * 128 + (i & 31) * 4;
             if (i < last && col < p.n) {
                 const long long row = row0 + (i >> 5);
                 const float f[4] = {sum[u].x * alpha, sum[u].y * alpha, sum[u].z * alpha, sum[u].w * alpha};
 #pragma unroll
                 for (int c = 0; c < 4; ++c) {
                     if (col + c < p.n) {
-                        nv_store_one<OUT>(p, row, col + c, f[c] + (p.bias != nullptr ? __ldg(p.bias + col + c) : 0.0f));
+                        nv_store_one<OUT>(p, row, col + c, f[c] + bias[c]);
                     }
                 }
             }
@@ -666,7 +676,7 @@ __global__ void __launch_bounds__(kNvFewThreads, 2)
             const int in_tile = quarter * 32 + lane;
             const int col = ni * 128 + in_tile;
             const float alpha = nv_alpha(p);
-            const float bias = (p.bias != nullptr && col < p.n) ? __ldg(p.bias + col) : 0.0f;
+            const float bias = (p.bias != nullptr && col < p.n) ? p.bias[col] : 0.0f;
             float* part = reinterpret_cast<float*>(smem); // [BLOCK_T][128]; every load and product of the ring is done
             uint32_t v[32];
 #pragma unroll

@@ -202,9 +202,9 @@ struct WgElem<WG_OUT_F16> {
 constexpr int kWgConvertThreads = 256;
 
 template <bool F16>
-__global__ void __launch_bounds__(kWgConvertThreads) mx_to_16bit_kernel(const uint8_t* __restrict__ data,
-                                                                         const uint8_t* __restrict__ scales,
-                                                                         uint16_t* __restrict__ out, int rows, int k,
+__global__ void __launch_bounds__(kWgConvertThreads) mx_to_16bit_kernel(const uint8_t* data,
+                                                                         const uint8_t* scales,
+                                                                         uint16_t* out, int rows, int k,
                                                                          long long ld_data, long long ld_scales)
 {
     const int row_items = k / 16;
@@ -227,8 +227,8 @@ __global__ void __launch_bounds__(kWgConvertThreads) mx_to_16bit_kernel(const ui
             in[u] = make_uint4(0u, 0u, 0u, 0u);
             e[u] = 127u;
             if (i < total) {
-                in[u] = __ldcs(reinterpret_cast<const uint4*>(data + row * ld_data) + c);
-                e[u] = __ldg(scales + row * ld_scales + (c >> 1));
+                in[u] = nv_ld16_once(reinterpret_cast<const uint4*>(data + row * ld_data) + c);
+                e[u] = nv_ld_byte(scales + row * ld_scales + (c >> 1));
             }
             i += stride;
             row += row_step;
@@ -544,13 +544,13 @@ __global__ void __launch_bounds__(kWgThreads, 1)
             if (visit_token + kWgStageTokens <= p.t) {
 #pragma unroll
                 for (int h = 0; h < 4; ++h) {
-                    e[h] = __ldg(base + 16 * h * p.ld_scales + scale_off);
+                    e[h] = nv_ld_byte(base + 16 * h * p.ld_scales + scale_off);
                 }
             } else if (visit_token < p.t) {
                 const int last_row = p.t - 1 - visit_token;
 #pragma unroll
                 for (int h = 0; h < 4; ++h) {
-                    e[h] = __ldg(base + (min(row + 16 * h, last_row) - row) * p.ld_scales + scale_off);
+                    e[h] = nv_ld_byte(base + (min(row + 16 * h, last_row) - row) * p.ld_scales + scale_off);
                 }
             }
             visit_token += kWgGroups * kWgStageTokens;

@@ -154,9 +154,9 @@ __global__ void __launch_bounds__(kQuantThreads) mx_quantize_e4m3_kernel(const f
 constexpr int kQuant16Items = 2;
 
 template <int ALG, int SRC, int VEC>
-__global__ void __launch_bounds__(kQuantThreads) mx_quantize_e4m3_16bit_kernel(const uint16_t* __restrict__ src,
-                                                                                uint8_t* __restrict__ data,
-                                                                                uint8_t* __restrict__ scales, int rows, int k,
+__global__ void __launch_bounds__(kQuantThreads) mx_quantize_e4m3_16bit_kernel(const uint16_t* src,
+                                                                                uint8_t* data,
+                                                                                uint8_t* scales, int rows, int k,
                                                                                 long long ld_src, long long ld_data,
                                                                                 long long ld_scales)
 {

@@ -182,8 +182,8 @@ constexpr int kNvItems = 2;
 
 template <int SRC, int VEC>
 __global__ void __launch_bounds__(kNvQuantThreads)
-    nvfp4_quantize_kernel(const void* __restrict__ src, const float* __restrict__ amax, uint8_t* __restrict__ data,
-                          uint8_t* __restrict__ scales, float* __restrict__ tensor_scale, int rows, int k,
+    nvfp4_quantize_kernel(const void* src, const float* amax, uint8_t* data,
+                          uint8_t* scales, float* tensor_scale, int rows, int k,
                           long long ld_src, long long ld_data)
 {
     using T = typename NvElem<SRC>::type;
@@ -245,9 +245,9 @@ __global__ void __launch_bounds__(kNvQuantThreads)
 // (Through a shared-memory tile of 256 x 64: 118 us for bf16 and 249 us for fp32 on 16384 x 8192.)
 template <int SRC, bool PAIRS>
 __global__ void __launch_bounds__(kNvQuantThreads)
-    nvfp4_quantize_transposed_kernel(const void* __restrict__ src, const float* __restrict__ amax,
-                                     uint8_t* __restrict__ data, uint8_t* __restrict__ scales,
-                                     float* __restrict__ tensor_scale, int rows, int k, long long ld_src, long long ld_data)
+    nvfp4_quantize_transposed_kernel(const void* src, const float* amax,
+                                     uint8_t* data, uint8_t* scales,
+                                     float* tensor_scale, int rows, int k, long long ld_src, long long ld_data)
 {
     using T = typename NvElem<SRC>::type;
     constexpr int kCols = PAIRS ? 2 : 1;
@@ -282,7 +282,7 @@ __global__ void __launch_bounds__(kNvQuantThreads)
                 for (int j = 0; j < 16; ++j) {
                     const T* at = p + static_cast<long long>(b * 16 + j) * ld_src;
                     if constexpr (PAIRS) {
-                        nv_unpack2<SRC>(__ldcs(reinterpret_cast<const uint32_t*>(at)), x[0][j], x[1][j]);
+                        nv_unpack2<SRC>(nv_ld_word_once(at), x[0][j], x[1][j]);
                     } else {
                         x[0][j] = nv_to_float<SRC>(*at);
                     }
@@ -351,7 +351,7 @@ constexpr int kAmaxSingleElems = 65536; // what one block of that many threads i
 
 template <int SRC, int VEC>
 __global__ void __launch_bounds__(kAmaxSingleThreads)
-    amax_kernel(const void* __restrict__ src, uint32_t* __restrict__ out, int rows, int k, long long ld_src)
+    amax_kernel(const void* src, uint32_t* out, int rows, int k, long long ld_src)
 {
     using T = typename NvElem<SRC>::type;
     constexpr int kAmaxItems = SRC == NV_F32 ? 2 : 4; // 128 bytes in flight per thread
@@ -417,8 +417,8 @@ constexpr int kNvOneBlocks = kNvOneCtas * 1024 * kNvItems; // of 16 elements, a 
 
 template <int SRC, int VEC, int THREADS>
 __global__ void __launch_bounds__(THREADS)
-    nvfp4_quantize_one_kernel(const void* __restrict__ src, float* __restrict__ amax, uint8_t* __restrict__ data,
-                              uint8_t* __restrict__ scales, float* __restrict__ tensor_scale, int rows, int k,
+    nvfp4_quantize_one_kernel(const void* src, float* amax, uint8_t* data,
+                              uint8_t* scales, float* tensor_scale, int rows, int k,
                               long long ld_src, long long ld_data)
 {
     using T = typename NvElem<SRC>::type;
@@ -525,8 +525,8 @@ __device__ __forceinline__ __half2 nv_e2m1x2_to_half2(uint32_t byte)
 // elements - two of them in flight. VEC: the result's rows start on 32-byte boundaries.
 template <int DST, bool VEC>
 __global__ void __launch_bounds__(kNvQuantThreads)
-    nvfp4_dequantize_kernel(const uint8_t* __restrict__ data, const uint8_t* __restrict__ scales,
-                            const float* __restrict__ tensor_scale, void* __restrict__ out, int rows, int k,
+    nvfp4_dequantize_kernel(const uint8_t* data, const uint8_t* scales,
+                            const float* tensor_scale, void* out, int rows, int k,
                             long long ld_data, long long ld_out)
 {
     using T = typename NvElem<DST>::type;
@@ -556,11 +556,11 @@ __global__ void __launch_bounds__(kNvQuantThreads)
                 const uint32_t* p = reinterpret_cast<const uint32_t*>(data + row * ld_data) + static_cast<long long>(c) * kWords;
 #pragma unroll
                 for (int w = 0; w < kWords; ++w) {
-                    codes[u][w] = c * kElems + 8 * w < k ? __ldcs(p + w) : 0u;
+                    codes[u][w] = c * kElems + 8 * w < k ? nv_ld_word_once(p + w) : 0u;
                 }
                 const int kb = c * kElems / 16;
                 const long long tile = (row >> 7) * k_atoms + (kb >> 2);
-                s_code[u] = __ldg(scales + tile * 512 + (row & 31) * 16 + ((row >> 5) & 3) * 4 + (kb & 3));
+                s_code[u] = nv_ld_byte(scales + tile * 512 + (row & 31) * 16 + ((row >> 5) & 3) * 4 + (kb & 3));
             }
             i += stride;
             row += row_step;

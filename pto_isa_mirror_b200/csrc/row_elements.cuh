@@ -47,8 +47,11 @@ __device__ __forceinline__ void nv_unpack2(uint32_t w, float& lo, float& hi)
     }
 }
 
-// One float that every thread of a grid reads, kept behind what stands before it in the program (a wait for an earlier
-// launch), which a load of constant data need not be. (A volatile load passes the first-level cache by: 2 us more for a
+// Loads of what an earlier launch may still be writing when this one starts (programmatic serialisation). They stand behind
+// ptx::grid_dependency_wait in the program, and have to stay there: as volatile asm, and never through the read-only path
+// (.nc, __ldg, or what the compiler makes of a const __restrict__ source), which is for memory that nothing writes while the
+// kernel runs.
+// One float that every thread of a grid reads: through the first-level cache. (A volatile load passes it by: 2 us more for a
 // cast of 4093x2904 and back.)
 __device__ __forceinline__ float nv_ld_common(const float* ptr)
 {
@@ -57,13 +60,35 @@ __device__ __forceinline__ float nv_ld_common(const float* ptr)
     return f;
 }
 
+__device__ __forceinline__ uint32_t nv_ld_byte(const uint8_t* ptr)
+{
+    uint32_t b;
+    asm volatile("ld.global.u8 %0, [%1];" : "=r"(b) : "l"(ptr) : "memory");
+    return b;
+}
+
+__device__ __forceinline__ uint32_t nv_ld_word_once(const void* ptr)
+{
+    uint32_t w;
+    asm volatile("ld.global.cs.b32 %0, [%1];" : "=r"(w) : "l"(ptr) : "memory");
+    return w;
+}
+
+__device__ __forceinline__ uint4 nv_ld16_once(const void* ptr)
+{
+    uint4 a;
+    asm volatile("ld.global.cs.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(a.x), "=r"(a.y), "=r"(a.z), "=r"(a.w) : "l"(ptr) : "memory");
+    return a;
+}
+
 // 32 bytes in one access (32-byte aligned): a warp's accesses are then whole lines. With two of 16 bytes each covers
 // half of every sector (dequantising 16384 x 8192 to bf16 took 92 us that way).
 __device__ __forceinline__ void nv_ld32(const void* ptr, uint4& a, uint4& b)
 {
-    asm volatile("ld.global.nc.L1::no_allocate.v8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
+    asm volatile("ld.global.L1::no_allocate.v8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
                  : "=r"(a.x), "=r"(a.y), "=r"(a.z), "=r"(a.w), "=r"(b.x), "=r"(b.y), "=r"(b.z), "=r"(b.w)
-                 : "l"(ptr));
+                 : "l"(ptr)
+                 : "memory");
 }
 
 __device__ __forceinline__ void nv_st32(void* ptr, const uint4& a, const uint4& b)
@@ -90,7 +115,7 @@ struct NvRaw16 {
         } else {
 #pragma unroll
             for (int i = 0; i < kQuads; ++i) {
-                q[i] = __ldcs(static_cast<const uint4*>(ptr) + i);
+                q[i] = nv_ld16_once(static_cast<const uint4*>(ptr) + i);
             }
         }
     }

@@ -60,3 +60,14 @@ def test_no_signal_reaches_a_cta_of_the_pair_after_it_has_left(name, stages, wai
     issue = text.index("umma_commit_pair(")
     waits = [m.start() for m in re.finditer(wait + r"\(&?acc_empty_bar", text)]
     assert len(waits) == 2 and waits[0] < issue < waits[1]
+
+
+@pytest.mark.parametrize("name", ["row_elements.cuh", "nvfp4_quantize.cuh", "gemm_nvfp4.cuh", "gemm_wgrad_mx.cuh", "mx_quantize.cuh"])
+def test_launches_that_may_start_early_use_no_read_only_loads(name):
+    # such a launch runs while the one before it still writes what it is going to read
+    text = source(name)
+    if name == "mx_quantize.cuh":  # its other kernels wait for the launch before them as a whole
+        kernels = [t for t in re.split(r"template <", text) if "grid_dependency_wait()" in t]
+        assert len(kernels) == 1
+        text = kernels[0]
+    assert not re.search(r"\.nc\b|__ldg\(|__restrict__", text)
