@@ -219,14 +219,6 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kNvPairThreads)
                 }
             }
         }
-#pragma unroll 1
-        for (int i = 0; ok && i < STAGES; ++i) { // the leader's last signals have come before this CTA may leave
-            ok = bounded_wait_warp(&empty_bar[stage], phase ^ 1u, abort_flag, p.status, ST_NV_PRODUCER, p.wait_limit);
-            if (++stage == STAGES) {
-                stage = 0;
-                phase ^= 1u;
-            }
-        }
     } else if (warp == 1) {
         // ---------------------------------------------------------------- scale copies and products (leader)
         // cta_group::2 copies the same shared-memory offsets of both CTAs into both CTAs' tensor memory; a thread's copies
@@ -240,6 +232,9 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kNvPairThreads)
             const uint64_t b_desc0 = ptx::make_smem_desc(ptx::smem_u32(smem + L::kBOff), 16, 1024, ptx::kSwizzle128B);
             const uint64_t sfa_desc0 = ptx::make_smem_desc(ptx::smem_u32(smem + L::kSfaOff), 0, 128, ptx::kSwizzleNone);
             const uint64_t sfb_desc0 = ptx::make_smem_desc(ptx::smem_u32(smem + L::kSfbOff), 0, 128, ptx::kSwizzleNone);
+            // stages left of all units: the last round of the ring is not handed back, since nobody would wait for that and a
+            // signal could reach the other CTA after it has left
+            long long left = static_cast<long long>((p.units - pair + num_pairs - 1) / num_pairs) * p.k_stages;
             for (int u = pair; ok && u < p.units; u += num_pairs) {
                 ok = bounded_wait_warp(acc_empty_bar, acc_phase ^ 1u, abort_flag, p.status, ST_NV_MMA, p.wait_limit);
                 if (!ok) {
@@ -277,11 +272,14 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kNvPairThreads)
                                                     sf + 16u + 8u * g, (ks > 0 || g > 0) ? 1u : 0u);
                             }
                         }
-                        ptx::umma_commit_pair(&empty_bar[stage], 0x3);
+                        if (left > STAGES) {
+                            ptx::umma_commit_pair(&empty_bar[stage], 0x3);
+                        }
                         if (ks == p.k_stages - 1) {
                             ptx::umma_commit_pair(acc_full_bar, 0x3);
                         }
                     }
+                    --left;
                     __syncwarp();
                     if (++stage == STAGES) {
                         stage = 0;
