@@ -31,7 +31,8 @@ namespace pto_b200 {
 
 constexpr int kNvQuantThreads = 256;
 
-// Exponent field of g for a tensor maximum: amax / 2688 rounded up to a power of two, 2688 = 1.3125 * 2^11.
+// Exponent field of g for a tensor maximum: amax / 2688 rounded up to a power of two, 2688 = 1.3125 * 2^11. An infinity or a
+// NaN counts as the largest number.
 __device__ __forceinline__ uint32_t nv_scale_exponent(float amax)
 {
     const uint32_t bits = min(__float_as_uint(amax) & 0x7FFFFFFFu, 0x7F7FFFFFu);
@@ -199,9 +200,10 @@ __global__ void __launch_bounds__(kNvQuantThreads)
     long long row = i / row_blocks;
     int kb = static_cast<int>(i - row * row_blocks);
     ptx::grid_dependency_wait();
-    const NvTensorScale t(nv_ld_common(amax));
-    if (blockIdx.x == 0 && threadIdx.x == 0) {
-        *tensor_scale = t.g;
+    const float top_of_tensor = nv_ld_common(amax);
+    const NvTensorScale t(top_of_tensor);
+    if (blockIdx.x == 0 && threadIdx.x == 0) { // a maximum gone wrong stays visible in every number and product
+        *tensor_scale = isfinite(top_of_tensor) ? t.g : __uint_as_float(0x7FC00000u);
     }
     while (i - static_cast<int>(threadIdx.x & 31u) < total) { // the warp goes on together
         NvRaw16<SRC> raw[kNvItems];
@@ -256,9 +258,10 @@ __global__ void __launch_bounds__(kNvQuantThreads)
     const long long total = static_cast<long long>(k_atoms) * col_items;
     const bool wide = (reinterpret_cast<uintptr_t>(data) & 31u) == 0 && (ld_data & 31) == 0;
     ptx::grid_dependency_wait();
-    const NvTensorScale t(nv_ld_common(amax));
-    if (blockIdx.x == 0 && threadIdx.x == 0) {
-        *tensor_scale = t.g;
+    const float top_of_tensor = nv_ld_common(amax);
+    const NvTensorScale t(top_of_tensor);
+    if (blockIdx.x == 0 && threadIdx.x == 0) { // a maximum gone wrong stays visible in every number and product
+        *tensor_scale = isfinite(top_of_tensor) ? t.g : __uint_as_float(0x7FC00000u);
     }
     for (long long it = blockIdx.x * static_cast<long long>(blockDim.x) + threadIdx.x; it < total;
          it += static_cast<long long>(gridDim.x) * blockDim.x) {

@@ -52,9 +52,9 @@ def nvfp4_quantize(src: torch.Tensor, amax: Optional[torch.Tensor] = None, trans
     scales [ceil(rows / 128), ceil(K / 64), 512] uint8, tensor_scale [1] float32), K16 = K rounded up to 16 with zeros:
     the operands :func:`gemm_nvfp4` takes.
 
-    tensor_scale: the smallest power of two >= amax / 2688 (1 for amax = 0). ``amax``: one float32 on the device, finite
-    and not negative, for a largest magnitude known from calibration (what exceeds it saturates); without it the largest
-    finite magnitude of src is found first: in the same launch for small sources, in a pass of its own for others. Block scale: the e4m3 value nearest to
+    tensor_scale: the smallest power of two >= amax / 2688 (1 for amax = 0). ``amax``: one float32 on the device, not
+    negative, for a largest magnitude known from calibration (what exceeds it saturates; from an infinite or NaN one
+    tensor_scale is NaN, and so is every number that uses it); without it the largest finite magnitude of src is found first: in the same launch for small sources, in a pass of its own for others. Block scale: the e4m3 value nearest to
     max|x| / (6 tensor_scale), at most 448; code: the e2m1 value nearest to x / (scale tensor_scale), ties to the even
     code, at most 6 in magnitude. A block with an infinity or a NaN gets the scale NaN.
 
