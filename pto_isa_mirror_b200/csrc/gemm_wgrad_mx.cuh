@@ -4,9 +4,8 @@
 // quantised, read as it is. The sum runs over tokens, so both operands lie with their summed index outermost
 // ("MN-major"): the tensor core takes them in that order from 128-byte swizzled rows and nothing is transposed.
 //
-// x becomes 16-bit on the way: every e4m3 value times a power of two is a bf16 value exactly (below 2^-126 in magnitude
-// the smallest bits are cut off), and an fp16 value where it lies in fp16's range (above it: infinity, below 2^-14:
-// rounded). So dy meets the numbers the checkpoint stands for, at the 16-bit rate of the tensor core.
+// x becomes 16-bit on the way: every e4m3 value times a power of two is a bf16 value exactly (below 2^-126 in magnitude:
+// rounded), and an fp16 value where it lies in fp16's range (above it: infinity, below 2^-14: rounded). So dy meets the numbers the checkpoint stands for, at the 16-bit rate of the tensor core.
 //
 // Two ways to the same bits. Without scratch memory x is converted tile by tile in shared memory, beside the products
 // (SCRATCH = false); every tile of x then is converted once for each 256 columns of dy. With scratch for T x K 16-bit
@@ -123,8 +122,10 @@ __device__ __forceinline__ void wg_convert16_any(const uint4& raw, uint32_t e, u
             const __half2 v = __floats2half2_rn(lo, hi);
             o[i] = *reinterpret_cast<const uint32_t*>(&v);
         } else {
-            // at most four significant bits: the upper half of the float is the bf16 value
-            o[i] = __byte_perm(__float_as_uint(lo), __float_as_uint(hi), 0x7632);
+            // exact but below 2^-126, where it rounds as the short form's multiplication does: which of the two a value meets
+            // depends on its neighbours
+            const __nv_bfloat162 v = __floats2bfloat162_rn(lo, hi);
+            o[i] = *reinterpret_cast<const uint32_t*>(&v);
         }
     }
 }

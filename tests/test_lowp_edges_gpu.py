@@ -34,3 +34,30 @@ def test_a_maximum_gone_wrong_stays_visible(rows, k, transpose, bad):
     x[0, 5] = bad
     found = pto.nvfp4_quantize(x, transpose=transpose)[2]
     assert float(found) == ref.power_of_two_scale(float(x[torch.isfinite(x)].abs().max()))
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("form", ["fused", "scratch", "default"])
+@pytest.mark.parametrize("e", [0, 1, 3, 7, 9, 12, 101, 102, 103, 110, 127, 134, 135, 142, 143, 180, 200])
+@pytest.mark.parametrize("broken", [False, True])
+def test_every_byte_with_every_neighbour(broken, e, form, dtype):
+    # dy picks out one token a row, so dW is x as the product meets it: rounded once to dy's type, whatever stands beside it
+    # (a NaN or another block's scale takes a warp, or a thread, to the conversion that holds for all bytes)
+    t, k = 64, 256
+    byte = (torch.arange(t)[:, None] * 37 + torch.arange(k)[None, :]) % 256
+    byte[(byte & 0x7F) == 0x7F] = 0x7E
+    scales = torch.full((t, k // 32), e, dtype=torch.uint8)
+    if broken:
+        byte[5, 3], byte[40, 200] = 0x7F, 0xFF
+        scales[17, 4] = 254
+    data = byte.to(torch.uint8)
+    x = data.view(torch.float8_e4m3fn).double().view(t, -1, 32) * torch.exp2(scales.double() - 127)[:, :, None]
+    x = x.view(t, k).float().to(dtype).double()  # exact as float: at most four bits, down to 2^-136
+    up = 2.0 ** 60 if dtype == torch.bfloat16 and e < 64 else 1.0  # out of the range where fp32 sums have few bits
+    dy = (torch.eye(t) * up).to(dtype).to(DEV)
+    workspace = {"fused": False, "scratch": torch.empty(2 * t * k, dtype=torch.uint8, device=DEV), "default": None}[form]
+    got = pto.gemm_wgrad_mx(dy, data.to(DEV), scales.to(DEV), workspace=workspace).double().cpu()
+    clean = torch.isfinite(x).all(0)  # an infinity or a NaN times 0 is a NaN: its column is
+    assert torch.equal(got[:, clean], (x[:, clean] * up).float().double())  # fp32 ends at 2^128, where 2^60 times x may not
+    assert not torch.isfinite(got[:, ~clean]).all(0).any()
+    assert int(clean.sum()) > 0 or (dtype == torch.float16 and e > 134)
