@@ -266,10 +266,7 @@ int launch_nv_few(cudaStream_t stream, const HostContext& host, const NvProblem&
         return rc;
     }
     const long long n_tiles = (static_cast<long long>(q.n) + 127) / 128;
-    const long long t_tiles = (static_cast<long long>(q.m) + BLOCK_T - 1) / BLOCK_T;
-    if (n_tiles > 65535 || t_tiles > 65535) {
-        return PTO_B200_EINVAL;
-    }
+    const long long t_tiles = (static_cast<long long>(q.m) + BLOCK_T - 1) / BLOCK_T; // both fit a grid: launch_nv sees to it
     // K parts: as many as keep all of them resident at two CTAs per SM, each with four stages of K at least (with two,
     // 128x4096x4096 took 11.9 us instead of 9.9)
     int splits = 1;
@@ -301,9 +298,10 @@ int launch_nv(cudaStream_t stream, const HostContext& host, const NvProblem& q, 
     // is long enough to gain by it (beyond eight 256-element stages). Measured, few rows / pairs, us: 512x8192x8192 (64
     // tiles of 256 x 256) 23.1 / 16.9, 200x8192x4096 (32) 11.6 / 10.3, 200x4096x8192 (16) 11.2 / 14.6, 256x512x8192 (2)
     // 7.6 / 14.2, 144x512x1024 (2, four stages) 7.8 / 6.1. At most 128 rows: half of a pair's rows would be empty,
-    // 128x8192x8192 12.2 / 15.5, 48x14336x4096 9.2 / 10.7.
+    // 128x8192x8192 12.2 / 15.5, 48x14336x4096 9.2 / 10.7. More columns than a grid's second axis counts in tiles of 128: pairs.
     const long long tiles256 = ((static_cast<long long>(q.m) + 255) / 256) * ((static_cast<long long>(q.n) + 255) / 256);
-    if (q.m > 128 && (8 * tiles256 > host.sm_count || p.k_stages <= 8)) {
+    constexpr int kMostFewColumns = 65535 * 128;
+    if (q.n > kMostFewColumns || (q.m > 128 && (8 * tiles256 > host.sm_count || p.k_stages <= 8))) {
         return launch_nv_pair<OUT>(stream, host, q, p);
     }
     if (q.m <= 16) {

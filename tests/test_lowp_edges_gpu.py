@@ -61,3 +61,20 @@ def test_every_byte_with_every_neighbour(broken, e, form, dtype):
     assert torch.equal(got[:, clean], (x[:, clean] * up).float().double())  # fp32 ends at 2^128, where 2^60 times x may not
     assert not torch.isfinite(got[:, ~clean]).all(0).any()
     assert int(clean.sum()) > 0 or (dtype == torch.float16 and e > 134)
+
+
+def test_few_rows_of_more_columns_than_a_grids_second_axis_counts():
+    m, n, k = 3, 65535 * 128 + 129, 16
+    g = gen(3)
+    codes = torch.randint(0, 256, (2048, k // 2), generator=g, dtype=torch.uint8)  # the columns repeat these
+    a = torch.zeros((m, 16), dtype=torch.uint8)
+    a[:, :8] = torch.randint(0, 256, (m, k // 2), generator=g, dtype=torch.uint8)
+    sfa = ref.tile_scales(torch.randint(0x30, 0x40, (m, 1), generator=g))
+    sfb_rows = torch.randint(0x30, 0x40, (2048, 1), generator=g)
+    tiles = ref.tile_scales(sfb_rows)
+    b = torch.zeros((n, 16), dtype=torch.uint8, device=DEV)
+    b[:, :8] = codes.to(DEV).repeat((n + 2047) // 2048, 1)[:n]
+    sfb = tiles.to(DEV).repeat(((n + 127) // 128 + 15) // 16, 1, 1)[: (n + 127) // 128].contiguous()
+    out = pto.gemm_nvfp4(a.to(DEV)[:, :8], b[:, :8], sfa.to(DEV), sfb, out_dtype=torch.float32)
+    want = (ref.values(a[:, :8].contiguous(), sfa) @ ref.values(codes, tiles).t()).float().to(DEV)  # sums of 16: exact in fp32
+    assert torch.equal(out, want.repeat(1, (n + 2047) // 2048)[:, :n])
