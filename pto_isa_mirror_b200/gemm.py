@@ -355,7 +355,7 @@ def mx_quantize_e4m3(src: torch.Tensor, stream: Optional[torch.cuda.Stream] = No
     """OCP MX quantisation (TQUANT, MXFP8): float32, bfloat16 or float16 src [rows, K] -> (e4m3 bytes [rows, K] uint8, e8m0
     scales [rows, K/32] uint8), one scale per 32 elements along K. float32: finite input only; a 16-bit block with an
     infinity or a NaN gets the scale 255, a NaN. ``data`` / ``scales``: caller's output
-    buffers of those shapes (allocated when omitted). ``scale_alg``: ``_capi.SCALE_OCP`` (default) or ``_capi.SCALE_NV``,
+    buffers of those shapes (allocated when omitted, on ``stream`` when one is given). ``scale_alg``: ``_capi.SCALE_OCP`` (default) or ``_capi.SCALE_NV``,
     the reference's QuantScaleAlg."""
     lib = _capi.load()
     _require_cuda_2d(src, "src")
@@ -370,14 +370,15 @@ def mx_quantize_e4m3(src: torch.Tensor, stream: Optional[torch.cuda.Stream] = No
             if t.dtype != torch.uint8 or tuple(t.shape) != shape:
                 raise ValueError(f"{name} must be a uint8 CUDA tensor of shape {shape}")
     device = _device_of(src, data, scales)
-    if device != torch.cuda.current_device():
-        with torch.cuda.device(device):
-            return mx_quantize_e4m3(src, stream, data, scales, scale_alg)
+    there = _elsewhere(device, stream)
+    if there is not None:
+        with there:
+            return mx_quantize_e4m3(src, None, data, scales, scale_alg)
     if data is None:
         data = src.new_empty_strided((rows, k), (k, 1), dtype=torch.uint8)
     if scales is None:
         scales = src.new_empty_strided((rows, k // 32), (k // 32, 1), dtype=torch.uint8)
-    rc = lib.pto_b200_mx_quantize_e4m3_src(_stream_ptr(stream), data.data_ptr(), scales.data_ptr(), src.data_ptr(), rows, k,
+    rc = lib.pto_b200_mx_quantize_e4m3_src(_raw_stream(device), data.data_ptr(), scales.data_ptr(), src.data_ptr(), rows, k,
                                            src.stride()[0] if rows > 1 else k, data.stride()[0] if rows > 1 else k,
                                            scales.stride()[0] if rows > 1 else k // 32, _TORCH_TO_PTO[src.dtype],
                                            scale_alg)

@@ -78,3 +78,19 @@ def test_few_rows_of_more_columns_than_a_grids_second_axis_counts():
     out = pto.gemm_nvfp4(a.to(DEV)[:, :8], b[:, :8], sfa.to(DEV), sfb, out_dtype=torch.float32)
     want = (ref.values(a[:, :8].contiguous(), sfa) @ ref.values(codes, tiles).t()).float().to(DEV)  # sums of 16: exact in fp32
     assert torch.equal(out, want.repeat(1, (n + 2047) // 2048)[:, :n])
+
+
+def test_outputs_of_another_stream_are_not_blocks_still_in_use():
+    x = torch.randn((2048, 2048), generator=gen(6)).to(torch.bfloat16).to(DEV)
+    want = pto.mx_quantize_e4m3(x)
+    side = torch.cuda.Stream()
+    for _ in range(4):
+        torch.cuda.synchronize()
+        blocks = [torch.empty_like(w) for w in want]
+        torch.cuda._sleep(20_000_000)  # the current stream is busy for some ten milliseconds
+        for b in blocks:
+            b.fill_(0x55)  # and still to write these
+        del blocks, b
+        got = pto.mx_quantize_e4m3(x, stream=side)
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(got, want))

@@ -1,0 +1,76 @@
+"""The host side of the low-precision entry points without a GPU: which stream outputs belong to, what import needs."""
+import contextlib
+import sys
+
+import pytest
+import torch
+
+import pto_isa_mirror_b200 as pto
+from pto_isa_mirror_b200 import _capi
+
+gemm = sys.modules["pto_isa_mirror_b200.gemm"]  # the package's `gemm` is the function
+
+
+class OnDevice:
+    """Stands for a CUDA tensor."""
+
+    def __init__(self, shape, dtype, events):
+        self.shape, self.dtype, self.events = torch.Size(shape), dtype, events
+
+    def stride(self):
+        return (self.shape[1], 1)
+
+    def data_ptr(self):
+        return 4096
+
+    def get_device(self):
+        return 0
+
+    def new_empty_strided(self, size, stride, dtype):
+        self.events.append("allocate")
+        return OnDevice(size, dtype, self.events)
+
+
+class Stream:
+    def __init__(self, device_index):
+        self.device_index, self.cuda_stream = device_index, 77
+
+
+@pytest.fixture
+def events(monkeypatch):
+    seen = []
+
+    @contextlib.contextmanager
+    def on(stream):
+        seen.append("enter")
+        yield
+        seen.append("leave")
+
+    class Lib:
+        @staticmethod
+        def pto_b200_mx_quantize_e4m3_src(stream, *args):
+            seen.append(("launch", stream))
+            return 0
+
+    inside = lambda: seen.count("enter") - seen.count("leave")  # noqa: E731
+    monkeypatch.setattr(torch.cuda, "stream", on)
+    monkeypatch.setattr(torch.cuda, "current_device", lambda: 0)
+    monkeypatch.setattr(gemm, "_raw_stream", lambda device: 77 if inside() else 5)
+    monkeypatch.setattr(gemm, "_require_cuda_2d", lambda t, name: None)
+    monkeypatch.setattr(_capi, "load", lambda: Lib)
+    return seen
+
+
+def test_the_mx_quantisers_outputs_belong_to_the_stream_it_launches_on(events):
+    # blocks of the current stream's pool may still be used by work queued there, which the other stream does not wait for
+    pto.mx_quantize_e4m3(OnDevice((4, 64), torch.bfloat16, events), stream=Stream(0))
+    assert events == ["enter", "allocate", "allocate", ("launch", 77), "leave"]
+    events.clear()
+    pto.mx_quantize_e4m3(OnDevice((4, 64), torch.bfloat16, events))
+    assert events == ["allocate", "allocate", ("launch", 5)]
+
+
+def test_the_mx_quantiser_refuses_a_stream_of_another_device(events):
+    with pytest.raises(ValueError, match="another device"):
+        pto.mx_quantize_e4m3(OnDevice((4, 64), torch.bfloat16, events), stream=Stream(1))
+    assert events == []
