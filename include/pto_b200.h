@@ -246,7 +246,7 @@ int pto_b200_amax(void* stream, float* amax, const uint8_t* src, int rows, int k
 /*
  * Quantise src (rows x k; F32, BF16 or F16; leading dimension ld_src elements) to NVFP4:
  *   *tensor_scale = g = the smallest power of two >= *amax / 2688 (1 for 0; NaN for an infinite or NaN *amax, so that what
- *                   went wrong stays visible; *amax is not negative)
+ *                   went wrong stays visible; *amax is not negative and is not *tensor_scale itself)
  *   scale         = the e4m3 value nearest to max|x| / (6 g) of its 16 elements, at most 448
  *   code          = the e2m1 value nearest to x / (scale g), ties to the even code, at most 6; 0 where the scale is 0
  * Decisions are those of exact arithmetic. A block with an infinity or a NaN gets the scale NaN (0x7F) and zero codes;

@@ -332,7 +332,7 @@ int check_quantize(const void* data, const void* scales, const void* tensor_scal
         misaligned(tensor_scale, 4) || misaligned(amax, 4)) {
         return PTO_B200_EALIGN;
     }
-    return PTO_B200_OK;
+    return tensor_scale == amax ? PTO_B200_EINVAL : PTO_B200_OK; // one block writes the one while others still read the other
 }
 
 } // namespace

@@ -67,6 +67,8 @@ def nvfp4_quantize(src: torch.Tensor, amax: Optional[torch.Tensor] = None, trans
         raise ValueError("src must be float32, bfloat16 or float16")
     _require_float_scalar(amax, "amax")
     _require_float_scalar(tensor_scale, "tensor_scale")
+    if amax is not None and tensor_scale is not None and amax.data_ptr() == tensor_scale.data_ptr():
+        raise ValueError("tensor_scale must not be amax itself")
     rows, k = src.shape
     if rows == 0 or k == 0:
         raise ValueError("src must not be empty")

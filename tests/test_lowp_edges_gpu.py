@@ -94,3 +94,10 @@ def test_outputs_of_another_stream_are_not_blocks_still_in_use():
         got = pto.mx_quantize_e4m3(x, stream=side)
         torch.cuda.synchronize()
         assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+def test_refusals_of_maxima_and_widths():
+    x = torch.randn((8, 64), generator=gen(7)).to(DEV)
+    place = torch.ones(1, device=DEV)
+    with pytest.raises(ValueError):
+        pto.nvfp4_quantize(x, amax=place, tensor_scale=place)

@@ -1,12 +1,13 @@
 """The host side of the low-precision entry points without a GPU: which stream outputs belong to, what import needs."""
 import contextlib
+import ctypes
 import sys
 
 import pytest
 import torch
 
 import pto_isa_mirror_b200 as pto
-from pto_isa_mirror_b200 import _capi
+from pto_isa_mirror_b200 import _capi, build
 
 gemm = sys.modules["pto_isa_mirror_b200.gemm"]  # the package's `gemm` is the function
 
@@ -74,3 +75,17 @@ def test_the_mx_quantiser_refuses_a_stream_of_another_device(events):
     with pytest.raises(ValueError, match="another device"):
         pto.mx_quantize_e4m3(OnDevice((4, 64), torch.bfloat16, events), stream=Stream(1))
     assert events == []
+
+
+@pytest.mark.parametrize("transpose", [0, 1])
+@pytest.mark.parametrize("rows", [4, 1 << 20])
+def test_a_quantisers_maximum_and_tensor_scale_are_two_places(rows, transpose):
+    build.build()
+    lib = _capi.load()
+    buf = (ctypes.c_uint8 * 4096)()
+    p = (ctypes.addressof(buf) + 63) & ~63
+    before = lib.pto_b200_launch_count()
+    tail = (rows, 64, 64, 1 << 20, _capi.BF16, transpose)  # rows, k, ld_src, ld_data, source type
+    assert lib.pto_b200_nvfp4_quantize(None, p, p + 512, p + 256, p + 1024, p + 256, *tail) == _capi.EINVAL
+    assert lib.pto_b200_nvfp4_quantize_dynamic(None, p, p + 512, p + 256, p + 256, p + 1024, *tail) == _capi.EINVAL
+    assert lib.pto_b200_launch_count() == before
