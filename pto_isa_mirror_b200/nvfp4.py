@@ -113,16 +113,16 @@ def nvfp4_quantize(src: torch.Tensor, amax: Optional[torch.Tensor] = None, trans
 def nvfp4_dequantize(data: torch.Tensor, scales: torch.Tensor, tensor_scale: Optional[torch.Tensor] = None,
                      out_dtype: torch.dtype = torch.bfloat16, out: Optional[torch.Tensor] = None,
                      stream: Optional[torch.cuda.Stream] = None) -> torch.Tensor:
-    """The numbers [rows, K] that packed codes data [rows, K / 2] with their scale tiles stand for: code * scale *
-    tensor_scale (None: 1), float32, bfloat16 or float16. Exact before the output's own rounding when tensor_scale is a
+    """The numbers [rows, K] that packed codes data [rows, K / 2] with their scale tiles stand for, K a multiple of 16: code *
+    scale * tensor_scale (None: 1), float32, bfloat16 or float16. Exact before the output's own rounding when tensor_scale is a
     power of two. ``out`` may lack up to 15 of the last columns, those that filled up the last block."""
     lib = _capi.load()
     _require_cuda_2d(data, "data")
     if data.dtype not in _CODES:
         raise ValueError("data must be packed codes, uint8")
     rows, k = data.shape[0], data.shape[1] * 2
-    if rows == 0 or k == 0:
-        raise ValueError("data must not be empty")
+    if rows == 0 or k == 0 or k % 16 != 0:
+        raise ValueError("data must hold whole blocks of 16 codes, 8 bytes each, and not be empty")
     _require_scales(scales, rows, k, "scales")
     _require_float_scalar(tensor_scale, "tensor_scale")
     if out is not None:
@@ -141,7 +141,7 @@ def nvfp4_dequantize(data: torch.Tensor, scales: torch.Tensor, tensor_scale: Opt
     cols = out.shape[1]
     rc = lib.pto_b200_nvfp4_dequantize(_raw_stream(device), out.data_ptr(), data.data_ptr(), scales.data_ptr(),
                                        _ptr(tensor_scale), rows, cols,
-                                       data.stride()[0] if rows > 1 else (k // 2 + 3) // 4 * 4,
+                                       data.stride()[0] if rows > 1 else k // 2,
                                        out.stride()[0] if rows > 1 else cols, _TORCH_TO_PTO[out.dtype])
     _capi.check(rc, "pto_b200_nvfp4_dequantize")
     return out

@@ -101,3 +101,8 @@ def test_refusals_of_maxima_and_widths():
     place = torch.ones(1, device=DEV)
     with pytest.raises(ValueError):
         pto.nvfp4_quantize(x, amax=place, tensor_scale=place)
+    data, scales, g = pto.nvfp4_quantize(x[:1])
+    for width in (1, 3, 12, 28):
+        with pytest.raises(ValueError):
+            pto.nvfp4_dequantize(data[:, :width], scales, g)
+    assert torch.equal(pto.nvfp4_dequantize(data[:, :24], scales, g), pto.nvfp4_dequantize(data, scales, g)[:, :48])

@@ -89,3 +89,25 @@ def test_a_quantisers_maximum_and_tensor_scale_are_two_places(rows, transpose):
     assert lib.pto_b200_nvfp4_quantize(None, p, p + 512, p + 256, p + 1024, p + 256, *tail) == _capi.EINVAL
     assert lib.pto_b200_nvfp4_quantize_dynamic(None, p, p + 512, p + 256, p + 256, p + 1024, *tail) == _capi.EINVAL
     assert lib.pto_b200_launch_count() == before
+
+
+@pytest.mark.parametrize("shape", [(1, 1), (1, 3), (1, 36), (5, 4), (130, 33), (2, 12), (0, 8), (3, 0)])
+def test_codes_to_dequantise_come_in_whole_blocks(monkeypatch, shape):
+    # the kernel reads whole words of codes, and a row's scale tiles are counted from its blocks
+    nvfp4 = sys.modules["pto_isa_mirror_b200.nvfp4"]
+    launches = []
+
+    class Lib:
+        pto_b200_nvfp4_dequantize = staticmethod(lambda *args: launches.append(args) or 0)
+
+    monkeypatch.setattr(nvfp4, "_require_cuda_2d", lambda t, name: None)
+    monkeypatch.setattr(nvfp4, "_require_scales", lambda *args: None)
+    monkeypatch.setattr(nvfp4, "_raw_stream", lambda device: 5)
+    monkeypatch.setattr(nvfp4, "_elsewhere", lambda device, stream: None)
+    monkeypatch.setattr(_capi, "load", lambda: Lib)
+    scales = OnDevice((1, 1, 512), torch.uint8, [])
+    with pytest.raises(ValueError, match="blocks of 16"):
+        pto.nvfp4_dequantize(OnDevice(shape, torch.uint8, []), scales)
+    assert launches == []
+    assert pto.nvfp4_dequantize(OnDevice((1, 40), torch.uint8, []), scales).shape == (1, 80)
+    assert len(launches) == 1 and launches[0][5:9] == (1, 80, 40, 80)  # rows, k, ld_data, ld_out
