@@ -9,6 +9,8 @@ from . import _capi
 from .gemm import _TORCH_TO_PTO, _device_of, _elsewhere, _raw_stream, _require_cuda_2d
 from .nvfp4 import _FLOATS, _new, _ptr
 
+_E8M0_BYTES = (torch.uint8,) + ((torch.float8_e8m0fnu,) if hasattr(torch, "float8_e8m0fnu") else ())
+
 
 def _scratch_pays(t: int, n: int, k: int) -> bool:
     """Converting x once against converting it for every 256 columns of dy. Measured, us without / with scratch (T x N x K):
@@ -36,8 +38,8 @@ def gemm_wgrad_mx(dy: torch.Tensor, data: torch.Tensor, scales: torch.Tensor, ou
         _require_cuda_2d(t, name)
     if dy.dtype not in (torch.bfloat16, torch.float16):
         raise ValueError("dy must be bfloat16 or float16")
-    if data.dtype not in (torch.uint8, torch.float8_e4m3fn) or scales.element_size() != 1:
-        raise ValueError("data must be e4m3 bytes (uint8 or float8_e4m3fn) and scales e8m0 bytes")
+    if data.dtype not in (torch.uint8, torch.float8_e4m3fn) or scales.dtype not in _E8M0_BYTES:
+        raise ValueError("data must be e4m3 bytes (uint8 or float8_e4m3fn) and scales e8m0 bytes (uint8 or float8_e8m0fnu)")
     t, n = dy.shape
     k = data.shape[1]
     if data.shape[0] != t:

@@ -111,3 +111,25 @@ def test_codes_to_dequantise_come_in_whole_blocks(monkeypatch, shape):
     assert launches == []
     assert pto.nvfp4_dequantize(OnDevice((1, 40), torch.uint8, []), scales).shape == (1, 80)
     assert len(launches) == 1 and launches[0][5:9] == (1, 80, 40, 80)  # rows, k, ld_data, ld_out
+
+
+def test_the_weight_gradients_scales_are_e8m0_bytes(monkeypatch):
+    wgrad = sys.modules["pto_isa_mirror_b200.wgrad"]
+    launches = []
+
+    class Lib:
+        pto_b200_gemm_wgrad_mx = staticmethod(lambda *args: launches.append(args) or 0)
+
+    monkeypatch.setattr(wgrad, "_require_cuda_2d", lambda t, name: None)
+    monkeypatch.setattr(wgrad, "_raw_stream", lambda device: 5)
+    monkeypatch.setattr(wgrad, "_elsewhere", lambda device, stream: None)
+    monkeypatch.setattr(_capi, "load", lambda: Lib)
+    call = lambda dtype: pto.gemm_wgrad_mx(  # noqa: E731
+        OnDevice((8, 16), torch.bfloat16, []), OnDevice((8, 64), torch.uint8, []), OnDevice((8, 2), dtype, []))
+    for dtype in (torch.bool, torch.int8, torch.float8_e4m3fn, torch.float8_e5m2):
+        with pytest.raises(ValueError, match="e8m0"):
+            call(dtype)
+    assert launches == []
+    for dtype in (torch.uint8, torch.float8_e8m0fnu):
+        assert call(dtype).shape == (16, 64)
+    assert len(launches) == 2
