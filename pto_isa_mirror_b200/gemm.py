@@ -29,7 +29,8 @@ if hasattr(torch, "float8_e4m3fn"):
     _TORCH_TO_PTO[torch.float8_e5m2] = E5M2
 
 
-_raw_stream = torch._C._cuda_getCurrentRawStream  # the current stream of a device as a pointer, without a Stream object
+# the current stream of a device as a pointer, without a Stream object; a torch built without CUDA has none
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
 
 
 def _stream_ptr(stream: Optional[torch.cuda.Stream]) -> int:

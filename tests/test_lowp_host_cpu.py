@@ -1,6 +1,8 @@
 """The host side of the low-precision entry points without a GPU: which stream outputs belong to, what import needs."""
 import contextlib
 import ctypes
+import os
+import subprocess
 import sys
 
 import pytest
@@ -133,3 +135,19 @@ def test_the_weight_gradients_scales_are_e8m0_bytes(monkeypatch):
     for dtype in (torch.uint8, torch.float8_e8m0fnu):
         assert call(dtype).shape == (16, 64)
     assert len(launches) == 2
+
+
+def test_the_package_imports_with_a_torch_built_without_cuda():
+    code = """
+import torch
+del torch._C._cuda_getCurrentRawStream  # what such a build lacks
+import pto_isa_mirror_b200 as pto
+from pto_isa_mirror_b200 import build, gen_data
+try:
+    pto.gemm(torch.zeros((4, 4)), torch.zeros((4, 4)))
+except ValueError as e:
+    print("refused:", e)
+"""
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    got = subprocess.run([sys.executable, "-c", code], cwd=root, capture_output=True, text=True, timeout=600)
+    assert got.returncode == 0 and got.stdout.startswith("refused:"), got.stderr
