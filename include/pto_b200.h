@@ -307,8 +307,9 @@ int pto_b200_mx_quantize_e4m3_src(void* stream, uint8_t* data, uint8_t* scales, 
  *   workspace : null, or t * k * 2 bytes, 32-byte aligned: the activations are then converted to dy's type once, into it,
  *               instead of tile by tile for every 256 columns of dy; the result is the same to the bit
  * The activations are multiplied as the numbers they stand for, in dy's type: exact for BF16 down to 2^-126 and rounded
- * below; for F16 what lies above 65504 becomes infinite and what lies below 2^-14 is rounded. Sums are fp32, rounded at
- * least every 2048 tokens where the tensor core's own sum cuts off. The result does not depend on timing.
+ * below; for F16 what lies above 65504 becomes infinite and what lies below 2^-14 is rounded. Sums are fp32, those of at
+ * most 1024 tokens the tensor core's own, which cuts off, and these are added with rounding. The result does not depend on
+ * timing.
  */
 int pto_b200_gemm_wgrad_mx(void* stream, uint8_t* out, const uint8_t* dy, const uint8_t* data, const uint8_t* scales,
                            const uint8_t* addend, uint8_t* workspace, size_t workspace_bytes, int t, int n, int k,

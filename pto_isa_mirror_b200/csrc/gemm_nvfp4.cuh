@@ -8,6 +8,11 @@
 // The last stage of K may hold fewer than four 64-element groups: only those that exist are multiplied, so what stands
 // in the scale buffers past them never matters.
 //
+// The tensor core's fp32 sums cut off instead of rounding. They are not joined in parts: an instruction adds 64 of K at once,
+// and products of 4-bit numbers and their scales have few bits. Measured, relative (plain fp32 product of the same numbers):
+// K = 16384, normal numbers exact, of one sign 4.9e-8 (7.5e-7); 65536, 2e-9 (3e-9) and 5.9e-7 (3.3e-6); 262144 of one sign
+// 7.8e-6.
+//
 // gemm_nvfp4_2cta: a cluster of two CTAs owns a 256 x 256 tile (many rows). gemm_nvfp4_few_rows: few rows of A, the
 // bound is reading B; see there.
 #pragma once

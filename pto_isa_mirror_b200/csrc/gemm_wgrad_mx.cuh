@@ -24,12 +24,13 @@
 // once per 64 values of a thread), scales are fetched by the threads that use them, and the product warp keeps its
 // descriptors in uniform registers (its issue alone took 800 cycles of a stage's 513 before).
 //
-// Sums: the tensor core adds into its accumulator by cutting off, not by rounding (measured here: 1.9e-5 of the result
-// lost after 16384 terms, 3.8e-5 after 32768). So an accumulator takes kWgFoldStages x 64 = 1024 tokens at most; the
-// converting warps then add it to fp32 sums in their registers, with rounding, while the other accumulator fills.
+// Sums: the tensor core adds into its accumulator by cutting off, not by rounding. One accumulator for all tokens would lose
+// (measured here, relative, normal numbers / of one sign) 8.8e-6 / 3.5e-5 of 16384 of them and 2.1e-5 / 9.1e-5 of 32768. So
+// an accumulator takes kWgFoldStages x 64 = 1024 tokens at most; the converting warps then add it to fp32 sums in their
+// registers, with rounding, while the other accumulator fills.
 // Relative error of 16384 tokens, and time of 16384x8192x8192 with and without scratch, by tokens per accumulator:
 //   2048   6.3e-7 (terms of one sign 2.4e-6)   1456 / 1739 us
-//   1024   2.8e-7 (9.4e-7)                     1440 / 1778 us
+//   1024   2.9e-7 (9.5e-7)                     1440 / 1778 us
 //    512   1.5e-7 (3.6e-7)                     1470 / 1863 us
 //    256   1.1e-7 (1.5e-7)                     1515 / 2595 us
 // A plain fp32 matrix product of the same numbers has 5.7e-7 there.

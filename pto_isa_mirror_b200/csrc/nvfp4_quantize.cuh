@@ -9,8 +9,9 @@
 //
 // g is a power of two on purpose: x / g is then exact, and so is every decision below. A border between two codes
 // times s has at most seven bits, so a quotient that is rounded correctly never moves onto a border that the exact
-// quotient misses, and fp32 gives the codes that real arithmetic gives. It costs no accuracy: the block scales keep
-// their relative precision wherever in their range they lie.
+// quotient misses, and fp32 gives the codes that real arithmetic gives. It costs up to one binade at the top of e4m3's
+// range: blocks that are small beside the tensor's maximum reach the subnormal scales, and zero, up to a factor of two
+// earlier. Elsewhere the block scales keep their relative precision.
 //
 // Scales are stored as the block-scaled tensor-core instruction reads them: 512-byte tiles of 128 rows x 4 scales (64
 // elements of K), tile (row / 128, k / 64) in row-major order, byte (row % 32) * 16 + (row % 128) / 32 * 4 + j. The

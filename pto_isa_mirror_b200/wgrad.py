@@ -26,7 +26,7 @@ def gemm_wgrad_mx(dy: torch.Tensor, data: torch.Tensor, scales: torch.Tensor, ou
     bytes and ``scales`` [T, K / 32] e8m0 bytes, as :func:`mx_quantize_e4m3` returns them (and :func:`gemm_mx` reads them
     in the forward pass). dy [T, N]: bfloat16 or float16, rows on 16-byte boundaries; K a multiple of 32.
 
-    x enters as the numbers the bytes stand for, in dy's type - exact for bfloat16; float16 has its range. Sums are
+    x enters as the numbers the bytes stand for, in dy's type - exact for bfloat16 down to 2^-126; float16 has its range. Sums are
     float32; dW is float32, bfloat16 or float16. ``addend`` [N, K], of dW's type, is added before the rounding; it may be
     ``out`` itself, which accumulates gradients in place.
 
