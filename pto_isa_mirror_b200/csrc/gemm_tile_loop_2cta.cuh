@@ -321,6 +321,13 @@ __global__ void __cluster_dims__(2, 1, 1)
                     }
                 }
             }
+            for (int i = 0; ok && i < STAGES; ++i) { // the leader's last signals have come before this CTA may leave
+                ok = bounded_wait(&empty_bar[stage], phase ^ 1u, abort_flag, p.status, ST_PRODUCER_TIMEOUT, p.wait_limit);
+                if (++stage == STAGES) {
+                    stage = 0;
+                    phase ^= 1u;
+                }
+            }
         }
     } else if (warp == 1) {
         if constexpr (KIND == KIND_MXF8) {
@@ -417,6 +424,13 @@ __global__ void __cluster_dims__(2, 1, 1)
                     break;
                 }
                 ptx::umma_commit_pair(&acc_full_bar[acc], 0x3);
+                if (++acc == kNumAcc) {
+                    acc = 0;
+                    acc_phase ^= 1u;
+                }
+            }
+            for (int i = 0; ok && i < kNumAcc; ++i) { // the other CTA's last signals have come before this one may leave
+                ok = bounded_wait(&acc_empty_bar[acc], acc_phase ^ 1u, abort_flag, p.status, ST_MMA_ACC_TIMEOUT, p.wait_limit);
                 if (++acc == kNumAcc) {
                     acc = 0;
                     acc_phase ^= 1u;

@@ -75,3 +75,12 @@ def test_launches_that_may_start_early_use_no_read_only_loads(name):
         assert len(kernels) == 1
         text = kernels[0]
     assert not re.search(r"\.nc\b|__ldg\(|__restrict__", text)
+
+
+def test_no_signal_reaches_a_cta_of_the_tile_loops_pair_after_it_has_left():
+    # both sides wait once more, behind their last load and their last product, for what the other still signals
+    text = source("gemm_tile_loop_2cta.cuh")
+    for last, bar, rounds in (("tma_load_2d_pair(", "empty_bar[stage], phase", "STAGES"),
+                              ("umma_commit_pair(&acc_full_bar", "acc_empty_bar[acc], acc_phase", "kNumAcc")):
+        behind = text[text.rindex(last):]
+        assert re.search(r"for \(int i = 0; ok && i < " + rounds + r"; \+\+i\) {\s*ok = bounded_wait\(&" + re.escape(bar) + r" \^ 1u", behind)
