@@ -475,14 +475,15 @@ __device__ __forceinline__ void nv_store_one(const NvGemmParams& p, long long ro
 // CTA's shared memory and are added in rank order. Four columns per thread and step, kAtOnce steps at a time, all their reads
 // in flight together (a read from another SM takes about a thousand cycles: one value at a time this took 12000 cycles for
 // 48 rows, one step at a time 4300). The arrival that lets the other CTAs leave comes behind the last reads, in the releasing
-// form, behind which no read is under way any more; it waits for stores, too, so up to 64 rows keep their sums until then.
-// Sums kept / stored as they come: 1x4096x4096 6.4 / 6.6 us, 64x4096x4096 7.9 / 8.3; 128x8192x8192 16.6 / 15.7.
+// form, behind which no read is under way any more; it waits for stores, too, so few steps (up to 64 rows, or an eighth of
+// 128) keep their sums until then. Sums kept / stored as they come, weights in L2: 1x4096x4096 5.2 / 5.3 us, 256x512x8192
+// 8.0 / 8.2; 128x8192x8192, eleven steps, 12.8 / 12.4, 200x4096x8192, six, 12.0 / 11.6.
 template <int BLOCK_T, int SPLITS, int OUT>
 __device__ __forceinline__ void nv_add_parts(const NvGemmParams& p, uint32_t base, int rank, int ni, int row0, int rows)
 {
     constexpr int kSteps = (BLOCK_T * 32 / SPLITS + kNvFewThreads - 1) / kNvFewThreads;
     constexpr int kAtOnce = 8 / SPLITS;
-    constexpr int kKept = BLOCK_T <= 64 ? (kSteps + kAtOnce - 1) / kAtOnce * kAtOnce : kAtOnce;
+    constexpr int kKept = BLOCK_T <= 64 || SPLITS == 8 ? (kSteps + kAtOnce - 1) / kAtOnce * kAtOnce : kAtOnce;
     const int items = rows * 32;
     const int first = items * rank / SPLITS + static_cast<int>(threadIdx.x);
     const int last = items * (rank + 1) / SPLITS;

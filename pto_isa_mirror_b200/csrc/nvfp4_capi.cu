@@ -296,9 +296,9 @@ int launch_nv(cudaStream_t stream, const HostContext& host, const NvProblem& q, 
 {
     // More than 128 rows: CTA pairs, unless the tiles are so few that the other kernel cuts K into four parts or more and K
     // is long enough to gain by it (beyond eight 256-element stages). Measured, few rows / pairs, us: 512x8192x8192 (64
-    // tiles of 256 x 256) 23.1 / 16.9, 200x8192x4096 (32) 11.6 / 10.3, 200x4096x8192 (16) 11.2 / 14.6, 256x512x8192 (2)
-    // 7.6 / 14.2, 144x512x1024 (2, four stages) 7.8 / 6.1. At most 128 rows: half of a pair's rows would be empty,
-    // 128x8192x8192 12.2 / 15.5, 48x14336x4096 9.2 / 10.7. More columns than a grid's second axis counts in tiles of 128: pairs.
+    // tiles of 256 x 256) 22.1 / 16.5, 200x8192x4096 (32) 10.5 / 10.0, 200x4096x8192 (16) 11.5 / 14.6, 256x512x8192 (2)
+    // 8.0 / 14.4, 144x512x1024 (2, four stages) 7.1 / 6.1. At most 128 rows: half of a pair's rows would be empty,
+    // 128x8192x8192 12.4 / 14.9, 48x14336x4096 8.9 / 10.7. More columns than a grid's second axis counts in tiles of 128: pairs.
     const long long tiles256 = ((static_cast<long long>(q.m) + 255) / 256) * ((static_cast<long long>(q.n) + 255) / 256);
     constexpr int kMostFewColumns = 65535 * 128;
     if (q.n > kMostFewColumns || (q.m > 128 && (8 * tiles256 > host.sm_count || p.k_stages <= 8))) {

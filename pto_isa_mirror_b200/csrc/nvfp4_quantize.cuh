@@ -415,7 +415,7 @@ __global__ void __launch_bounds__(kAmaxSingleThreads)
 // Few rows: the largest magnitude and the codes in one launch. A cluster of up to eight CTAs holds the matrix in registers
 // between the two, kNvItems blocks of 16 per thread, and exchanges its maxima over distributed shared memory. The CTAs have
 // 256, 512 or 1024 threads, the fewest that hold it, since large ones start and meet slowly: 8x4096 bf16 2.9 us with 256,
-// 4.1 with 1024 (2.5 as it is launched now). In two launches / in one: 1x4096 4.0 / 2.6, 8x4096 4.6 / 2.5, 64x4096 7.8 / 4.5.
+// 4.1 with 1024 (2.6 as it is launched now). In two launches / in one: 1x4096 4.4 / 2.8, 8x4096 4.9 / 2.6, 64x4096 7.4 / 4.9.
 constexpr int kNvOneCtas = 8;
 constexpr int kNvOneBlocks = kNvOneCtas * 1024 * kNvItems; // of 16 elements, a row's filled up to 64
 
