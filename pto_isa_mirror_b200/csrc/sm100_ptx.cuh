@@ -310,9 +310,10 @@ __device__ __forceinline__ uint32_t map_to_cta(uint32_t smem_addr, uint32_t rank
 }
 
 __device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory"); }
-// Arrival that orders no memory: for a rendezvous that only says "I no longer touch your shared memory, barriers or
-// tensor memory". (The releasing form also waits for this CTA's outstanding stores, the TMA stores of the last tile
-// among them: measured 1.0 us against 0.43 us at the end of the pair kernel.)
+// Arrival that orders no memory: for a rendezvous behind which a CTA may leave, where nothing is under way to it any more.
+// Signals on its barriers have been waited for; reads of its shared memory have not, so behind those stands the releasing
+// form. (That one also waits for this CTA's outstanding stores, the TMA stores of the last tile among them: measured 1.0 us
+// against 0.43 us at the end of the pair kernel.)
 __device__ __forceinline__ void cluster_arrive_relaxed() { asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory"); }
 __device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory"); }
 
